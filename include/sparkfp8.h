@@ -467,6 +467,78 @@ int sfp8_bf16_fold_grads(const void* dwp, const float* w, const float* nw, int64
                          float* dnw, float* part, int64_t part_floats, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Routing of tokens to experts: what runs around the grouped expert kernels.
+ * dtype codes: 0 fp32, 1 bf16, 2 fp16.
+ * ------------------------------------------------------------------------- */
+
+/* Each token's top_k experts and their weights from logits [T, E] (rows ld
+ * elements apart).  Scores s: score 0 softmax, 1 sigmoid of the logits.  The
+ * order value of an expert is its logit, or s + bias when bias (fp32 [E]) is
+ * not NULL; an expert whose logit or order value is -inf is never taken, NaN
+ * ranks above everything, and the lowest index comes first among equals.
+ * groups > 1: the experts are groups of E / groups in a row, and only the
+ * top_groups best groups take part, a group's value being its best order
+ * value (group_best 1) or the sum of its two best scores with their biases
+ * (group_best 2).  weights = scale * s, or scale * s / (sum of the chosen s)
+ * when renorm.  Writes weights fp32, selected int64 and picked fp32 (the
+ * chosen logits; may be NULL), each [T, top_k] in descending order; slots
+ * without an expert and every slot of a token whose mask byte is 0 (mask may
+ * be NULL) get 0, -1 and 0.  E <= 1024, groups <= 64 dividing E, top_k <= 64
+ * and at most the experts of the kept groups, T <= 2^25. */
+int sfp8_moe_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, const float* bias,
+                   const void* mask, int score, int64_t groups, int64_t top_groups, int64_t group_best,
+                   int64_t top_k, int renorm, float scale, float* weights, int64_t* selected, float* picked,
+                   void* stream);
+
+/* The gradient dlogits [T, E] (the logits' type, contiguous) from dweights
+ * fp32 [T, top_k]; selected and picked as sfp8_moe_route wrote them (no expert
+ * twice in a row).  logits (rows ld apart) is read for score 0 without renorm
+ * only, and may be NULL otherwise. */
+int sfp8_moe_route_bwd(const float* dweights, const int64_t* selected, const float* picked, const void* logits,
+                       int dtype, int64_t T, int64_t E, int64_t ld, int score, int64_t top_k, int renorm, float scale,
+                       void* dlogits, void* stream);
+
+/* The stable order of R = T * top_k slots by expert (selected int64; a slot
+ * outside [0, E) names no expert and comes last): token_index[row] = slot /
+ * top_k, inverse[slot] = row (-1 for a slot without an expert), offsets[e] =
+ * inclusive row counts (int32 [E]).  R <= 2^30, E <= 1024; ws of
+ * sfp8_moe_expert_order_workspace_ints(R, E) ints (NULL when that is 0). */
+int64_t sfp8_moe_expert_order_workspace_ints(int64_t R, int64_t E);
+int sfp8_moe_expert_order(const int64_t* selected, int64_t R, int64_t top_k, int64_t E, int64_t* token_index,
+                          int64_t* inverse, int* offsets, int* ws, int64_t ws_ints, void* stream);
+
+/* out[t] = sum over j < top_k of weights[t, j] * rows[inverse[t, j]] (rows
+ * [R, D] and out [T, D] of one type, weights fp32), summed in fp32 in slot
+ * order and rounded once; slots whose row is outside [0, R) add nothing.
+ * Backward: drows[inverse[t, j]] = weights[t, j] * dout[t] and dweights[t, j]
+ * = the dot product of dout[t] and that row (0 for slots without one); either
+ * may be NULL.  Each row below offsets[E - 1] is named by one slot; rows from
+ * there on get zeros.  top_k <= 64, T <= 2^25. */
+int sfp8_moe_combine(const void* rows, int dtype, int64_t R, int64_t D, const float* weights, const int64_t* inverse,
+                     int64_t T, int64_t top_k, void* out, void* stream);
+int sfp8_moe_combine_bwd(const void* dout, const void* rows, int dtype, int64_t R, int64_t D, const float* weights,
+                         const int64_t* inverse, int64_t T, int64_t top_k, const int* offsets, int64_t E, void* drows,
+                         float* dweights, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The global norm of many gradients, and clipping to a largest norm.
+ * ------------------------------------------------------------------------- */
+
+/* norm = sqrt(sum of squares over all elements of count gradients) (fp32 at a
+ * device pointer; summed in 64 bits, in an order that the sizes alone give).
+ * grads, n (elements) and dtype are host arrays, read before the call
+ * returns; ws: sfp8_grad_norm_workspace_doubles(count) doubles.
+ * sfp8_grad_clip also writes out[i] = grads[i] * min(1, max_norm / (norm +
+ * 1e-6)), rounded to the gradient's type; out[i] == grads[i] clips in place
+ * (nothing is written where the factor is 1), any other overlap of what is
+ * written is the caller's error.  Pointers are aligned to their elements. */
+int64_t sfp8_grad_norm_workspace_doubles(int64_t count);
+int sfp8_grad_norm(int64_t count, const void* const* grads, const int64_t* n, const int* dtype, float* norm,
+                   double* ws, int64_t ws_doubles, void* stream);
+int sfp8_grad_clip(int64_t count, const void* const* grads, void* const* out, const int64_t* n, const int* dtype,
+                   float max_norm, float* norm, double* ws, int64_t ws_doubles, void* stream);
+
+/* ---------------------------------------------------------------------------
  * The consumer of the fp32 weight gradients: the Muon optimizer's momentum
  * stage (train.py:2805-2839), alone and fused into the weight gradient.
  * ------------------------------------------------------------------------- */

@@ -14,7 +14,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsparkfp8.so")
-SOURCES = ("quant.hip", "gemm.hip", "moe.hip", "bf16.hip", "optim.hip")
+SOURCES = ("quant.hip", "gemm.hip", "moe.hip", "bf16.hip", "optim.hip", "route.hip", "clip.hip")
 NATIVE = os.path.join(HERE, "_native.so")
 NATIVE_SOURCE = "native.cpp"
 ARCH = "gfx950"

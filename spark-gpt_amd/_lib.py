@@ -77,6 +77,18 @@ SIGNATURES = {
     "sfp8_bf16_fold_grads": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _P, _I64, _P]),
     "sfp8_wgrad_rows_workspace_floats": (_I64, [_I64, _I64, _I64]),
     "sfp8_gemm_wgrad_rows": (_INT, [_P, _INT, _INT, _P, _INT, _INT, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
+    # routing of tokens to experts
+    "sfp8_moe_route": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _P, _INT, _I64, _I64, _I64, _I64, _INT, _F32, _P, _P, _P,
+                              _P]),
+    "sfp8_moe_route_bwd": (_INT, [_P, _P, _P, _P, _INT, _I64, _I64, _I64, _INT, _I64, _INT, _F32, _P, _P]),
+    "sfp8_moe_expert_order_workspace_ints": (_I64, [_I64, _I64]),
+    "sfp8_moe_expert_order": (_INT, [_P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
+    "sfp8_moe_combine": (_INT, [_P, _INT, _I64, _I64, _P, _P, _I64, _I64, _P, _P]),
+    "sfp8_moe_combine_bwd": (_INT, [_P, _P, _INT, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P]),
+    # the global gradient norm and clipping
+    "sfp8_grad_norm_workspace_doubles": (_I64, [_I64]),
+    "sfp8_grad_norm": (_INT, [_I64, _P, _P, _P, _P, _P, _I64, _P]),
+    "sfp8_grad_clip": (_INT, [_I64, _P, _P, _P, _P, _F32, _P, _P, _I64, _P]),
     # the optimizer's momentum stage, and the weight gradient fused with it
     "sfp8_momentum_stage": (_INT, [_P, _P, _P, _I64, _F32, _F32, _P]),
     "sfp8_wgrad_momentum_workspace_floats": (_I64, [_I64, _I64, _I64]),

@@ -1,0 +1,294 @@
+// The global norm of many gradients and their scaling to a largest norm
+// (gfx950): what a training step does between the backward pass and the
+// optimizer's momentum stage (optim.hip).
+//
+//   n = sqrt(sum over all tensors and elements of g^2)
+//   c = min(1, max_norm / (n + 1e-6)),  out = round(c * g)
+//
+// The squares are summed in 64 bits (a square of a 32-bit number cannot
+// overflow there, and 64-bit FMAs cost a few percent of the time the bytes
+// take), in an order that depends on the sizes alone: every work-group sums
+// its own chunks, then the sums are added in order.  Bound by HBM: each
+// gradient is read once for the norm and, where c != 1 or the result goes
+// elsewhere, read again and written.
+#include "common.h"
+
+namespace sfp8 {
+
+enum : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
+
+// The tensors of one launch, passed by value: 4 KiB of kernel arguments.
+constexpr int kClipTensors = 120;
+constexpr int kClipChunk = 65536;   // bytes of a gradient that one work-group takes at a time
+constexpr int kClipBlocks = 2048;   // work-groups of a launch, at most
+constexpr int kClipThreads = 256;
+
+struct ClipTable {
+  const void* in[kClipTensors];
+  void* out[kClipTensors];
+  int64_t n[kClipTensors];
+  uint32_t first[kClipTensors + 1];  // first chunk of each tensor; [count]: all chunks
+  uint8_t dtype[kClipTensors];
+  int count;
+};
+
+SFP8_DEV float half_to_f32(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (uint16_t)b); }
+
+// Tensor of chunk c: the largest i with first[i] <= c.
+SFP8_DEV int clip_tensor(const ClipTable& tab, uint32_t c) {
+  int lo = 0, hi = tab.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tab.first[mid] <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Elements 0 .. U - 1 of 16 bytes as fp32.
+template <int DT>
+struct Pack {
+  static constexpr int U = DT == kF32 ? 4 : 8;
+  static constexpr int kSize = DT == kF32 ? 4 : 2;
+  SFP8_DEV static float get(const intx4& v, int i) {
+    if (DT == kF32) return __uint_as_float((uint32_t)v[i]);
+    const uint32_t b = ((uint32_t)v[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+    return DT == kBf16 ? bf16_bits_to_f32(b) : half_to_f32(b);
+  }
+  SFP8_DEV static float load(const void* p, int64_t i) {
+    if (DT == kF32) return reinterpret_cast<const float*>(p)[i];
+    const uint32_t b = reinterpret_cast<const uint16_t*>(p)[i];
+    return DT == kBf16 ? bf16_bits_to_f32(b) : half_to_f32(b);
+  }
+  SFP8_DEV static uint32_t bits(float f) {
+    if (DT == kF32) return __float_as_uint(f);
+    return DT == kBf16 ? f32_to_bf16_bits(f) : (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f);
+  }
+  SFP8_DEV static void store(void* p, int64_t i, float f) {
+    if (DT == kF32) reinterpret_cast<float*>(p)[i] = f;
+    else reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)bits(f);
+  }
+  SFP8_DEV static intx4 scaled(const intx4& v, float c) {
+    intx4 o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (DT == kF32) o[q] = (int)bits(get(v, q) * c);
+      else o[q] = (int)(bits(get(v, 2 * q) * c) | bits(get(v, 2 * q + 1) * c) << 16);
+    }
+    return o;
+  }
+};
+
+// The elements [e0, e1) of a chunk: those before the first 16-byte boundary,
+// whole 16-byte vectors, and the rest.  one(i) takes element i, vec(i) the
+// vector that starts at element i.
+template <int DT, typename One, typename Vec>
+SFP8_DEV void clip_walk(const void* p, int64_t e0, int64_t e1, One one, Vec vec) {
+  using P = Pack<DT>;
+  const uintptr_t at = (uintptr_t)p + e0 * P::kSize;
+  const int64_t lead = (int64_t)(((16 - (at & 15)) & 15) / P::kSize);
+  const int64_t v0 = e0 + lead < e1 ? e0 + lead : e1;
+  const int64_t v1 = v0 + (e1 - v0) / P::U * P::U;
+  for (int64_t i = e0 + threadIdx.x; i < v0; i += kClipThreads) one(i);
+  for (int64_t i = v0 + (int64_t)threadIdx.x * P::U; i < v1; i += kClipThreads * P::U) vec(i);
+  for (int64_t i = v1 + threadIdx.x; i < e1; i += kClipThreads) one(i);
+}
+
+template <int DT>
+SFP8_DEV double clip_squares(const void* p, int64_t e0, int64_t e1) {
+  using P = Pack<DT>;
+  double s = 0.0;
+  clip_walk<DT>(
+      p, e0, e1,
+      [&](int64_t i) {
+        const double x = P::load(p, i);
+        s = __builtin_fma(x, x, s);
+      },
+      [&](int64_t i) {
+        const intx4 v = *reinterpret_cast<const intx4*>(reinterpret_cast<const char*>(p) + i * P::kSize);
+#pragma unroll
+        for (int q = 0; q < P::U; ++q) {
+          const double x = P::get(v, q);
+          s = __builtin_fma(x, x, s);
+        }
+      });
+  return s;
+}
+
+template <int DT>
+SFP8_DEV void clip_scale(const void* p, void* o, int64_t e0, int64_t e1, float c, bool aligned) {
+  using P = Pack<DT>;
+  const auto one = [&](int64_t i) { P::store(o, i, P::load(p, i) * c); };
+  if (!aligned) {  // in and out sit differently in their 16 bytes
+    for (int64_t i = e0 + threadIdx.x; i < e1; i += kClipThreads) one(i);
+    return;
+  }
+  clip_walk<DT>(p, e0, e1, one, [&](int64_t i) {
+    const intx4 v = *reinterpret_cast<const intx4*>(reinterpret_cast<const char*>(p) + i * P::kSize);
+    *reinterpret_cast<intx4*>(reinterpret_cast<char*>(o) + i * P::kSize) = P::scaled(v, c);
+  });
+}
+
+// part[blockIdx.x] = the squares of this work-group's chunks.
+__global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(const ClipTable tab, double* __restrict__ part) {
+  __shared__ double red[kClipThreads / 64];
+  double s = 0.0;
+  for (uint32_t c = blockIdx.x; c < tab.first[tab.count]; c += gridDim.x) {
+    const int i = clip_tensor(tab, c);
+    const int dt = tab.dtype[i];
+    const int64_t per = kClipChunk / (dt == kF32 ? 4 : 2);
+    const int64_t e0 = (int64_t)(c - tab.first[i]) * per;
+    const int64_t e1 = e0 + per < tab.n[i] ? e0 + per : tab.n[i];
+    s += dt == kF32 ? clip_squares<kF32>(tab.in[i], e0, e1)
+                    : dt == kBf16 ? clip_squares<kBf16>(tab.in[i], e0, e1) : clip_squares<kF16>(tab.in[i], e0, e1);
+  }
+  s = wave_sum_f64(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// The norm from the partial sums, the same in every work-group that asks.
+SFP8_DEV float clip_norm_of(const double* part, int parts) {
+  __shared__ double red[kClipThreads / 64];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kClipThreads) s += part[i];
+  s = wave_sum_f64(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return (float)sqrt((red[0] + red[1]) + (red[2] + red[3]));
+}
+
+__global__ __launch_bounds__(kClipThreads) void clip_norm_out_kernel(const double* __restrict__ part, int parts,
+                                                                     float* __restrict__ norm) {
+  const float n = clip_norm_of(part, parts);
+  if (threadIdx.x == 0) *norm = n;
+}
+
+__global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipTable tab, const double* __restrict__ part,
+                                                                  int parts, float max_norm,
+                                                                  float* __restrict__ norm) {
+  const float n = clip_norm_of(part, parts);
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
+  float f = max_norm / (n + 1e-6f);
+  f = f > 1.0f ? 1.0f : f;  // keeps NaN
+  for (uint32_t c = blockIdx.x; c < tab.first[tab.count]; c += gridDim.x) {
+    const int i = clip_tensor(tab, c);
+    if (f == 1.0f && tab.in[i] == tab.out[i]) continue;  // x * 1 is x
+    const int dt = tab.dtype[i];
+    const int64_t per = kClipChunk / (dt == kF32 ? 4 : 2);
+    const int64_t e0 = (int64_t)(c - tab.first[i]) * per;
+    const int64_t e1 = e0 + per < tab.n[i] ? e0 + per : tab.n[i];
+    const bool aligned = (((uintptr_t)tab.in[i] ^ (uintptr_t)tab.out[i]) & 15u) == 0;
+    if (dt == kF32) clip_scale<kF32>(tab.in[i], tab.out[i], e0, e1, f, aligned);
+    else if (dt == kBf16) clip_scale<kBf16>(tab.in[i], tab.out[i], e0, e1, f, aligned);
+    else clip_scale<kF16>(tab.in[i], tab.out[i], e0, e1, f, aligned);
+  }
+}
+
+}  // namespace sfp8
+
+// ============================================================================
+// C ABI
+// ============================================================================
+using namespace sfp8;
+
+namespace {
+inline int clip_status() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? kOk : (int)e;
+}
+inline int64_t clip_chunks(int64_t n, int dtype) {
+  const int64_t bytes = n * (dtype == kF32 ? 4 : 2);
+  return (bytes + kClipChunk - 1) / kClipChunk;
+}
+
+// Tables of up to kClipTensors tensors each (tensors without elements are left
+// out): f(table, work-groups).
+template <typename F>
+void clip_tables(int64_t count, const void* const* in, void* const* out, const int64_t* n, const int* dtype, F f) {
+  ClipTable tab;
+  tab.count = 0;
+  tab.first[0] = 0;
+  const auto flush = [&] {
+    if (tab.count == 0) return;
+    const uint32_t chunks = tab.first[tab.count];
+    f(tab, (int)(chunks < (uint32_t)kClipBlocks ? chunks : (uint32_t)kClipBlocks));
+    tab.count = 0;
+  };
+  for (int64_t i = 0; i < count; ++i) {
+    if (n[i] == 0) continue;
+    const int64_t c = clip_chunks(n[i], dtype[i]);
+    if (tab.count == kClipTensors || (tab.count && tab.first[tab.count] + c > 0x7fffffff)) flush();
+    const int j = tab.count++;
+    tab.in[j] = in[i];
+    tab.out[j] = out ? out[i] : nullptr;
+    tab.n[j] = n[i];
+    tab.dtype[j] = (uint8_t)dtype[i];
+    tab.first[j + 1] = (j ? tab.first[j] : 0) + (uint32_t)c;
+  }
+  flush();
+}
+
+int clip_check(int64_t count, const void* const* in, const int64_t* n, const int* dtype) {
+  if (count < 0) return kErrBadShape;
+  if (count > 0 && (!in || !n || !dtype)) return kErrNullPointer;
+  for (int64_t i = 0; i < count; ++i) {
+    if (n[i] < 0 || n[i] > (int64_t)1 << 40 || dtype[i] < 0 || dtype[i] > 2) return kErrBadShape;
+    if (n[i] > 0 && !in[i]) return kErrNullPointer;
+    if ((uintptr_t)in[i] % (dtype[i] == kF32 ? 4 : 2)) return kErrBadAlignment;
+  }
+  return kOk;
+}
+}  // namespace
+
+extern "C" {
+
+int64_t sfp8_grad_norm_workspace_doubles(int64_t count) {
+  return count < 0 ? -1 : (count + kClipTensors - 1) / kClipTensors * kClipBlocks + kClipBlocks;
+}
+
+int sfp8_grad_norm(int64_t count, const void* const* grads, const int64_t* n, const int* dtype, float* norm,
+                   double* ws, int64_t ws_doubles, void* stream) {
+  if (const int rc = clip_check(count, grads, n, dtype)) return rc;
+  if (!norm || !ws) return kErrNullPointer;
+  if (ws_doubles < sfp8_grad_norm_workspace_doubles(count)) return kErrWorkspaceTooSmall;
+  hipStream_t st = (hipStream_t)stream;
+  int parts = 0;
+  clip_tables(count, grads, nullptr, n, dtype, [&](const ClipTable& tab, int blocks) {
+    hipLaunchKernelGGL(clip_norm_kernel, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws + parts);
+    parts += blocks;
+  });
+  hipLaunchKernelGGL(clip_norm_out_kernel, dim3(1), dim3(kClipThreads), 0, st, ws, parts, norm);
+  return clip_status();
+}
+
+int sfp8_grad_clip(int64_t count, const void* const* grads, void* const* out, const int64_t* n, const int* dtype,
+                   float max_norm, float* norm, double* ws, int64_t ws_doubles, void* stream) {
+  if (const int rc = clip_check(count, grads, n, dtype)) return rc;
+  if (!norm || !ws || (count > 0 && !out)) return kErrNullPointer;
+  if (!(max_norm >= 0.0f)) return kErrBadShape;
+  for (int64_t i = 0; i < count; ++i) {
+    if (n[i] > 0 && !out[i]) return kErrNullPointer;
+    if ((uintptr_t)out[i] % (dtype[i] == kF32 ? 4 : 2)) return kErrBadAlignment;
+  }
+  if (ws_doubles < sfp8_grad_norm_workspace_doubles(count)) return kErrWorkspaceTooSmall;
+  hipStream_t st = (hipStream_t)stream;
+  int parts = 0;
+  clip_tables(count, grads, out, n, dtype, [&](const ClipTable& tab, int blocks) {
+    hipLaunchKernelGGL(clip_norm_kernel, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws + parts);
+    parts += blocks;
+  });
+  if (parts == 0) {  // nothing to scale: the norm is 0
+    hipLaunchKernelGGL(clip_norm_out_kernel, dim3(1), dim3(kClipThreads), 0, st, ws, 0, norm);
+    return clip_status();
+  }
+  float* first = norm;
+  clip_tables(count, grads, out, n, dtype, [&](const ClipTable& tab, int blocks) {
+    hipLaunchKernelGGL(clip_scale_kernel, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws, parts, max_norm, first);
+    first = nullptr;
+  });
+  return clip_status();
+}
+
+}  // extern "C"

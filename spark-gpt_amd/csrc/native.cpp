@@ -14,6 +14,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <c10/core/DeviceGuard.h>
+
+#include <algorithm>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -369,6 +372,219 @@ Tensor moe_topk_sum(const Tensor& dx, const Tensor& inverse_permutation, int64_t
   return out;
 }
 
+// ------------------------------------------------------------------ routing
+constexpr auto kI64 = ScalarType::Long;
+
+inline int64_t* lptr(const Tensor& t) { return static_cast<int64_t*>(t.data_ptr()); }
+
+// The library's code of a 32- or 16-bit floating type (-1: none of them).
+inline int dtype_code(ScalarType t) {
+  return t == kF32 ? 0 : t == kBF16 ? 1 : t == ScalarType::Half ? 2 : -1;
+}
+int float_code(const char* name, const Tensor& t) {
+  if (!t.is_cuda()) refuse(std::string(name) + " must be a ROCm device tensor");
+  const int c = dtype_code(t.scalar_type());
+  if (c < 0) refuse(std::string(name) + " must be fp32, bf16 or fp16, got " + c10::toString(t.scalar_type()));
+  return c;
+}
+void same_device(const char* name, const Tensor& t, const Tensor& like) {
+  if (t.device() != like.device()) refuse(std::string(name) + " must be on " + like.device().str());
+}
+int score_code(const std::string& score) {
+  if (score != "softmax" && score != "sigmoid") refuse("score must be 'softmax' or 'sigmoid', got '" + score + "'");
+  return score == "sigmoid";
+}
+// Logits are [T, E] with any row stride; another column stride is copied.
+Tensor logit_rows(const Tensor& t) {
+  if (t.dim() != 2) refuse("logits must be 2-D, got shape " + shape_of(t));
+  need(t.size(1) > 0, "logits need at least one expert");
+  return t.size(1) == 1 || t.stride(1) == 1 ? t : t.contiguous();
+}
+
+std::tuple<Tensor, Tensor, Tensor> moe_route(const Tensor& logits_, const OptTensor& bias, const OptTensor& mask,
+                                             const std::string& score, int64_t groups, int64_t top_groups,
+                                             int64_t group_best, int64_t top_k, bool renormalize, double scale) {
+  const int dtype = float_code("logits", logits_), sc = score_code(score);
+  const c10::DeviceGuard guard(logits_.device());
+  const Tensor logits = logit_rows(logits_);
+  const int64_t T = logits.size(0), E = logits.size(1);
+  if (bias) {
+    contig("bias", *bias, kF32, 1);
+    same_device("bias", *bias, logits);
+    need(bias->size(0) == E, "bias must have one entry per expert");
+  }
+  if (mask) {
+    contig("mask", *mask, ScalarType::Bool, 1);
+    same_device("mask", *mask, logits);
+    need(mask->size(0) == T, "mask must have one entry per token");
+  }
+  need(E <= 1024, "at most 1024 experts");
+  if (groups < 1 || groups > 64 || E % groups)
+    refuse("groups must be 1 .. 64 and divide the " + std::to_string(E) + " experts, got " + std::to_string(groups));
+  need(top_groups >= 1 && top_groups <= groups, "top_groups must be 1 .. groups");
+  need(group_best == 1 || group_best == 2, "group_best must be 1 or 2");
+  if (top_k < 1 || top_k > 64 || top_k > top_groups * (E / groups))
+    refuse("top_k must be 1 .. 64 and no more than the experts of the kept groups, got " + std::to_string(top_k));
+  Tensor w = empty({T, top_k}, kF32, logits), sel = empty({T, top_k}, kI64, logits),
+         picked = empty({T, top_k}, kF32, logits);
+  CALL(sfp8_moe_route, ptr(logits), dtype, T, E, logits.stride(0), fptr(bias), ptr(mask), sc, groups, top_groups,
+       group_best, top_k, (int)renormalize, (float)scale, fptr(w), lptr(sel), fptr(picked), stream_of(logits));
+  return {w, sel, picked};
+}
+
+Tensor moe_route_bwd(const Tensor& dweights_, const Tensor& selected, const Tensor& picked, const Tensor& logits_,
+                     const std::string& score, bool renormalize, double scale) {
+  const int dtype = float_code("logits", logits_), sc = score_code(score);
+  const c10::DeviceGuard guard(logits_.device());
+  const Tensor logits = logit_rows(logits_);
+  const int64_t T = logits.size(0), E = logits.size(1);
+  contig("selected", selected, kI64, 2);
+  const int64_t k = selected.size(1);
+  const Tensor dweights = dweights_.contiguous();
+  for (const auto& [n, t] : {std::pair<const char*, const Tensor&>{"dweights", dweights}, {"picked", picked}}) {
+    contig(n, t, kF32, 2);
+    if (!(t.sizes() == selected.sizes())) refuse(std::string(n) + " must have the shape of selected");
+  }
+  for (const auto& [n, t] : {std::pair<const char*, const Tensor&>{"dweights", dweights}, {"picked", picked},
+                             {"selected", selected}})
+    same_device(n, t, logits);
+  need(selected.size(0) == T, "selected must have one row per token");
+  need(E <= 1024 && k >= 1 && k <= 64 && k <= E, "1 .. 64 slots of at most 1024 experts");
+  Tensor d = empty({T, E}, logits.scalar_type(), logits);
+  CALL(sfp8_moe_route_bwd, fptr(dweights), lptr(selected), fptr(picked), ptr(logits), dtype, T, E, logits.stride(0), sc,
+       k, (int)renormalize, (float)scale, ptr(d), stream_of(logits));
+  return d;
+}
+
+std::tuple<Tensor, Tensor, Tensor> moe_expert_order(const Tensor& selected, int64_t E) {
+  contig("selected", selected, kI64, 2);
+  need(E >= 1 && E <= 1024, "1 .. 1024 experts");
+  need(selected.size(1) >= 1, "selected must have at least one slot per token");
+  const int64_t R = selected.numel();
+  need(R <= (int64_t)1 << 30, "at most 2^30 slots");
+  const c10::DeviceGuard guard(selected.device());
+  Tensor token_index = empty({R}, kI64, selected), inverse = empty({R}, kI64, selected),
+         offsets = empty({E}, ScalarType::Int, selected);
+  const int64_t n = sfp8_moe_expert_order_workspace_ints(R, E);
+  OptTensor ws;
+  if (n > 0) ws = empty({n}, ScalarType::Int, selected);
+  CALL(sfp8_moe_expert_order, lptr(selected), R, selected.size(1), E, lptr(token_index), lptr(inverse), iptr(offsets),
+       iptr(ws), n, stream_of(selected));
+  return {token_index, inverse, offsets};
+}
+
+// rows [R, D], weights [T, k], inverse of T * k entries, one device
+int combine_args(const Tensor& rows, const Tensor& weights, const Tensor& inverse) {
+  const int dtype = float_code("rows", rows);
+  contig("rows", rows, rows.scalar_type(), 2);
+  contig("weights", weights, kF32, 2);
+  contig("inverse_permutation", inverse, kI64, 1);
+  same_device("weights", weights, rows);
+  same_device("inverse_permutation", inverse, rows);
+  need(rows.size(1) > 0, "rows need at least one column");
+  need(weights.size(1) >= 1 && weights.size(1) <= 64, "1 .. 64 slots per token");
+  need(inverse.numel() == weights.numel(), "inverse_permutation must have one entry per weight");
+  return dtype;
+}
+
+Tensor moe_combine(const Tensor& rows, const Tensor& weights, const Tensor& inverse_permutation) {
+  const int dtype = combine_args(rows, weights, inverse_permutation);
+  const c10::DeviceGuard guard(rows.device());
+  Tensor out = empty({weights.size(0), rows.size(1)}, rows.scalar_type(), rows);
+  CALL(sfp8_moe_combine, ptr(rows), dtype, rows.size(0), rows.size(1), fptr(weights), lptr(inverse_permutation),
+       weights.size(0), weights.size(1), ptr(out), stream_of(rows));
+  return out;
+}
+
+std::tuple<OptTensor, OptTensor> moe_combine_bwd(const Tensor& dout, const Tensor& rows, const Tensor& weights,
+                                                 const Tensor& inverse_permutation, const Tensor& offsets,
+                                                 bool need_rows, bool need_weights) {
+  const int dtype = combine_args(rows, weights, inverse_permutation);
+  contig("dout", dout, rows.scalar_type(), 2);
+  contig("offsets", offsets, ScalarType::Int, 1);
+  same_device("dout", dout, rows);
+  same_device("offsets", offsets, rows);
+  need(offsets.size(0) >= 1, "offsets must have one entry per expert");
+  need(dout.size(0) == weights.size(0) && dout.size(1) == rows.size(1), "dout must be [tokens, columns of rows]");
+  const c10::DeviceGuard guard(rows.device());
+  OptTensor drows, dweights;
+  if (need_rows) drows = empty(rows.sizes(), rows.scalar_type(), rows);
+  if (need_weights) dweights = empty(weights.sizes(), kF32, rows);
+  CALL(sfp8_moe_combine_bwd, ptr(dout), ptr(rows), dtype, rows.size(0), rows.size(1), fptr(weights),
+       lptr(inverse_permutation), weights.size(0), weights.size(1), iptr(offsets), offsets.size(0), ptr(drows),
+       fptr(dweights), stream_of(rows));
+  return {drows, dweights};
+}
+
+// ------------------------------------------------------------------ gradient norm and clipping
+struct GradList {
+  std::vector<const void*> in;
+  std::vector<void*> out;
+  std::vector<int64_t> n;
+  std::vector<int> dtype;
+};
+
+// Gradients of one device, each one dense block of memory in some order of its dimensions.
+GradList grad_list(const std::vector<Tensor>& grads) {
+  need(!grads.empty(), "at least one gradient");
+  GradList g;
+  for (const Tensor& t : grads) {
+    g.dtype.push_back(float_code("a gradient", t));
+    if (t.layout() != at::kStrided || !t.is_non_overlapping_and_dense())
+      refuse("a gradient must be dense and must not overlap itself, got shape " + shape_of(t));
+    same_device("every gradient", t, grads[0]);
+    g.in.push_back(t.data_ptr());
+    g.n.push_back(t.numel());
+  }
+  return g;
+}
+
+Tensor grad_norm(const std::vector<Tensor>& grads) {
+  const GradList g = grad_list(grads);
+  const c10::DeviceGuard guard(grads[0].device());
+  const int64_t count = (int64_t)grads.size(), nws = sfp8_grad_norm_workspace_doubles(count);
+  Tensor norm = empty({}, kF32, grads[0]), ws = empty({nws}, ScalarType::Double, grads[0]);
+  CALL(sfp8_grad_norm, count, g.in.data(), g.n.data(), g.dtype.data(), fptr(norm), static_cast<double*>(ws.data_ptr()),
+       nws, stream_of(grads[0]));
+  return norm;
+}
+
+Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::optional<std::vector<Tensor>>& out) {
+  GradList g = grad_list(grads);
+  need(max_norm >= 0.0, "max_norm must not be negative");
+  if (out) need(out->size() == grads.size(), "out must have one tensor per gradient");
+  // what is written: [first byte, one past the last), and whether another gradient is read there
+  struct Span {
+    uintptr_t begin, end;
+    bool written;
+  };
+  std::vector<Span> spans;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& o = out ? (*out)[i] : grads[i];
+    if (out && !(o.scalar_type() == grads[i].scalar_type() && o.device() == grads[i].device() &&
+                 o.sizes() == grads[i].sizes() && o.strides() == grads[i].strides()))
+      refuse("out must have the types, shapes and strides of the gradients");
+    g.out.push_back(o.data_ptr());
+    const uintptr_t bytes = (uintptr_t)(g.n[i] * o.element_size()), a = (uintptr_t)o.data_ptr();
+    if (!bytes) continue;
+    spans.push_back({a, a + bytes, true});
+    if (g.in[i] != g.out[i]) spans.push_back({(uintptr_t)g.in[i], (uintptr_t)g.in[i] + bytes, false});
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.begin < y.begin; });
+  uintptr_t any_end = 0, written_end = 0;
+  for (const Span& s : spans) {
+    need(!(s.begin < written_end || (s.written && s.begin < any_end)), "the tensors that are written must not overlap");
+    any_end = std::max(any_end, s.end);
+    if (s.written) written_end = std::max(written_end, s.end);
+  }
+  const c10::DeviceGuard guard(grads[0].device());
+  const int64_t count = (int64_t)grads.size(), nws = sfp8_grad_norm_workspace_doubles(count);
+  Tensor norm = empty({}, kF32, grads[0]), ws = empty({nws}, ScalarType::Double, grads[0]);
+  CALL(sfp8_grad_clip, count, g.in.data(), g.out.data(), g.n.data(), g.dtype.data(), (float)max_norm, fptr(norm),
+       static_cast<double*>(ws.data_ptr()), nws, stream_of(grads[0]));
+  return norm;
+}
+
 // ------------------------------------------------------------------ bf16 SwiGLU path
 std::tuple<OptTensor, OptTensor> bf16_weight_slabs(const Tensor& w, const OptTensor& norm_w, bool rows,
                                                    bool transposed) {
@@ -567,6 +783,25 @@ PYBIND11_MODULE(_native, m) {
         "([rows/64, ldp, 64]: read through transposing LDS reads) instead of the token-contiguous copy.");
   m.def("moe_topk_sum", &moe_topk_sum, arg("dx"), arg("inverse_permutation"), arg("T"), arg("top_k"),
         "out[t] = sum of the top_k expert-order rows of token t (bf16 [T, D]).");
+  m.def("moe_route", &moe_route, arg("logits"), arg("bias"), arg("mask"), arg("score"), arg("groups"),
+        arg("top_groups"), arg("group_best"), arg("top_k"), arg("renormalize"), arg("scale"),
+        "(weights fp32, selected int64, picked fp32), each [T, top_k]: the experts of each token in descending order, "
+        "their weights and their logits; -1, 0 and 0 where no expert is left or the token is masked.");
+  m.def("moe_route_bwd", &moe_route_bwd, arg("dweights"), arg("selected"), arg("picked"), arg("logits"), arg("score"),
+        arg("renormalize"), arg("scale"),
+        "The gradient [T, E] of the logits (their type) from that of the weights; selected and picked as moe_route "
+        "returned them.");
+  m.def("moe_expert_order", &moe_expert_order, arg("selected"), arg("num_experts"),
+        "(token_index, inverse_permutation, offsets): the slots of selected [T, top_k] in stable order by expert, those "
+        "that name none last (inverse_permutation -1); offsets the experts' inclusive row counts (int32).");
+  m.def("moe_combine", &moe_combine, arg("rows"), arg("weights"), arg("inverse_permutation"),
+        "out[t] = sum of weights[t, j] * rows[inverse_permutation[t, j]] over the slots, summed in 32 bits in order.");
+  m.def("moe_combine_bwd", &moe_combine_bwd, arg("dout"), arg("rows"), arg("weights"), arg("inverse_permutation"),
+        arg("offsets"), arg("need_rows") = true, arg("need_weights") = true,
+        "(drows, dweights) of moe_combine; rows from offsets[-1] on get zeros.");
+  m.def("grad_norm", &grad_norm, arg("grads"), "The 2-norm over all elements of all gradients (fp32 scalar tensor).");
+  m.def("clip_grads", &clip_grads, arg("grads"), arg("max_norm"), arg("out") = py::none(),
+        "grad_norm(grads); every gradient times min(1, max_norm / (norm + 1e-6)), in place or into out.");
   m.def("bf16_weight_slabs", &bf16_weight_slabs, arg("w"), arg("norm_w") = py::none(), kw, arg("rows") = true,
         arg("transposed") = true,
         "bf16 K-slabs of W [E, R, C] (fp32, times norm_w[c] when given, or bf16): (ws: stacked K-slabs of W[e] [R, C] "

@@ -22,6 +22,9 @@ _NATIVE = ("norm_quant", "block_weight_quant", "weight_quant_experts", "gateup_s
            "moe_gateup_swiglu_fwd", "moe_down_fwd", "moe_down_dgrad_swiglu", "moe_gateup_dgrad", "moe_wgrad_rows",
            "moe_topk_sum", "bf16_weight_slabs", "bf16_rows_prep", "bf16_swiglu_fwd", "bf16_swiglu_eval",
            "bf16_swiglu_bwd", "bf16_gemm", "bf16_norm_dh", "bf16_wgrad_rows", "bf16_fold_grads")
+# those around the experts and between the backward pass and the optimizer
+_NATIVE_STEP = ("moe_route", "moe_route_bwd", "moe_expert_order", "moe_combine", "moe_combine_bwd", "grad_norm",
+                "clip_grads")
 
 
 def _missing(name: str, why: str):
@@ -35,9 +38,9 @@ def _missing(name: str, why: str):
 try:
     from . import _native
 except ImportError as _e:
-    globals().update({_n: _missing(_n, str(_e)) for _n in _NATIVE})
+    globals().update({_n: _missing(_n, str(_e)) for _n in _NATIVE + _NATIVE_STEP})
 else:
-    globals().update({_n: getattr(_native, _n) for _n in _NATIVE})
+    globals().update({_n: getattr(_native, _n) for _n in _NATIVE + _NATIVE_STEP})
 
 E4M3 = torch.float8_e4m3fn
 E5M2 = torch.float8_e5m2

@@ -28,7 +28,7 @@ from __future__ import annotations
 
 import threading
 import weakref
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -438,3 +438,78 @@ swiglu_bwd = torch.library.custom_op("sparkfp8::swiglu_bwd", swiglu_bwd_impl, mu
 @swiglu_bwd.register_fake
 def _swiglu_bwd_fake(dh, x, weight, gu, plan):
     return x.new_empty(tuple(x.shape), dtype=BF16), x.new_empty(tuple(weight.shape), dtype=BF16)
+
+
+# ------------------------------------------------------------------ routing
+def route_fwd_impl(logits: Tensor, bias: Optional[Tensor], mask: Optional[Tensor], score: str, groups: int,
+                   top_groups: int, group_best: int, top_k: int, renormalize: bool,
+                   scale: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """(weights fp32, selected int64, picked fp32), each [T, top_k]."""
+    return ops.moe_route(logits, bias, mask, score, groups, top_groups, group_best, top_k, renormalize, scale)
+
+
+route_fwd = torch.library.custom_op("sparkfp8::route_fwd", route_fwd_impl, mutates_args=())
+
+
+@route_fwd.register_fake
+def _route_fwd_fake(logits, bias, mask, score, groups, top_groups, group_best, top_k, renormalize, scale):
+    shape = (logits.shape[0], top_k)
+    return (logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int64),
+            logits.new_empty(shape, dtype=torch.float32))
+
+
+def route_bwd_impl(dweights: Tensor, selected: Tensor, picked: Tensor, logits: Tensor, score: str, renormalize: bool,
+                   scale: float) -> Tensor:
+    """The gradient of the logits, in their type."""
+    return ops.moe_route_bwd(dweights, selected, picked, logits, score, renormalize, scale)
+
+
+route_bwd = torch.library.custom_op("sparkfp8::route_bwd", route_bwd_impl, mutates_args=())
+
+
+@route_bwd.register_fake
+def _route_bwd_fake(dweights, selected, picked, logits, score, renormalize, scale):
+    return logits.new_empty(tuple(logits.shape))
+
+
+def expert_order_impl(selected: Tensor, num_experts: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """(token_index, inverse_permutation, offsets) of the slots in expert order."""
+    return ops.moe_expert_order(selected.contiguous(), num_experts)
+
+
+expert_order = torch.library.custom_op("sparkfp8::expert_order", expert_order_impl, mutates_args=())
+
+
+@expert_order.register_fake
+def _expert_order_fake(selected, num_experts):
+    R = selected.shape[0] * selected.shape[1]
+    return (selected.new_empty((R,), dtype=torch.int64), selected.new_empty((R,), dtype=torch.int64),
+            selected.new_empty((num_experts,), dtype=torch.int32))
+
+
+def combine_fwd_impl(rows: Tensor, weights: Tensor, inverse_permutation: Tensor) -> Tensor:
+    """The weighted sum of each token's rows, [T, D] in the rows' type."""
+    return ops.moe_combine(rows.contiguous(), weights.contiguous(), inverse_permutation.contiguous())
+
+
+combine_fwd = torch.library.custom_op("sparkfp8::combine_fwd", combine_fwd_impl, mutates_args=())
+
+
+@combine_fwd.register_fake
+def _combine_fwd_fake(rows, weights, inverse_permutation):
+    return rows.new_empty((weights.shape[0], rows.shape[1]))
+
+
+def combine_bwd_impl(dout: Tensor, rows: Tensor, weights: Tensor, inverse_permutation: Tensor,
+                     offsets: Tensor) -> Tuple[Tensor, Tensor]:
+    """(drows in the rows' type, dweights fp32); both are computed."""
+    return ops.moe_combine_bwd(dout.contiguous(), rows.contiguous(), weights.contiguous(),
+                               inverse_permutation.contiguous(), offsets.contiguous())
+
+
+combine_bwd = torch.library.custom_op("sparkfp8::combine_bwd", combine_bwd_impl, mutates_args=())
+
+
+@combine_bwd.register_fake
+def _combine_bwd_fake(dout, rows, weights, inverse_permutation, offsets):
+    return rows.new_empty(tuple(rows.shape)), weights.new_empty(tuple(weights.shape))

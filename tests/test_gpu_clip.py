@@ -1,0 +1,190 @@
+"""GPU tests of the global gradient norm and clipping against 64 bits.
+
+The squares are summed in 64 bits, so the norm is off by its rounding to fp32,
+2^-24 relative (and 1e-9 for up to 10^7 additions of 2^-53).  The factor adds
+that, the sum with 1e-6 and the quotient, 2^-24 each; a scaled gradient its
+product and half a step of its type."""
+import pytest
+import torch
+
+import spark_gpt_amd as sg
+from oracle import routing as O
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+NORM_TOL = 2.0 ** -24 * 1.02
+
+
+def _grads(dev, shapes, dtypes, seed, std=1e-2):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return [(torch.randn(s, device=dev, generator=g) * std).to(dtypes[i % len(dtypes)]) for i, s in enumerate(shapes)]
+
+
+def _check(before, after, norm, max_norm):
+    ref, factor = O.clip(before, max_norm)
+    assert norm.dtype == torch.float32 and norm.dim() == 0
+    assert abs(float(norm) - ref) <= NORM_TOL * ref
+    for b, a in zip(before, after):
+        if factor == 1.0:
+            assert torch.equal(a, b)
+            continue
+        want = b.double() * factor
+        step = 5 * 2.0 ** -24 if b.dtype == torch.float32 else 5 * 2.0 ** -24 + torch.finfo(b.dtype).eps / 2
+        tiny = torch.finfo(b.dtype).tiny * torch.finfo(b.dtype).eps
+        assert a.dtype == b.dtype and ((a.double() - want).abs() <= step * want.abs() + tiny).all()
+
+
+SHAPES = {"one": [(1,)], "scalars": [(), (1,), (3,)], "odd": [(7, 13), (1025,), (3, 5, 7), (16384,), (16385,), (32768 + 5,)],
+          "weights": [(512, 256), (256, 1024), (256,)] * 3, "empty": [(0,), (4, 0), (5,)],
+          "many": [(i % 97 + 1,) for i in range(500)], "large": [(3000, 1111)]}
+
+
+@pytest.mark.parametrize("shapes", list(SHAPES))
+@pytest.mark.parametrize("dtypes", [[d] for d in DTYPES] + [DTYPES])
+@pytest.mark.parametrize("max_norm", [1e-3, 1e6])
+def test_norm_and_clip(dev, shapes, dtypes, max_norm):
+    grads = _grads(dev, SHAPES[shapes], dtypes, 3)
+    before = [g.clone() for g in grads]
+    ref, _ = O.clip(before, max_norm)
+    assert abs(float(sg.grad_norm(grads)) - ref) <= NORM_TOL * ref
+    out = [torch.full_like(g, 7.0) for g in grads]
+    norm = sg.clip_grads(grads, max_norm, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    _check(before, out, norm, max_norm)
+    norm2 = sg.clip_grads(grads, max_norm)
+    assert torch.equal(norm2, norm)
+    _check(before, grads, norm2, max_norm)
+    assert all(torch.equal(a, b) for a, b in zip(grads, out))  # in place or not: the same bits
+
+
+def test_parameters(dev):
+    """clip_grad_norm_ on parameters, some without a gradient, some transposed,
+    against torch's own on copies (its fp32 norm: 1e-5)."""
+    params = [torch.nn.Parameter(torch.zeros(s, device=dev)) for s in ((40, 30), (7,), (9, 9), (64, 3))]
+    other = [torch.nn.Parameter(torch.zeros_like(p)) for p in params]
+    g = torch.Generator(device=dev).manual_seed(1)
+    for i, (p, q) in enumerate(zip(params, other)):
+        if i == 1:
+            continue
+        x = torch.randn(p.shape[::-1], device=dev, generator=g).t() if i == 0 else torch.randn(p.shape, device=dev, generator=g)
+        p.grad, q.grad = x.clone(memory_format=torch.preserve_format), x.clone()
+    assert not params[0].grad.is_contiguous()
+    norm = sg.clip_grad_norm_(iter(params), 0.5)
+    want = torch.nn.utils.clip_grad_norm_(other, 0.5)
+    assert abs(float(norm) - float(want)) <= 1e-5 * float(want)
+    for p, q in zip(params, other):
+        if q.grad is not None:
+            assert ((p.grad - q.grad).abs() <= 1e-5 * q.grad.abs()).all()
+    single = sg.clip_grad_norm_(params[2], 100.0)
+    assert float(single) > 0 and params[1].grad is None
+
+
+def test_extremes(dev):
+    """Squares beyond fp32's range on either side, infinite and NaN gradients,
+    a largest norm of zero and of infinity."""
+    for v in (1e25, 1e-25, 3e38, 1e-40):
+        g = torch.full((1000,), v, device=dev)
+        ref = min(float(g[0].double()) * 1000 ** 0.5, float("inf"))
+        got = float(sg.grad_norm([g]))
+        if ref > torch.finfo(torch.float32).max:
+            assert got == float("inf")
+        else:
+            assert abs(got - ref) <= NORM_TOL * ref + 2.0 ** -150
+    for bad in (float("inf"), float("nan")):
+        a, b = torch.ones(10, device=dev), torch.ones(5000, device=dev)
+        b[77] = bad
+        want = torch.nn.Parameter(torch.zeros(5000, device=dev))
+        want.grad = b.clone()
+        torch.nn.utils.clip_grad_norm_([want], 1.0)
+        norm = sg.clip_grads([a, b], 1.0)
+        assert torch.equal(norm.isnan(), torch.tensor(bad != bad, device=dev)) and not bool(norm.isfinite())
+        assert torch.equal(b.isnan(), want.grad.isnan()) and torch.equal(b.nan_to_num(3.0), want.grad.nan_to_num(3.0))
+    g = torch.ones(10, device=dev)
+    sg.clip_grads([g], 0.0)
+    assert bool((g == 0).all())
+    g = torch.ones(10, device=dev)
+    assert float(sg.clip_grads([g], float("inf"))) > 3 and bool((g == 1).all())
+    z = torch.zeros(10, device=dev)
+    assert float(sg.clip_grads([z], 1.0)) == 0.0 and bool((z == 0).all())
+    p = torch.nn.Parameter(torch.zeros(4, device=dev))
+    p.grad = torch.full((4,), float("nan"), device=dev)
+    with pytest.raises(RuntimeError):
+        sg.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)
+    p.grad = torch.ones(4, device=dev)
+    assert abs(float(sg.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)) - 2.0) < 1e-6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_offsets_and_neighbours(dev, dtype):
+    """Gradients at every offset of their storage; what lies beside them stays."""
+    for off in range(0, 9):
+        for n in (1, 5, 8, 40, 70000):
+            store = torch.full((n + 32,), 3.0, device=dev, dtype=dtype)
+            g = store[off:off + n]
+            g.copy_(torch.randn(n, device=dev, generator=torch.Generator(device=dev).manual_seed(n)))
+            before = g.clone()
+            other = torch.full((n + 32,), 5.0, device=dev, dtype=dtype)
+            o = other[3:3 + n]
+            norm = sg.clip_grads([g], 0.1, out=[o])
+            _check([before], [o], norm, 0.1)
+            norm = sg.clip_grads([g], 0.1)
+            assert torch.equal(g, o)
+            assert bool((store[:off] == 3).all()) and bool((store[off + n:] == 3).all())
+            assert bool((other[:3] == 5).all()) and bool((other[3 + n:] == 5).all())
+
+
+def test_refusals(dev):
+    a, b = torch.ones(64, device=dev), torch.ones(64, device=dev)
+    store = torch.ones(100, device=dev)
+    for grads in ([a, a], [store[:60], store[59:]], [store, store[10:20]]):
+        with pytest.raises(ValueError, match="overlap"):
+            sg.clip_grads(grads, 1.0)
+        assert abs(float(sg.grad_norm(grads)) - O.clip(grads, 1.0)[0]) < 1e-5  # reading twice is fine
+    assert bool((a == 1).all()) and bool((store == 1).all())
+    for out in ([a], [a.double(), b], [a[:5], b], [b, b], [store[:64], store[1:65]], [b, a], [a.cpu(), b]):
+        with pytest.raises(ValueError):
+            sg.clip_grads([a, b], 1.0, out=out)
+    for grads in ([a.double()], [a.int()], [a[:1].expand(8)], [store[::2]], [a.cpu()], []):
+        with pytest.raises(ValueError):
+            sg.clip_grads(grads, 1.0)
+    for mx in (-1.0, float("nan")):
+        with pytest.raises(ValueError):
+            sg.clip_grads([a], mx)
+    torch.cuda.synchronize()
+    assert bool((a == 1).all()) and bool((b == 1).all()) and bool((store == 1).all())
+
+
+def test_deterministic_and_partly_in_place(dev):
+    grads = _grads(dev, [(700, 900), (33,), (70000,)], DTYPES, 6)
+    norms = {float(sg.grad_norm(grads)) for _ in range(5)}
+    assert len(norms) == 1
+    out = [torch.empty_like(grads[0]), grads[1], torch.empty_like(grads[2])]
+    before = [g.clone() for g in grads]
+    norm = sg.clip_grads(grads, 0.01, out=out)
+    _check(before, out, norm, 0.01)
+    assert torch.equal(grads[0], before[0]) and torch.equal(grads[2], before[2])
+
+
+def test_captured_and_replayed(dev):
+    """A captured clip, replayed on new gradients between eager calls."""
+    shapes = [(512, 256), (1000,), (64, 64)]
+    static = _grads(dev, shapes, DTYPES, 1)
+    out = [torch.empty_like(g) for g in static]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        sg.clip_grads(static, 1.0, out=out)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = sg.clip_grads(static, 1.0, out=out)
+    for rep in range(4):
+        new = _grads(dev, shapes, DTYPES, 50 + rep, std=10.0 ** (rep - 3))
+        for a, b in zip(static, new):
+            a.copy_(b)
+        graph.replay()
+        want = [torch.empty_like(g) for g in new]
+        wn = sg.clip_grads(new, 1.0, out=want)
+        torch.cuda.synchronize()
+        assert torch.equal(norm, wn) and all(torch.equal(a, b) for a, b in zip(out, want)), rep

@@ -1,0 +1,567 @@
+"""GPU tests of the routing operators against a plain restatement in 64 bits
+(oracle/routing.py): selection (equal, ties and borders included), weights and
+gradients, the expert order, the combine, and the layer that runs them around
+the FP8 experts.
+
+Tolerances.  A score is exp of an argument d = l - max (softmax) or -|l|
+(sigmoid): the argument's rounding, the product with log2(e) and that constant
+give |d| * 2.5 * 2^-24, exp2 and the reciprocal 2 * 2^-24 each; sums of up to
+1024 positive terms in lanes' order 22 * 2^-24, the scale 2^-24.  With D the
+largest |d| of the row: (32 + 5 D) * 2^-24 relative, below 2^-100 nothing is
+asked.  A gradient is a product of such weights: twice that, of the sum of the
+absolute products, and half a step of its type."""
+import threading
+
+import pytest
+import torch
+
+import spark_gpt_amd as sg
+from oracle import routing as O
+
+pytestmark = pytest.mark.gpu
+DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+INF, NAN = float("inf"), float("nan")
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _row_tol(low, score):
+    x = low.detach().cpu().double()
+    x = torch.where(x.isfinite(), x, 0.0)
+    span = (x.amax(1, keepdim=True) - x.amin(1, keepdim=True)) if score == "softmax" else x.abs().amax(1, keepdim=True)
+    return (32 + 5 * span) * 2.0 ** -24
+
+
+def _check_weights(w, ref, tol):
+    w = w.detach().cpu().double()
+    assert torch.equal(w.isnan(), ref.isnan())
+    ok = ref.isnan() | ((w - ref).abs() <= tol * ref.abs() + 2.0 ** -100)
+    assert ok.all(), (w[~ok][:4], ref[~ok][:4])
+
+
+def _run(low, k, dw=None, mask=None, bias=None, **kw):
+    """route_tokens against the oracle: selection, weights and, with dw, the gradient."""
+    leaf = low.detach().requires_grad_(dw is not None)
+    w, sel = sg.route_tokens(leaf, k, mask=mask, bias=bias, **kw)
+    rw, rsel = O.route(low, k, mask=mask, bias=bias, **kw)
+    assert sel.dtype == torch.int64 and torch.equal(sel.cpu(), rsel), kw
+    score = kw.get("score", "softmax")
+    tol = _row_tol(low, score)
+    _check_weights(w, rw, tol)
+    if dw is not None:
+        d, = torch.autograd.grad(w, leaf, dw)
+        kg = {x: kw[x] for x in ("score", "renormalize", "scale") if x in kw}
+        rd, size = O.route_grad(low, rsel, dw, **kg)
+        assert d.dtype == low.dtype and d.shape == low.shape
+        x = d.cpu().double()
+        assert torch.equal(x.isnan(), rd.isnan())
+        # the smallest step of the type (fp16 has a large one) bounds the rounding of tiny values;
+        # a score below 2^-126 is subnormal in 32 bits, off by up to its own size where it is flushed
+        # to zero, and a gradient is a score times at most the sum of the row's |g|, or that of two
+        tiny = torch.finfo(low.dtype).tiny * torch.finfo(low.dtype).eps
+        g = (kw.get("scale", 1.0) * dw.cpu().double()).abs().sum(1, keepdim=True)
+        tiny = tiny + 2.0 ** -125 * g
+        bound = 2 * tol * size + _half_step(low.dtype) * rd.abs() * (1 + 2.0 ** -8) + tiny
+        ok = rd.isnan() | ((x - rd).abs() <= bound)
+        assert ok.all(), (x[~ok][:4], rd[~ok][:4], bound[~ok][:4])
+    return w, sel
+
+
+def _logits(dev, T, E, dtype, seed, spread=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return (torch.randn(T, E, device=dev, generator=g) * spread + 0.5 * torch.randn(E, device=dev, generator=g)).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 8, 2), (7, 8, 8), (130, 16, 5), (65, 60, 4), (33, 64, 6), (5, 100, 64),
+                                   (41, 128, 8), (19, 256, 8), (3, 257, 1), (9, 384, 8), (4, 1000, 10), (2, 1024, 64)])
+def test_route_and_gradient(dev, T, E, k, score, renorm, dtype):
+    low = _logits(dev, T, E, DTYPES[dtype], T + E)
+    dw = torch.randn(T, k, device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+    _run(low, k, dw, score=score, renormalize=renorm, scale=2.5)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,top_groups,best", [(8, 4, 2), (8, 3, 1), (4, 1, 2), (6, 5, 2), (3, 2, 1), (1, 1, 1),
+                                                    (64, 20, 1), (16, 16, 2)])
+@pytest.mark.parametrize("with_bias", [True, False])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_route_groups_and_bias(dev, score, groups, top_groups, best, with_bias, dtype):
+    T = 70
+    for per in (1, 3, 8, 20, 32):
+        E = groups * per
+        if E > 1024:
+            continue
+        k = min(8, top_groups * per)
+        low = _logits(dev, T, E, DTYPES[dtype], E + best)
+        g = torch.Generator(device=dev).manual_seed(E)
+        bias = torch.randn(E, device=dev, generator=g) * 0.05 if with_bias else None
+        dw = torch.randn(T, k, device=dev, generator=g)
+        mask = torch.rand(T, device=dev, generator=g) > 0.2
+        _run(low, k, dw, mask=mask, bias=bias, score=score, groups=groups, top_groups=top_groups, group_best=best)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups", [(8, 1), (64, 4), (256, 8)])
+@pytest.mark.parametrize("with_bias", [True, False])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_route_special_rows(dev, score, E, groups, with_bias, dtype):
+    """Rows that are equal, tied, nearly tied, masked by -inf in part, but for
+    one expert or whole, NaN and infinite ones, far apart and tiny."""
+    k, per = 6, E // groups
+    base = torch.randn(E, generator=torch.Generator().manual_seed(E))
+    rows = [torch.zeros(E), torch.full((E,), -3.5), base.sign(), base.round()]
+    up = torch.full((E,), 1.0)
+    up[E // 2:] = torch.nextafter(torch.tensor(1.0), torch.tensor(2.0))  # one step of fp32 apart
+    rows += [up, torch.where(torch.arange(E) % 3 == 0, up, up.flip(0))]
+    x = base.clone()
+    x[::2] = -INF
+    rows += [x, torch.full((E,), -INF)]
+    x = torch.full((E,), -INF)
+    x[E - 1] = 0.25
+    rows.append(x)
+    x = torch.full((E,), -INF)
+    x[per - 1:per + 2] = torch.tensor([1.0, -2.0, 1.0])[:len(x[per - 1:per + 2])]
+    rows.append(x)
+    for at, v in ((3, NAN), (0, INF), (5, -INF)):
+        x = base.clone()
+        x[at] = v
+        rows.append(x)
+    x = base.clone()
+    x[1], x[2], x[4] = NAN, INF, NAN
+    rows += [x, base * 1e4, base * 1e-6, base * 60, base - 200, base + 200, base * 1e-3 + 1]
+    x = base.clone()
+    x[2] = 3e4
+    rows.append(x)
+    low = torch.stack(rows).to(dev).to(DTYPES[dtype])
+    low = torch.cat([low, low.flip(0), low.flip(1)])
+    for bias in ([torch.zeros(E, device=dev), (torch.arange(E, device=dev) % 4) * 0.25] if with_bias else [None]):
+        for best in ((1, 2) if groups > 1 else (1,)):
+            kw = dict(score=score, groups=groups, top_groups=max(1, groups // 2), group_best=best)
+            _run(low, k, None, bias=bias, **kw)
+            fine = low.isfinite().all(1) & (low.float().abs().amax(1) < 1e3)
+            dw = torch.randn(int(fine.sum()), k, device=dev)
+            for renorm in (True, False):
+                _run(low[fine], k, dw, bias=bias, renormalize=renorm, **kw)
+
+
+def test_route_bias_special(dev):
+    """A bias of -inf takes an expert out, +inf puts it first, NaN ranks above."""
+    low = _logits(dev, 20, 16, torch.float32, 5)
+    bias = torch.zeros(16, device=dev)
+    bias[3], bias[7], bias[9] = -INF, INF, INF
+    _run(low, 4, torch.ones(20, 4, device=dev), bias=bias, score="sigmoid")
+    bias[12] = NAN
+    _run(low, 4, bias=bias, score="sigmoid")
+    _run(low, 14, bias=torch.full((16,), -INF, device=dev), score="sigmoid")
+    _run(low, 4, bias=torch.linspace(-1e6, 1e6, 16, device=dev), score="softmax")
+
+
+def test_route_close_scores(dev):
+    """Biased scores that differ by less than fp32 holds: the order is the 64-bit one."""
+    g = torch.Generator(device=dev).manual_seed(2)
+    E, T = 64, 256
+    low = torch.randn(T, E, device=dev, generator=g)
+    # every score within a few 1e-8 of 1/2, in steps of 2^-30
+    low = torch.round(low * 8) * 2.0 ** -28
+    bias = torch.randint(-4, 4, (E,), device=dev, generator=g) * 2.0 ** -31
+    for groups, best in ((1, 1), (8, 1), (8, 2)):
+        _run(low, 8, bias=bias, score="sigmoid", groups=groups, top_groups=max(1, groups // 2), group_best=best)
+    far = torch.randn(T, E, device=dev, generator=g) * 1e-3 + 20.0  # 1 - s of about 2e-9
+    _run(far, 8, bias=torch.zeros(E, device=dev), score="sigmoid")
+    _run(far, 8, score="sigmoid")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_route_strides(dev, dtype):
+    """Any row stride and offset, a transposed view, an expanded row, no tokens."""
+    big = _logits(dev, 40, 77, DTYPES[dtype], 11)
+    dw = torch.randn(40, 3, device=dev)
+    for low in (big[:, 5:69], big[:, 1:65], big[:, :64]):
+        _run(low, 3, dw)
+        _run(low, 3, dw, renormalize=False)
+    _run(big[::2, 3:35], 3, dw[::2])
+    _run(big.t(), 3, torch.randn(77, 3, device=dev))
+    _run(big[:1, :64].expand(9, 64), 3, dw[:9], renormalize=False)
+    w, sel = sg.route_tokens(big[:0], 2)
+    assert w.shape == sel.shape == (0, 2)
+    leaf = big[:0].detach().requires_grad_(True)
+    d, = torch.autograd.grad(sg.route_tokens(leaf, 2)[0].sum(), leaf)
+    assert d.shape == (0, 77)
+
+
+def test_route_deterministic_and_large(dev):
+    """Twice the same bits; token counts past one pass of the chip against a
+    second call on parts of the rows."""
+    for T, E, k, kw in ((70001, 8, 2, {}), (50001, 64, 6, dict(score="sigmoid")),
+                        (30001, 256, 8, dict(score="sigmoid", groups=8, top_groups=4, group_best=2,
+                                             bias=torch.linspace(-0.1, 0.1, 256, device=dev)))):
+        low = _logits(dev, T, E, torch.float32, T).requires_grad_(True)
+        dw = torch.randn(T, k, device=dev)
+        w, sel = sg.route_tokens(low, k, **kw)
+        d, = torch.autograd.grad(w, low, dw)
+        w2, sel2 = sg.route_tokens(low, k, **kw)
+        assert torch.equal(w, w2) and torch.equal(sel, sel2)
+        for a, b in ((0, 100), (T // 2, T // 2 + 333), (T - 50, T)):
+            part = low.detach()[a:b].clone().requires_grad_(True)
+            pw, psel = sg.route_tokens(part, k, **kw)
+            pd, = torch.autograd.grad(pw, part, dw[a:b])
+            assert torch.equal(psel, sel[a:b]) and torch.equal(pw, w[a:b]) and torch.equal(pd, d[a:b])
+        _run(low.detach()[-64:], k, dw[-64:], **kw)
+
+
+def test_route_refusals(dev):
+    low = torch.zeros(4, 12, device=dev)
+    one = torch.ones(12, device=dev)
+    for kw in (dict(score="tanh"), dict(groups=5), dict(groups=0), dict(groups=3, top_groups=4), dict(top_groups=0),
+               dict(group_best=3), dict(bias=one.double()), dict(bias=one[:5]), dict(bias=one.cpu()),
+               dict(mask=torch.ones(5, dtype=torch.bool, device=dev)), dict(mask=torch.ones(4, device=dev)),
+               dict(mask=torch.ones(4, dtype=torch.bool)), dict(groups=4, top_groups=1)):
+        with pytest.raises(ValueError):
+            sg.route_tokens(low, 4, **kw)
+    for bad, k in ((low, 0), (low, 13), (low[0], 1), (low.double(), 1), (torch.zeros(2, 1025, device=dev), 1),
+                   (torch.zeros(2, 0, device=dev), 1), (torch.zeros(2, 128, device=dev), 65)):
+        with pytest.raises(ValueError):
+            sg.route_tokens(bad, k)
+    sel = torch.zeros(4, 2, dtype=torch.int64, device=dev)
+    for args in ((sel.int(), 8), (sel[0], 8), (sel, 0), (sel, 1025), (sel[:, :0], 8)):
+        with pytest.raises(ValueError):
+            sg.expert_order(*args)
+    rows, w, inv = torch.zeros(8, 16, device=dev), torch.zeros(4, 2, device=dev), sel.view(-1)
+    off = torch.zeros(8, dtype=torch.int32, device=dev)
+    for args in ((rows.double(), w, inv, off), (rows, w, inv[:-1], off), (rows, w, inv.int(), off),
+                 (rows[0], w, inv, off), (rows[:, :0], w, inv, off), (rows, w.cpu(), inv, off)):
+        with pytest.raises(ValueError):
+            sg.combine_experts(*args)
+    with pytest.raises(ValueError):
+        sg.ops.moe_combine_bwd(rows[:4], rows, w, inv, off.long())
+    with pytest.raises(ValueError):
+        sg.ops.moe_combine_bwd(rows, rows, w, inv, off)
+    torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ expert order
+@pytest.mark.parametrize("T,k,E", [(0, 2, 8), (1, 1, 1), (1, 8, 128), (8, 8, 128), (63, 3, 7), (1000, 2, 8), (4096, 1, 1),
+                                   (4097, 1, 3), (5003, 6, 60), (9001, 8, 256), (2049, 4, 1023), (3000, 7, 1024)])
+@pytest.mark.parametrize("fill", ["random", "some unrouted", "one expert", "none"])
+def test_expert_order(dev, T, k, E, fill):
+    g = torch.Generator().manual_seed(T + E)
+    sel = torch.randint(0, E, (T, k), generator=g)
+    if fill == "some unrouted":
+        sel[torch.rand(T, k, generator=g) < 0.2] = -1
+        sel[torch.rand(T, k, generator=g) < 0.05] = E + 3
+        sel[torch.rand(T, k, generator=g) < 0.05] = -(2 ** 40)
+    elif fill == "one expert":
+        sel[:] = E - 1
+    elif fill == "none":
+        sel[:] = -1
+    got = sg.expert_order(sel.to(dev), E)
+    for name, a, b in zip(("token_index", "inverse", "offsets"), got, O.expert_order(sel, E)):
+        assert a.dtype == b.dtype and torch.equal(a.cpu(), b), name
+
+
+def test_expert_order_large_matches_sort(dev):
+    """More slots than one pass of the work-groups, against torch's stable sort."""
+    T, k, E = 300007, 5, 200
+    sel = torch.randint(-1, E, (T, k), device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+    tok, inv, off = sg.expert_order(sel, E)
+    flat = sel.view(-1).cpu()
+    key = torch.where(flat < 0, E, flat)
+    order = torch.sort(key, stable=True).indices
+    assert torch.equal(tok.cpu(), order // k)
+    want = torch.empty_like(order)
+    want[order] = torch.arange(T * k)
+    assert torch.equal(inv.cpu(), torch.where(flat < 0, -1, want))
+    assert torch.equal(off.cpu(), torch.cumsum(torch.bincount(key, minlength=E + 1)[:E], 0).int())
+
+
+# ------------------------------------------------------------------ combine
+def _sum_steps(n):
+    """Roundings on the way of one product through a sum of n terms spread over
+    the lanes of a wave: its lane's chain and the tree."""
+    return n / 16 + 24
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,k,D", [(1, 1, 1), (1, 8, 2048), (5, 2, 7), (64, 2, 8), (33, 6, 1000), (50, 3, 130), (9, 8, 4096),
+                                   (17, 64, 24), (300, 2, 256), (12, 4, 5003)])
+@pytest.mark.parametrize("unrouted", [False, True])
+def test_combine_and_gradients(dev, T, k, D, dtype, unrouted):
+    g = torch.Generator().manual_seed(T * k + D)
+    E, dt = 16, DTYPES[dtype]
+    sel = torch.randint(0, E, (T, k), generator=g)
+    if unrouted:
+        sel[torch.rand(T, k, generator=g) < 0.3] = -1
+    _, inv, off = O.expert_order(sel, E)
+    rows = torch.randn(T * k, D, generator=g).to(dt)
+    n = int(off[-1])
+    rows[n:] = NAN  # what no slot names is not read
+    w = torch.rand(T, k, generator=g)
+    w[sel < 0] = NAN if unrouted else 0.0
+    dout = torch.randn(T, D, generator=g).to(dt)
+    r, ww = rows.to(dev).requires_grad_(True), w.to(dev).requires_grad_(True)
+    y = sg.combine_experts(r, ww, inv.to(dev), off.to(dev))
+    dr, dw = torch.autograd.grad(y, [r, ww], dout.to(dev))
+    step, tiny = _half_step(dt), torch.finfo(dt).tiny * torch.finfo(dt).eps
+    ref, size = O.combine(rows, w, inv)
+    assert y.dtype == dt and ((y.cpu().double() - ref).abs()
+                              <= (k + 1) * 2.0 ** -24 * size + step * (1 + 2.0 ** -8) * ref.abs() + tiny).all()
+    rdr, rdw, dsize = O.combine_grad(dout, rows, w, inv)
+    assert dr.dtype == dt and ((dr.cpu().double() - rdr).abs() <= (2.0 ** -24 + step * 1.01) * rdr.abs() + tiny).all()
+    assert (dr[n:] == 0).all()
+    assert dw.dtype == torch.float32
+    assert ((dw.cpu().double() - rdw).abs() <= _sum_steps(D) * 2.0 ** -24 * dsize + 2.0 ** -120).all()
+
+
+def test_combine_layouts(dev):
+    """Rows at an odd offset of their storage, strided views, bf16 weights, one
+    gradient alone, row indices beyond the rows, no tokens."""
+    g = torch.Generator(device=dev).manual_seed(8)
+    T, k, D, E = 40, 2, 64, 4
+    sel = torch.randint(0, E, (T, k), device=dev, generator=g)
+    _, inv, off = sg.expert_order(sel, E)
+    store = torch.randn(T * k * D + 1, device=dev, generator=g).to(torch.bfloat16)
+    w = torch.rand(T, k, device=dev, generator=g)
+    odd = store[1:].view(T * k, D)
+    want = sg.combine_experts(odd.clone(), w, inv, off)
+    assert torch.equal(sg.combine_experts(odd, w, inv, off), want)
+    wide = torch.randn(T * k, 2 * D, device=dev, generator=g).to(torch.bfloat16)
+    assert torch.equal(sg.combine_experts(wide[:, ::2], w, inv, off), sg.combine_experts(wide[:, ::2].clone(), w, inv, off))
+    wb = w.to(torch.bfloat16).requires_grad_(True)
+    y = sg.combine_experts(odd, wb, inv, off)
+    gw, = torch.autograd.grad(y, wb, torch.ones_like(y))
+    assert gw.dtype == torch.bfloat16 and torch.equal(y, sg.combine_experts(odd, wb.float(), inv, off))
+    dout = torch.randn(T, D, device=dev, generator=g).to(torch.bfloat16)
+    dr, dw = sg.ops.moe_combine_bwd(dout, odd, w, inv, off)
+    only, none = sg.ops.moe_combine_bwd(dout, odd, w, inv, off, True, False)
+    assert none is None and torch.equal(only, dr)
+    none, only = sg.ops.moe_combine_bwd(dout, odd, w, inv, off, False, True)
+    assert none is None and torch.equal(only, dw)
+    far = inv.clone()
+    far[::3] = T * k + 5
+    want, size = O.combine(odd, torch.where((far < T * k).view(T, k), w, 0.0), torch.where(far < T * k, far, -1))
+    got = sg.combine_experts(odd, w, far, off).cpu().double()
+    assert ((got - want).abs() <= 3 * 2.0 ** -24 * size + 2.0 ** -8 * 1.01 * want.abs()).all()
+    empty = sg.combine_experts(odd[:0], w[:0], inv[:0], torch.zeros(E, dtype=torch.int32, device=dev))
+    assert empty.shape == (0, D)
+
+
+# ------------------------------------------------------------------ together
+class _Experts(torch.nn.Module):
+    def __init__(self, E, D, I, dev, seed=0):
+        super().__init__()
+        g = torch.Generator(device=dev).manual_seed(seed)
+        self.gate_up_proj = torch.nn.Parameter(torch.randn(E, 2 * I, D, device=dev, generator=g) * D ** -0.5)
+        self.down_proj = torch.nn.Parameter(torch.randn(E, D, I, device=dev, generator=g) * I ** -0.5)
+        self.register_buffer("fp8_scale", torch.ones(5, device=dev), persistent=False)
+        self.register_buffer("fp8_amax", torch.zeros(5, device=dev), persistent=False)
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_routed_layer_matches_its_parts(dev, padded):
+    """fp8_routed_experts, forward and backward, against torch's sort and
+    products around _FP8Experts on the same scales: the rows, and so dx and the
+    experts' gradients, are equal to the bit; a padded batch gives its valid
+    tokens what they get without the padding."""
+    T, D, I, E, k = 600, 256, 384, 8, 2
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(T, D, device=dev, generator=g).to(torch.bfloat16)
+    low = torch.randn(T, E, device=dev, generator=g)
+    low[:, 5] = -INF  # an expert that nothing reaches
+    dout = (torch.randn(T, D, device=dev, generator=g) * 1e-3).to(torch.bfloat16)
+    mask = (torch.arange(T, device=dev) % 5 != 0) if padded else None
+    m = _Experts(E, D, I, dev).train()
+    m.fp8_scale.copy_(torch.tensor([32.0, 32, 16, 2.0 ** 20, 2.0 ** 20], device=dev))
+    xx, ll = x.clone().requires_grad_(True), low.clone().requires_grad_(True)
+    y, sel = sg.fp8_routed_experts(xx, ll, m, k, mask=mask)
+    params = [m.gate_up_proj, m.down_proj]
+    dx, dl, dgu, dd = torch.autograd.grad(y, [xx, ll] + params, dout)
+    amax = m.fp8_amax.clone()
+
+    # the same on the valid tokens alone, in torch around the experts
+    keep = mask if padded else torch.ones(T, dtype=torch.bool, device=dev)
+    n = int(keep.sum())
+    m.fp8_amax.zero_()
+    xv, lv = x[keep].clone().requires_grad_(True), low[keep].double().requires_grad_(True)
+    p = torch.softmax(lv, 1)
+    want_sel = torch.sort(low[keep], dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(sel[keep], want_sel) and bool((sel[~keep] == -1).all())
+    w = p.gather(1, want_sel)
+    w = w / w.sum(1, keepdim=True)
+    flat = want_sel.reshape(-1)
+    perm = torch.sort(flat, stable=True).indices
+    inv = torch.empty_like(perm)
+    inv[perm] = torch.arange(n * k, device=dev)
+    off = torch.cumsum(torch.bincount(flat, minlength=E), 0).int()
+    rows = sg._FP8Experts.apply(xv, m.gate_up_proj, m.down_proj, perm // k, inv, off, k, m.fp8_scale, m.fp8_amax)
+    yv = (rows.double()[inv].view(n, k, D) * w[:, :, None]).sum(1)
+    # k products and sums in 32 bits of weights within (32 + 5 * 8) 2^-24, rounded to bf16
+    size = (rows.double()[inv].view(n, k, D) * w[:, :, None]).abs().sum(1)
+    assert ((y[keep].double() - yv).abs() <= 76 * 2.0 ** -24 * size + 2.0 ** -8 * 1.01 * yv.abs()).all()
+    assert bool((y[~keep] == 0).all())
+    drows = torch.empty_like(rows)
+    w32 = sg.route_tokens(low[keep], k)[0]
+    drows[inv] = (w32.reshape(-1, 1) * dout[keep].float().repeat_interleave(k, 0)).to(torch.bfloat16)
+    vx, vgu, vd = torch.autograd.grad(rows, [xv] + params, drows, retain_graph=True)
+    assert torch.equal(dx[keep], vx) and bool((dx[~keep] == 0).all())
+    assert torch.equal(dgu, vgu) and torch.equal(dd, vd) and torch.equal(amax, m.fp8_amax)
+    assert bool((dgu[5] == 0).all()) and bool((dd[5] == 0).all())
+    vl, = torch.autograd.grad(yv, lv, dout[keep].double())
+    # dweights: dot products of D terms, 2^-24 of their absolute sum a step; then the route's own bound
+    dots = (rows.double()[inv].view(n, k, D) * dout[keep].double()[:, None]).abs().sum(2)
+    bound = (2 * 72 + _sum_steps(D)) * 2.0 ** -24 * 2 * dots.sum(1, keepdim=True)
+    assert ((dl[keep].double() - vl).abs() <= bound).all() and bool((dl[~keep] == 0).all())
+
+
+def test_training_step(dev):
+    """A router, the layer, clipping over its parameters and the momentum stage:
+    the norm, the clipped gradients and the stage's results against torch."""
+    T, D, I, E, k = 512, 256, 256, 4, 2
+    g = torch.Generator(device=dev).manual_seed(9)
+    x = torch.randn(T, D, device=dev, generator=g).to(torch.bfloat16)
+    router = torch.nn.Parameter(torch.randn(E, D, device=dev, generator=g) * D ** -0.5)
+    m = _Experts(E, D, I, dev).train()
+    params = [router, m.gate_up_proj, m.down_proj]
+    for step in range(2):
+        for p in params:
+            p.grad = None
+        y, sel = sg.fp8_routed_experts(x, torch.nn.functional.linear(x.float(), router), m, k, score="sigmoid", scale=1.5)
+        (y.float().square().mean()).backward()
+        assert all(bool(p.grad.isfinite().all()) and float(p.grad.abs().max()) > 0 for p in params)
+        before = [p.grad.clone() for p in params]
+        norm, factor = O.clip(before, 1e-3)
+        assert factor < 1
+        got = sg.clip_grad_norm_(params, 1e-3)
+        assert abs(float(got) - norm) <= 2.0 ** -24 * 1.01 * norm
+        for p, b in zip(params, before):
+            assert ((p.grad.double() - b.double() * factor).abs() <= 5 * 2.0 ** -24 * (b.double() * factor).abs() + 1e-44).all()
+        for p in params[1:]:
+            v = torch.zeros_like(p)
+            u = torch.empty(p.shape, dtype=torch.bfloat16, device=dev)
+            sg._momentum_stage(p.grad, v, u, 0.95)
+            rv = torch.zeros_like(p).lerp_(p.grad, 1 - 0.95)
+            assert torch.equal(v, rv)
+        sg.fp8_update_scales(m)
+
+
+def test_side_stream_and_threads(dev):
+    """Calls on another stream than the default, and from two threads at once,
+    each on a stream of its own, give the same bits."""
+    low = _logits(dev, 3000, 64, torch.float32, 3)
+    rows = torch.randn(3000 * 4, 128, device=dev).to(torch.bfloat16)
+
+    def work():
+        w, sel = sg.route_tokens(low, 4)
+        tok, inv, off = sg.expert_order(sel, 64)
+        return w, sel, tok, inv, off, sg.combine_experts(rows, w, inv, off)
+
+    want = work()
+    torch.cuda.synchronize()
+    got = {}
+
+    def go(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(5):
+                got[i] = work()
+        s.synchronize()
+
+    go(0)
+    threads = [threading.Thread(target=go, args=(i,)) for i in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want))
+
+
+def test_captured_and_replayed(dev):
+    """Route, order and combine captured into a graph: every replay on new data
+    equals the eager call, with eager work between the replays; two graphs side
+    by side do not disturb each other."""
+    T, E, k, D = 700, 32, 4, 96
+
+    def data(seed):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        return (torch.randn(T, E, device=dev, generator=g), torch.randn(T * k, D, device=dev, generator=g).to(torch.bfloat16),
+                torch.randn(T, k, device=dev, generator=g), torch.randn(T, D, device=dev, generator=g).to(torch.bfloat16))
+
+    def work(low, rows, dw, dout):
+        w, sel, picked = sg.ops.moe_route(low, None, None, "sigmoid", 4, 2, 2, k, True, 1.0)
+        dl = sg.ops.moe_route_bwd(dw, sel, picked, low, "sigmoid", True, 1.0)
+        tok, inv, off = sg.ops.moe_expert_order(sel, E)
+        y = sg.ops.moe_combine(rows, w, inv)
+        dr, dwt = sg.ops.moe_combine_bwd(dout, rows, w, inv, off)
+        return w, sel, dl, tok, inv, off, y, dr, dwt
+
+    graphs = []
+    for i in range(2):
+        ins = data(100 + i)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            work(*ins)
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = work(*ins)
+        graphs.append((graph, ins, outs))
+    for rep in range(4):
+        for i, (graph, ins, outs) in enumerate(graphs):
+            new = data(10 * rep + i)
+            for a, b in zip(ins, new):
+                a.copy_(b)
+            graph.replay()
+            want = work(*new)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), (rep, i)
+
+
+def test_compiled_matches_eager(dev):
+    T, E, k, D = 300, 16, 2, 64
+    low = _logits(dev, T, E, torch.float32, 21)
+    rows = torch.randn(T * k, D, device=dev).to(torch.bfloat16)
+    dout = torch.randn(T, D, device=dev).to(torch.bfloat16)
+
+    def f(low, rows):
+        w, sel = sg.route_tokens(low, k, score="sigmoid")
+        tok, inv, off = sg.expert_order(sel, E)
+        return sg.combine_experts(rows, w, inv, off), sel
+
+    outs = []
+    for fn in (f, torch.compile(f, dynamic=False, fullgraph=True)):
+        a, b = low.clone().requires_grad_(True), rows.clone().requires_grad_(True)
+        y, sel = fn(a, b)
+        outs.append((y, sel) + torch.autograd.grad(y, [a, b], dout))
+    assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
+def test_operators_opcheck(dev):
+    low = _logits(dev, 20, 16, torch.bfloat16, 2)
+    args = (low, None, None, "softmax", 1, 1, 1, 3, False, 1.0)
+    w, sel, picked = torch.ops.sparkfp8.route_fwd(*args)
+    torch.library.opcheck(torch.ops.sparkfp8.route_fwd.default, args)
+    torch.library.opcheck(torch.ops.sparkfp8.route_bwd.default, (w, sel, picked, low, "softmax", False, 1.0))
+    torch.library.opcheck(torch.ops.sparkfp8.expert_order.default, (sel, 16))
+    _, inv, off = torch.ops.sparkfp8.expert_order(sel, 16)
+    rows = torch.randn(60, 24, device=dev)
+    torch.library.opcheck(torch.ops.sparkfp8.combine_fwd.default, (rows, w, inv))
+    torch.library.opcheck(torch.ops.sparkfp8.combine_bwd.default, (rows[:20], rows, w, inv, off))
+
+
+def test_no_gradient_and_one_gradient(dev):
+    """Nothing asked of the logits costs no backward; weights alone carry one."""
+    low = _logits(dev, 10, 8, torch.float32, 6)
+    with torch.no_grad():
+        assert not sg.route_tokens(low, 2)[0].requires_grad
+    leaf = low.clone().requires_grad_(True)
+    w, sel = sg.route_tokens(leaf, 2)
+    assert w.requires_grad and not sel.requires_grad
+    with pytest.raises(RuntimeError):
+        d, = torch.autograd.grad(w.sum(), leaf, create_graph=True)
+        torch.autograd.grad(d.sum(), leaf)
