@@ -58,117 +58,479 @@ struct RouteArgs {
   float* picked;
 };
 
-// One wave per token, everything in 64 bits: v[e] is the order value of
-// expert e (LDS), -inf where it cannot be taken (any more).
-__global__ __launch_bounds__(256) void moe_route_kernel(const RouteArgs a) {
-  extern __shared__ __align__(16) double lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-  if (t >= a.T) return;
-  double* v = lds + (int64_t)wave * a.E;
+// ---------------------------------------------------------------------------
+// Reductions over the L lanes of a token (L a power of two, its lanes aligned
+// to L).  share<S>(x) gives two values whose combination is that of x with the
+// lane S away, where the S lanes below already agree: DPP within 16 lanes
+// (quad permutes, mirrors of half rows and rows), the lane swaps beyond.
+// ---------------------------------------------------------------------------
+struct Two {
+  uint32_t a, b;
+};
+template <int S>
+SFP8_DEV Two share(uint32_t x) {
+  static_assert(S == 1 || S == 2 || S == 4 || S == 8 || S == 16 || S == 32, "");
+  if constexpr (S == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return {r[0], r[1]};
+  } else if constexpr (S == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return {r[0], r[1]};
+  } else {
+    constexpr int ctrl = S == 1 ? 0xB1 : S == 2 ? 0x4E : S == 4 ? 0x141 : 0x140;
+    return {x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, ctrl, 0xf, 0xf, true)};
+  }
+}
+template <int S>
+SFP8_DEV void share_f(float x, float& a, float& b) {
+  const Two t = share<S>(__float_as_uint(x));
+  a = __uint_as_float(t.a);
+  b = __uint_as_float(t.b);
+}
+template <int L, int S = 1, class F>
+SFP8_DEV float reduce_f(float x, F f) {
+  if constexpr (S < L) {
+    float a, b;
+    share_f<S>(x, a, b);
+    return reduce_f<L, S * 2>(f(a, b), f);
+  } else {
+    return x;
+  }
+}
+template <int L, int S = 1>
+SFP8_DEV uint32_t reduce_max_u(uint32_t x) {
+  if constexpr (S < L) {
+    const Two t = share<S>(x);
+    return reduce_max_u<L, S * 2>(t.a > t.b ? t.a : t.b);
+  } else {
+    return x;
+  }
+}
+template <int L>
+SFP8_DEV float lanes_max(float x) {
+  return reduce_f<L>(x, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int L>
+SFP8_DEV float lanes_min(float x) {
+  return reduce_f<L>(x, [](float a, float b) { return fminf(a, b); });
+}
+template <int L>
+SFP8_DEV float lanes_sum(float x) {
+  return reduce_f<L>(x, [](float a, float b) { return a + b; });
+}
+
+constexpr float kLog2E = 1.4426950408889634f;
+SFP8_DEV float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2E); }
+
+// How the experts of a token lie in its L lanes: each group (all of them, when
+// there are none) has the G lanes g * G .. g * G + G - 1 of group g, and lane
+// `sub` of them holds, in chunks of four, members 4 * (c * G + sub) + i.
+struct RouteLayout {
+  int G, gs;  // lanes and members of a group
+  int g, sub;
+  SFP8_DEV int member(int c) const { return 4 * (c * G + sub); }
+};
+
+// The V logits of a lane: those past the group's members, and all where `on` is
+// false, read as -inf.  at: the group's first logit.
+template <int V>
+SFP8_DEV void load_logits(float (&l)[V], const void* p, int dtype, bool vec, int64_t at, const RouteLayout& lay, bool on) {
+  const float ninf = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < V; ++j) l[j] = ninf;
+  if (!on) return;
+  if (vec && dtype == kF32) {  // gs % 4 == 0 and aligned: a chunk is in or out as a whole
+    const float* q = reinterpret_cast<const float*>(p) + at;
+#pragma unroll
+    for (int c = 0; c < V / 4; ++c)
+      if (lay.member(c) < lay.gs) {
+        const floatx4 v = *reinterpret_cast<const floatx4*>(q + lay.member(c));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[4 * c + i] = v[i];
+      }
+  } else if (vec) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + at;
+#pragma unroll
+    for (int c = 0; c < V / 4; ++c)
+      if (lay.member(c) < lay.gs) {
+        const intx2 v = *reinterpret_cast<const intx2*>(q + lay.member(c));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t b = ((uint32_t)v[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+          l[4 * c + i] = dtype == kBf16 ? bf16_bits_to_f32(b) : half_bits_to_f32(b);
+        }
+      }
+  } else {
+#pragma unroll
+    for (int c = 0; c < V / 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lay.member(c) + i < lay.gs) l[4 * c + i] = load_as_f32(p, dtype, at + lay.member(c) + i);
+  }
+}
+
+// A double as an integer in the order of ranks_above: NaN is all ones, -inf
+// (what cannot be taken) is 0.
+SFP8_DEV uint64_t rank_bits(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.0);
+  const uint64_t ord = b >> 63 ? ~b : b | 1ull << 63;
+  return x != x ? ~0ull : x == -__builtin_inf() ? 0ull : ord;
+}
+template <int S = 1>
+SFP8_DEV uint64_t wave_max_u64(uint64_t x) {
+  if constexpr (S < 64) {
+    const Two lo = share<S>((uint32_t)x), hi = share<S>((uint32_t)(x >> 32));
+    const uint64_t a = (uint64_t)hi.a << 32 | lo.a, b = (uint64_t)hi.b << 32 | lo.b;
+    return wave_max_u64<S * 2>(a > b ? a : b);
+  } else {
+    return x;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The selection by the definition, in 64 bits, of one token by a whole wave:
+// for rows that hold NaN or +inf and for those whose order 32 bits do not
+// settle.  Returns the expert of slot `lane`, or -1.  v[e] (LDS) is the order
+// value of expert e as rank_bits, 0 where it cannot be taken (any more).  One
+// exponential and one quotient in the code, which is seldom run and so comes
+// from memory: its length counts for as much as its steps.
+// ---------------------------------------------------------------------------
+SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
+  const int lane = threadIdx.x & 63;
   const double ninf = -__builtin_inf();
   const int64_t row = t * a.ld;
-  if (a.mask && !a.mask[t]) {
-    if (lane < a.k) {
-      a.weights[t * a.k + lane] = 0.0f;
-      a.selected[t * a.k + lane] = -1;
-      if (a.picked) a.picked[t * a.k + lane] = 0.0f;
+  const bool softmax = a.score == kSoftmax;
+  const bool two_best = a.groups > 1 && a.group_best == 2;
+  const bool scores = a.bias || two_best;
+  if (scores) {
+    double m = 0.0, z = 0.0;
+    if (softmax) {
+      m = ninf;
+      for (int e = lane; e < a.E; e += 64) {
+        const double l = load_as_f32(a.logits, a.dtype, row + e);
+        m = ranks_above(l, m) ? l : m;
+      }
+      m = wave_max_nan_f64(m);
     }
-    return;
-  }
-  double m = 0.0, z = 1.0;
-  if (a.score == kSoftmax) {
-    m = ninf;
+    double* d = reinterpret_cast<double*>(v);
     for (int e = lane; e < a.E; e += 64) {
       const double l = load_as_f32(a.logits, a.dtype, row + e);
-      m = ranks_above(l, m) ? l : m;
+      const double x = exp(softmax ? l - m : -l);
+      z += x;
+      d[e] = x;
     }
-    m = wave_max_nan_f64(m);
-    z = 0.0;
-    for (int e = lane; e < a.E; e += 64) z += exp((double)load_as_f32(a.logits, a.dtype, row + e) - m);
-    z = wave_sum_f64(z);
-  }
-  const auto score_of = [&](double l) { return a.score == kSoftmax ? exp(l - m) / z : 1.0 / (1.0 + exp(-l)); };
-  for (int e = lane; e < a.E; e += 64) {
-    const double l = load_as_f32(a.logits, a.dtype, row + e);
-    v[e] = l == ninf ? ninf : a.bias ? score_of(l) + (double)a.bias[e] : l;
+    z = softmax ? wave_sum_f64(z) : 0.0;
+    for (int e = lane; e < a.E; e += 64) {
+      const double l = load_as_f32(a.logits, a.dtype, row + e);
+      const double s = (softmax ? d[e] : 1.0) / (softmax ? z : 1.0 + d[e]);
+      v[e] = l == ninf ? 0ull : rank_bits(a.bias ? s + (double)a.bias[e] : s);
+    }
+  } else {
+    for (int e = lane; e < a.E; e += 64) v[e] = rank_bits((double)load_as_f32(a.logits, a.dtype, row + e));
   }
   __builtin_amdgcn_wave_barrier();
   if (a.groups > 1) {
     const int gs = a.E / a.groups;
-    double g = ninf;  // the value of group `lane`
+    uint64_t b1 = 0, b2 = 0;  // the best two of group `lane`
     if (lane < a.groups) {
-      double b1 = ninf, b2 = ninf;
       for (int e = lane * gs; e < lane * gs + gs; ++e) {
-        const double x = v[e];
-        if (ranks_above(x, b1)) {
-          b2 = b1;
-          b1 = x;
-        } else if (ranks_above(x, b2)) {
-          b2 = x;
-        }
+        const uint64_t x = v[e];
+        b2 = x > b1 ? b1 : x > b2 ? x : b2;
+        b1 = x > b1 ? x : b1;
       }
-      if (a.group_best == 1 || b1 == ninf) {
-        g = b1;
-      } else if (a.bias) {
-        g = b1 + (b2 == ninf ? 0.0 : b2);
-      } else {
-        g = score_of(b1) + (b2 == ninf ? 0.0 : score_of(b2));
-      }
+    }
+    uint64_t g = b1;
+    if (two_best && b2) {
+      const auto value = [](uint64_t x) {
+        return x == ~0ull ? __builtin_nan("") : __builtin_bit_cast(double, x >> 63 ? x & ~(1ull << 63) : ~x);
+      };
+      g = rank_bits(value(b1) + value(b2));
     }
     int rank = 0;
     for (int j = 0; j < a.groups; ++j) {
-      const double o = __shfl(g, j, 64);
-      rank += ranks_above(o, g) || (j < lane && !ranks_above(g, o));
+      const uint64_t o = (uint64_t)__shfl((unsigned long long)g, j, 64);
+      rank += o > g || (o == g && j < lane);
     }
-    if (lane < a.groups && (g == ninf || rank >= a.top_groups))
-      for (int e = lane * gs; e < lane * gs + gs; ++e) v[e] = ninf;
+    const uint64_t keep = __ballot(lane < a.groups && g && rank < a.top_groups);
+    __builtin_amdgcn_wave_barrier();
+    for (int e = lane; e < a.E; e += 64) {
+      const uint64_t x = a.bias || !two_best ? v[e] : rank_bits((double)load_as_f32(a.logits, a.dtype, row + e));
+      v[e] = keep >> (e / gs) & 1 ? x : 0ull;
+    }
     __builtin_amdgcn_wave_barrier();
   }
-  int mine = -1;  // the expert of slot `lane`
+  int mine = -1;
   for (int s = 0; s < a.k; ++s) {
-    double best = ninf;
+    uint64_t best = 0;
     int at = a.E;
     for (int e = lane; e < a.E; e += 64) {
-      const double x = v[e];
-      if (ranks_above(x, best)) {
-        best = x;
-        at = e;
-      }
+      const uint64_t x = v[e];
+      at = x > best ? e : at;
+      best = x > best ? x : best;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const double ob = __shfl_xor(best, o, 64);
-      const int oa = __shfl_xor(at, o, 64);
-      if (ranks_above(ob, best) || (!ranks_above(best, ob) && oa < at)) {
-        best = ob;
-        at = oa;
-      }
-    }
-    if (best == ninf) break;
-    if (lane == s) mine = at;
-    if (lane == 0) v[at] = ninf;
+    const uint64_t m = wave_max_u64(best);
+    if (m == 0) break;
+    // the lowest index of them
+    at = a.E - (int)reduce_max_u<64>(best == m ? (uint32_t)(a.E - at) : 0u);
+    mine = lane == s ? at : mine;
+    if (lane == 0) v[at] = 0ull;
     __builtin_amdgcn_wave_barrier();
   }
-  const bool live = lane < a.k && mine >= 0;
-  const double l = live ? (double)load_as_f32(a.logits, a.dtype, row + mine) : ninf;
-  double w = 0.0;
-  if (!a.renorm) {
-    w = live ? score_of(l) : 0.0;
-  } else {
-    // shares of the chosen scores, scaled so that the largest cannot vanish
-    const double x = a.score == kSoftmax ? l : (l < 0.0 || l != l ? l : 0.0);
-    double mx = live ? x : ninf;
-    mx = wave_max_nan_f64(mx);
-    double q = live ? exp(x - mx) : 0.0;
-    if (a.score == kSigmoid && live) q /= 1.0 + exp(-__builtin_fabs(l));
-    const double sum = wave_sum_f64(q);
-    w = live ? q / sum : 0.0;
+  return mine;
+}
+
+// ---------------------------------------------------------------------------
+// Routing, L lanes a token, V values a lane, 64 / L tokens a wave at a time.
+//
+// The order.  Each expert gets a key of 31 bits, its order value above its
+// inverted index, so that keys differ and the larger key comes first; 0 where
+// it cannot be taken.  16-bit logits without a bias fit whole, with their bits
+// in the order of their values.  Others are put on a fixed-point scale of up to 24 bits
+// between the row's smallest and largest value: the steps to it (a
+// difference, a product, a truncation) keep the order, so keys that differ
+// there are in the order of the 32-bit values.  The next key below m is
+// max(key - m) + m in wrapping arithmetic (keys below m wrap to 2^31 and
+// above, those from m on stay below), one subtraction and half a max3 for each
+// value and log2(L) lane steps, with nothing to clear.
+//
+// Its limits.  Where two neighbours of the k + 1 first are closer than their
+// 32-bit errors, or two groups are at the border of those kept, the token is
+// done again by the definition in 64 bits (route_exact), as are rows with NaN
+// or +inf.  Without a bias that is where two logits fall on one step of the
+// scale and differ (equal ones are in the order of their indices): 3 of 10^4
+// tokens at 256 normal logits.  With one, scores are off: a softmax by at most
+// (2.5 |d| + 30) 2^-24 of itself, below 2^-19 in all (d is the exponent's
+// argument, |d| e^-|d| < 0.4), a sigmoid, which has no sum over the experts, by
+// at most 2^-21; the sums with the bias round once more.
+//
+// A token's result depends on its row and on E, top_k and the groups alone,
+// not on the batch it comes in.
+// ---------------------------------------------------------------------------
+template <int L, int V, bool BIAS>
+__global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, int G, int idx_bits, bool vec) {
+  extern __shared__ __align__(16) uint64_t lds[];
+  constexpr int kTok = 64 / L;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tl = lane & (L - 1);  // lane of the token
+  const RouteLayout lay{G, a.E / a.groups, tl / G, tl % G};
+  const bool in_group = lay.g < a.groups;
+  const float ninf = -__builtin_inff();
+  const uint32_t idx_mask = (1u << idx_bits) - 1;
+  const bool half16 = !BIAS && a.dtype != kF32;  // keys hold the whole logit
+  const bool softmax = a.score == kSoftmax;
+  const bool two_best = a.groups > 1 && a.group_best == 2;
+  const bool scores = BIAS || !a.renorm || two_best;  // scores of all experts, not of the chosen alone
+  const int first = lay.g * lay.gs;                   // the group's first expert
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * kTok;
+  if (t0 >= a.T) return;
+  const int64_t t = t0 + lane / L;
+  const bool on = t < a.T && !(a.mask && !a.mask[t]);
+  float l[V];
+  load_logits<V>(l, a.logits, a.dtype, vec, t * a.ld + first, lay, on && in_group);
+  bool odd = false;  // done again in 64 bits
+  float m = ninf;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    l[j] += 0.0f;  // -0 is 0
+    odd |= !(l[j] < __builtin_inff());
+    m = fmaxf(m, l[j]);
   }
-  if (lane < a.k) {
-    a.weights[t * a.k + lane] = live ? a.scale * (float)w : 0.0f;
-    a.selected[t * a.k + lane] = mine;
-    if (a.picked) a.picked[t * a.k + lane] = live ? (float)l : 0.0f;
+  float z = 1.0f;
+  if (softmax && scores) {
+    m = lanes_max<L>(m);
+    z = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) z += l[j] == ninf ? 0.0f : exp_fast(l[j] - m);
+    z = lanes_sum<L>(z);
+  }
+  // the order values
+  float o[V], bias[V];
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int c = 0; c < V / 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int mem = lay.member(c) + i;
+        bias[4 * c + i] = in_group && mem < lay.gs ? a.bias[first + mem] : 0.0f;
+      }
+  }
+  float err = 0.0f;  // how far one may be off
+  if constexpr (BIAS) {
+    const float rz = 1.0f / z;
+    float big = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float sc;
+      if (softmax) {
+        sc = exp_fast(l[j] - m) * rz;
+      } else {
+        const float en = exp_fast(-fabsf(l[j]));
+        sc = (l[j] > 0.0f ? 1.0f : en) * __builtin_amdgcn_rcpf(1.0f + en);
+      }
+      o[j] = l[j] == ninf ? ninf : sc + bias[j];
+      odd |= !(o[j] < __builtin_inff());
+      big = o[j] == ninf ? big : fmaxf(big, fabsf(o[j]));
+    }
+    err = (softmax ? 0x1p-19f : 0x1p-21f) + 0x1p-24f * lanes_max<L>(big);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = l[j];
+  }
+  bool kept = in_group;
+  if (a.groups > 1) {
+    // the best two of this lane, then of its group
+    float b1 = ninf, b2 = ninf;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      b2 = fmaxf(b2, fminf(b1, o[j]));
+      b1 = fmaxf(b1, o[j]);
+    }
+    const auto merge = [&](float p1, float q1, float p2, float q2) {
+      b1 = fmaxf(p1, q1);
+      b2 = fmaxf(fminf(p1, q1), fmaxf(p2, q2));
+    };
+    float p1, q1, p2, q2;
+    if constexpr (L > 1)
+      if (G > 1) share_f<1>(b1, p1, q1), share_f<1>(b2, p2, q2), merge(p1, q1, p2, q2);
+    if constexpr (L > 2)
+      if (G > 2) share_f<2>(b1, p1, q1), share_f<2>(b2, p2, q2), merge(p1, q1, p2, q2);
+    if constexpr (L > 4)
+      if (G > 4) share_f<4>(b1, p1, q1), share_f<4>(b2, p2, q2), merge(p1, q1, p2, q2);
+    if constexpr (L > 8)
+      if (G > 8) share_f<8>(b1, p1, q1), share_f<8>(b2, p2, q2), merge(p1, q1, p2, q2);
+    if constexpr (L > 16)
+      if (G > 16) share_f<16>(b1, p1, q1), share_f<16>(b2, p2, q2), merge(p1, q1, p2, q2);
+    if constexpr (L > 32)
+      if (G > 32) share_f<32>(b1, p1, q1), share_f<32>(b2, p2, q2), merge(p1, q1, p2, q2);
+    float val = b1, tol = 2.0f * err;
+    if (two_best && b1 != ninf) {
+      if constexpr (!BIAS) {
+        const auto part = [&](float x) {
+          if (softmax) return exp_fast(x - m);  // z is the same for all
+          const float en = exp_fast(-fabsf(x));
+          return (x > 0.0f ? 1.0f : en) * __builtin_amdgcn_rcpf(1.0f + en);
+        };
+        b1 = part(b1);
+        b2 = b2 == ninf ? ninf : part(b2);
+      }
+      val = b1 + (b2 == ninf ? 0.0f : b2);
+      // of scores: (2.5 |d| + 8) 2^-24 of each, |d| < 104 (below, they vanish)
+      tol = BIAS ? 4.0f * err + 0x1p-22f * fabsf(val) : 0x1p-14f * val + 0x1p-120f;
+    }
+    int rank = 0, over = 0, near = 0;
+    for (int j = 1; j < L / G; ++j) {
+      const int from = (tl + j * G) & (L - 1);
+      const float other = __shfl(val, (lane & ~(L - 1)) + from, 64);
+      rank += other > val || (other == val && from < tl);
+      over += other > val + tol;
+      near += other >= val - tol;
+    }
+    kept = in_group && val != ninf && rank < a.top_groups;
+    odd |= tol > 0.0f && val != ninf && over < a.top_groups && near >= a.top_groups;
+  }
+  // the keys
+  uint32_t key[V];
+  float gap = 0.0f;  // keys that are no further apart on the scale may be in the wrong order
+  if (half16) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int32_t b = a.dtype == kBf16 ? (int32_t)__float_as_uint(o[j]) >> 16
+                                         : (int32_t)(int16_t)f32_to_half_bits(o[j]);
+      const uint32_t ord = (uint32_t)(b ^ (b < 0 ? 0xffff : 0x8000)) & 0xffffu;
+      key[j] = o[j] == ninf ? 0u : ord << idx_bits;
+    }
+  } else {
+    float lo = __builtin_inff(), hi = ninf;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      lo = fminf(lo, o[j] == ninf ? lo : o[j]);
+      hi = fmaxf(hi, o[j]);
+    }
+    lo = lanes_min<L>(lo);
+    hi = lanes_max<L>(hi);
+    const int bits = 31 - idx_bits < 24 ? 31 - idx_bits : 24;
+    const float range = hi - lo;
+    const float scale = range > 0.0f ? ((float)(1u << bits) - 4.0f) / range : 0.0f;
+    // a range outside 2^+-100 is left to 64 bits
+    odd |= range > 0.0f && !(range > 0x1p-100f && range < 0x1p100f);
+    gap = BIAS ? 2.0f * err * scale + 3.0f : 0.0f;  // the scale's own roundings: 3
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      key[j] = o[j] == ninf ? 0u
+                            : ((uint32_t)__builtin_amdgcn_fmed3f((o[j] - lo) * scale, 0.0f, 0x1p24f) + 1u) << idx_bits;
+  }
+#pragma unroll
+  for (int c = 0; c < V / 4; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t& x = key[4 * c + i];
+      x = kept && x ? x | (idx_mask - (uint32_t)(first + lay.member(c) + i)) : 0u;
+    }
+  // the first top_k keys, and the one after them
+  uint32_t top = 1u << 31, mine = 0u;
+  bool near = false;  // neighbours no further apart than their errors
+  const int rounds = a.k + (half16 ? 0 : 1);
+  for (int s = 0; s < rounds; ++s) {
+    uint32_t r = 0u;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const uint32_t x = key[j] - top;
+      r = x > r ? x : r;
+    }
+    r = reduce_max_u<L>(r);
+    const uint32_t next = r & 0x80000000u ? r + top : 0u;
+    if (!half16 && s > 0 && next) near |= (float)((top >> idx_bits) - (next >> idx_bits)) <= gap;
+    mine = s == tl && s < a.k ? next : mine;
+    top = next;
+  }
+  int e = mine ? (int)(idx_mask - (mine & idx_mask)) : -1;
+  float le = e >= 0 ? load_as_f32(a.logits, a.dtype, t * a.ld + e) : ninf;
+  if (!half16 && __any(near)) {
+    // Near neighbours with the same logit and bias are equal, and in the order
+    // of their indices: that leaves those that differ, among the chosen or
+    // between the last of them and the rest.
+    const float be = BIAS && e >= 0 ? a.bias[e] : 0.0f;
+    const uint32_t above = __shfl_up(mine, 1, 64);
+    const float la = __shfl_up(le, 1, 64), ba = __shfl_up(be, 1, 64);
+    odd |= tl > 0 && e >= 0 && (float)((above >> idx_bits) - (mine >> idx_bits)) <= gap && !(la == le && ba == be);
+    const int from = (lane & ~(L - 1)) + a.k - 1;
+    const uint32_t last = __shfl(mine, from, 64);
+    const float ll = __shfl(le, from, 64), bl = __shfl(be, from, 64);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (key[j] && key[j] < last && (float)((last >> idx_bits) - (key[j] >> idx_bits)) <= gap) {
+        const int x = (int)(idx_mask - (key[j] & idx_mask));
+        odd |= load_as_f32(a.logits, a.dtype, t * a.ld + x) != ll || (BIAS && a.bias[x] != bl);
+      }
+  }
+  const uint64_t any_odd = __ballot(odd && on);
+  if (any_odd) {  // wave uniform
+    for (int i = 0; i < kTok; ++i) {
+      if (!(any_odd >> (i * L) & (L == 64 ? ~0ull : (1ull << L) - 1))) continue;
+      const int again = __shfl(route_exact(a, t0 + i, lds + wave * a.E), tl, 64);
+      if (lane / L == i) {
+        e = tl < a.k ? again : -1;
+        le = e >= 0 ? load_as_f32(a.logits, a.dtype, t * a.ld + e) : ninf;
+      }
+    }
+  }
+  // the weights: lane s of the token has slot s
+  const bool live = e >= 0;
+  float w;
+  if (softmax) {
+    const float top_l = a.renorm ? lanes_max<L>(le) : m;
+    w = live ? exp_fast(le - top_l) : 0.0f;
+    w /= a.renorm ? lanes_sum<L>(w) : z;
+  } else {
+    const float en = exp_fast(-fabsf(le)), low = fminf(le, 0.0f);
+    const float top_l = a.renorm ? lanes_max<L>(low) : 0.0f;
+    w = live ? exp_fast(low - top_l) / (1.0f + en) : 0.0f;
+    if (a.renorm) w /= lanes_sum<L>(w);
+  }
+  if (t < a.T && tl < a.k) {
+    a.weights[t * a.k + tl] = live ? a.scale * w : 0.0f;
+    a.selected[t * a.k + tl] = e;
+    if (a.picked) a.picked[t * a.k + tl] = live ? le : 0.0f;
   }
 }
 
@@ -500,6 +862,55 @@ void by_type(int dtype, bool vec, A... args) {
   else vec ? F<kF16, true>::run(args...) : F<kF16, false>::run(args...);
 }
 
+// Lanes of a token and of a group, and values of a lane: the fewest lanes that
+// hold every group at 16 values each and have one for every slot; at most 64,
+// with up to 32 values where the number of groups is no power of two.
+struct RouteShape {
+  int L, G, V;
+};
+RouteShape route_shape(int64_t E, int64_t groups, int64_t k) {
+  int gp = 1;
+  while (gp < groups) gp *= 2;
+  const int gs = (int)(E / groups);
+  int G = 1;
+  while ((G * 16 < gs || gp * G < k) && gp * G < 64) G *= 2;
+  const int need = (gs + G - 1) / G;  // above 16 where gp lanes of G would be more than a wave
+  return {gp * G, G, need <= 4 ? 4 : need <= 8 ? 8 : need <= 16 ? 16 : 32};
+}
+
+template <int L, int V>
+void route_launch_lv(const RouteArgs& a, const RouteShape& sh, bool vec, int idx_bits, hipStream_t st) {
+  const int64_t per = 4 * (64 / L);  // tokens of a work-group
+  const dim3 grid((unsigned)((a.T + per - 1) / per));
+  const size_t lds = 4 * (size_t)a.E * 8;
+  if (a.bias) hipLaunchKernelGGL((moe_route_kernel<L, V, true>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec);
+  else hipLaunchKernelGGL((moe_route_kernel<L, V, false>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec);
+}
+template <int L>
+void route_launch_l(const RouteArgs& a, const RouteShape& sh, bool vec, int idx_bits, hipStream_t st) {
+  if (sh.V == 4) route_launch_lv<L, 4>(a, sh, vec, idx_bits, st);
+  else if (sh.V == 8) route_launch_lv<L, 8>(a, sh, vec, idx_bits, st);
+  else route_launch_lv<L, 16>(a, sh, vec, idx_bits, st);
+}
+void route_launch(const RouteArgs& a, hipStream_t st) {
+  const RouteShape sh = route_shape(a.E, a.groups, a.k);
+  int idx_bits = 0;
+  while ((1 << idx_bits) < a.E) ++idx_bits;
+  const uintptr_t unit = a.dtype == kF32 ? 16 : 8;  // four logits
+  const bool vec = (a.E / a.groups) % 4 == 0 && (a.ld % 4 == 0 || a.T == 1) && (uintptr_t)a.logits % unit == 0;
+  switch (sh.L) {
+    case 1: return route_launch_l<1>(a, sh, vec, idx_bits, st);
+    case 2: return route_launch_l<2>(a, sh, vec, idx_bits, st);
+    case 4: return route_launch_l<4>(a, sh, vec, idx_bits, st);
+    case 8: return route_launch_l<8>(a, sh, vec, idx_bits, st);
+    case 16: return route_launch_l<16>(a, sh, vec, idx_bits, st);
+    case 32: return route_launch_l<32>(a, sh, vec, idx_bits, st);
+    default:
+      if (sh.V == 32) return route_launch_lv<64, 32>(a, sh, vec, idx_bits, st);
+      return route_launch_l<64>(a, sh, vec, idx_bits, st);
+  }
+}
+
 template <int DT, bool VEC>
 struct Combine {
   static void run(const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv, int64_t T, int k,
@@ -537,8 +948,7 @@ int sfp8_moe_route(const void* logits, int dtype, int64_t T, int64_t E, int64_t 
   if (T == 0) return kOk;
   const RouteArgs a{logits, dtype, T, ld, (int)E, (int)top_k, score, (int)groups, (int)top_groups, (int)group_best,
                     renorm, scale, bias, (const uint8_t*)mask, weights, selected, picked};
-  hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)((T + 3) / 4)), dim3(256), 4 * (size_t)E * 8,
-                     (hipStream_t)stream, a);
+  route_launch(a, (hipStream_t)stream);
   return route_status();
 }
 
