@@ -12,6 +12,8 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -110,8 +112,10 @@ inline void* stream_of(const Tensor& t) {
 template <class F, class... A>
 void call(const char* name, F fn, A... args) {
   int rc;
-  {
+  if (PyGILState_Check()) {
     py::gil_scoped_release nogil;
+    rc = fn(args...);
+  } else {  // a backward pass, in a thread of the autograd engine
     rc = fn(args...);
   }
   if (rc == 0) return;
@@ -401,9 +405,10 @@ Tensor logit_rows(const Tensor& t) {
   return t.size(1) == 1 || t.stride(1) == 1 ? t : t.contiguous();
 }
 
-std::tuple<Tensor, Tensor, Tensor> moe_route(const Tensor& logits_, const OptTensor& bias, const OptTensor& mask,
+std::tuple<Tensor, Tensor, OptTensor> moe_route(const Tensor& logits_, const OptTensor& bias, const OptTensor& mask,
                                              const std::string& score, int64_t groups, int64_t top_groups,
-                                             int64_t group_best, int64_t top_k, bool renormalize, double scale) {
+                                             int64_t group_best, int64_t top_k, bool renormalize, double scale,
+                                             bool need_picked) {
   const int dtype = float_code("logits", logits_), sc = score_code(score);
   const c10::DeviceGuard guard(logits_.device());
   const Tensor logits = logit_rows(logits_);
@@ -425,8 +430,9 @@ std::tuple<Tensor, Tensor, Tensor> moe_route(const Tensor& logits_, const OptTen
   need(group_best == 1 || group_best == 2, "group_best must be 1 or 2");
   if (top_k < 1 || top_k > 64 || top_k > top_groups * (E / groups))
     refuse("top_k must be 1 .. 64 and no more than the experts of the kept groups, got " + std::to_string(top_k));
-  Tensor w = empty({T, top_k}, kF32, logits), sel = empty({T, top_k}, kI64, logits),
-         picked = empty({T, top_k}, kF32, logits);
+  Tensor w = empty({T, top_k}, kF32, logits), sel = empty({T, top_k}, kI64, logits);
+  OptTensor picked;
+  if (need_picked) picked = empty({T, top_k}, kF32, logits);
   CALL(sfp8_moe_route, ptr(logits), dtype, T, E, logits.stride(0), fptr(bias), ptr(mask), sc, groups, top_groups,
        group_best, top_k, (int)renormalize, (float)scale, fptr(w), lptr(sel), fptr(picked), stream_of(logits));
   return {w, sel, picked};
@@ -514,6 +520,85 @@ std::tuple<OptTensor, OptTensor> moe_combine_bwd(const Tensor& dout, const Tenso
        lptr(inverse_permutation), weights.size(0), weights.size(1), iptr(offsets), offsets.size(0), ptr(drows),
        fptr(dweights), stream_of(rows));
   return {drows, dweights};
+}
+
+// The autograd nodes of routing.py's eager calls: what _RouteTokens and
+// _CombineExperts do there, without Python's share of a node (a training pass
+// of a few tokens, bound by host time: 77 us with the Python nodes, 56 with
+// these, 49 for a torch product and its gradient).
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that can be taken once: a second derivative raises.
+variable_list once(variable_list grads, const char* what) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  const int64_t n = (int64_t)grads.size();
+  return std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", n)
+      ->apply(std::move(grads));
+}
+
+struct RouteTokens : torch::autograd::Function<RouteTokens> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& bias, const OptTensor& mask,
+                               const std::string& score, int64_t groups, int64_t top_groups, int64_t group_best,
+                               int64_t top_k, bool renormalize, double scale, bool needs_grad) {
+    auto [w, sel, picked] = moe_route(logits, bias, mask, score, groups, top_groups, group_best, top_k, renormalize,
+                                      scale, needs_grad);
+    if (needs_grad) ctx->save_for_backward({logits, sel, *picked});
+    ctx->saved_data["score"] = score;
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({sel});
+    ctx->set_materialize_grads(false);
+    return {w, sel};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    variable_list out(11);
+    if (!grads[0].defined()) return out;
+    const variable_list v = ctx->get_saved_variables();
+    {
+      const c10::AutoGradMode off(false);
+      out[0] = moe_route_bwd(grads[0], v[1], v[2], v[0], ctx->saved_data["score"].toStringRef(),
+                             ctx->saved_data["renormalize"].toBool(), ctx->saved_data["scale"].toDouble());
+    }
+    return once(std::move(out), "route_tokens");
+  }
+};
+
+std::tuple<Tensor, Tensor> route_tokens(const Tensor& logits, const OptTensor& bias, const OptTensor& mask,
+                                        const std::string& score, int64_t groups, int64_t top_groups,
+                                        int64_t group_best, int64_t top_k, bool renormalize, double scale) {
+  variable_list out = RouteTokens::apply(logits, bias, mask, score, groups, top_groups, group_best, top_k, renormalize,
+                                         scale, c10::GradMode::is_enabled() && logits.requires_grad());
+  return {out[0], out[1]};
+}
+
+struct CombineExperts : torch::autograd::Function<CombineExperts> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& inverse,
+                        const Tensor& offsets) {
+    ctx->save_for_backward({rows, weights, inverse, offsets});
+    return moe_combine(rows.contiguous(), weights.contiguous(), inverse.contiguous());
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const variable_list v = ctx->get_saved_variables();
+    variable_list out(4);
+    {
+      const c10::AutoGradMode off(false);
+      auto [drows, dweights] = moe_combine_bwd(grads[0].contiguous(), v[0].contiguous(), v[1].contiguous(),
+                                               v[2].contiguous(), v[3].contiguous(), ctx->needs_input_grad(0),
+                                               ctx->needs_input_grad(1));
+      if (drows) out[0] = *drows;
+      if (dweights) out[1] = *dweights;
+    }
+    return once(std::move(out), "combine_experts");
+  }
+};
+
+Tensor combine_experts(const Tensor& rows, const Tensor& weights, const Tensor& inverse_permutation,
+                       const Tensor& offsets) {
+  return CombineExperts::apply(rows, weights.scalar_type() == kF32 ? weights : weights.to(kF32), inverse_permutation,
+                               offsets);
 }
 
 // ------------------------------------------------------------------ gradient norm and clipping
@@ -785,7 +870,8 @@ PYBIND11_MODULE(_native, m) {
         "out[t] = sum of the top_k expert-order rows of token t (bf16 [T, D]).");
   m.def("moe_route", &moe_route, arg("logits"), arg("bias"), arg("mask"), arg("score"), arg("groups"),
         arg("top_groups"), arg("group_best"), arg("top_k"), arg("renormalize"), arg("scale"),
-        "(weights fp32, selected int64, picked fp32), each [T, top_k]: the experts of each token in descending order, "
+        arg("need_picked") = true,
+        "(weights fp32, selected int64, picked fp32 or None), each [T, top_k]: the experts of each token in descending order, "
         "their weights and their logits; -1, 0 and 0 where no expert is left or the token is masked.");
   m.def("moe_route_bwd", &moe_route_bwd, arg("dweights"), arg("selected"), arg("picked"), arg("logits"), arg("score"),
         arg("renormalize"), arg("scale"),
@@ -799,6 +885,11 @@ PYBIND11_MODULE(_native, m) {
   m.def("moe_combine_bwd", &moe_combine_bwd, arg("dout"), arg("rows"), arg("weights"), arg("inverse_permutation"),
         arg("offsets"), arg("need_rows") = true, arg("need_weights") = true,
         "(drows, dweights) of moe_combine; rows from offsets[-1] on get zeros.");
+  m.def("route_tokens", &route_tokens, arg("logits"), arg("bias"), arg("mask"), arg("score"), arg("groups"),
+        arg("top_groups"), arg("group_best"), arg("top_k"), arg("renormalize"), arg("scale"),
+        "(weights, selected) of moe_route, differentiable in the logits.");
+  m.def("combine_experts", &combine_experts, arg("rows"), arg("weights"), arg("inverse_permutation"), arg("offsets"),
+        "moe_combine, differentiable in the rows and the weights.");
   m.def("grad_norm", &grad_norm, arg("grads"), "The 2-norm over all elements of all gradients (fp32 scalar tensor).");
   m.def("clip_grads", &clip_grads, arg("grads"), arg("max_norm"), arg("out") = py::none(),
         "grad_norm(grads); every gradient times min(1, max_norm / (norm + 1e-6)), in place or into out.");

@@ -546,60 +546,91 @@ struct RouteBwdArgs {
   void* dlogits;
 };
 
-// One wave per token: the row's gradient in LDS, then written whole.
-__global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a) {
-  extern __shared__ __align__(16) float row_lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * 4 + wave;
-  if (t >= a.T) return;
-  float* d = row_lds + (int64_t)wave * a.E;
+// The gradient of the logits, L lanes a token and V values a lane as the
+// forward has them without groups.  Lane s of a token computes what slot s gives
+// its expert, from the chosen logits alone; the plain softmax also reads the
+// row again, for p of every expert.  The row is put together in LDS (zeros or
+// the dense part, then the slots' values) and written whole, once: bound by
+// those bytes.
+template <int L, int V>
+__global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a, bool vec_in, bool vec_out) {
+  __shared__ __align__(16) float rows[256 * V];
+  constexpr int kTok = 64 / L;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tl = lane & (L - 1);
+  const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * kTok;
+  if (t0 >= a.T) return;
+  const int64_t t = t0 + lane / L;
+  const bool on = t < a.T;
   const float ninf = -__builtin_inff();
-  const int64_t sel = lane < a.k ? a.selected[t * a.k + lane] : -1;
+  const RouteLayout lay{L, a.E, 0, tl};
+  float* row = rows + (wave * kTok + lane / L) * (L * V);
+  const int64_t sel = on && tl < a.k ? a.selected[t * a.k + tl] : -1;
   const bool live = sel >= 0 && sel < a.E;
-  const float g = live ? a.scale * a.dweights[t * a.k + lane] : 0.0f;
-  const float l = live ? a.picked[t * a.k + lane] : ninf;
-  float mine = 0.0f;
+  const float g = live ? a.scale * a.dweights[t * a.k + tl] : 0.0f;
+  const float le = live ? a.picked[t * a.k + tl] : ninf;
   const bool dense = a.score == kSoftmax && !a.renorm;
-  if (a.renorm) {
-    const float x = a.score == kSoftmax ? l : (l < 0.0f || l != l ? l : 0.0f);
-    const float mx = (float)wave_max_nan_f64(live ? x : ninf);
-    float q = live ? expf(x - mx) : 0.0f;
-    const float en = expf(-fabsf(l));
-    if (a.score == kSigmoid && live) q /= 1.0f + en;
-    const float sum = wave_sum_f32(q);
-    const float w = live ? q / sum : 0.0f;
-    const float dot = wave_sum_f32(g * w);
-    mine = w * (g - dot);
-    // 1 - sigmoid(l)
-    if (a.score == kSigmoid) mine *= (l > 0.0f ? en : 1.0f) / (1.0f + en);
-  } else if (a.score == kSigmoid) {
-    const float en = expf(-fabsf(l)), r = 1.0f / (1.0f + en);
-    mine = g * en * r * r;
-  }
-  if (!dense || !__any(live)) {
-    for (int e = lane; e < a.E; e += 64) d[e] = 0.0f;
-    __builtin_amdgcn_wave_barrier();
-    if (live && !dense) d[sel] = mine;
-  } else {
-    float m = ninf;
-    bool bad = false;
-    for (int e = lane; e < a.E; e += 64) {
-      const float x = load_as_f32(a.logits, a.dtype, t * a.ld + e);
-      m = fmaxf(m, x);
-      bad |= x != x;
+  float mine, d[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) d[j] = 0.0f;
+  if (dense) {
+    float l[V], m = ninf, z = 0.0f;
+    load_logits<V>(l, a.logits, a.dtype, vec_in, t * a.ld, lay, on);
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = fmaxf(m, l[j]);
+    m = lanes_max<L>(m);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      l[j] = l[j] == ninf ? 0.0f : exp_fast(l[j] - m);
+      z += l[j];
     }
-    m = __any(bad) ? __builtin_nanf("") : wave_max(m);
-    float z = 0.0f;
-    for (int e = lane; e < a.E; e += 64) z += expf(load_as_f32(a.logits, a.dtype, t * a.ld + e) - m);
-    z = wave_sum_f32(z);
-    const float p = live ? expf(l - m) / z : 0.0f;
-    const float dot = wave_sum_f32(g * p);
-    for (int e = lane; e < a.E; e += 64) d[e] = -dot * (expf(load_as_f32(a.logits, a.dtype, t * a.ld + e) - m) / z);
-    __builtin_amdgcn_wave_barrier();
-    if (live) d[sel] += g * p;
+    z = lanes_sum<L>(z);
+    const float some = lanes_max<L>(live ? 1.0f : 0.0f);
+    const float p = live ? exp_fast(le - m) / z : 0.0f;
+    mine = g * p;
+    const float dot = lanes_sum<L>(mine), f = -dot / z;
+#pragma unroll
+    for (int j = 0; j < V; ++j) d[j] = some > 0.0f ? f * l[j] : 0.0f;
+  } else {
+    const float en = exp_fast(-fabsf(le)), r = 1.0f / (1.0f + en);
+    if (a.renorm) {
+      const float x = a.score == kSoftmax ? le : fminf(le, 0.0f);
+      const float top = lanes_max<L>(x);
+      float q = live ? exp_fast(x - top) : 0.0f;
+      if (a.score == kSigmoid) q *= r;
+      const float w = q / lanes_sum<L>(q);
+      const float share = live ? w : 0.0f;
+      mine = share * (g - lanes_sum<L>(g * share));
+      if (a.score == kSigmoid) mine *= (le > 0.0f ? en : 1.0f) * r;  // 1 - sigmoid
+    } else {
+      mine = g * en * r * r;
+    }
   }
+#pragma unroll
+  for (int c = 0; c < V / 4; ++c)
+    *reinterpret_cast<floatx4*>(row + lay.member(c)) = floatx4{d[4 * c], d[4 * c + 1], d[4 * c + 2], d[4 * c + 3]};
   __builtin_amdgcn_wave_barrier();
-  for (int e = lane; e < a.E; e += 64) store_f32_as(a.dlogits, a.dtype, t * a.E + e, d[e]);
+  if (live) row[sel] += mine;  // each expert at most once in a token
+  __builtin_amdgcn_wave_barrier();
+  if (!on) return;
+#pragma unroll
+  for (int c = 0; c < V / 4; ++c) {
+    const int mem = lay.member(c);
+    if (mem >= a.E) continue;
+    const floatx4 v = *reinterpret_cast<const floatx4*>(row + mem);
+    const int64_t at = t * a.E + mem;
+    if (vec_out && a.dtype == kF32) {
+      *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(a.dlogits) + at) = v;
+    } else if (vec_out) {
+      const intx2 o = a.dtype == kBf16 ? intx2{(int)pack2_bf16(v[0], v[1]), (int)pack2_bf16(v[2], v[3])}
+                                       : intx2{(int)(f32_to_half_bits(v[0]) | f32_to_half_bits(v[1]) << 16),
+                                               (int)(f32_to_half_bits(v[2]) | f32_to_half_bits(v[3]) << 16)};
+      *reinterpret_cast<intx2*>(reinterpret_cast<uint16_t*>(a.dlogits) + at) = o;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (mem + i < a.E) store_f32_as(a.dlogits, a.dtype, at + i, v[i]);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -879,37 +910,50 @@ RouteShape route_shape(int64_t E, int64_t groups, int64_t k) {
 }
 
 template <int L, int V>
-void route_launch_lv(const RouteArgs& a, const RouteShape& sh, bool vec, int idx_bits, hipStream_t st) {
+void route_run(const RouteArgs& a, const RouteShape& sh, hipStream_t st) {
+  int idx_bits = 0;
+  while ((1 << idx_bits) < a.E) ++idx_bits;
+  const uintptr_t unit = a.dtype == kF32 ? 16 : 8;  // four logits
+  const bool vec = (a.E / a.groups) % 4 == 0 && (a.ld % 4 == 0 || a.T == 1) && (uintptr_t)a.logits % unit == 0;
   const int64_t per = 4 * (64 / L);  // tokens of a work-group
   const dim3 grid((unsigned)((a.T + per - 1) / per));
   const size_t lds = 4 * (size_t)a.E * 8;
   if (a.bias) hipLaunchKernelGGL((moe_route_kernel<L, V, true>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec);
   else hipLaunchKernelGGL((moe_route_kernel<L, V, false>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec);
 }
-template <int L>
-void route_launch_l(const RouteArgs& a, const RouteShape& sh, bool vec, int idx_bits, hipStream_t st) {
-  if (sh.V == 4) route_launch_lv<L, 4>(a, sh, vec, idx_bits, st);
-  else if (sh.V == 8) route_launch_lv<L, 8>(a, sh, vec, idx_bits, st);
-  else route_launch_lv<L, 16>(a, sh, vec, idx_bits, st);
+template <int L, int V>
+void route_run(const RouteBwdArgs& a, const RouteShape&, hipStream_t st) {
+  const uintptr_t unit = a.dtype == kF32 ? 16 : 8;
+  const bool vec_in = a.E % 4 == 0 && (a.ld % 4 == 0 || a.T == 1) && (uintptr_t)a.logits % unit == 0;
+  const bool vec_out = a.E % 4 == 0 && (uintptr_t)a.dlogits % unit == 0;
+  const int64_t per = 4 * (64 / L);
+  hipLaunchKernelGGL((moe_route_bwd_kernel<L, V>), dim3((unsigned)((a.T + per - 1) / per)), dim3(256), 0, st, a, vec_in,
+                     vec_out);
+}
+template <int L, class Args>
+void route_run_l(const Args& a, const RouteShape& sh, hipStream_t st) {
+  if (sh.V == 4) route_run<L, 4>(a, sh, st);
+  else if (sh.V == 8) route_run<L, 8>(a, sh, st);
+  else route_run<L, 16>(a, sh, st);
+}
+template <class Args>
+void route_by_shape(const Args& a, const RouteShape& sh, hipStream_t st) {
+  switch (sh.L) {
+    case 1: return route_run_l<1>(a, sh, st);
+    case 2: return route_run_l<2>(a, sh, st);
+    case 4: return route_run_l<4>(a, sh, st);
+    case 8: return route_run_l<8>(a, sh, st);
+    case 16: return route_run_l<16>(a, sh, st);
+    case 32: return route_run_l<32>(a, sh, st);
+    default: return route_run_l<64>(a, sh, st);
+  }
 }
 void route_launch(const RouteArgs& a, hipStream_t st) {
   const RouteShape sh = route_shape(a.E, a.groups, a.k);
-  int idx_bits = 0;
-  while ((1 << idx_bits) < a.E) ++idx_bits;
-  const uintptr_t unit = a.dtype == kF32 ? 16 : 8;  // four logits
-  const bool vec = (a.E / a.groups) % 4 == 0 && (a.ld % 4 == 0 || a.T == 1) && (uintptr_t)a.logits % unit == 0;
-  switch (sh.L) {
-    case 1: return route_launch_l<1>(a, sh, vec, idx_bits, st);
-    case 2: return route_launch_l<2>(a, sh, vec, idx_bits, st);
-    case 4: return route_launch_l<4>(a, sh, vec, idx_bits, st);
-    case 8: return route_launch_l<8>(a, sh, vec, idx_bits, st);
-    case 16: return route_launch_l<16>(a, sh, vec, idx_bits, st);
-    case 32: return route_launch_l<32>(a, sh, vec, idx_bits, st);
-    default:
-      if (sh.V == 32) return route_launch_lv<64, 32>(a, sh, vec, idx_bits, st);
-      return route_launch_l<64>(a, sh, vec, idx_bits, st);
-  }
+  if (sh.V == 32) return route_run<64, 32>(a, sh, st);
+  route_by_shape(a, sh, st);
 }
+void route_bwd_launch(const RouteBwdArgs& a, hipStream_t st) { route_by_shape(a, route_shape(a.E, 1, a.k), st); }
 
 template <int DT, bool VEC>
 struct Combine {
@@ -962,8 +1006,7 @@ int sfp8_moe_route_bwd(const float* dweights, const int64_t* selected, const flo
   if (T == 0) return kOk;
   const RouteBwdArgs a{dweights, selected, picked, logits, dtype, T, ld, (int)E, (int)top_k, score, renorm, scale,
                        dlogits};
-  hipLaunchKernelGGL(moe_route_bwd_kernel, dim3((unsigned)((T + 3) / 4)), dim3(256), 4 * (size_t)E * 4,
-                     (hipStream_t)stream, a);
+  route_bwd_launch(a, (hipStream_t)stream);
   return route_status();
 }
 

@@ -25,6 +25,8 @@ _NATIVE = ("norm_quant", "block_weight_quant", "weight_quant_experts", "gateup_s
 # those around the experts and between the backward pass and the optimizer
 _NATIVE_STEP = ("moe_route", "moe_route_bwd", "moe_expert_order", "moe_combine", "moe_combine_bwd", "grad_norm",
                 "clip_grads")
+# differentiable as they are: the eager calls of routing.py
+_NATIVE_AUTOGRAD = ("route_tokens", "combine_experts")
 
 
 def _missing(name: str, why: str):
@@ -38,9 +40,9 @@ def _missing(name: str, why: str):
 try:
     from . import _native
 except ImportError as _e:
-    globals().update({_n: _missing(_n, str(_e)) for _n in _NATIVE + _NATIVE_STEP})
+    globals().update({_n: _missing(_n, str(_e)) for _n in _NATIVE + _NATIVE_STEP + _NATIVE_AUTOGRAD})
 else:
-    globals().update({_n: getattr(_native, _n) for _n in _NATIVE + _NATIVE_STEP})
+    globals().update({_n: getattr(_native, _n) for _n in _NATIVE + _NATIVE_STEP + _NATIVE_AUTOGRAD})
 
 E4M3 = torch.float8_e4m3fn
 E5M2 = torch.float8_e5m2

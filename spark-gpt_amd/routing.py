@@ -20,12 +20,14 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import ops
 from . import torch_ops  # the sparkfp8:: operators and their implementations
 from .moe import _FP8Experts
 
 
 class _RouteTokens(torch.autograd.Function):
-    """(weights, selected) of ``route_tokens``; the selection has no gradient."""
+    """(weights, selected) of ``route_tokens`` in a compiled graph (an eager call
+    makes the same node in C++); the selection has no gradient."""
 
     @staticmethod
     def forward(ctx, logits, bias, mask, score, groups, top_groups, group_best, top_k, renormalize, scale):
@@ -70,8 +72,9 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bi
     Equal order values go to the lowest index; an expert whose logit (or order
     value) is -inf is never taken, and NaN ranks first.  Slots that no expert
     is left for, and those of masked tokens, get index -1 and weight 0."""
-    return _RouteTokens.apply(logits, bias, mask, score, groups, groups if top_groups is None else top_groups,
-                              group_best, top_k, renormalize, float(scale))
+    apply = _RouteTokens.apply if torch.compiler.is_compiling() else ops.route_tokens
+    return apply(logits, bias, mask, score, groups, groups if top_groups is None else top_groups, group_best, top_k,
+                 renormalize, float(scale))
 
 
 def expert_order(selected: torch.Tensor, num_experts: int):
@@ -85,7 +88,7 @@ def expert_order(selected: torch.Tensor, num_experts: int):
 
 
 class _CombineExperts(torch.autograd.Function):
-    """The weighted top-k sum of ``combine_experts``."""
+    """The weighted top-k sum of ``combine_experts`` in a compiled graph."""
 
     @staticmethod
     def forward(ctx, rows, weights, inverse_permutation, offsets):
@@ -108,7 +111,9 @@ def combine_experts(rows: torch.Tensor, weights: torch.Tensor, inverse_permutati
     sum is taken in 32 bits in slot order and rounded once; slots without a row
     add nothing.  In the backward pass rows that no slot names get zeros; a row
     that two slots name (``expert_order`` gives no such) is not supported."""
-    return _CombineExperts.apply(rows, weights.float(), inverse_permutation, offsets)
+    if torch.compiler.is_compiling():
+        return _CombineExperts.apply(rows, weights.float(), inverse_permutation, offsets)
+    return ops.combine_experts(rows, weights, inverse_permutation, offsets)
 
 
 def fp8_routed_experts(x: torch.Tensor, logits: torch.Tensor, experts, top_k: int, **route):
