@@ -191,9 +191,10 @@ SFP8_DEV uint64_t wave_max_u64(uint64_t x) {
 // The selection by the definition, in 64 bits, of one token by a whole wave:
 // for rows that hold NaN or +inf and for those whose order 32 bits do not
 // settle.  Returns the expert of slot `lane`, or -1.  v[e] (LDS) is the order
-// value of expert e as rank_bits, 0 where it cannot be taken (any more).  One
-// exponential and one quotient in the code, which is seldom run and so comes
-// from memory: its length counts for as much as its steps.
+// value of expert e as rank_bits, 0 where it cannot be taken (any more); the
+// row's logits follow it.  The code is seldom run and so comes from memory: its
+// length counts for more than its steps, hence one exponential, one quotient
+// and few unrolled loops.
 // ---------------------------------------------------------------------------
 SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
   const int lane = threadIdx.x & 63;
@@ -201,42 +202,55 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
   const int64_t row = t * a.ld;
   const bool softmax = a.score == kSoftmax;
   const bool two_best = a.groups > 1 && a.group_best == 2;
-  const bool scores = a.bias || two_best;
-  if (scores) {
-    double m = 0.0, z = 0.0;
-    if (softmax) {
-      m = ninf;
-      for (int e = lane; e < a.E; e += 64) {
-        const double l = load_as_f32(a.logits, a.dtype, row + e);
-        m = ranks_above(l, m) ? l : m;
-      }
-      m = wave_max_nan_f64(m);
+  float* l = reinterpret_cast<float*>(v + a.E);  // the row
+  double m = ninf;
+#pragma unroll 1
+  for (int e0 = lane; e0 < a.E; e0 += 256) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = e0 + 64 * i < a.E ? load_as_f32(a.logits, a.dtype, row + e0 + 64 * i) : -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (e0 + 64 * i < a.E) l[e0 + 64 * i] = x[i];
+      m = ranks_above(x[i], m) ? (double)x[i] : m;
     }
+  }
+  const bool scores = a.bias || two_best;
+  if (scores) {  // which d holds until they are ranked
+    m = wave_max_nan_f64(m);
+    double z = 0.0;
     double* d = reinterpret_cast<double*>(v);
+#pragma unroll 1
     for (int e = lane; e < a.E; e += 64) {
-      const double l = load_as_f32(a.logits, a.dtype, row + e);
-      const double x = exp(softmax ? l - m : -l);
+      const double x = exp(softmax ? l[e] - m : -(double)l[e]);
       z += x;
       d[e] = x;
     }
-    z = softmax ? wave_sum_f64(z) : 0.0;
+    z = wave_sum_f64(z);
+#pragma unroll 1
     for (int e = lane; e < a.E; e += 64) {
-      const double l = load_as_f32(a.logits, a.dtype, row + e);
-      const double s = (softmax ? d[e] : 1.0) / (softmax ? z : 1.0 + d[e]);
-      v[e] = l == ninf ? 0ull : rank_bits(a.bias ? s + (double)a.bias[e] : s);
+      const double x = (softmax ? d[e] : 1.0) / (softmax ? z : 1.0 + d[e]);
+      v[e] = l[e] == -__builtin_inff() ? 0ull : rank_bits(a.bias ? x + (double)a.bias[e] : x);
     }
   } else {
-    for (int e = lane; e < a.E; e += 64) v[e] = rank_bits((double)load_as_f32(a.logits, a.dtype, row + e));
+#pragma unroll 1
+    for (int e = lane; e < a.E; e += 64) v[e] = rank_bits(l[e]);
   }
   __builtin_amdgcn_wave_barrier();
   if (a.groups > 1) {
     const int gs = a.E / a.groups;
     uint64_t b1 = 0, b2 = 0;  // the best two of group `lane`
     if (lane < a.groups) {
-      for (int e = lane * gs; e < lane * gs + gs; ++e) {
-        const uint64_t x = v[e];
-        b2 = x > b1 ? b1 : x > b2 ? x : b2;
-        b1 = x > b1 ? x : b1;
+#pragma unroll 1
+      for (int e0 = 0; e0 < gs; e0 += 4) {
+        uint64_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = e0 + i < gs ? v[lane * gs + e0 + i] : 0ull;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          b2 = x[i] > b1 ? b1 : x[i] > b2 ? x[i] : b2;
+          b1 = x[i] > b1 ? x[i] : b1;
+        }
       }
     }
     uint64_t g = b1;
@@ -247,26 +261,34 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
       g = rank_bits(value(b1) + value(b2));
     }
     int rank = 0;
+#pragma unroll 1
     for (int j = 0; j < a.groups; ++j) {
-      const uint64_t o = (uint64_t)__shfl((unsigned long long)g, j, 64);
+      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(g >> 32), j) << 32 |
+                         (uint32_t)__builtin_amdgcn_readlane((int)g, j);
       rank += o > g || (o == g && j < lane);
     }
     const uint64_t keep = __ballot(lane < a.groups && g && rank < a.top_groups);
     __builtin_amdgcn_wave_barrier();
-    for (int e = lane; e < a.E; e += 64) {
-      const uint64_t x = a.bias || !two_best ? v[e] : rank_bits((double)load_as_f32(a.logits, a.dtype, row + e));
-      v[e] = keep >> (e / gs) & 1 ? x : 0ull;
-    }
+    const bool again = two_best && !a.bias;  // the order is that of the logits
+#pragma unroll 1
+    for (int e = lane; e < a.E; e += 64) v[e] = keep >> (e / gs) & 1 ? (again ? rank_bits(l[e]) : v[e]) : 0ull;
     __builtin_amdgcn_wave_barrier();
   }
   int mine = -1;
+#pragma unroll 1
   for (int s = 0; s < a.k; ++s) {
     uint64_t best = 0;
     int at = a.E;
-    for (int e = lane; e < a.E; e += 64) {
-      const uint64_t x = v[e];
-      at = x > best ? e : at;
-      best = x > best ? x : best;
+#pragma unroll 1
+    for (int e0 = lane; e0 < a.E; e0 += 256) {
+      uint64_t x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = e0 + 64 * i < a.E ? v[e0 + 64 * i] : 0ull;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        at = x[i] > best ? e0 + 64 * i : at;
+        best = x[i] > best ? x[i] : best;
+      }
     }
     const uint64_t m = wave_max_u64(best);
     if (m == 0) break;
@@ -280,25 +302,28 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
 }
 
 // ---------------------------------------------------------------------------
-// Routing, L lanes a token, V values a lane, 64 / L tokens a wave at a time.
+// Routing, L lanes a token, V values a lane, 64 / L tokens a wave.
 //
-// The order.  Each expert gets a key of 31 bits, its order value above its
-// inverted index, so that keys differ and the larger key comes first; 0 where
-// it cannot be taken.  16-bit logits without a bias fit whole, with their bits
-// in the order of their values.  Others are put on a fixed-point scale of up to 24 bits
-// between the row's smallest and largest value: the steps to it (a
-// difference, a product, a truncation) keep the order, so keys that differ
-// there are in the order of the 32-bit values.  The next key below m is
-// max(key - m) + m in wrapping arithmetic (keys below m wrap to 2^31 and
-// above, those from m on stay below), one subtraction and half a max3 for each
-// value and log2(L) lane steps, with nothing to clear.
+// The order.  Each expert gets a key of 31 bits, a rank of 21 to 23 bits above
+// its inverted index, so that keys differ and the larger key comes first.
+// 16-bit logits without a bias have the order of their own bits as the rank.
+// Others are put on a fixed-point scale between a low value and the row's
+// largest: rank = 1 + (value - low) * scale, with the mantissa of a number
+// from 2^23 on as the integer; what is below low has rank 0 and is not taken.  Each
+// step to it keeps the order, so ranks that differ are in the order of the
+// 32-bit values.  Without groups and with more lanes than slots the low value
+// is the smallest of the lanes' largest: L values are no smaller, so the
+// top_k + 1 first are among them.  The next key below `top` is max(key - top)
+// + top in wrapping arithmetic (keys below top wrap to 2^31 and above, those
+// from top on stay below), a subtraction and half a max3 for each value and
+// log2(L) lane steps, with nothing to clear.
 //
-// Its limits.  Where two neighbours of the k + 1 first are closer than their
-// 32-bit errors, or two groups are at the border of those kept, the token is
-// done again by the definition in 64 bits (route_exact), as are rows with NaN
-// or +inf.  Without a bias that is where two logits fall on one step of the
-// scale and differ (equal ones are in the order of their indices): 3 of 10^4
-// tokens at 256 normal logits.  With one, scores are off: a softmax by at most
+// Its limits.  Where two neighbours of the top_k + 1 first are closer than
+// their errors, or two groups are at the border of those kept, the token is
+// selected again by the definition in 64 bits (route_exact), as are rows with
+// NaN or +inf.  Without a bias that takes two logits that differ on one step of the
+// scale (equal ones are in the order of their indices): about 1 of 10^4 tokens
+// at 256 normal logits.  With one, scores are off: a softmax by at most
 // (2.5 |d| + 30) 2^-24 of itself, below 2^-19 in all (d is the exponent's
 // argument, |d| e^-|d| < 0.4), a sigmoid, which has no sum over the experts, by
 // at most 2^-21; the sums with the bias round once more.
@@ -306,72 +331,68 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
 // A token's result depends on its row and on E, top_k and the groups alone,
 // not on the batch it comes in.
 // ---------------------------------------------------------------------------
+template <int V>
+SFP8_DEV float max_nan(const float (&x)[V]) {
+  float m = x[0];
+#pragma unroll
+  for (int j = 1; j + 1 < V; j += 2) m = max3_nan(m, x[j], x[j + 1]);
+  return V % 2 ? m : __builtin_elementwise_maximum(m, x[V - 1]);
+}
+
+// sigmoid(x) without its sum's cancellation: e^x / (1 + e^x) below 0.
+SFP8_DEV float sigmoid_of(float x) {
+  const float en = exp_fast(-fabsf(x));
+  return (x > 0.0f ? 1.0f : en) * __builtin_amdgcn_rcpf(1.0f + en);
+}
+
 template <int L, int V, bool BIAS>
-__global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, int G, int idx_bits, bool vec) {
+__global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, int G, int idx_bits, bool vec,
+                                                           bool vec_bias) {
   extern __shared__ __align__(16) uint64_t lds[];
   constexpr int kTok = 64 / L;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int tl = lane & (L - 1);  // lane of the token
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tl = lane & (L - 1), tok = lane / L;  // lane of the token, token of the wave
   const RouteLayout lay{G, a.E / a.groups, tl / G, tl % G};
   const bool in_group = lay.g < a.groups;
   const float ninf = -__builtin_inff();
-  const uint32_t idx_mask = (1u << idx_bits) - 1;
-  const bool half16 = !BIAS && a.dtype != kF32;  // keys hold the whole logit
+  const bool half16 = !BIAS && a.dtype != kF32;  // ranks hold the whole logit
   const bool softmax = a.score == kSoftmax;
   const bool two_best = a.groups > 1 && a.group_best == 2;
   const bool scores = BIAS || !a.renorm || two_best;  // scores of all experts, not of the chosen alone
   const int first = lay.g * lay.gs;                   // the group's first expert
   const int64_t t0 = ((int64_t)blockIdx.x * 4 + wave) * kTok;
   if (t0 >= a.T) return;
-  const int64_t t = t0 + lane / L;
-  const bool on = t < a.T && !(a.mask && !a.mask[t]);
+  const bool on = t0 + tok < a.T && !(a.mask && !a.mask[t0 + tok]);
+  const int64_t row = t0 * a.ld + tok * a.ld;
   float l[V];
-  load_logits<V>(l, a.logits, a.dtype, vec, t * a.ld + first, lay, on && in_group);
-  bool odd = false;  // done again in 64 bits
-  float m = ninf;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    l[j] += 0.0f;  // -0 is 0
-    odd |= !(l[j] < __builtin_inff());
-    m = fmaxf(m, l[j]);
-  }
-  float z = 1.0f;
+  load_logits<V>(l, a.logits, a.dtype, vec, row + first, lay, on && in_group);
+  float mine_max = max_nan<V>(l);             // NaN if one is
+  bool odd = !(mine_max < __builtin_inff());  // selected again in 64 bits
+  float m = ninf, z = 1.0f;
   if (softmax && scores) {
-    m = lanes_max<L>(m);
+    m = lanes_max<L>(mine_max);
     z = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) z += l[j] == ninf ? 0.0f : exp_fast(l[j] - m);
     z = lanes_sum<L>(z);
   }
   // the order values
-  float o[V], bias[V];
+  float o[V];
+  const float err = !BIAS ? 0.0f : softmax ? 0x1p-19f : 0x1p-21f;  // how far a score may be off
   if constexpr (BIAS) {
+    const float rz = __builtin_amdgcn_rcpf(z);
+    float bias[V];
+    load_logits<V>(bias, a.bias, kF32, vec_bias, first, lay, in_group);
 #pragma unroll
     for (int c = 0; c < V / 4; ++c)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int mem = lay.member(c) + i;
-        bias[4 * c + i] = in_group && mem < lay.gs ? a.bias[first + mem] : 0.0f;
+        const int j = 4 * c + i;
+        const float sc = softmax ? exp_fast(l[j] - m) * rz : sigmoid_of(l[j]);
+        o[j] = l[j] == ninf ? ninf : sc + bias[j];
       }
-  }
-  float err = 0.0f;  // how far one may be off
-  if constexpr (BIAS) {
-    const float rz = 1.0f / z;
-    float big = 0.0f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float sc;
-      if (softmax) {
-        sc = exp_fast(l[j] - m) * rz;
-      } else {
-        const float en = exp_fast(-fabsf(l[j]));
-        sc = (l[j] > 0.0f ? 1.0f : en) * __builtin_amdgcn_rcpf(1.0f + en);
-      }
-      o[j] = l[j] == ninf ? ninf : sc + bias[j];
-      odd |= !(o[j] < __builtin_inff());
-      big = o[j] == ninf ? big : fmaxf(big, fabsf(o[j]));
-    }
-    err = (softmax ? 0x1p-19f : 0x1p-21f) + 0x1p-24f * lanes_max<L>(big);
+    mine_max = max_nan<V>(o);
+    odd |= !(mine_max < __builtin_inff());
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = l[j];
@@ -382,7 +403,7 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
     float b1 = ninf, b2 = ninf;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      b2 = fmaxf(b2, fminf(b1, o[j]));
+      b2 = __builtin_amdgcn_fmed3f(b1, b2, o[j]);
       b1 = fmaxf(b1, o[j]);
     }
     const auto merge = [&](float p1, float q1, float p2, float q2) {
@@ -402,20 +423,19 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
       if (G > 16) share_f<16>(b1, p1, q1), share_f<16>(b2, p2, q2), merge(p1, q1, p2, q2);
     if constexpr (L > 32)
       if (G > 32) share_f<32>(b1, p1, q1), share_f<32>(b2, p2, q2), merge(p1, q1, p2, q2);
-    float val = b1, tol = 2.0f * err;
+    float val = b1, tol = 0.0f;  // tol: how far two groups' values may be off together
+    if constexpr (BIAS) {
+      const float big = lanes_max<L>(b1 == ninf ? 0.0f : fmaxf(fabsf(b1), b2 == ninf ? 0.0f : fabsf(b2)));
+      tol = (two_best ? 4.0f : 2.0f) * (err + 0x1p-23f * big);
+    }
     if (two_best && b1 != ninf) {
       if constexpr (!BIAS) {
-        const auto part = [&](float x) {
-          if (softmax) return exp_fast(x - m);  // z is the same for all
-          const float en = exp_fast(-fabsf(x));
-          return (x > 0.0f ? 1.0f : en) * __builtin_amdgcn_rcpf(1.0f + en);
-        };
-        b1 = part(b1);
-        b2 = b2 == ninf ? ninf : part(b2);
+        b1 = softmax ? exp_fast(b1 - m) : sigmoid_of(b1);  // z is the same for all
+        b2 = b2 == ninf ? ninf : softmax ? exp_fast(b2 - m) : sigmoid_of(b2);
       }
       val = b1 + (b2 == ninf ? 0.0f : b2);
       // of scores: (2.5 |d| + 8) 2^-24 of each, |d| < 104 (below, they vanish)
-      tol = BIAS ? 4.0f * err + 0x1p-22f * fabsf(val) : 0x1p-14f * val + 0x1p-120f;
+      if constexpr (!BIAS) tol = 0x1p-14f * val + 0x1p-120f;
     }
     int rank = 0, over = 0, near = 0;
     for (int j = 1; j < L / G; ++j) {
@@ -428,49 +448,56 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
     kept = in_group && val != ninf && rank < a.top_groups;
     odd |= tol > 0.0f && val != ninf && over < a.top_groups && near >= a.top_groups;
   }
-  // the keys
-  uint32_t key[V];
-  float gap = 0.0f;  // keys that are no further apart on the scale may be in the wrong order
+  // the keys: rank << idx_bits, and the inverted index
+  const uint32_t idx_mask = (1u << idx_bits) - 1, idx_top = idx_mask - (uint32_t)first;
+  uint32_t key[V], least;  // keys from `least` on can be taken
+  float gap = 0.0f;        // ranks that are no further apart may be in the wrong order
   if (half16) {
+    const bool bf16 = a.dtype == kBf16;
+    least = (bf16 ? 0x80u : 0x400u) << idx_bits;  // above -inf
+    const uint32_t keep = kept ? ~idx_mask : 0u;
+    const int down = 16 - idx_bits;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int32_t b = a.dtype == kBf16 ? (int32_t)__float_as_uint(o[j]) >> 16
-                                         : (int32_t)(int16_t)f32_to_half_bits(o[j]);
-      const uint32_t ord = (uint32_t)(b ^ (b < 0 ? 0xffff : 0x8000)) & 0xffffu;
-      key[j] = o[j] == ninf ? 0u : ord << idx_bits;
-    }
+    for (int c = 0; c < V / 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = l[4 * c + i] + 0.0f;  // -0 is 0
+        const uint32_t b = bf16 ? __float_as_uint(x) : f32_to_half_bits(x) << 16;
+        const uint32_t ord = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+        key[4 * c + i] = (ord >> down & keep) | (idx_top - (uint32_t)(lay.member(c) + i));
+      }
   } else {
-    float lo = __builtin_inff(), hi = ninf;
+    least = 1u << idx_bits;
+    float lo;
+    if (a.groups == 1 && L > a.k) lo = lanes_min<L>(mine_max);
+    else lo = ninf;
+    if (__any(lo == ninf)) {  // a lane without an expert, a group that is out: the row's smallest
+      float least_o = __builtin_inff();
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      lo = fminf(lo, o[j] == ninf ? lo : o[j]);
-      hi = fmaxf(hi, o[j]);
+      for (int j = 0; j < V; ++j) least_o = fminf(least_o, o[j] == ninf ? least_o : o[j]);
+      lo = lanes_min<L>(least_o);
     }
-    lo = lanes_min<L>(lo);
-    hi = lanes_max<L>(hi);
-    const int bits = 31 - idx_bits < 24 ? 31 - idx_bits : 24;
+    const float hi = lanes_max<L>(mine_max);
     const float range = hi - lo;
-    const float scale = range > 0.0f ? ((float)(1u << bits) - 4.0f) / range : 0.0f;
+    // below 2^(31 - idx_bits) at the largest value, by two steps and the quotient's 2^-22
+    const float steps = (float)(1u << (31 - idx_bits)) * (1.0f - 0x1p-19f) - 4.0f;
+    const float scale = kept && range > 0.0f ? steps * __builtin_amdgcn_rcpf(range) : 0.0f;
+    const float base = kept ? 0x1p23f + 1.0f : 0x1p23f;
     // a range outside 2^+-100 is left to 64 bits
     odd |= range > 0.0f && !(range > 0x1p-100f && range < 0x1p100f);
-    gap = BIAS ? 2.0f * err * scale + 3.0f : 0.0f;  // the scale's own roundings: 3
+    // a value's error, and three steps for the scale's own roundings
+    if constexpr (BIAS) gap = 2.0f * (err + 0x1p-23f * fmaxf(fabsf(lo), fabsf(hi))) * lanes_max<L>(scale) + 3.0f;
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      key[j] = o[j] == ninf ? 0u
-                            : ((uint32_t)__builtin_amdgcn_fmed3f((o[j] - lo) * scale, 0.0f, 0x1p24f) + 1u) << idx_bits;
+    for (int c = 0; c < V / 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = fmaxf(__builtin_fmaf(o[4 * c + i] - lo, scale, base), 0x1p23f);
+        key[4 * c + i] = __float_as_uint(x) << idx_bits | (idx_top - (uint32_t)(lay.member(c) + i));
+      }
   }
-#pragma unroll
-  for (int c = 0; c < V / 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t& x = key[4 * c + i];
-      x = kept && x ? x | (idx_mask - (uint32_t)(first + lay.member(c) + i)) : 0u;
-    }
-  // the first top_k keys, and the one after them
-  uint32_t top = 1u << 31, mine = 0u;
-  bool near = false;  // neighbours no further apart than their errors
-  const int rounds = a.k + (half16 ? 0 : 1);
-  for (int s = 0; s < rounds; ++s) {
+  // the first top_k keys, lane s of the token keeping that of slot s, and the one after them
+  uint32_t top = 1u << 31, mine = 0u, after = 0u;
+  for (int s = 0; s <= a.k; ++s) {
     uint32_t r = 0u;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -478,59 +505,65 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
       r = x > r ? x : r;
     }
     r = reduce_max_u<L>(r);
-    const uint32_t next = r & 0x80000000u ? r + top : 0u;
-    if (!half16 && s > 0 && next) near |= (float)((top >> idx_bits) - (next >> idx_bits)) <= gap;
-    mine = s == tl && s < a.k ? next : mine;
-    top = next;
+    top = r & 0x80000000u ? r + top : 0u;
+    if (s < a.k) mine = s == tl ? top : mine;  // uniform
+    else after = top;
   }
-  int e = mine ? (int)(idx_mask - (mine & idx_mask)) : -1;
-  float le = e >= 0 ? load_as_f32(a.logits, a.dtype, t * a.ld + e) : ninf;
-  if (!half16 && __any(near)) {
-    // Near neighbours with the same logit and bias are equal, and in the order
-    // of their indices: that leaves those that differ, among the chosen or
-    // between the last of them and the rest.
-    const float be = BIAS && e >= 0 ? a.bias[e] : 0.0f;
-    const uint32_t above = __shfl_up(mine, 1, 64);
-    const float la = __shfl_up(le, 1, 64), ba = __shfl_up(be, 1, 64);
-    odd |= tl > 0 && e >= 0 && (float)((above >> idx_bits) - (mine >> idx_bits)) <= gap && !(la == le && ba == be);
-    const int from = (lane & ~(L - 1)) + a.k - 1;
-    const uint32_t last = __shfl(mine, from, 64);
-    const float ll = __shfl(le, from, 64), bl = __shfl(be, from, 64);
+  int e = mine >= least ? (int)(idx_mask - (mine & idx_mask)) : -1;
+  float le = e >= 0 ? load_as_f32(a.logits, a.dtype, row + e) : ninf;
+  if (!half16) {
+    const uint32_t up = __shfl_up(mine, 1, 64);
+    const uint32_t last = __shfl(mine, (lane & ~(L - 1)) + a.k - 1, 64);
+    const auto close = [&](uint32_t x, uint32_t y) {  // x comes first
+      return y >= least && (float)((x >> idx_bits) - (y >> idx_bits)) <= gap;
+    };
+    if (__any((tl > 0 && tl < a.k && close(up, mine)) || close(last, after))) {
+      // Near neighbours with the same logit and bias are equal, and in the order
+      // of their indices: that leaves those that differ, among the chosen or
+      // between the last of them and the rest.
+      const float be = BIAS && e >= 0 ? a.bias[e] : 0.0f;
+      const float la = __shfl_up(le, 1, 64), ba = __shfl_up(be, 1, 64);
+      odd |= tl > 0 && e >= 0 && close(up, mine) && !(la == le && ba == be);
+      const int from = (lane & ~(L - 1)) + a.k - 1;
+      const float ll = __shfl(le, from, 64), bl = __shfl(be, from, 64);
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (key[j] && key[j] < last && (float)((last >> idx_bits) - (key[j] >> idx_bits)) <= gap) {
-        const int x = (int)(idx_mask - (key[j] & idx_mask));
-        odd |= load_as_f32(a.logits, a.dtype, t * a.ld + x) != ll || (BIAS && a.bias[x] != bl);
-      }
+      for (int j = 0; j < V; ++j)
+        if (key[j] < last && close(last, key[j])) {
+          const int x = (int)(idx_mask - (key[j] & idx_mask));
+          odd |= load_as_f32(a.logits, a.dtype, row + x) != ll || (BIAS && a.bias[x] != bl);
+        }
+    }
   }
   const uint64_t any_odd = __ballot(odd && on);
   if (any_odd) {  // wave uniform
     for (int i = 0; i < kTok; ++i) {
       if (!(any_odd >> (i * L) & (L == 64 ? ~0ull : (1ull << L) - 1))) continue;
-      const int again = __shfl(route_exact(a, t0 + i, lds + wave * a.E), tl, 64);
-      if (lane / L == i) {
+      const int again = __shfl(route_exact(a, t0 + i, lds + wave * ((3 * a.E + 1) / 2)), tl, 64);
+      if (tok == i) {
         e = tl < a.k ? again : -1;
-        le = e >= 0 ? load_as_f32(a.logits, a.dtype, t * a.ld + e) : ninf;
+        le = e >= 0 ? load_as_f32(a.logits, a.dtype, row + e) : ninf;
       }
     }
   }
-  // the weights: lane s of the token has slot s
+  // the weights
   const bool live = e >= 0;
   float w;
   if (softmax) {
     const float top_l = a.renorm ? lanes_max<L>(le) : m;
     w = live ? exp_fast(le - top_l) : 0.0f;
-    w /= a.renorm ? lanes_sum<L>(w) : z;
+    w *= __builtin_amdgcn_rcpf(a.renorm ? lanes_sum<L>(w) : z);
   } else {
     const float en = exp_fast(-fabsf(le)), low = fminf(le, 0.0f);
     const float top_l = a.renorm ? lanes_max<L>(low) : 0.0f;
-    w = live ? exp_fast(low - top_l) / (1.0f + en) : 0.0f;
-    if (a.renorm) w /= lanes_sum<L>(w);
+    w = live ? exp_fast(low - top_l) * __builtin_amdgcn_rcpf(1.0f + en) : 0.0f;
+    if (a.renorm) w *= __builtin_amdgcn_rcpf(lanes_sum<L>(w));
   }
-  if (t < a.T && tl < a.k) {
-    a.weights[t * a.k + tl] = live ? a.scale * w : 0.0f;
-    a.selected[t * a.k + tl] = e;
-    if (a.picked) a.picked[t * a.k + tl] = live ? le : 0.0f;
+  if (t0 + tok < a.T && tl < a.k) {
+    const int64_t base = t0 * a.k;
+    const int at = tok * a.k + tl;
+    (a.weights + base)[at] = live ? a.scale * w : 0.0f;
+    (a.selected + base)[at] = e;
+    if (a.picked) (a.picked + base)[at] = live ? le : 0.0f;
   }
 }
 
@@ -911,15 +944,18 @@ RouteShape route_shape(int64_t E, int64_t groups, int64_t k) {
 
 template <int L, int V>
 void route_run(const RouteArgs& a, const RouteShape& sh, hipStream_t st) {
-  int idx_bits = 0;
+  int idx_bits = 8;  // at least: a rank's mantissa then leaves its exponent behind (moe_route_kernel)
   while ((1 << idx_bits) < a.E) ++idx_bits;
   const uintptr_t unit = a.dtype == kF32 ? 16 : 8;  // four logits
   const bool vec = (a.E / a.groups) % 4 == 0 && (a.ld % 4 == 0 || a.T == 1) && (uintptr_t)a.logits % unit == 0;
   const int64_t per = 4 * (64 / L);  // tokens of a work-group
   const dim3 grid((unsigned)((a.T + per - 1) / per));
-  const size_t lds = 4 * (size_t)a.E * 8;
-  if (a.bias) hipLaunchKernelGGL((moe_route_kernel<L, V, true>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec);
-  else hipLaunchKernelGGL((moe_route_kernel<L, V, false>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec);
+  const size_t lds = 4 * (size_t)((3 * a.E + 1) / 2) * 8;  // of each wave: an order value and a logit per expert
+  const bool vec_bias = (a.E / a.groups) % 4 == 0 && (uintptr_t)a.bias % 16 == 0;
+  if (a.bias)
+    hipLaunchKernelGGL((moe_route_kernel<L, V, true>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec, vec_bias);
+  else
+    hipLaunchKernelGGL((moe_route_kernel<L, V, false>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec, vec_bias);
 }
 template <int L, int V>
 void route_run(const RouteBwdArgs& a, const RouteShape&, hipStream_t st) {
