@@ -669,7 +669,11 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
 // ---------------------------------------------------------------------------
 // Expert order: a stable counting sort of the R = T * k slots by expert, bin E
 // holding the slots that name none.  A work-group takes `chunk` consecutive
-// slots, wave w of it the w-th sixteenth.
+// slots, wave w of it the w-th sixteenth.  One launch counts each group's bins;
+// in the second every group adds up the counts itself (at most 256 rows of E +
+// 1, from the L2), which is cheaper than a third launch that would scan them.
+// Up to 4096 slots are one group and one launch.  Bound by its launches: the
+// bytes are 24 a slot.
 // ---------------------------------------------------------------------------
 constexpr int kOrderWaves = 16;
 constexpr int kOrderThreads = 64 * kOrderWaves;
@@ -681,6 +685,8 @@ __host__ __device__ inline int64_t order_chunk(int64_t R) {
   const int64_t least = c < 4096 ? 4096 : c;
   return (least + kOrderThreads - 1) / kOrderThreads * kOrderThreads;
 }
+// Bins of a row of counts: E + 1, in whole 16-byte units.
+__host__ __device__ inline int order_stride(int E) { return (E + 4) / 4 * 4; }
 
 SFP8_DEV int order_bin(const int64_t* sel, int64_t i, int E) {
   const int64_t e = sel[i];
@@ -691,28 +697,48 @@ SFP8_DEV int order_bin(const int64_t* sel, int64_t i, int E) {
 __global__ __launch_bounds__(kOrderThreads) void moe_order_count_kernel(const int64_t* __restrict__ sel, int64_t R,
                                                                          int64_t chunk, int E,
                                                                          int* __restrict__ counts) {
-  extern __shared__ int hist[];
-  for (int e = threadIdx.x; e <= E; e += kOrderThreads) hist[e] = 0;
+  extern __shared__ __align__(16) int hist[];
+  const int stride = order_stride(E);
+  for (int e = threadIdx.x; e < stride; e += kOrderThreads) hist[e] = 0;
   __syncthreads();
   const int64_t i0 = (int64_t)blockIdx.x * chunk;
   const int64_t i1 = i0 + chunk < R ? i0 + chunk : R;
+#pragma unroll 4
   for (int64_t i = i0 + threadIdx.x; i < i1; i += kOrderThreads) atomicAdd(&hist[order_bin(sel, i, E)], 1);
   __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += kOrderThreads) counts[(int64_t)blockIdx.x * (E + 1) + e] = hist[e];
+  for (int e = threadIdx.x; e < stride; e += kOrderThreads) counts[(int64_t)blockIdx.x * stride + e] = hist[e];
 }
 
 __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
     const int64_t* __restrict__ sel, int64_t R, int64_t chunk, int k, int E, const int* __restrict__ counts,
     int64_t* __restrict__ token_index, int64_t* __restrict__ inverse, int* __restrict__ offsets) {
-  extern __shared__ int next[];  // [waves][E + 1]: the next row of each bin, per wave
-  __shared__ int part[kOrderWaves + 1];
+  // next[wave][bin]: the next row of each bin, per wave; then, while the counts
+  // are added up, the sums of each part of the work-group
+  extern __shared__ __align__(16) int next[];
+  __shared__ int part[kOrderWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nb = gridDim.x, bins = E + 1;
-  for (int e = threadIdx.x; e < kOrderWaves * bins; e += kOrderThreads) next[e] = 0;
+  const int stride = order_stride(E), cols = stride / 4;
+  const int parts = counts ? kOrderThreads / cols : 0;  // at least 3: 257 columns at most
+  int* sums = next + kOrderWaves * stride;              // [parts][2][stride]: all rows, the rows before this group's
+  for (int e = threadIdx.x; e < kOrderWaves * stride; e += kOrderThreads) next[e] = 0;
+  if (counts && (int)threadIdx.x < parts * cols) {
+    const int p = threadIdx.x / cols, c = threadIdx.x % cols;
+    intx4 total = {0, 0, 0, 0}, before = {0, 0, 0, 0};
+#pragma unroll 8
+    for (int b = p; b < nb; b += parts) {
+      const intx4 x = *reinterpret_cast<const intx4*>(counts + (int64_t)b * stride + 4 * c);
+      total += x;
+      before += b < (int)blockIdx.x ? x : intx4{0, 0, 0, 0};
+    }
+    *reinterpret_cast<intx4*>(sums + (2 * p) * stride + 4 * c) = total;
+    *reinterpret_cast<intx4*>(sums + (2 * p + 1) * stride + 4 * c) = before;
+  }
   __syncthreads();
-  int* mine = next + wave * bins;
+  int* mine = next + wave * stride;
   const int64_t per = chunk / kOrderWaves;
   const int64_t i0 = (int64_t)blockIdx.x * chunk + wave * per;
   const int64_t i1 = i0 + per < R ? i0 + per : R;
+#pragma unroll 4
   for (int64_t i = i0 + lane; i < i1; i += 64) atomicAdd(&mine[order_bin(sel, i, E)], 1);
   __syncthreads();
   // start of each bin: the totals of the bins before it, then this bin's slots of earlier work-groups
@@ -721,13 +747,13 @@ __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
     int total = 0, before = 0;
     if (e < bins) {
       if (counts) {
-        for (int b = 0; b < nb; ++b) {
-          const int c = counts[(int64_t)b * bins + e];
-          before += b < (int)blockIdx.x ? c : 0;
-          total += c;
+        for (int p = 0; p < parts; ++p) {
+          total += sums[(2 * p) * stride + e];
+          before += sums[(2 * p + 1) * stride + e];
         }
       } else {
-        for (int w = 0; w < kOrderWaves; ++w) total += next[w * bins + e];
+#pragma unroll
+        for (int w = 0; w < kOrderWaves; ++w) total += next[w * stride + e];
       }
     }
     int scan = total;  // inclusive over the wave's bins
@@ -739,6 +765,7 @@ __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
     if (lane == 63) part[wave] = scan;
     __syncthreads();
     int base = carry, all = carry;
+#pragma unroll
     for (int w = 0; w < kOrderWaves; ++w) {
       base += w < wave ? part[w] : 0;
       all += part[w];
@@ -748,9 +775,10 @@ __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
     if (e < bins) {
       if (blockIdx.x == 0 && e < E) offsets[e] = base + scan;
       int at = base + scan - total + before;
+#pragma unroll
       for (int w = 0; w < kOrderWaves; ++w) {
-        const int c = next[w * bins + e];
-        next[w * bins + e] = at;
+        const int c = next[w * stride + e];
+        next[w * stride + e] = at;
         at += c;
       }
     }
@@ -773,7 +801,7 @@ __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
     __builtin_amdgcn_wave_barrier();
     if (in) {
       inverse[i] = e < E ? row : -1;
-      token_index[row] = i / k;
+      token_index[row] = (uint32_t)i / (uint32_t)k;  // i < 2^30
     }
   }
 }
@@ -1049,7 +1077,7 @@ int sfp8_moe_route_bwd(const float* dweights, const int64_t* selected, const flo
 int64_t sfp8_moe_expert_order_workspace_ints(int64_t R, int64_t E) {
   if (R < 0 || R > (int64_t)1 << 30 || E <= 0 || E > kRouteMaxExperts) return -1;
   const int64_t chunk = order_chunk(R), nb = (R + chunk - 1) / chunk;
-  return nb > 1 ? nb * (E + 1) : 0;
+  return nb > 1 ? nb * order_stride((int)E) : 0;
 }
 
 int sfp8_moe_expert_order(const int64_t* selected, int64_t R, int64_t top_k, int64_t E, int64_t* token_index,
@@ -1060,10 +1088,12 @@ int sfp8_moe_expert_order(const int64_t* selected, int64_t R, int64_t top_k, int
   if (need > 0 && (!ws || ws_ints < need)) return kErrWorkspaceTooSmall;
   const int64_t chunk = order_chunk(R);
   const int64_t nb = R > chunk ? (R + chunk - 1) / chunk : 1;
-  const size_t lds = (size_t)kOrderWaves * (E + 1) * 4;
+  const int stride = order_stride((int)E);
+  // 16 rows of bins, and up to 1024 columns of 16 bytes for two sums
+  const size_t lds = (size_t)kOrderWaves * stride * 4 + (nb > 1 ? (size_t)kOrderThreads / (stride / 4) * 2 * stride * 4 : 0);
   if (const int rc = route_allow_lds(moe_order_place_kernel, lds)) return rc;
   if (nb > 1)
-    hipLaunchKernelGGL(moe_order_count_kernel, dim3((unsigned)nb), dim3(kOrderThreads), (size_t)(E + 1) * 4,
+    hipLaunchKernelGGL(moe_order_count_kernel, dim3((unsigned)nb), dim3(kOrderThreads), (size_t)stride * 4,
                        (hipStream_t)stream, selected, R, chunk, (int)E, ws);
   hipLaunchKernelGGL(moe_order_place_kernel, dim3((unsigned)nb), dim3(kOrderThreads), lds, (hipStream_t)stream,
                      selected, R, chunk, (int)top_k, (int)E, nb > 1 ? ws : nullptr, token_index, inverse, offsets);
