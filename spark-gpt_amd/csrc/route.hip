@@ -680,11 +680,18 @@ constexpr int kOrderThreads = 64 * kOrderWaves;
 constexpr int kOrderBlocks = 256;
 
 // Slots per work-group: a multiple of its threads, at most kOrderBlocks groups.
-__host__ __device__ inline int64_t order_chunk(int64_t R) {
+// Below that many, shorter groups are faster where the counts that each adds up
+// stay short too (us at 2048 and 4096 slots a group: 131072 slots of 8 experts
+// 9.3 and 11.0, of 256 experts 11.4 and 13.1; 524288 slots of 1024 experts 29
+// and 23), and one group alone up to 4096 (7.8, against 8.7 in two).
+inline int64_t order_chunk(int64_t R, int64_t E) {
   const int64_t c = (R + kOrderBlocks - 1) / kOrderBlocks;
-  const int64_t least = c < 4096 ? 4096 : c;
+  const int64_t few = R <= 4096 || E >= 512 ? 4096 : 2048;
+  const int64_t least = c < few ? few : c;
   return (least + kOrderThreads - 1) / kOrderThreads * kOrderThreads;
 }
+// Parts of the rows that are added up side by side: 3 (257 columns) to 32.
+__host__ __device__ inline int order_parts(int cols) { return kOrderThreads / cols < 32 ? kOrderThreads / cols : 32; }
 // Bins of a row of counts: E + 1, in whole 16-byte units.
 __host__ __device__ inline int order_stride(int E) { return (E + 4) / 4 * 4; }
 
@@ -718,7 +725,7 @@ __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
   __shared__ int part[kOrderWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nb = gridDim.x, bins = E + 1;
   const int stride = order_stride(E), cols = stride / 4;
-  const int parts = counts ? kOrderThreads / cols : 0;  // at least 3: 257 columns at most
+  const int parts = counts ? order_parts(cols) : 0;
   int* sums = next + kOrderWaves * stride;              // [parts][2][stride]: all rows, the rows before this group's
   for (int e = threadIdx.x; e < kOrderWaves * stride; e += kOrderThreads) next[e] = 0;
   if (counts && (int)threadIdx.x < parts * cols) {
@@ -848,26 +855,57 @@ struct Unit {  // U consecutive elements as fp32
   }
 };
 
-template <int DT, bool VEC>
+// One unit a lane: `lanes` (a power of two) lanes for the D / U units of a token
+// where those are fewer than a wave's, else whole waves.  K slots' rows are in
+// flight at once.  Bound by the rows' bytes; for few tokens by two dependent
+// loads, which one unit a lane keeps from repeating.
+template <int DT, bool VEC, int K>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict__ rows, int64_t R, int64_t D,
                                                           const float* __restrict__ weights,
                                                           const int64_t* __restrict__ inv, int64_t T, int k,
-                                                          void* __restrict__ out, int lanes) {
+                                                          void* __restrict__ out, int lanes, int waves) {
   using X = Unit<DT, VEC>;
-  const int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  int64_t t, d0, step;
+  if (lanes == 64) {  // `waves` waves a token
+    const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    const uint32_t tt = w / (uint32_t)waves;
+    t = tt;
+    d0 = ((int64_t)(w - tt * (uint32_t)waves) * 64 + (threadIdx.x & 63)) * X::U;
+    step = (int64_t)waves * 64 * X::U;
+  } else {
+    t = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    d0 = (int64_t)(threadIdx.x & (lanes - 1)) * X::U;
+    step = (int64_t)lanes * X::U;
+  }
   if (t >= T) return;
-  for (int64_t d = (int64_t)(threadIdx.x & (lanes - 1)) * X::U; d < D; d += (int64_t)lanes * X::U) {
+  for (int64_t d = d0; d < D; d += step) {  // once, but for launches beyond 2^32 work-items
     X acc;
 #pragma unroll
     for (int q = 0; q < X::U; ++q) acc.x[q] = 0.0f;
-    for (int j = 0; j < k; ++j) {
-      const int64_t r = inv[t * k + j];
-      if (r < 0 || r >= R) continue;
-      const float w = weights[t * k + j];
-      X v;
-      v.load(rows, r * D + d);
+    for (int j0 = 0; j0 < k; j0 += K) {
+      int64_t r[K];
+      float w[K];
+      X v[K];
 #pragma unroll
-      for (int q = 0; q < X::U; ++q) acc.x[q] = __builtin_fmaf(w, v.x[q], acc.x[q]);
+      for (int j = 0; j < K; ++j) {
+        const bool in = j0 + j < k;
+        r[j] = in ? inv[t * k + j0 + j] : -1;
+        w[j] = in ? weights[t * k + j0 + j] : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if (r[j] >= 0 && r[j] < R) {
+          v[j].load(rows, r[j] * D + d);
+        } else {
+          w[j] = 0.0f;
+#pragma unroll
+          for (int q = 0; q < X::U; ++q) v[j].x[q] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < K; ++j)
+#pragma unroll
+        for (int q = 0; q < X::U; ++q) acc.x[q] = __builtin_fmaf(w[j], v[j].x[q], acc.x[q]);
     }
     acc.store(out, t * D + d);
   }
@@ -875,40 +913,40 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
 
 // drows[inv[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], rows[inv[t, j]]>
 // (either may be null); rows from offsets[E - 1] on, which no slot names, get
-// zeros.  One wave per token.
+// zeros.  One wave a slot: the waves of a token share its gradient through the
+// caches.  Bound by the rows' bytes, read and written.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
     const void* __restrict__ dout, const void* __restrict__ rows, int64_t R, int64_t D,
-    const float* __restrict__ weights, const int64_t* __restrict__ inv, int64_t T, int k,
+    const float* __restrict__ weights, const int64_t* __restrict__ inv, int64_t slots, int k,
     const int* __restrict__ offsets, int E, void* __restrict__ drows, float* __restrict__ dweights) {
   using X = Unit<DT, VEC>;
   const int lane = threadIdx.x & 63;
-  const int64_t gw = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), nw = (int64_t)gridDim.x * 4;
-  for (int64_t t = gw; t < T; t += nw) {
-    for (int j = 0; j < k; ++j) {
-      const int64_t r = inv[t * k + j];
-      float dot = 0.0f;
-      if (r >= 0 && r < R) {
-        const float w = weights[t * k + j];
-        for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) {
-          X g, v;
-          g.load(dout, t * D + d);
-          if (dweights) {
-            v.load(rows, r * D + d);
+  const int64_t gw = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), nw = (int64_t)gridDim.x * 4;
+  for (int64_t s = gw; s < slots; s += nw) {
+    const int64_t t = (uint32_t)s / (uint32_t)k, r = inv[s];
+    float dot = 0.0f;
+    if (r >= 0 && r < R) {
+      const float w = weights[s];
+#pragma unroll 2
+      for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) {
+        X g, v;
+        g.load(dout, t * D + d);
+        if (dweights) {
+          v.load(rows, r * D + d);
 #pragma unroll
-            for (int q = 0; q < X::U; ++q) dot = __builtin_fmaf(g.x[q], v.x[q], dot);
-          }
-          if (drows) {
+          for (int q = 0; q < X::U; ++q) dot = __builtin_fmaf(g.x[q], v.x[q], dot);
+        }
+        if (drows) {
 #pragma unroll
-            for (int q = 0; q < X::U; ++q) g.x[q] *= w;
-            g.store(drows, r * D + d);
-          }
+          for (int q = 0; q < X::U; ++q) g.x[q] *= w;
+          g.store(drows, r * D + d);
         }
       }
-      if (dweights) {
-        dot = wave_sum_f32(dot);
-        if (lane == 0) dweights[t * k + j] = dot;
-      }
+    }
+    if (dweights) {
+      dot = lanes_sum<64>(dot);
+      if (lane == 0) dweights[s] = dot;
     }
   }
   if (!drows) return;
@@ -1021,13 +1059,24 @@ void route_bwd_launch(const RouteBwdArgs& a, hipStream_t st) { route_by_shape(a,
 
 template <int DT, bool VEC>
 struct Combine {
+  template <int K>
+  static void go(const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv, int64_t T, int k, void* out,
+                 hipStream_t st) {
+    constexpr int U = Unit<DT, VEC>::U;
+    const int64_t units = (D + U - 1) / U, most = ((int64_t)1 << 25) / T;  // waves: 2^31 work-items
+    const int64_t waves = (units + 63) / 64 < most ? (units + 63) / 64 : most;
+    int lanes = 64;
+    while (lanes > 1 && lanes / 2 >= units) lanes /= 2;
+    const int64_t per = 256 / lanes, blocks = lanes == 64 ? (T * waves + 3) / 4 : (T + per - 1) / per;
+    hipLaunchKernelGGL((moe_combine_kernel<DT, VEC, K>), dim3((unsigned)blocks), dim3(256), 0, st, rows, R, D, w, inv, T,
+                       k, out, lanes, (int)waves);
+  }
   static void run(const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv, int64_t T, int k,
                   void* out, hipStream_t st) {
-    int lanes = 64;
-    while (lanes > 1 && (int64_t)(lanes / 2) * Unit<DT, VEC>::U >= D) lanes /= 2;
-    const int64_t per = 256 / lanes;
-    hipLaunchKernelGGL((moe_combine_kernel<DT, VEC>), dim3((unsigned)((T + per - 1) / per)), dim3(256), 0, st, rows, R,
-                       D, w, inv, T, k, out, lanes);
+    if (k == 1) go<1>(rows, R, D, w, inv, T, k, out, st);
+    else if (k == 2) go<2>(rows, R, D, w, inv, T, k, out, st);
+    else if (k <= 4) go<4>(rows, R, D, w, inv, T, k, out, st);
+    else go<8>(rows, R, D, w, inv, T, k, out, st);
   }
 };
 
@@ -1035,9 +1084,10 @@ template <int DT, bool VEC>
 struct CombineBwd {
   static void run(const void* dout, const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv,
                   int64_t T, int k, const int* offsets, int E, void* drows, float* dw, hipStream_t st) {
-    const int64_t nb = (T + 3) / 4;
-    hipLaunchKernelGGL((moe_combine_bwd_kernel<DT, VEC>), dim3((unsigned)(nb < 1 ? 1 : nb)), dim3(256), 0, st, dout,
-                       rows, R, D, w, inv, T, k, offsets, E, drows, dw);
+    const int64_t slots = T * k, work = slots > 0 ? slots : R, most = (int64_t)1 << 22;
+    const int64_t nb = (work + 3) / 4 < most ? (work + 3) / 4 : most;
+    hipLaunchKernelGGL((moe_combine_bwd_kernel<DT, VEC>), dim3((unsigned)nb), dim3(256), 0, st, dout, rows, R, D, w, inv,
+                       slots, k, offsets, E, drows, dw);
   }
 };
 }  // namespace
@@ -1076,7 +1126,7 @@ int sfp8_moe_route_bwd(const float* dweights, const int64_t* selected, const flo
 
 int64_t sfp8_moe_expert_order_workspace_ints(int64_t R, int64_t E) {
   if (R < 0 || R > (int64_t)1 << 30 || E <= 0 || E > kRouteMaxExperts) return -1;
-  const int64_t chunk = order_chunk(R), nb = (R + chunk - 1) / chunk;
+  const int64_t chunk = order_chunk(R, E), nb = (R + chunk - 1) / chunk;
   return nb > 1 ? nb * order_stride((int)E) : 0;
 }
 
@@ -1086,11 +1136,11 @@ int sfp8_moe_expert_order(const int64_t* selected, int64_t R, int64_t top_k, int
   const int64_t need = sfp8_moe_expert_order_workspace_ints(R, E);
   if (need < 0 || top_k <= 0 || R % top_k) return kErrBadShape;
   if (need > 0 && (!ws || ws_ints < need)) return kErrWorkspaceTooSmall;
-  const int64_t chunk = order_chunk(R);
+  const int64_t chunk = order_chunk(R, E);
   const int64_t nb = R > chunk ? (R + chunk - 1) / chunk : 1;
   const int stride = order_stride((int)E);
   // 16 rows of bins, and up to 1024 columns of 16 bytes for two sums
-  const size_t lds = (size_t)kOrderWaves * stride * 4 + (nb > 1 ? (size_t)kOrderThreads / (stride / 4) * 2 * stride * 4 : 0);
+  const size_t lds = (size_t)kOrderWaves * stride * 4 + (nb > 1 ? (size_t)order_parts(stride / 4) * 2 * stride * 4 : 0);
   if (const int rc = route_allow_lds(moe_order_place_kernel, lds)) return rc;
   if (nb > 1)
     hipLaunchKernelGGL(moe_order_count_kernel, dim3((unsigned)nb), dim3(kOrderThreads), (size_t)stride * 4,

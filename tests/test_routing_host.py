@@ -109,7 +109,8 @@ def test_c_abi_refuses_before_launch():
 def test_workspace_sizes():
     q = lambda R, E: _lib.query("sfp8_moe_expert_order_workspace_ints", R, E)
     assert q(0, 8) == q(4096, 8) == 0  # one work-group needs none
-    assert q(4097, 8) == 2 * 12 and q(65536 * 8, 256) == 128 * 260  # rows of E + 1 bins, in fours
+    assert q(4097, 8) == 3 * 12 and q(65536 * 8, 256) == 256 * 260  # rows of E + 1 bins, in fours
+    assert q(65536 * 8, 1023) == 128 * 1024
     assert q(1 << 30, 1024) == 256 * 1028  # never more than 256 work-groups
     assert q(-1, 8) == q(8, 0) == q(8, 1025) == q((1 << 30) + 1, 8) == -1
     assert _lib.query("sfp8_grad_norm_workspace_doubles", -1) == -1
