@@ -667,6 +667,9 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
   Tensor norm = empty({}, kF32, grads[0]), ws = empty({nws}, ScalarType::Double, grads[0]);
   CALL(sfp8_grad_clip, count, g.in.data(), g.out.data(), g.n.data(), g.dtype.data(), (float)max_norm, fptr(norm),
        static_cast<double*>(ws.data_ptr()), nws, stream_of(grads[0]));
+  // written in place, as autograd's checks of saved tensors have to see
+  for (const Tensor& t : out ? *out : grads)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 

@@ -497,7 +497,8 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
   }
   // the first top_k keys, lane s of the token keeping that of slot s, and the one after them
   uint32_t top = 1u << 31, mine = 0u, after = 0u;
-  for (int s = 0; s <= a.k; ++s) {
+  const int rounds = a.k + (half16 ? 0 : 1);
+  for (int s = 0; s < rounds; ++s) {
     uint32_t r = 0u;
 #pragma unroll
     for (int j = 0; j < V; ++j) {

@@ -109,8 +109,10 @@ def combine_experts(rows: torch.Tensor, weights: torch.Tensor, inverse_permutati
     [T, D]: rows [R, D] bf16, fp16 or fp32 in expert order, weights [T, k]
     (k <= 64), ``inverse_permutation`` and ``offsets`` of ``expert_order``.  The
     sum is taken in 32 bits in slot order and rounded once; slots without a row
-    add nothing.  In the backward pass rows that no slot names get zeros; a row
-    that two slots name (``expert_order`` gives no such) is not supported."""
+    add nothing.  In the backward pass rows from ``offsets[-1]`` on get zeros, and
+    each row before is expected to be the row of one slot, as in what
+    ``expert_order`` returns: a slot is left out by its -1 in ``selected``, before
+    the order is made, not by a change to ``inverse_permutation``."""
     if torch.compiler.is_compiling():
         return _CombineExperts.apply(rows, weights.float(), inverse_permutation, offsets)
     return ops.combine_experts(rows, weights, inverse_permutation, offsets)
@@ -122,6 +124,9 @@ def fp8_routed_experts(x: torch.Tensor, logits: torch.Tensor, experts, top_k: in
     has the reference's packed ``gate_up_proj`` [E, 2I, D], ``down_proj`` [E, D, I],
     ``fp8_scale`` and ``fp8_amax`` (train.py:2252-2260); ``route`` are the keyword
     arguments of ``route_tokens``."""
+    if logits.dim() != 2 or logits.shape != (x.shape[0], experts.gate_up_proj.shape[0]):
+        raise ValueError(f"logits must be [{x.shape[0]}, {experts.gate_up_proj.shape[0]}], one row for each token and one "
+                         f"column for each expert, got {tuple(logits.shape)}")
     weights, selected = route_tokens(logits, top_k, **route)
     token_index, inverse_permutation, offsets = expert_order(selected, logits.shape[1])
     rows = _FP8Experts.apply(x, experts.gate_up_proj, experts.down_proj, token_index, inverse_permutation, offsets,

@@ -154,6 +154,20 @@ def test_refusals(dev):
     assert bool((a == 1).all()) and bool((b == 1).all()) and bool((store == 1).all())
 
 
+def test_written_tensors_count_a_version(dev):
+    """Clipping is an in-place write to autograd too."""
+    a, b, o = (torch.ones(8, device=dev) for _ in range(3))
+    v = a._version, b._version, o._version
+    sg.clip_grads([a, b], 1.0, out=[o, b])
+    assert (a._version, b._version, o._version) == (v[0], v[1] + 1, v[2] + 1)
+    x = torch.ones(8, device=dev, requires_grad=True)
+    y = torch.ones(8, device=dev)
+    z = (x * y).sum()  # saves y
+    sg.clip_grads([y], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
 def test_deterministic_and_partly_in_place(dev):
     grads = _grads(dev, [(700, 900), (33,), (70000,)], DTYPES, 6)
     norms = {float(sg.grad_norm(grads)) for _ in range(5)}

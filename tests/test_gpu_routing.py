@@ -429,6 +429,19 @@ def test_routed_layer_matches_its_parts(dev, padded):
     assert ((dl[keep].double() - vl).abs() <= bound).all() and bool((dl[~keep] == 0).all())
 
 
+def test_routed_layer_without_tokens_and_all_masked(dev):
+    """No tokens, and a batch that is all padding: zeros, and zero gradients."""
+    D, I, E, k = 128, 128, 4, 2
+    m = _Experts(E, D, I, dev).train()
+    for T, mask in ((0, None), (70, torch.zeros(70, dtype=torch.bool, device=dev))):
+        x = torch.randn(T, D, device=dev).to(torch.bfloat16).requires_grad_(True)
+        low = torch.randn(T, E, device=dev).requires_grad_(True)
+        y, sel = sg.fp8_routed_experts(x, low, m, k, mask=mask)
+        assert y.shape == (T, D) and bool((y == 0).all()) and bool((sel == -1).all())
+        for g in torch.autograd.grad(y, [x, low, m.gate_up_proj, m.down_proj], torch.ones_like(y)):
+            assert bool((g == 0).all())
+
+
 def test_training_step(dev):
     """A router, the layer, clipping over its parameters and the momentum stage:
     the norm, the clipped gradients and the stage's results against torch."""

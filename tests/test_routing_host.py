@@ -144,6 +144,17 @@ def test_wrappers_refuse_host_tensors():
         sg.clip_grad_norm_(p, 1.0)
 
 
+def test_routed_experts_refuse_other_shapes():
+    """One row of logits for each token and one column for each expert: a plan of
+    more experts than there are weights would read past them."""
+    m = torch.nn.Module()
+    m.gate_up_proj = torch.nn.Parameter(torch.zeros(4, 256, 128))
+    x = torch.zeros(6, 128, dtype=torch.bfloat16)
+    for shape in ((6, 5), (6, 3), (5, 4), (4,)):
+        with pytest.raises(ValueError, match="one row for each token"):
+            sg.fp8_routed_experts(x, torch.zeros(shape), m, 2)
+
+
 def test_fake_shapes():
     from torch._subclasses.fake_tensor import FakeTensorMode
 
