@@ -131,41 +131,54 @@ struct RouteLayout {
   SFP8_DEV int member(int c) const { return 4 * (c * G + sub); }
 };
 
+// Four values of a row at `at`, of which the first is at q + at elements.
+SFP8_DEV void load4(float (&x)[4], const void* p, int dtype, int64_t at) {
+  if (dtype == kF32) {
+    const floatx4 v = *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v[i];
+  } else {
+    const intx2 v = *reinterpret_cast<const intx2*>(reinterpret_cast<const uint16_t*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t b = ((uint32_t)v[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+      x[i] = dtype == kBf16 ? bf16_bits_to_f32(b) : half_bits_to_f32(b);
+    }
+  }
+}
+
 // The V logits of a lane: those past the group's members, and all where `on` is
-// false, read as -inf.  at: the group's first logit.
+// false, read as -inf.  at: the group's first logit.  vec: aligned chunks of
+// four, each in or out as a whole.
 template <int V>
 SFP8_DEV void load_logits(float (&l)[V], const void* p, int dtype, bool vec, int64_t at, const RouteLayout& lay, bool on) {
   const float ninf = -__builtin_inff();
+  if (vec && lay.gs == lay.G * V && __all(on)) {  // nothing to leave out
+    if (dtype == kF32) {  // uniform, once: the loads go out together
+#pragma unroll
+      for (int c = 0; c < V / 4; ++c) load4(*reinterpret_cast<float(*)[4]>(l + 4 * c), p, kF32, at + lay.member(c));
+    } else if (dtype == kBf16) {
+#pragma unroll
+      for (int c = 0; c < V / 4; ++c) load4(*reinterpret_cast<float(*)[4]>(l + 4 * c), p, kBf16, at + lay.member(c));
+    } else {
+#pragma unroll
+      for (int c = 0; c < V / 4; ++c) load4(*reinterpret_cast<float(*)[4]>(l + 4 * c), p, kF16, at + lay.member(c));
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < V; ++j) l[j] = ninf;
   if (!on) return;
-  if (vec && dtype == kF32) {  // gs % 4 == 0 and aligned: a chunk is in or out as a whole
-    const float* q = reinterpret_cast<const float*>(p) + at;
 #pragma unroll
-    for (int c = 0; c < V / 4; ++c)
-      if (lay.member(c) < lay.gs) {
-        const floatx4 v = *reinterpret_cast<const floatx4*>(q + lay.member(c));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l[4 * c + i] = v[i];
-      }
-  } else if (vec) {
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(p) + at;
-#pragma unroll
-    for (int c = 0; c < V / 4; ++c)
-      if (lay.member(c) < lay.gs) {
-        const intx2 v = *reinterpret_cast<const intx2*>(q + lay.member(c));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t b = ((uint32_t)v[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-          l[4 * c + i] = dtype == kBf16 ? bf16_bits_to_f32(b) : half_bits_to_f32(b);
-        }
-      }
-  } else {
-#pragma unroll
-    for (int c = 0; c < V / 4; ++c)
+  for (int c = 0; c < V / 4; ++c) {
+    const int m = lay.member(c);
+    if (vec) {
+      if (m < lay.gs) load4(*reinterpret_cast<float(*)[4]>(l + 4 * c), p, dtype, at + m);
+    } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (lay.member(c) + i < lay.gs) l[4 * c + i] = load_as_f32(p, dtype, at + lay.member(c) + i);
+        if (m + i < lay.gs) l[4 * c + i] = load_as_f32(p, dtype, at + m + i);
+    }
   }
 }
 
@@ -346,13 +359,14 @@ SFP8_DEV float sigmoid_of(float x) {
 }
 
 template <int L, int V, bool BIAS>
-__global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, int G, int idx_bits, bool vec,
-                                                           bool vec_bias) {
+__global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, int log_g, int gs, int idx_bits,
+                                                           bool vec, bool vec_bias) {
   extern __shared__ __align__(16) uint64_t lds[];
   constexpr int kTok = 64 / L;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tl = lane & (L - 1), tok = lane / L;  // lane of the token, token of the wave
-  const RouteLayout lay{G, a.E / a.groups, tl / G, tl % G};
+  const int G = 1 << log_g;
+  const RouteLayout lay{G, gs, tl >> log_g, tl & (G - 1)};
   const bool in_group = lay.g < a.groups;
   const float ninf = -__builtin_inff();
   const bool half16 = !BIAS && a.dtype != kF32;  // ranks hold the whole logit
@@ -438,7 +452,7 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
       if constexpr (!BIAS) tol = 0x1p-14f * val + 0x1p-120f;
     }
     int rank = 0, over = 0, near = 0;
-    for (int j = 1; j < L / G; ++j) {
+    for (int j = 1; j < L >> log_g; ++j) {
       const int from = (tl + j * G) & (L - 1);
       const float other = __shfl(val, (lane & ~(L - 1)) + from, 64);
       rank += other > val || (other == val && from < tl);
@@ -506,7 +520,7 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
       r = x > r ? x : r;
     }
     r = reduce_max_u<L>(r);
-    top = r & 0x80000000u ? r + top : 0u;
+    top += r;
     if (s < a.k) mine = s == tl ? top : mine;  // uniform
     else after = top;
   }
@@ -1018,11 +1032,16 @@ void route_run(const RouteArgs& a, const RouteShape& sh, hipStream_t st) {
   const int64_t per = 4 * (64 / L);  // tokens of a work-group
   const dim3 grid((unsigned)((a.T + per - 1) / per));
   const size_t lds = 4 * (size_t)((3 * a.E + 1) / 2) * 8;  // of each wave: an order value and a logit per expert
+  const int gs = a.E / a.groups;
+  int log_g = 0;
+  while ((1 << log_g) < sh.G) ++log_g;
   const bool vec_bias = (a.E / a.groups) % 4 == 0 && (uintptr_t)a.bias % 16 == 0;
   if (a.bias)
-    hipLaunchKernelGGL((moe_route_kernel<L, V, true>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec, vec_bias);
+    hipLaunchKernelGGL((moe_route_kernel<L, V, true>), grid, dim3(256), lds, st, a, log_g, gs, idx_bits, vec,
+                       vec_bias);
   else
-    hipLaunchKernelGGL((moe_route_kernel<L, V, false>), grid, dim3(256), lds, st, a, sh.G, idx_bits, vec, vec_bias);
+    hipLaunchKernelGGL((moe_route_kernel<L, V, false>), grid, dim3(256), lds, st, a, log_g, gs, idx_bits, vec,
+                       vec_bias);
 }
 template <int L, int V>
 void route_run(const RouteBwdArgs& a, const RouteShape&, hipStream_t st) {
