@@ -332,9 +332,11 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
 // log2(L) lane steps, with nothing to clear.
 //
 // Its limits.  Where two neighbours of the top_k + 1 first are closer than
-// their errors, or two groups are at the border of those kept, the token is
-// selected again by the definition in 64 bits (route_exact), as are rows with
-// NaN or +inf.  Without a bias that takes two logits that differ on one step of the
+// their errors, the first few are put in order again by their values in 64 bits.
+// Where more than four behind the last are that close, or two groups at the
+// border of those kept (or a biased softmax, whose sum is over the whole row),
+// the whole selection is done again by the definition in 64 bits (route_exact),
+// as it is for rows with NaN or +inf.  Without a bias that takes two logits that differ on one step of the
 // scale (equal ones are in the order of their indices): about 1 of 10^4 tokens
 // at 256 normal logits.  With one, scores are off: a softmax by at most
 // (2.5 |d| + 30) 2^-24 of itself, below 2^-19 in all (d is the exponent's
@@ -538,15 +540,55 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
       // between the last of them and the rest.
       const float be = BIAS && e >= 0 ? a.bias[e] : 0.0f;
       const float la = __shfl_up(le, 1, 64), ba = __shfl_up(be, 1, 64);
-      odd |= tl > 0 && e >= 0 && close(up, mine) && !(la == le && ba == be);
+      bool differ = tl > 0 && e >= 0 && close(up, mine) && !(la == le && ba == be);
       const int from = (lane & ~(L - 1)) + a.k - 1;
       const float ll = __shfl(le, from, 64), bl = __shfl(be, from, 64);
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (key[j] < last && close(last, key[j])) {
           const int x = (int)(idx_mask - (key[j] & idx_mask));
-          odd |= load_as_f32(a.logits, a.dtype, row + x) != ll || (BIAS && a.bias[x] != bl);
+          differ |= load_as_f32(a.logits, a.dtype, row + x) != ll || (BIAS && a.bias[x] != bl);
         }
+      differ = lanes_max<L>(differ && on ? 1.0f : 0.0f) > 0.0f;  // the token
+      if (__any(differ)) {
+        // The chosen and the next few, each in a lane, by their values in 64 bits.
+        // What is not among them is further from the last chosen than the errors.
+        const int n = a.k + 4 < L ? a.k + 4 : L;
+        uint32_t cand = tl == a.k ? after : mine, tail = after;
+        for (int s = a.k + 1; s < n; ++s) {
+          uint32_t r = 0u;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const uint32_t x = key[j] - tail;
+            r = x > r ? x : r;
+          }
+          tail += reduce_max_u<L>(r);
+          cand = s == tl ? tail : cand;
+        }
+        // tail > last: the keys are used up
+        odd |= differ && ((tail < last && close(last, tail)) || (BIAS && softmax));
+        const bool is = tl < n && cand >= least && (tl < a.k || cand < last);
+        const int ce = is ? (int)(idx_mask - (cand & idx_mask)) : -1;
+        double val = 0.0;
+        if (is) {
+          val = load_as_f32(a.logits, a.dtype, row + ce);
+          if constexpr (BIAS) val = 1.0 / (1.0 + exp(-val)) + (double)a.bias[ce];
+        }
+        int place = 0;
+        for (int j = 0; j < n; ++j) {
+          const int src = (lane & ~(L - 1)) + j;
+          const double ov = __shfl(val, src, 64);
+          const int oe = __shfl(ce, src, 64);
+          place += oe >= 0 && (ov > val || (ov == val && oe < ce));
+        }
+        // those that are none stay in the lanes behind
+        const int to = (lane & ~(L - 1)) + (is ? place : tl);
+        const int placed = __builtin_amdgcn_ds_permute(to << 2, ce);
+        if (differ) {
+          e = tl < a.k ? placed : -1;
+          le = e >= 0 ? load_as_f32(a.logits, a.dtype, row + e) : ninf;
+        }
+      }
     }
   }
   const uint64_t any_odd = __ballot(odd && on);
