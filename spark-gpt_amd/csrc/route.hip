@@ -879,20 +879,27 @@ template <int DT, bool VEC>
 struct Unit {  // U consecutive elements as fp32
   static constexpr int U = VEC ? (DT == kF32 ? 4 : 8) : 1;
   float x[U];
-  SFP8_DEV void load(const void* p, int64_t i) {
-    if constexpr (!VEC) {
-      x[0] = load_as_f32(p, DT, i);
-    } else if constexpr (DT == kF32) {
-      const floatx4 v = *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(p) + i);
+  // as they are in memory: what a load in flight holds
+  struct Raw {
+    intx4 v;
+    SFP8_DEV void load(const void* p, int64_t i) {
+      if constexpr (!VEC) {
+        v[0] = DT == kF32 ? reinterpret_cast<const int*>(p)[i] : reinterpret_cast<const uint16_t*>(p)[i];
+      } else {
+        v = *reinterpret_cast<const intx4*>(reinterpret_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2));
+      }
+    }
+  };
+  SFP8_DEV Unit() = default;
+  SFP8_DEV explicit Unit(const Raw& r) {
+    if constexpr (DT == kF32) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) x[q] = v[q];
+      for (int q = 0; q < U; ++q) x[q] = __uint_as_float((uint32_t)r.v[q]);
     } else {
-      const intx4 v = *reinterpret_cast<const intx4*>(reinterpret_cast<const uint16_t*>(p) + i);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t lo = (uint32_t)v[q] & 0xffffu, hi = (uint32_t)v[q] >> 16;
-        x[2 * q] = DT == kBf16 ? bf16_bits_to_f32(lo) : half_bits_to_f32(lo);
-        x[2 * q + 1] = DT == kBf16 ? bf16_bits_to_f32(hi) : half_bits_to_f32(hi);
+      for (int q = 0; q < U; ++q) {
+        const uint32_t b = ((uint32_t)r.v[q >> 1] >> (16 * (q & 1))) & 0xffffu;
+        x[q] = DT == kBf16 ? bf16_bits_to_f32(b) : half_bits_to_f32(b);
       }
     }
   }
@@ -942,7 +949,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
     for (int j0 = 0; j0 < k; j0 += K) {
       int64_t r[K];
       float w[K];
-      X v[K];
+      typename X::Raw v[K];
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         const bool in = j0 + j < k;
@@ -955,14 +962,15 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
           v[j].load(rows, r[j] * D + d);
         } else {
           w[j] = 0.0f;
-#pragma unroll
-          for (int q = 0; q < X::U; ++q) v[j].x[q] = 0.0f;
+          v[j].v = intx4{0, 0, 0, 0};
         }
       }
 #pragma unroll
-      for (int j = 0; j < K; ++j)
+      for (int j = 0; j < K; ++j) {
+        const X x(v[j]);
 #pragma unroll
-        for (int q = 0; q < X::U; ++q) acc.x[q] = __builtin_fmaf(w[j], v[j].x[q], acc.x[q]);
+        for (int q = 0; q < X::U; ++q) acc.x[q] = __builtin_fmaf(w[j], x.x[q], acc.x[q]);
+      }
     }
     acc.store(out, t * D + d);
   }
@@ -987,10 +995,12 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
       const float w = weights[s];
 #pragma unroll 2
       for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) {
-        X g, v;
-        g.load(dout, t * D + d);
+        typename X::Raw rg, rv;
+        rg.load(dout, t * D + d);
+        if (dweights) rv.load(rows, r * D + d);
+        X g(rg);
         if (dweights) {
-          v.load(rows, r * D + d);
+          const X v(rv);
 #pragma unroll
           for (int q = 0; q < X::U; ++q) dot = __builtin_fmaf(g.x[q], v.x[q], dot);
         }
