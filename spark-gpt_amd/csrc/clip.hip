@@ -10,11 +10,7 @@
 // take), in an order that depends on the sizes alone: every work-group sums
 // its own chunks, then the sums are added in order.  Bound by HBM: each
 // gradient is read once for the norm and, where c != 1 or the result goes
-// elsewhere, read again and written.  The second pass walks from the end, where
-// the last-level cache still holds what the norm read last, and its stores pass
-// the caches by: 1208 MB in 24 tensors 698 -> 678 -> 663 us (the norm alone 210,
-// 5.8 TB/s); 63 MB in 60 tensors 34, below the limit (the norm, and a launch
-// that ends at once) 15.7.
+// elsewhere, read again and written.
 #include "common.h"
 
 namespace sfp8 {
@@ -26,6 +22,7 @@ constexpr int kClipTensors = 120;
 constexpr int kClipChunk = 65536;   // bytes of a gradient that one work-group takes at a time
 constexpr int kClipBlocks = 2048;   // work-groups of a launch, at most
 constexpr int kClipThreads = 256;
+constexpr int64_t kClipLastLevelCache = (int64_t)256 << 20;
 constexpr int kClipUnroll = 8;      // 16-byte loads of a thread in flight
 
 struct ClipTable {
@@ -90,8 +87,8 @@ struct Pack {
 
 // The elements [e0, e1) of a chunk: those before the first 16-byte boundary,
 // whole 16-byte vectors, and the rest.  one(i) takes element i, vec(i, v) the
-// vector v that starts at element i.
-template <int DT, typename One, typename Vec>
+// vector v that starts at element i.  ONCE: loads that pass the caches by.
+template <int DT, bool ONCE, typename One, typename Vec>
 SFP8_DEV void clip_walk(const void* p, int64_t e0, int64_t e1, One one, Vec vec) {
   using P = Pack<DT>;
   constexpr int kStep = kClipThreads * P::U;
@@ -104,7 +101,10 @@ SFP8_DEV void clip_walk(const void* p, int64_t e0, int64_t e1, One one, Vec vec)
   for (; i + (kClipUnroll - 1) * kStep < v1; i += kClipUnroll * kStep) {  // kClipUnroll loads in flight
     intx4 v[kClipUnroll];
 #pragma unroll
-    for (int q = 0; q < kClipUnroll; ++q) v[q] = *reinterpret_cast<const intx4*>(at + (i + q * kStep) * P::kSize);
+    for (int q = 0; q < kClipUnroll; ++q) {
+      const intx4* x = reinterpret_cast<const intx4*>(at + (i + q * kStep) * P::kSize);
+      v[q] = ONCE ? __builtin_nontemporal_load(x) : *x;
+    }
 #pragma unroll
     for (int q = 0; q < kClipUnroll; ++q) vec(e0 + i + q * kStep, v[q]);
   }
@@ -112,11 +112,11 @@ SFP8_DEV void clip_walk(const void* p, int64_t e0, int64_t e1, One one, Vec vec)
   if (v1 + (int)threadIdx.x < n) one(e0 + v1 + threadIdx.x);
 }
 
-template <int DT>
+template <int DT, bool ONCE>
 SFP8_DEV double clip_squares(const void* p, int64_t e0, int64_t e1) {
   using P = Pack<DT>;
   double s = 0.0;
-  clip_walk<DT>(
+  clip_walk<DT, ONCE>(
       p, e0, e1,
       [&](int64_t i) {
         const double x = P::load(p, i);
@@ -132,7 +132,7 @@ SFP8_DEV double clip_squares(const void* p, int64_t e0, int64_t e1) {
   return s;
 }
 
-template <int DT>
+template <int DT, bool ONCE>
 SFP8_DEV void clip_scale(const void* p, void* o, int64_t e0, int64_t e1, float c, bool aligned) {
   using P = Pack<DT>;
   const auto one = [&](int64_t i) { P::store(o, i, P::load(p, i) * c); };
@@ -140,12 +140,13 @@ SFP8_DEV void clip_scale(const void* p, void* o, int64_t e0, int64_t e1, float c
     for (int64_t i = e0 + threadIdx.x; i < e1; i += kClipThreads) one(i);
     return;
   }
-  clip_walk<DT>(p, e0, e1, one, [&](int64_t i, const intx4& v) {
+  clip_walk<DT, ONCE>(p, e0, e1, one, [&](int64_t i, const intx4& v) {
     __builtin_nontemporal_store(P::scaled(v, c), reinterpret_cast<intx4*>(reinterpret_cast<char*>(o) + i * P::kSize));
   });
 }
 
 // part[blockIdx.x] = the squares of this work-group's chunks.
+template <bool ONCE>
 __global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(const ClipTable tab, double* __restrict__ part) {
   __shared__ double red[kClipThreads / 64];
   const ClipFinder find(tab);
@@ -157,8 +158,9 @@ __global__ __launch_bounds__(kClipThreads) void clip_norm_kernel(const ClipTable
     const int64_t per = kClipChunk / (dt == kF32 ? 4 : 2);
     const int64_t e0 = (int64_t)(c - tab.first[i]) * per;
     const int64_t e1 = e0 + per < tab.n[i] ? e0 + per : tab.n[i];
-    s += dt == kF32 ? clip_squares<kF32>(tab.in[i], e0, e1)
-                    : dt == kBf16 ? clip_squares<kBf16>(tab.in[i], e0, e1) : clip_squares<kF16>(tab.in[i], e0, e1);
+    s += dt == kF32 ? clip_squares<kF32, ONCE>(tab.in[i], e0, e1)
+                    : dt == kBf16 ? clip_squares<kBf16, ONCE>(tab.in[i], e0, e1)
+                                  : clip_squares<kF16, ONCE>(tab.in[i], e0, e1);
   }
   s = wave_sum_f64(s);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -183,8 +185,9 @@ __global__ __launch_bounds__(kClipThreads) void clip_norm_out_kernel(const doubl
   if (threadIdx.x == 0) *norm = n;
 }
 
+template <bool ONCE>
 __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipTable tab, const double* __restrict__ part,
-                                                                  int parts, float max_norm,
+                                                                  int parts, float max_norm, bool backwards,
                                                                   float* __restrict__ norm) {
   const float n = clip_norm_of(part, parts);
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
@@ -193,9 +196,8 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipTabl
   if (f == 1.0f && tab.in_place) return;  // x * 1 is x
   const ClipFinder find(tab);
   const uint32_t chunks = tab.first[tab.count];
-  // from the end, of which the caches still hold what the norm read last
   for (uint32_t b = blockIdx.x; b < chunks; b += gridDim.x) {
-    const uint32_t c = chunks - 1 - b;
+    const uint32_t c = backwards ? chunks - 1 - b : b;
     const int i = find(c);
     if (f == 1.0f && tab.in[i] == tab.out[i]) continue;
     const int dt = tab.dtype[i];
@@ -203,9 +205,9 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale_kernel(const ClipTabl
     const int64_t e0 = (int64_t)(c - tab.first[i]) * per;
     const int64_t e1 = e0 + per < tab.n[i] ? e0 + per : tab.n[i];
     const bool aligned = (((uintptr_t)tab.in[i] ^ (uintptr_t)tab.out[i]) & 15u) == 0;
-    if (dt == kF32) clip_scale<kF32>(tab.in[i], tab.out[i], e0, e1, f, aligned);
-    else if (dt == kBf16) clip_scale<kBf16>(tab.in[i], tab.out[i], e0, e1, f, aligned);
-    else clip_scale<kF16>(tab.in[i], tab.out[i], e0, e1, f, aligned);
+    if (dt == kF32) clip_scale<kF32, ONCE>(tab.in[i], tab.out[i], e0, e1, f, aligned);
+    else if (dt == kBf16) clip_scale<kBf16, ONCE>(tab.in[i], tab.out[i], e0, e1, f, aligned);
+    else clip_scale<kF16, ONCE>(tab.in[i], tab.out[i], e0, e1, f, aligned);
   }
 }
 
@@ -282,7 +284,7 @@ int sfp8_grad_norm(int64_t count, const void* const* grads, const int64_t* n, co
   hipStream_t st = (hipStream_t)stream;
   int parts = 0;
   clip_tables(count, grads, nullptr, n, dtype, [&](const ClipTable& tab, int blocks) {
-    hipLaunchKernelGGL(clip_norm_kernel, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws + parts);
+    hipLaunchKernelGGL(clip_norm_kernel<true>, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws + parts);
     parts += blocks;
   });
   hipLaunchKernelGGL(clip_norm_out_kernel, dim3(1), dim3(kClipThreads), 0, st, ws, parts, norm);
@@ -300,9 +302,23 @@ int sfp8_grad_clip(int64_t count, const void* const* grads, void* const* out, co
   }
   if (ws_doubles < sfp8_grad_norm_workspace_doubles(count)) return kErrWorkspaceTooSmall;
   hipStream_t st = (hipStream_t)stream;
+  int64_t bytes = 0;
+  bool elsewhere = false;
+  for (int64_t i = 0; i < count; ++i) {
+    bytes += n[i] * (dtype[i] == kF32 ? 4 : 2);
+    elsewhere |= n[i] > 0 && out[i] != grads[i];
+  }
+  // Which loads pass the caches by, and which way the second pass goes.  us of
+  // 63 / 151 / 1208 MB, below the limit, scaled in place, scaled elsewhere:
+  //   neither, the second backwards   16 31 211 | 34 75 677 | 34 73 655
+  //   both, backwards                 13 29 183 | 38 83 643 | 36 80 634
+  //   the norm's, forwards            13 30 183 | 35 73 647 | 35 80 666
+  const bool large = bytes > kClipLastLevelCache;
+  const bool norm_once = !elsewhere || large, scale_once = elsewhere && large;
   int parts = 0;
   clip_tables(count, grads, out, n, dtype, [&](const ClipTable& tab, int blocks) {
-    hipLaunchKernelGGL(clip_norm_kernel, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws + parts);
+    if (norm_once) hipLaunchKernelGGL(clip_norm_kernel<true>, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws + parts);
+    else hipLaunchKernelGGL(clip_norm_kernel<false>, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws + parts);
     parts += blocks;
   });
   if (parts == 0) {  // nothing to scale: the norm is 0
@@ -311,7 +327,12 @@ int sfp8_grad_clip(int64_t count, const void* const* grads, void* const* out, co
   }
   float* first = norm;
   clip_tables(count, grads, out, n, dtype, [&](const ClipTable& tab, int blocks) {
-    hipLaunchKernelGGL(clip_scale_kernel, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws, parts, max_norm, first);
+    if (scale_once)
+      hipLaunchKernelGGL(clip_scale_kernel<true>, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws, parts, max_norm,
+                         elsewhere, first);
+    else
+      hipLaunchKernelGGL(clip_scale_kernel<false>, dim3(blocks), dim3(kClipThreads), 0, st, tab, ws, parts, max_norm,
+                         elsewhere, first);
     first = nullptr;
   });
   return clip_status();

@@ -889,6 +889,12 @@ struct Unit {  // U consecutive elements as fp32
         v = *reinterpret_cast<const intx4*>(reinterpret_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2));
       }
     }
+    // the same of data that is read once
+    SFP8_DEV void load_once(const void* p, int64_t i) {
+      if constexpr (!VEC) load(p, i);
+      else v = __builtin_nontemporal_load(
+          reinterpret_cast<const intx4*>(reinterpret_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2)));
+    }
   };
   SFP8_DEV Unit() = default;
   SFP8_DEV explicit Unit(const Raw& r) {
@@ -903,18 +909,22 @@ struct Unit {  // U consecutive elements as fp32
       }
     }
   }
+  // ONCE: past the caches
+  template <bool ONCE = false>
   SFP8_DEV void store(void* p, int64_t i) const {
     if constexpr (!VEC) {
       store_f32_as(p, DT, i, x[0]);
-    } else if constexpr (DT == kF32) {
-      *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(p) + i) = floatx4{x[0], x[1], x[2], x[3]};
     } else {
       intx4 o;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        o[q] = (int)(DT == kBf16 ? pack2_bf16(x[2 * q], x[2 * q + 1])
-                                 : f32_to_half_bits(x[2 * q]) | f32_to_half_bits(x[2 * q + 1]) << 16);
-      *reinterpret_cast<intx4*>(reinterpret_cast<uint16_t*>(p) + i) = o;
+      for (int q = 0; q < 4; ++q) {
+        if constexpr (DT == kF32) o[q] = (int)__float_as_uint(x[q]);
+        else if constexpr (DT == kBf16) o[q] = (int)pack2_bf16(x[2 * q], x[2 * q + 1]);
+        else o[q] = (int)(f32_to_half_bits(x[2 * q]) | f32_to_half_bits(x[2 * q + 1]) << 16);
+      }
+      intx4* at = reinterpret_cast<intx4*>(reinterpret_cast<char*>(p) + i * (DT == kF32 ? 4 : 2));
+      if constexpr (ONCE) __builtin_nontemporal_store(o, at);
+      else *at = o;
     }
   }
 };
@@ -923,7 +933,7 @@ struct Unit {  // U consecutive elements as fp32
 // where those are fewer than a wave's, else whole waves.  K slots' rows are in
 // flight at once.  Bound by the rows' bytes; for few tokens by two dependent
 // loads, which one unit a lane keeps from repeating.
-template <int DT, bool VEC, int K>
+template <int DT, bool VEC, int K, bool NT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict__ rows, int64_t R, int64_t D,
                                                           const float* __restrict__ weights,
                                                           const int64_t* __restrict__ inv, int64_t T, int k,
@@ -959,7 +969,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         if (r[j] >= 0 && r[j] < R) {
-          v[j].load(rows, r[j] * D + d);
+          NT ? v[j].load_once(rows, r[j] * D + d) : v[j].load(rows, r[j] * D + d);
         } else {
           w[j] = 0.0f;
           v[j].v = intx4{0, 0, 0, 0};
@@ -980,7 +990,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
 // (either may be null); rows from offsets[E - 1] on, which no slot names, get
 // zeros.  One wave a slot: the waves of a token share its gradient through the
 // caches.  Bound by the rows' bytes, read and written.
-template <int DT, bool VEC>
+template <int DT, bool VEC, bool NT>
 __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
     const void* __restrict__ dout, const void* __restrict__ rows, int64_t R, int64_t D,
     const float* __restrict__ weights, const int64_t* __restrict__ inv, int64_t slots, int k,
@@ -997,7 +1007,7 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
       for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) {
         typename X::Raw rg, rv;
         rg.load(dout, t * D + d);
-        if (dweights) rv.load(rows, r * D + d);
+        if (dweights) NT ? rv.load_once(rows, r * D + d) : rv.load(rows, r * D + d);
         X g(rg);
         if (dweights) {
           const X v(rv);
@@ -1007,7 +1017,7 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
         if (drows) {
 #pragma unroll
           for (int q = 0; q < X::U; ++q) g.x[q] *= w;
-          g.store(drows, r * D + d);
+          g.template store<NT>(drows, r * D + d);
         }
       }
     }
@@ -1129,6 +1139,13 @@ void route_launch(const RouteArgs& a, hipStream_t st) {
 }
 void route_bwd_launch(const RouteBwdArgs& a, hipStream_t st) { route_by_shape(a, route_shape(a.E, 1, a.k), st); }
 
+// What no longer fits the last-level cache passes it by: the rows, and in the
+// backward pass their gradients too.  us with that and without, by MiB of rows
+// and results, forward: 192 36.5 and 31.7, 216 40.6 and 34.2, 288 52 and 52, 336
+// 59 and 64, 384 66.5 and 77, 768 124 and 146; backward: 160 31 and 27, 240 42 and
+// 39, 272 53 and 55, 320 51 and 61, 480 80 and 98, 640 102 and 129, 1088 211 and 225.
+constexpr int64_t kLastLevelCache = (int64_t)256 << 20;
+
 template <int DT, bool VEC>
 struct Combine {
   template <int K>
@@ -1140,8 +1157,12 @@ struct Combine {
     int lanes = 64;
     while (lanes > 1 && lanes / 2 >= units) lanes /= 2;
     const int64_t per = 256 / lanes, blocks = lanes == 64 ? (T * waves + 3) / 4 : (T + per - 1) / per;
-    hipLaunchKernelGGL((moe_combine_kernel<DT, VEC, K>), dim3((unsigned)blocks), dim3(256), 0, st, rows, R, D, w, inv, T,
-                       k, out, lanes, (int)waves);
+    const auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, rows, R, D, w, inv, T, k, out, lanes,
+                         (int)waves);
+    };
+    if (VEC && (R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache) launch(moe_combine_kernel<DT, VEC, K, VEC>);
+    else launch(moe_combine_kernel<DT, VEC, K, false>);
   }
   static void run(const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv, int64_t T, int k,
                   void* out, hipStream_t st) {
@@ -1158,8 +1179,12 @@ struct CombineBwd {
                   int64_t T, int k, const int* offsets, int E, void* drows, float* dw, hipStream_t st) {
     const int64_t slots = T * k, work = slots > 0 ? slots : R, most = (int64_t)1 << 22;
     const int64_t nb = (work + 3) / 4 < most ? (work + 3) / 4 : most;
-    hipLaunchKernelGGL((moe_combine_bwd_kernel<DT, VEC>), dim3((unsigned)nb), dim3(256), 0, st, dout, rows, R, D, w, inv,
-                       slots, k, offsets, E, drows, dw);
+    const auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)nb), dim3(256), 0, st, dout, rows, R, D, w, inv, slots, k, offsets, E,
+                         drows, dw);
+    };
+    if (VEC && (2 * R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache) launch(moe_combine_bwd_kernel<DT, VEC, VEC>);
+    else launch(moe_combine_bwd_kernel<DT, VEC, false>);
   }
 };
 }  // namespace

@@ -179,6 +179,24 @@ def test_deterministic_and_partly_in_place(dev):
     assert torch.equal(grads[0], before[0]) and torch.equal(grads[2], before[2])
 
 
+def test_beyond_the_last_level_cache(dev):
+    """More gradients than the caches hold, in place and elsewhere, against torch in 64 bits."""
+    grads = _grads(dev, [(9000, 8001), (33,), (6000, 7000)], [torch.float32, torch.bfloat16], 2)
+    assert sum(g.numel() * g.element_size() for g in grads) > 300 << 20
+    ref = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
+    before = [g.clone() for g in grads]
+    out = [torch.empty_like(g) for g in grads]
+    for got in (sg.grad_norm(grads), sg.clip_grads(grads, 0.5, out=out)):
+        assert abs(float(got) - float(ref)) <= (2.0 ** -24 * 1.02 + 2e-8) * float(ref)  # 10^8 additions of 2^-53
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    sg.clip_grads(grads, 0.5)
+    factor = 0.5 / (ref + 1e-6)
+    for a, b, o in zip(grads, before, out):
+        step = 5 * 2.0 ** -24 + 2e-8 + (0 if b.dtype == torch.float32 else torch.finfo(b.dtype).eps / 2)
+        want = b.double() * factor
+        assert torch.equal(a, o) and bool(((a.double() - want).abs() <= step * want.abs() + 1e-40).all())
+
+
 def test_captured_and_replayed(dev):
     """A captured clip, replayed on new gradients between eager calls."""
     shapes = [(512, 256), (1000,), (64, 64)]

@@ -362,6 +362,33 @@ def test_combine_layouts(dev):
     assert empty.shape == (0, D)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_combine_beyond_the_last_level_cache(dev, dtype):
+    """Rows beyond the caches, which are read another way: the same bits as in parts."""
+    T, k, D, E = (70001, 2, 1024, 8) if dtype == "bf16" else (20001, 3, 1280, 8)
+    g = torch.Generator(device=dev).manual_seed(3)
+    sel = torch.randint(-1, E, (T, k), device=dev, generator=g)
+    _, inv, off = sg.expert_order(sel, E)
+    rows = torch.randn(T * k, D, device=dev, generator=g).to(DTYPES[dtype])
+    w, dout = torch.rand(T, k, device=dev, generator=g), torch.randn(T, D, device=dev, generator=g).to(DTYPES[dtype])
+    assert rows.numel() * rows.element_size() > 256 << 20
+    y = sg.ops.moe_combine(rows, w, inv)
+    dr, dw = sg.ops.moe_combine_bwd(dout, rows, w, inv, off)
+    n = int(off[-1])
+    assert 0 < n < T * k and bool((dr[n:] == 0).all())
+    for a in range(0, T, 9000):
+        b = min(a + 9000, T)
+        part = inv[a * k:b * k]
+        own = part[part >= 0]
+        few = rows[own].contiguous()  # the rows of these tokens alone
+        pinv = torch.full_like(part, -1)
+        pinv[part >= 0] = torch.arange(own.numel(), device=dev)
+        assert torch.equal(sg.ops.moe_combine(few, w[a:b], pinv), y[a:b])
+        poff = torch.tensor([own.numel()], dtype=torch.int32, device=dev)
+        pdr, pdw = sg.ops.moe_combine_bwd(dout[a:b], few, w[a:b], pinv, poff)
+        assert torch.equal(pdr, dr[own]) and torch.equal(pdw, dw[a:b])
+
+
 # ------------------------------------------------------------------ together
 class _Experts(torch.nn.Module):
     def __init__(self, E, D, I, dev, seed=0):
