@@ -23,13 +23,11 @@ import torch
 from . import ops
 
 
-@torch.no_grad()
 def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """sqrt(sum of squares over every element of ``grads``), an fp32 scalar tensor."""
     return ops.grad_norm(list(grads))
 
 
-@torch.no_grad()
 def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, out: Sequence[torch.Tensor] | None = None) -> torch.Tensor:
     """Scales ``grads`` to a norm of at most ``max_norm`` and returns the norm
     they had (an fp32 scalar tensor).  In place, or into ``out``: tensors of the

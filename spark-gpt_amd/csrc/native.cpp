@@ -613,6 +613,7 @@ struct GradList {
 GradList grad_list(const std::vector<Tensor>& grads) {
   need(!grads.empty(), "at least one gradient");
   GradList g;
+  g.in.reserve(grads.size()), g.out.reserve(grads.size()), g.n.reserve(grads.size()), g.dtype.reserve(grads.size());
   for (const Tensor& t : grads) {
     g.dtype.push_back(float_code("a gradient", t));
     if (t.layout() != at::kStrided || !t.is_non_overlapping_and_dense())
@@ -644,6 +645,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
     bool written;
   };
   std::vector<Span> spans;
+  spans.reserve(2 * grads.size());
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& o = out ? (*out)[i] : grads[i];
     if (out && !(o.scalar_type() == grads[i].scalar_type() && o.device() == grads[i].device() &&
