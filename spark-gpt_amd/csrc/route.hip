@@ -787,14 +787,15 @@ __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
   for (int e = threadIdx.x; e < kOrderWaves * stride; e += kOrderThreads) next[e] = 0;
   if (counts && (int)threadIdx.x < parts * cols) {
     const int p = threadIdx.x / cols, c = threadIdx.x % cols;
-    intx4 total = {0, 0, 0, 0}, before = {0, 0, 0, 0};
+    intx4 before = {0, 0, 0, 0}, after = {0, 0, 0, 0};
+    const intx4* row = reinterpret_cast<const intx4*>(counts) + p * cols + c;
+    const int step = parts * cols, own = blockIdx.x;
+    int b = p;
 #pragma unroll 8
-    for (int b = p; b < nb; b += parts) {
-      const intx4 x = *reinterpret_cast<const intx4*>(counts + (int64_t)b * stride + 4 * c);
-      total += x;
-      before += b < (int)blockIdx.x ? x : intx4{0, 0, 0, 0};
-    }
-    *reinterpret_cast<intx4*>(sums + (2 * p) * stride + 4 * c) = total;
+    for (; b < own; b += parts, row += step) before += *row;
+#pragma unroll 8
+    for (; b < nb; b += parts, row += step) after += *row;
+    *reinterpret_cast<intx4*>(sums + (2 * p) * stride + 4 * c) = before + after;
     *reinterpret_cast<intx4*>(sums + (2 * p + 1) * stride + 4 * c) = before;
   }
   __syncthreads();
@@ -850,22 +851,23 @@ __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
   __syncthreads();
   int bits = 0;
   while ((1 << bits) < bins) ++bits;
-  for (int64_t i = i0 + lane; i - lane < i1; i += 64) {
-    const bool in = i < i1;
+  for (int i = (int)i0 + lane; i - lane < (int)i1; i += 64) {  // R <= 2^30
+    const bool in = i < (int)i1;
     const int e = in ? order_bin(sel, i, E) : 0;
     uint64_t same = __ballot(in);  // the lanes of this step with the same bin
     for (int b = 0; b < bits; ++b) {
-      const uint64_t y = __ballot((e >> b) & 1);
-      same &= (e >> b) & 1 ? y : ~y;
+      const int bit = __builtin_amdgcn_sbfe(e, b, 1);  // 0 or -1
+      const uint64_t y = __ballot(bit);
+      same &= ~(y ^ (uint64_t)(int64_t)bit);
     }
-    const int rank = __popcll(same & ((1ull << lane) - 1));
+    const int rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
     const int row = in ? mine[e] + rank : 0;
     __builtin_amdgcn_wave_barrier();
     if (in && rank == 0) mine[e] = row + __popcll(same);
     __builtin_amdgcn_wave_barrier();
     if (in) {
       inverse[i] = e < E ? row : -1;
-      token_index[row] = (uint32_t)i / (uint32_t)k;  // i < 2^30
+      token_index[row] = (uint32_t)i / (uint32_t)k;
     }
   }
 }
