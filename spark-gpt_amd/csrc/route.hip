@@ -332,11 +332,12 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
 // log2(L) lane steps, with nothing to clear.
 //
 // Its limits.  Where two neighbours of the top_k + 1 first are closer than
-// their errors, the first few are put in order again by their values in 64 bits.
-// Where more than four behind the last are that close, or two groups at the
-// border of those kept (or a biased softmax, whose sum is over the whole row),
-// the whole selection is done again by the definition in 64 bits (route_exact),
-// as it is for rows with NaN or +inf.  Without a bias that takes two logits that differ on one step of the
+// their errors, the first few are put in order again by their values in 64 bits,
+// and so are the groups where two are that close at the border of those kept.
+// Where more than four experts behind the last are that close, or for a biased
+// softmax, whose sum is over the whole row, the whole selection is done again by
+// the definition in 64 bits (route_exact), as it is for rows with NaN or +inf.
+// Without a bias that takes two logits that differ on one step of the
 // scale (equal ones are in the order of their indices): about 1 of 10^4 tokens
 // at 256 normal logits.  With one, scores are off: a softmax by at most
 // (2.5 |d| + 30) 2^-24 of itself, below 2^-19 in all (d is the exponent's
@@ -462,7 +463,37 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
       near += other >= val - tol;
     }
     kept = in_group && val != ninf && rank < a.top_groups;
-    odd |= tol > 0.0f && val != ninf && over < a.top_groups && near >= a.top_groups;
+    const bool unsure = on && tol > 0.0f && val != ninf && over < a.top_groups && near >= a.top_groups;
+    if (BIAS && softmax) {
+      odd |= unsure;
+    } else if (__any(unsure)) {
+      // a group at the border of those kept: the groups' values in 64 bits
+      double d1 = ninf, d2 = ninf;
+#pragma unroll 1
+      for (int j = 0; j < V; ++j) {
+        const int mem = lay.member(j >> 2) + (j & 3);
+        if (!(on && in_group && mem < gs)) continue;
+        const float x = load_as_f32(a.logits, a.dtype, row + first + mem);
+        if (x == ninf) continue;
+        const double ex = exp(softmax ? (double)x - (double)m : -(double)x);
+        const double v = softmax ? ex : 1.0 / (1.0 + ex) + (BIAS ? (double)a.bias[first + mem] : 0.0);
+        d2 = fmax(d2, fmin(d1, v));
+        d1 = fmax(d1, v);
+      }
+      for (int s = 1; s < G; s <<= 1) {
+        const double o1 = __shfl_xor(d1, s, 64), o2 = __shfl_xor(d2, s, 64);
+        d2 = fmax(fmin(d1, o1), fmax(d2, o2));
+        d1 = fmax(d1, o1);
+      }
+      const double v = two_best && d2 != ninf ? d1 + d2 : d1;
+      int place = 0;
+      for (int j = 1; j < L >> log_g; ++j) {
+        const int from = (tl + j * G) & (L - 1);
+        const double other = __shfl(v, (lane & ~(L - 1)) + from, 64);
+        place += other > v || (other == v && from < tl);
+      }
+      kept = in_group && v != ninf && place < a.top_groups;
+    }
   }
   // the keys: rank << idx_bits, and the inverted index
   const uint32_t idx_mask = (1u << idx_bits) - 1, idx_top = idx_mask - (uint32_t)first;
