@@ -20,6 +20,12 @@ constexpr int kRouteMaxK = 64;
 enum : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 enum : int { kSoftmax = 0, kSigmoid = 1 };
 
+// 16 and 8 bytes at any element's address: global memory takes them there in
+// one access.
+typedef int intx4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef int intx2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef float floatx4_any __attribute__((ext_vector_type(4), aligned(4)));
+
 SFP8_DEV float half_bits_to_f32(uint32_t b) { return (float)__builtin_bit_cast(_Float16, (uint16_t)b); }
 SFP8_DEV uint32_t f32_to_half_bits(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
 
@@ -131,14 +137,14 @@ struct RouteLayout {
   SFP8_DEV int member(int c) const { return 4 * (c * G + sub); }
 };
 
-// Four values of a row at `at`, of which the first is at q + at elements.
+// Four values of a row, from element `at` of p on.
 SFP8_DEV void load4(float (&x)[4], const void* p, int dtype, int64_t at) {
   if (dtype == kF32) {
-    const floatx4 v = *reinterpret_cast<const floatx4*>(reinterpret_cast<const float*>(p) + at);
+    const floatx4_any v = *reinterpret_cast<const floatx4_any*>(reinterpret_cast<const float*>(p) + at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = v[i];
   } else {
-    const intx2 v = *reinterpret_cast<const intx2*>(reinterpret_cast<const uint16_t*>(p) + at);
+    const intx2_any v = *reinterpret_cast<const intx2_any*>(reinterpret_cast<const uint16_t*>(p) + at);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t b = ((uint32_t)v[i >> 1] >> (16 * (i & 1))) & 0xffffu;
@@ -148,12 +154,11 @@ SFP8_DEV void load4(float (&x)[4], const void* p, int dtype, int64_t at) {
 }
 
 // The V logits of a lane: those past the group's members, and all where `on` is
-// false, read as -inf.  at: the group's first logit.  vec: aligned chunks of
-// four, each in or out as a whole.
+// false, read as -inf.  at: the group's first logit.
 template <int V>
-SFP8_DEV void load_logits(float (&l)[V], const void* p, int dtype, bool vec, int64_t at, const RouteLayout& lay, bool on) {
+SFP8_DEV void load_logits(float (&l)[V], const void* p, int dtype, int64_t at, const RouteLayout& lay, bool on) {
   const float ninf = -__builtin_inff();
-  if (vec && lay.gs == lay.G * V && __all(on)) {  // nothing to leave out
+  if (lay.gs == lay.G * V && __all(on)) {  // nothing to leave out
     if (dtype == kF32) {  // uniform, once: the loads go out together
 #pragma unroll
       for (int c = 0; c < V / 4; ++c) load4(*reinterpret_cast<float(*)[4]>(l + 4 * c), p, kF32, at + lay.member(c));
@@ -172,11 +177,11 @@ SFP8_DEV void load_logits(float (&l)[V], const void* p, int dtype, bool vec, int
 #pragma unroll
   for (int c = 0; c < V / 4; ++c) {
     const int m = lay.member(c);
-    if (vec) {
-      if (m < lay.gs) load4(*reinterpret_cast<float(*)[4]>(l + 4 * c), p, dtype, at + m);
+    if (m + 4 <= lay.gs) {
+      load4(*reinterpret_cast<float(*)[4]>(l + 4 * c), p, dtype, at + m);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 3; ++i)
         if (m + i < lay.gs) l[4 * c + i] = load_as_f32(p, dtype, at + m + i);
     }
   }
@@ -362,8 +367,7 @@ SFP8_DEV float sigmoid_of(float x) {
 }
 
 template <int L, int V, bool BIAS>
-__global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, int log_g, int gs, int idx_bits,
-                                                           bool vec, bool vec_bias) {
+__global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, int log_g, int gs, int idx_bits) {
   extern __shared__ __align__(16) uint64_t lds[];
   constexpr int kTok = 64 / L;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -382,7 +386,7 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
   const bool on = t0 + tok < a.T && !(a.mask && !a.mask[t0 + tok]);
   const int64_t row = t0 * a.ld + tok * a.ld;
   float l[V];
-  load_logits<V>(l, a.logits, a.dtype, vec, row + first, lay, on && in_group);
+  load_logits<V>(l, a.logits, a.dtype, row + first, lay, on && in_group);
   float mine_max = max_nan<V>(l);             // NaN if one is
   bool odd = !(mine_max < __builtin_inff());  // selected again in 64 bits
   float m = ninf, z = 1.0f;
@@ -399,7 +403,7 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
   if constexpr (BIAS) {
     const float rz = __builtin_amdgcn_rcpf(z);
     float bias[V];
-    load_logits<V>(bias, a.bias, kF32, vec_bias, first, lay, in_group);
+    load_logits<V>(bias, a.bias, kF32, first, lay, in_group);
 #pragma unroll
     for (int c = 0; c < V / 4; ++c)
 #pragma unroll
@@ -674,7 +678,7 @@ struct RouteBwdArgs {
 // the dense part, then the slots' values) and written whole, once: bound by
 // those bytes.
 template <int L, int V>
-__global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a, bool vec_in, bool vec_out) {
+__global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a) {
   __shared__ __align__(16) float rows[256 * V];
   constexpr int kTok = 64 / L;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tl = lane & (L - 1);
@@ -695,7 +699,7 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
   for (int j = 0; j < V; ++j) d[j] = 0.0f;
   if (dense) {
     float l[V], m = ninf, z = 0.0f;
-    load_logits<V>(l, a.logits, a.dtype, vec_in, t * a.ld, lay, on);
+    load_logits<V>(l, a.logits, a.dtype, t * a.ld, lay, on);
 #pragma unroll
     for (int j = 0; j < V; ++j) m = fmaxf(m, l[j]);
     m = lanes_max<L>(m);
@@ -739,16 +743,16 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
     if (mem >= a.E) continue;
     const floatx4 v = *reinterpret_cast<const floatx4*>(row + mem);
     const int64_t at = t * a.E + mem;
-    if (vec_out && a.dtype == kF32) {
-      *reinterpret_cast<floatx4*>(reinterpret_cast<float*>(a.dlogits) + at) = v;
-    } else if (vec_out) {
+    if (mem + 4 <= a.E && a.dtype == kF32) {
+      *reinterpret_cast<floatx4_any*>(reinterpret_cast<float*>(a.dlogits) + at) = v;
+    } else if (mem + 4 <= a.E) {
       const intx2 o = a.dtype == kBf16 ? intx2{(int)pack2_bf16(v[0], v[1]), (int)pack2_bf16(v[2], v[3])}
                                        : intx2{(int)(f32_to_half_bits(v[0]) | f32_to_half_bits(v[1]) << 16),
                                                (int)(f32_to_half_bits(v[2]) | f32_to_half_bits(v[3]) << 16)};
-      *reinterpret_cast<intx2*>(reinterpret_cast<uint16_t*>(a.dlogits) + at) = o;
+      *reinterpret_cast<intx2_any*>(reinterpret_cast<uint16_t*>(a.dlogits) + at) = o;
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 3; ++i)
         if (mem + i < a.E) store_f32_as(a.dlogits, a.dtype, at + i, v[i]);
     }
   }
@@ -908,23 +912,32 @@ __global__ __launch_bounds__(kOrderThreads) void moe_order_place_kernel(
 // slot order and rounded once; slots whose row is out of range add nothing.
 // `lanes` lanes (a power of two) take one token, U elements at a time.
 // ---------------------------------------------------------------------------
-template <int DT, bool VEC>
+// How a row is cut into units: one element each (rows shorter than 16 bytes),
+// whole aligned 16-byte units, or 16 bytes at any address, where the last unit
+// of a row ends with it and so may hold elements of the one before.
+enum : int { kSingle = 0, kWhole = 1, kAny = 2 };
+
+template <int DT, int CUT>
 struct Unit {  // U consecutive elements as fp32
-  static constexpr int U = VEC ? (DT == kF32 ? 4 : 8) : 1;
+  static constexpr int U = CUT == kSingle ? 1 : DT == kF32 ? 4 : 8;
   float x[U];
+  // First element of the unit that would start at d; the elements before d - first are another unit's too.
+  SFP8_DEV static int64_t first(int64_t d, int64_t D) { return CUT == kAny && d > D - U ? D - U : d; }
   // as they are in memory: what a load in flight holds
   struct Raw {
     intx4 v;
     SFP8_DEV void load(const void* p, int64_t i) {
-      if constexpr (!VEC) {
+      if constexpr (CUT == kSingle) {
         v[0] = DT == kF32 ? reinterpret_cast<const int*>(p)[i] : reinterpret_cast<const uint16_t*>(p)[i];
       } else {
-        v = *reinterpret_cast<const intx4*>(reinterpret_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2));
+        const char* at = reinterpret_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2);
+        if constexpr (CUT == kWhole) v = *reinterpret_cast<const intx4*>(at);
+        else v = *reinterpret_cast<const intx4_any*>(at);
       }
     }
     // the same of data that is read once
     SFP8_DEV void load_once(const void* p, int64_t i) {
-      if constexpr (!VEC) load(p, i);
+      if constexpr (CUT != kWhole) load(p, i);
       else v = __builtin_nontemporal_load(
           reinterpret_cast<const intx4*>(reinterpret_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2)));
     }
@@ -945,7 +958,7 @@ struct Unit {  // U consecutive elements as fp32
   // ONCE: past the caches
   template <bool ONCE = false>
   SFP8_DEV void store(void* p, int64_t i) const {
-    if constexpr (!VEC) {
+    if constexpr (CUT == kSingle) {
       store_f32_as(p, DT, i, x[0]);
     } else {
       intx4 o;
@@ -955,9 +968,10 @@ struct Unit {  // U consecutive elements as fp32
         else if constexpr (DT == kBf16) o[q] = (int)pack2_bf16(x[2 * q], x[2 * q + 1]);
         else o[q] = (int)(f32_to_half_bits(x[2 * q]) | f32_to_half_bits(x[2 * q + 1]) << 16);
       }
-      intx4* at = reinterpret_cast<intx4*>(reinterpret_cast<char*>(p) + i * (DT == kF32 ? 4 : 2));
-      if constexpr (ONCE) __builtin_nontemporal_store(o, at);
-      else *at = o;
+      char* at = reinterpret_cast<char*>(p) + i * (DT == kF32 ? 4 : 2);
+      if constexpr (CUT == kAny) *reinterpret_cast<intx4_any*>(at) = o;
+      else if constexpr (ONCE) __builtin_nontemporal_store(o, reinterpret_cast<intx4*>(at));
+      else *reinterpret_cast<intx4*>(at) = o;
     }
   }
 };
@@ -966,12 +980,12 @@ struct Unit {  // U consecutive elements as fp32
 // where those are fewer than a wave's, else whole waves.  K slots' rows are in
 // flight at once.  Bound by the rows' bytes; for few tokens by two dependent
 // loads, which one unit a lane keeps from repeating.
-template <int DT, bool VEC, int K, bool NT>
+template <int DT, int CUT, int K, bool NT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict__ rows, int64_t R, int64_t D,
                                                           const float* __restrict__ weights,
                                                           const int64_t* __restrict__ inv, int64_t T, int k,
                                                           void* __restrict__ out, int lanes, int waves) {
-  using X = Unit<DT, VEC>;
+  using X = Unit<DT, CUT>;
   int64_t t, d0, step;
   if (lanes == 64) {  // `waves` waves a token
     const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -985,7 +999,8 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
     step = (int64_t)lanes * X::U;
   }
   if (t >= T) return;
-  for (int64_t d = d0; d < D; d += step) {  // once, but for launches beyond 2^32 work-items
+  for (int64_t at = d0; at < D; at += step) {  // once, but for launches beyond 2^32 work-items
+    const int64_t d = X::first(at, D);
     X acc;
 #pragma unroll
     for (int q = 0; q < X::U; ++q) acc.x[q] = 0.0f;
@@ -1023,12 +1038,12 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
 // (either may be null); rows from offsets[E - 1] on, which no slot names, get
 // zeros.  One wave a slot: the waves of a token share its gradient through the
 // caches.  Bound by the rows' bytes, read and written.
-template <int DT, bool VEC, bool NT>
+template <int DT, int CUT, bool NT>
 __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
     const void* __restrict__ dout, const void* __restrict__ rows, int64_t R, int64_t D,
     const float* __restrict__ weights, const int64_t* __restrict__ inv, int64_t slots, int k,
     const int* __restrict__ offsets, int E, void* __restrict__ drows, float* __restrict__ dweights) {
-  using X = Unit<DT, VEC>;
+  using X = Unit<DT, CUT>;
   const int lane = threadIdx.x & 63;
   const int64_t gw = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), nw = (int64_t)gridDim.x * 4;
   for (int64_t s = gw; s < slots; s += nw) {
@@ -1037,7 +1052,8 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
     if (r >= 0 && r < R) {
       const float w = weights[s];
 #pragma unroll 2
-      for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) {
+      for (int64_t at = (int64_t)lane * X::U; at < D; at += 64 * X::U) {
+        const int64_t d = X::first(at, D);
         typename X::Raw rg, rv;
         rg.load(dout, t * D + d);
         if (dweights) NT ? rv.load_once(rows, r * D + d) : rv.load(rows, r * D + d);
@@ -1045,7 +1061,8 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
         if (dweights) {
           const X v(rv);
 #pragma unroll
-          for (int q = 0; q < X::U; ++q) dot = __builtin_fmaf(g.x[q], v.x[q], dot);
+          for (int q = 0; q < X::U; ++q)
+            dot = CUT != kAny || q >= at - d ? __builtin_fmaf(g.x[q], v.x[q], dot) : dot;
         }
         if (drows) {
 #pragma unroll
@@ -1066,7 +1083,7 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
 #pragma unroll
   for (int q = 0; q < X::U; ++q) zero.x[q] = 0.0f;
   for (int64_t r = used + gw; r < R; r += nw)
-    for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) zero.store(drows, r * D + d);
+    for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) zero.store(drows, r * D + X::first(d, D));
 }
 
 }  // namespace sfp8
@@ -1094,12 +1111,20 @@ int route_allow_lds(K kernel, size_t bytes) {
   return e == hipSuccess ? kOk : (int)e;
 }
 
-// Calls f<dtype, whole 16-byte units>.
-template <template <int, bool> class F, typename... A>
-void by_type(int dtype, bool vec, A... args) {
-  if (dtype == kF32) vec ? F<kF32, true>::run(args...) : F<kF32, false>::run(args...);
-  else if (dtype == kBf16) vec ? F<kBf16, true>::run(args...) : F<kBf16, false>::run(args...);
-  else vec ? F<kF16, true>::run(args...) : F<kF16, false>::run(args...);
+// Calls F<dtype, cut>.
+template <template <int, int> class F, int DT, typename... A>
+void by_cut(int cut, A... args) {
+  cut == kWhole ? F<DT, kWhole>::run(args...) : cut == kAny ? F<DT, kAny>::run(args...) : F<DT, kSingle>::run(args...);
+}
+template <template <int, int> class F, typename... A>
+void by_type(int dtype, int cut, A... args) {
+  if (dtype == kF32) by_cut<F, kF32>(cut, args...);
+  else if (dtype == kBf16) by_cut<F, kBf16>(cut, args...);
+  else by_cut<F, kF16>(cut, args...);
+}
+int row_cut(int dtype, int64_t D, bool aligned) {
+  const int64_t unit = dtype == kF32 ? 4 : 8;
+  return D < unit ? kSingle : D % unit == 0 && aligned ? kWhole : kAny;
 }
 
 // Lanes of a token and of a group, and values of a lane: the fewest lanes that
@@ -1122,30 +1147,19 @@ template <int L, int V>
 void route_run(const RouteArgs& a, const RouteShape& sh, hipStream_t st) {
   int idx_bits = 8;  // at least: a rank's mantissa then leaves its exponent behind (moe_route_kernel)
   while ((1 << idx_bits) < a.E) ++idx_bits;
-  const uintptr_t unit = a.dtype == kF32 ? 16 : 8;  // four logits
-  const bool vec = (a.E / a.groups) % 4 == 0 && (a.ld % 4 == 0 || a.T == 1) && (uintptr_t)a.logits % unit == 0;
   const int64_t per = 4 * (64 / L);  // tokens of a work-group
   const dim3 grid((unsigned)((a.T + per - 1) / per));
   const size_t lds = 4 * (size_t)((3 * a.E + 1) / 2) * 8;  // of each wave: an order value and a logit per expert
   const int gs = a.E / a.groups;
   int log_g = 0;
   while ((1 << log_g) < sh.G) ++log_g;
-  const bool vec_bias = (a.E / a.groups) % 4 == 0 && (uintptr_t)a.bias % 16 == 0;
-  if (a.bias)
-    hipLaunchKernelGGL((moe_route_kernel<L, V, true>), grid, dim3(256), lds, st, a, log_g, gs, idx_bits, vec,
-                       vec_bias);
-  else
-    hipLaunchKernelGGL((moe_route_kernel<L, V, false>), grid, dim3(256), lds, st, a, log_g, gs, idx_bits, vec,
-                       vec_bias);
+  if (a.bias) hipLaunchKernelGGL((moe_route_kernel<L, V, true>), grid, dim3(256), lds, st, a, log_g, gs, idx_bits);
+  else hipLaunchKernelGGL((moe_route_kernel<L, V, false>), grid, dim3(256), lds, st, a, log_g, gs, idx_bits);
 }
 template <int L, int V>
 void route_run(const RouteBwdArgs& a, const RouteShape&, hipStream_t st) {
-  const uintptr_t unit = a.dtype == kF32 ? 16 : 8;
-  const bool vec_in = a.E % 4 == 0 && (a.ld % 4 == 0 || a.T == 1) && (uintptr_t)a.logits % unit == 0;
-  const bool vec_out = a.E % 4 == 0 && (uintptr_t)a.dlogits % unit == 0;
   const int64_t per = 4 * (64 / L);
-  hipLaunchKernelGGL((moe_route_bwd_kernel<L, V>), dim3((unsigned)((a.T + per - 1) / per)), dim3(256), 0, st, a, vec_in,
-                     vec_out);
+  hipLaunchKernelGGL((moe_route_bwd_kernel<L, V>), dim3((unsigned)((a.T + per - 1) / per)), dim3(256), 0, st, a);
 }
 template <int L, class Args>
 void route_run_l(const Args& a, const RouteShape& sh, hipStream_t st) {
@@ -1179,12 +1193,12 @@ void route_bwd_launch(const RouteBwdArgs& a, hipStream_t st) { route_by_shape(a,
 // 39, 272 53 and 55, 320 51 and 61, 480 80 and 98, 640 102 and 129, 1088 211 and 225.
 constexpr int64_t kLastLevelCache = (int64_t)256 << 20;
 
-template <int DT, bool VEC>
+template <int DT, int CUT>
 struct Combine {
   template <int K>
   static void go(const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv, int64_t T, int k, void* out,
                  hipStream_t st) {
-    constexpr int U = Unit<DT, VEC>::U;
+    constexpr int U = Unit<DT, CUT>::U;
     const int64_t units = (D + U - 1) / U, most = ((int64_t)1 << 25) / T;  // waves: 2^31 work-items
     const int64_t waves = (units + 63) / 64 < most ? (units + 63) / 64 : most;
     int lanes = 64;
@@ -1194,8 +1208,9 @@ struct Combine {
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, rows, R, D, w, inv, T, k, out, lanes,
                          (int)waves);
     };
-    if (VEC && (R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache) launch(moe_combine_kernel<DT, VEC, K, VEC>);
-    else launch(moe_combine_kernel<DT, VEC, K, false>);
+    constexpr bool kPast = CUT == kWhole;
+    if (kPast && (R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache) launch(moe_combine_kernel<DT, CUT, K, kPast>);
+    else launch(moe_combine_kernel<DT, CUT, K, false>);
   }
   static void run(const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv, int64_t T, int k,
                   void* out, hipStream_t st) {
@@ -1206,7 +1221,7 @@ struct Combine {
   }
 };
 
-template <int DT, bool VEC>
+template <int DT, int CUT>
 struct CombineBwd {
   static void run(const void* dout, const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv,
                   int64_t T, int k, const int* offsets, int E, void* drows, float* dw, hipStream_t st) {
@@ -1216,8 +1231,9 @@ struct CombineBwd {
       hipLaunchKernelGGL(kernel, dim3((unsigned)nb), dim3(256), 0, st, dout, rows, R, D, w, inv, slots, k, offsets, E,
                          drows, dw);
     };
-    if (VEC && (2 * R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache) launch(moe_combine_bwd_kernel<DT, VEC, VEC>);
-    else launch(moe_combine_bwd_kernel<DT, VEC, false>);
+    constexpr bool kPast = CUT == kWhole;
+    if (kPast && (2 * R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache) launch(moe_combine_bwd_kernel<DT, CUT, kPast>);
+    else launch(moe_combine_bwd_kernel<DT, CUT, false>);
   }
 };
 }  // namespace
@@ -1286,8 +1302,8 @@ int sfp8_moe_combine(const void* rows, int dtype, int64_t R, int64_t D, const fl
   if (R < 0 || T < 0 || T > kMaxTokens || D <= 0 || top_k <= 0 || top_k > kRouteMaxK || bad_dtype(dtype))
     return kErrBadShape;
   if (T == 0) return kOk;
-  const bool vec = D % (dtype == kF32 ? 4 : 8) == 0 && al16(rows) && al16(out);
-  by_type<Combine>(dtype, vec, rows, R, D, weights, inverse, T, (int)top_k, out, (hipStream_t)stream);
+  const int cut = row_cut(dtype, D, al16(rows) && al16(out));
+  by_type<Combine>(dtype, cut, rows, R, D, weights, inverse, T, (int)top_k, out, (hipStream_t)stream);
   return route_status();
 }
 
@@ -1299,8 +1315,8 @@ int sfp8_moe_combine_bwd(const void* dout, const void* rows, int dtype, int64_t 
   if (R < 0 || T < 0 || T > kMaxTokens || D <= 0 || top_k <= 0 || top_k > kRouteMaxK || bad_dtype(dtype) || E <= 0)
     return kErrBadShape;
   if ((T == 0 && R == 0) || (!drows && !dweights)) return kOk;
-  const bool vec = D % (dtype == kF32 ? 4 : 8) == 0 && al16(rows) && al16(dout) && al16(drows);
-  by_type<CombineBwd>(dtype, vec, dout, rows, R, D, weights, inverse, T, (int)top_k, offsets, (int)E, drows, dweights,
+  const int cut = row_cut(dtype, D, al16(rows) && al16(dout) && al16(drows));
+  by_type<CombineBwd>(dtype, cut, dout, rows, R, D, weights, inverse, T, (int)top_k, offsets, (int)E, drows, dweights,
                       (hipStream_t)stream);
   return route_status();
 }
