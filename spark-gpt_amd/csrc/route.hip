@@ -351,6 +351,12 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
 //
 // A token's result depends on its row and on E, top_k and the groups alone,
 // not on the batch it comes in.
+//
+// Bound by its vector instructions: 65536 tokens, 8 of 256 experts, fp32 19.5 us
+// (15 for the bytes), 545 instructions a wave of four tokens, 300 of them in the
+// selection; bf16 17.5; with sigmoid scores, a bias and groups 34 (998).  16
+// lanes of 16 logits take fewer of them a token than 64 of 4 (the lane steps are
+// shared by four tokens).
 // ---------------------------------------------------------------------------
 template <int V>
 SFP8_DEV float max_nan(const float (&x)[V]) {
@@ -676,7 +682,7 @@ struct RouteBwdArgs {
 // its expert, from the chosen logits alone; the plain softmax also reads the
 // row again, for p of every expert.  The row is put together in LDS (zeros or
 // the dense part, then the slots' values) and written whole, once: bound by
-// those bytes.
+// those bytes (65536 x 256 fp32 13.3 us, 5.0 TB/s; 65536 x 8 bf16 3.2).
 template <int L, int V>
 __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a) {
   __shared__ __align__(16) float rows[256 * V];
@@ -764,8 +770,10 @@ __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a
 // slots, wave w of it the w-th sixteenth.  One launch counts each group's bins;
 // in the second every group adds up the counts itself (at most 256 rows of E +
 // 1, from the L2), which is cheaper than a third launch that would scan them.
-// Up to 4096 slots are one group and one launch.  Bound by its launches: the
-// bytes are 24 a slot.
+// Up to 4096 slots are one group and one launch.  Bound by its launches and by
+// the chain of steps of the second (counts, sums, places), 24 bytes a slot are a
+// sixth of the time: 524288 slots of 256 experts 15.2 us, 131072 of 8 9.2, 64 of
+// 128 4.2.
 // ---------------------------------------------------------------------------
 constexpr int kOrderWaves = 16;
 constexpr int kOrderThreads = 64 * kOrderWaves;
@@ -937,9 +945,10 @@ struct Unit {  // U consecutive elements as fp32
     }
     // the same of data that is read once
     SFP8_DEV void load_once(const void* p, int64_t i) {
-      if constexpr (CUT != kWhole) load(p, i);
-      else v = __builtin_nontemporal_load(
-          reinterpret_cast<const intx4*>(reinterpret_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2)));
+      const char* at = reinterpret_cast<const char*>(p) + i * (DT == kF32 ? 4 : 2);
+      if constexpr (CUT == kSingle) load(p, i);
+      else if constexpr (CUT == kWhole) v = __builtin_nontemporal_load(reinterpret_cast<const intx4*>(at));
+      else v = __builtin_nontemporal_load(reinterpret_cast<const intx4_any*>(at));
     }
   };
   SFP8_DEV Unit() = default;
@@ -969,7 +978,8 @@ struct Unit {  // U consecutive elements as fp32
         else o[q] = (int)(f32_to_half_bits(x[2 * q]) | f32_to_half_bits(x[2 * q + 1]) << 16);
       }
       char* at = reinterpret_cast<char*>(p) + i * (DT == kF32 ? 4 : 2);
-      if constexpr (CUT == kAny) *reinterpret_cast<intx4_any*>(at) = o;
+      if constexpr (CUT == kAny && ONCE) __builtin_nontemporal_store(o, reinterpret_cast<intx4_any*>(at));
+      else if constexpr (CUT == kAny) *reinterpret_cast<intx4_any*>(at) = o;
       else if constexpr (ONCE) __builtin_nontemporal_store(o, reinterpret_cast<intx4*>(at));
       else *reinterpret_cast<intx4*>(at) = o;
     }
@@ -978,8 +988,9 @@ struct Unit {  // U consecutive elements as fp32
 
 // One unit a lane: `lanes` (a power of two) lanes for the D / U units of a token
 // where those are fewer than a wave's, else whole waves.  K slots' rows are in
-// flight at once.  Bound by the rows' bytes; for few tokens by two dependent
-// loads, which one unit a lane keeps from repeating.
+// flight at once.  Bound by the rows' bytes (65536 tokens of 2 rows of 1024 67
+// us, 6.0 TB/s; of 1022, at odd addresses, 70); for few tokens by two dependent
+// loads, which one unit a lane keeps from repeating (8 tokens of 8 of 2048 3.2).
 template <int DT, int CUT, int K, bool NT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict__ rows, int64_t R, int64_t D,
                                                           const float* __restrict__ weights,
@@ -1036,23 +1047,29 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
 
 // drows[inv[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], rows[inv[t, j]]>
 // (either may be null); rows from offsets[E - 1] on, which no slot names, get
-// zeros.  One wave a slot: the waves of a token share its gradient through the
-// caches.  Bound by the rows' bytes, read and written.
-template <int DT, int CUT, bool NT>
+// zeros.  One wave a slot, or `lanes` lanes (a power of two) where a row has
+// fewer units: the lanes of a token's slots share its gradient through the
+// caches.  Bound by the rows' bytes, read and written (65536 tokens of 2 rows of
+// 1024 99 us, 6.8 TB/s; 131072 of 2 of 128 28, in whole waves 53).
+template <int DT, int CUT, bool NT, bool WIDE>
 __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
     const void* __restrict__ dout, const void* __restrict__ rows, int64_t R, int64_t D,
     const float* __restrict__ weights, const int64_t* __restrict__ inv, int64_t slots, int k,
-    const int* __restrict__ offsets, int E, void* __restrict__ drows, float* __restrict__ dweights) {
+    const int* __restrict__ offsets, int E, void* __restrict__ drows, float* __restrict__ dweights, int lanes) {
   using X = Unit<DT, CUT>;
-  const int lane = threadIdx.x & 63;
-  const int64_t gw = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), nw = (int64_t)gridDim.x * 4;
-  for (int64_t s = gw; s < slots; s += nw) {
-    const int64_t t = (uint32_t)s / (uint32_t)k, r = inv[s];
+  const int per = WIDE ? 1 : 64 / lanes;  // slots of a wave
+  const int sub = WIDE ? threadIdx.x & 63 : threadIdx.x & (lanes - 1);
+  const int64_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int64_t first = wave * per + (WIDE ? 0 : (threadIdx.x & 63) / lanes), step = (int64_t)gridDim.x * 4 * per;
+  const int64_t stride = (int64_t)(WIDE ? 64 : lanes) * X::U;
+  for (int64_t s = first; s - first < slots - wave * per; s += step) {  // the lanes of a wave together
+    const bool in = s < slots;
+    const int64_t t = (uint32_t)s / (uint32_t)k, r = in ? inv[s] : -1;
     float dot = 0.0f;
     if (r >= 0 && r < R) {
       const float w = weights[s];
 #pragma unroll 2
-      for (int64_t at = (int64_t)lane * X::U; at < D; at += 64 * X::U) {
+      for (int64_t at = (int64_t)sub * X::U; at < D; at += stride) {
         const int64_t d = X::first(at, D);
         typename X::Raw rg, rv;
         rg.load(dout, t * D + d);
@@ -1072,8 +1089,10 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
       }
     }
     if (dweights) {
-      dot = lanes_sum<64>(dot);
-      if (lane == 0) dweights[s] = dot;
+      if constexpr (WIDE) dot = lanes_sum<64>(dot);
+      else
+        for (int o = 1; o < lanes; o <<= 1) dot += __shfl_xor(dot, o, 64);
+      if (in && sub == 0) dweights[s] = dot;
     }
   }
   if (!drows) return;
@@ -1082,8 +1101,8 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
   X zero;
 #pragma unroll
   for (int q = 0; q < X::U; ++q) zero.x[q] = 0.0f;
-  for (int64_t r = used + gw; r < R; r += nw)
-    for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) zero.store(drows, r * D + X::first(d, D));
+  for (int64_t r = used + first; r < R; r += step)
+    for (int64_t d = (int64_t)sub * X::U; d < D; d += stride) zero.store(drows, r * D + X::first(d, D));
 }
 
 }  // namespace sfp8
@@ -1208,7 +1227,7 @@ struct Combine {
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, rows, R, D, w, inv, T, k, out, lanes,
                          (int)waves);
     };
-    constexpr bool kPast = CUT == kWhole;
+    constexpr bool kPast = CUT != kSingle;
     if (kPast && (R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache) launch(moe_combine_kernel<DT, CUT, K, kPast>);
     else launch(moe_combine_kernel<DT, CUT, K, false>);
   }
@@ -1225,15 +1244,24 @@ template <int DT, int CUT>
 struct CombineBwd {
   static void run(const void* dout, const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv,
                   int64_t T, int k, const int* offsets, int E, void* drows, float* dw, hipStream_t st) {
+    constexpr int U = Unit<DT, CUT>::U;
+    int lanes = 64;
+    while (lanes > 1 && (int64_t)(lanes / 2) * U >= D) lanes /= 2;
     const int64_t slots = T * k, work = slots > 0 ? slots : R, most = (int64_t)1 << 22;
-    const int64_t nb = (work + 3) / 4 < most ? (work + 3) / 4 : most;
+    const int64_t per = 4 * (64 / lanes), need = (work + per - 1) / per, nb = need < most ? need : most;
     const auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)nb), dim3(256), 0, st, dout, rows, R, D, w, inv, slots, k, offsets, E,
-                         drows, dw);
+                         drows, dw, lanes);
     };
-    constexpr bool kPast = CUT == kWhole;
-    if (kPast && (2 * R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache) launch(moe_combine_bwd_kernel<DT, CUT, kPast>);
-    else launch(moe_combine_bwd_kernel<DT, CUT, false>);
+    constexpr bool kPast = CUT != kSingle;
+    const bool past = kPast && (2 * R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache;
+    if (lanes == 64) {
+      if (past) launch(moe_combine_bwd_kernel<DT, CUT, kPast, true>);
+      else launch(moe_combine_bwd_kernel<DT, CUT, false, true>);
+    } else {
+      if (past) launch(moe_combine_bwd_kernel<DT, CUT, kPast, false>);
+      else launch(moe_combine_bwd_kernel<DT, CUT, false, false>);
+    }
   }
 };
 }  // namespace
