@@ -344,10 +344,12 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
 // the definition in 64 bits (route_exact), as it is for rows with NaN or +inf.
 // Without a bias that takes two logits that differ on one step of the
 // scale (equal ones are in the order of their indices): about 1 of 10^4 tokens
-// at 256 normal logits.  With one, scores are off: a softmax by at most
-// (2.5 |d| + 30) 2^-24 of itself, below 2^-19 in all (d is the exponent's
-// argument, |d| e^-|d| < 0.4), a sigmoid, which has no sum over the experts, by
-// at most 2^-21; the sums with the bias round once more.
+// at 256 normal logits.  With one, scores are off.  An exponential of d is by
+// (2.5 |d| + 2) 2^-24 of itself (the argument, its product with log2(e), that
+// constant; exp2).  A softmax adds its sum, off by the terms' own errors (their
+// mean |d| is at most log(1024)) and up to 37 additions in a row, and the quotient: by
+// less than 64 2^-24 of the row's largest probability, 1 / z, in all (|d| e^-|d| <
+// 0.4).  A sigmoid is off by less than 2^-21.  The sums with the bias round once more.
 //
 // A token's result depends on its row and on E, top_k and the groups alone,
 // not on the batch it comes in.
@@ -405,9 +407,10 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
   }
   // the order values
   float o[V];
-  const float err = !BIAS ? 0.0f : softmax ? 0x1p-19f : 0x1p-21f;  // how far a score may be off
+  float err = 0.0f;  // how far a score may be off
   if constexpr (BIAS) {
     const float rz = __builtin_amdgcn_rcpf(z);
+    err = softmax ? 0x1p-18f * rz : 0x1p-21f;
     float bias[V];
     load_logits<V>(bias, a.bias, kF32, first, lay, in_group);
 #pragma unroll

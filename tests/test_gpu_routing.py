@@ -178,11 +178,21 @@ def test_route_close_scores(dev):
     g = torch.Generator(device=dev).manual_seed(2)
     E, T = 64, 256
     low = torch.randn(T, E, device=dev, generator=g)
-    # every score within a few 1e-8 of 1/2, in steps of 2^-30
+    # every score within a few 1e-8 of 1/2 (of 1/64), in steps of 2^-30 (2^-34), and biases in
+    # steps that have no common measure with them: two experts are the same or differ by more
+    # than a twentieth of a step, far above the errors of 64 bits
     low = torch.round(low * 8) * 2.0 ** -28
-    bias = torch.randint(-4, 4, (E,), device=dev, generator=g) * 2.0 ** -31
+    steps = torch.randint(-4, 4, (E,), device=dev, generator=g) * 2.0 ** 0.5
+    # sums of two such scores do tie: e^a + e^b and e^c + e^d with a + b = c + d differ by 2^-57 of
+    # themselves at these sizes, which 64 bits (2^-53) do not hold.  For sums the logits are
+    # continuous: two of them come within 2^-41 in a thousand borders, 2^12 times what 64 bits hold
+    loose = torch.randn(T, E, device=dev, generator=g) * 2.0 ** -26
     for groups, best in ((1, 1), (8, 1), (8, 2)):
-        _run(low, 8, bias=bias, score="sigmoid", groups=groups, top_groups=max(1, groups // 2), group_best=best)
+        x = low if best == 1 else loose
+        kw = dict(groups=groups, top_groups=max(1, groups // 2), group_best=best)
+        _run(x, 8, bias=steps * 2.0 ** -31, score="sigmoid", **kw)
+        _run(x, 8, bias=steps * 2.0 ** -35, score="softmax", **kw)
+        _run(x, 8, torch.ones(T, 8, device=dev), score="softmax", **kw)
     far = torch.randn(T, E, device=dev, generator=g) * 1e-3 + 20.0  # 1 - s of about 2e-9
     _run(far, 8, bias=torch.zeros(E, device=dev), score="sigmoid")
     _run(far, 8, score="sigmoid")
