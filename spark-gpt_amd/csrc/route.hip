@@ -508,7 +508,8 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
       kept = in_group && v != ninf && place < a.top_groups;
     }
   }
-  // the keys: rank << idx_bits, and the inverted index
+  // the keys: rank << idx_bits, and the inverted index (a padding lane's index may
+  // be past the mask: its key wraps to one that comes after all others)
   const uint32_t idx_mask = (1u << idx_bits) - 1, idx_top = idx_mask - (uint32_t)first;
   uint32_t key[V], least;  // keys from `least` on can be taken
   float gap = 0.0f;        // ranks that are no further apart may be in the wrong order
@@ -541,10 +542,12 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
     const float range = hi - lo;
     // below 2^(31 - idx_bits) at the largest value, by two steps and the quotient's 2^-22
     const float steps = (float)(1u << (31 - idx_bits)) * (1.0f - 0x1p-19f) - 4.0f;
-    const float scale = kept && range > 0.0f ? steps * __builtin_amdgcn_rcpf(range) : 0.0f;
+    // A range outside 2^+-100 is left to 64 bits, and its keys are all alike: a scale
+    // that overflows would take a rank past 31 bits, among the keys that wrap.
+    const bool fits = range > 0x1p-100f && range < 0x1p100f;
+    odd |= range > 0.0f && !fits;
+    const float scale = kept && fits ? steps * __builtin_amdgcn_rcpf(range) : 0.0f;
     const float base = kept ? 0x1p23f + 1.0f : 0x1p23f;
-    // a range outside 2^+-100 is left to 64 bits
-    odd |= range > 0.0f && !(range > 0x1p-100f && range < 0x1p100f);
     // a value's error, and three steps for the scale's own roundings
     if constexpr (BIAS) gap = 2.0f * (err + 0x1p-23f * fmaxf(fabsf(lo), fabsf(hi))) * lanes_max<L>(scale) + 3.0f;
 #pragma unroll

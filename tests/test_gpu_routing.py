@@ -161,6 +161,28 @@ def test_route_special_rows(dev, score, E, groups, with_bias, dtype):
                 _run(low[fine], k, dw, bias=bias, renormalize=renorm, **kw)
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,top_groups,k", [(8, 1, 1, 2), (60, 1, 1, 4), (1000, 1, 1, 10), (1023, 33, 9, 10),
+                                                   (1000, 20, 7, 64), (126, 63, 20, 33), (96, 3, 2, 8)])
+def test_route_tiny_and_huge_differences(dev, score, E, groups, top_groups, k):
+    """Rows whose largest difference is subnormal, or so large that its reciprocal is."""
+    g = torch.Generator().manual_seed(E + k)
+    step = torch.randint(0, 4, (6, E), generator=g).float()
+    one = torch.zeros(2, E)
+    one[0, E - 1] = one[1, E // 2] = 1.0
+    step = torch.cat([step, one])
+    low = torch.cat([step * v for v in (2.0 ** -149, 2.0 ** -140, 2.0 ** -128, 2.0 ** -126, 2.0 ** -101, 2.0 ** -99,
+                                        2.0 ** 99, 2.0 ** 101, 2.0 ** 125)])
+    low = torch.cat([low, low - 2.0 ** 126]).to(dev)
+    _run(low, k, score=score, groups=groups, top_groups=top_groups)
+    # scores that are all 0, so that biases alone differ, by the smallest steps and the largest
+    if score == "sigmoid":
+        flat = torch.full((5, E), -1e30, device=dev)
+        for v in (2.0 ** -149, 2.0 ** -128, 2.0 ** -101, 2.0 ** 125):
+            for best in (1, 2) if groups > 1 else (1,):
+                _run(flat, k, bias=step[0].to(dev) * v, score=score, groups=groups, top_groups=top_groups, group_best=best)
+
+
 def test_route_bias_special(dev):
     """A bias of -inf takes an expert out, +inf puts it first, NaN ranks above."""
     low = _logits(dev, 20, 16, torch.float32, 5)
