@@ -107,9 +107,10 @@ def test_route_groups_and_bias(dev, score, groups, top_groups, best, with_bias, 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("E,groups,top_groups,k", [(1023, 3, 2, 8), (1023, 33, 9, 10), (1000, 20, 7, 64), (1020, 5, 1, 6),
                                                    (1024, 64, 32, 3), (1024, 8, 4, 8), (126, 63, 20, 33), (992, 31, 30, 1)])
-def test_route_many_experts_in_groups(dev, score, E, groups, top_groups, k):
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_route_many_experts_in_groups(dev, score, E, groups, top_groups, k, dtype):
     """Group counts that are no power of two, of up to 1024 experts."""
-    low = _logits(dev, 23, E, torch.float32, E + groups)
+    low = _logits(dev, 23, E, DTYPES[dtype], E + groups)
     bias = torch.randn(E, device=dev, generator=torch.Generator(device=dev).manual_seed(E)) * 0.05
     for best in (1, 2):
         for b in (None, bias):
