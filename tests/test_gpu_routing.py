@@ -608,6 +608,45 @@ def test_captured_and_replayed(dev):
             assert all(torch.equal(a, b) for a, b in zip(outs, want)), (rep, i)
 
 
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True)])
+def test_gradients_captured_and_replayed(dev, score, renorm):
+    """The layer's steps and their gradients, through autograd, captured into a
+    graph: every replay on new data equals the eager gradients."""
+    T, E, k, D = 500, 24, 3, 72
+
+    def data(seed):
+        g = torch.Generator(device=dev).manual_seed(seed)
+        return (torch.randn(T, E, device=dev, generator=g).requires_grad_(),
+                torch.randn(T * k, D, device=dev, generator=g).to(torch.bfloat16).requires_grad_(),
+                torch.randn(T, D, device=dev, generator=g).to(torch.bfloat16))
+
+    def work(low, rows, dout):
+        w, sel = sg.route_tokens(low, k, score=score, renormalize=renorm)
+        tok, inv, off = sg.expert_order(sel, E)
+        y = sg.combine_experts(rows, w, inv, off)
+        return (y.detach(), sel) + torch.autograd.grad(y, (low, rows), dout)
+
+    ins = data(0)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        work(*ins)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work(*ins)
+    for rep in range(4):
+        new = data(rep + 1)
+        with torch.no_grad():
+            for a, b in zip(ins, new):
+                a.copy_(b)
+        graph.replay()
+        want = work(*new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)), rep
+
+
 def test_compiled_matches_eager(dev):
     T, E, k, D = 300, 16, 2, 64
     low = _logits(dev, T, E, torch.float32, 21)
