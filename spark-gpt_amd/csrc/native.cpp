@@ -569,7 +569,10 @@ struct RouteTokens : torch::autograd::Function<RouteTokens> {
 std::tuple<Tensor, Tensor> route_tokens(const Tensor& logits, const OptTensor& bias, const OptTensor& mask,
                                         const std::string& score, int64_t groups, int64_t top_groups,
                                         int64_t group_best, int64_t top_k, bool renormalize, double scale) {
-  variable_list out = RouteTokens::apply(logits, bias, mask, score, groups, top_groups, group_best, top_k, renormalize,
+  // The bias has no gradient, so it is no input of the node: one that requires a
+  // gradient would run a backward pass whose forward saved nothing.
+  const OptTensor order_bias = bias && bias->requires_grad() ? OptTensor(bias->detach()) : bias;
+  variable_list out = RouteTokens::apply(logits, order_bias, mask, score, groups, top_groups, group_best, top_k, renormalize,
                                          scale, c10::GradMode::is_enabled() && logits.requires_grad());
   return {out[0], out[1]};
 }

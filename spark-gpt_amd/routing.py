@@ -72,7 +72,10 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bi
     Equal order values go to the lowest index; an expert whose logit (or order
     value) is -inf is never taken, and NaN ranks first.  Slots that no expert
     is left for, and those of masked tokens, get index -1 and weight 0."""
-    apply = _RouteTokens.apply if torch.compiler.is_compiling() else ops.route_tokens
+    compiling = torch.compiler.is_compiling()
+    apply = _RouteTokens.apply if compiling else ops.route_tokens
+    if compiling and bias is not None:
+        bias = bias.detach()  # as in the eager call: weights require a gradient where the logits do
     return apply(logits, bias, mask, score, groups, groups if top_groups is None else top_groups, group_best, top_k,
                  renormalize, float(scale))
 

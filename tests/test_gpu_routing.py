@@ -690,3 +690,39 @@ def test_no_gradient_and_one_gradient(dev):
     with pytest.raises(RuntimeError):
         d, = torch.autograd.grad(w.sum(), leaf, create_graph=True)
         torch.autograd.grad(d.sum(), leaf)
+
+
+@pytest.mark.parametrize("compiled", [False, True])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_bias_that_requires_a_gradient(dev, score, compiled):
+    """A bias held as a Parameter has no gradient: a router whose logits need
+    none gives weights that need none, and one whose logits do gets the same
+    gradient as with a plain bias."""
+    T, E, k, D = 60, 16, 3, 40
+    low = _logits(dev, T, E, torch.float32, 12)
+    bias = torch.nn.Parameter(torch.linspace(-0.2, 0.2, E, device=dev))
+    rows = torch.randn(T * k, D, device=dev)
+    dout = torch.randn(T, D, device=dev)
+
+    def f(low, bias, rows):
+        w, sel = sg.route_tokens(low, k, score=score, bias=bias)
+        tok, inv, off = sg.expert_order(sel, E)
+        return sg.combine_experts(rows, w, inv, off), w
+
+    run = torch.compile(f, dynamic=False, fullgraph=True) if compiled else f
+    # a frozen router
+    r = rows.clone().requires_grad_(True)
+    y, w = run(low, bias, r)
+    assert not w.requires_grad
+    y.backward(dout)
+    want, = torch.autograd.grad(f(low, bias.detach(), r)[0], r, dout)
+    assert bias.grad is None and torch.equal(r.grad, want)
+    y, w = run(low, bias, rows)  # nothing needs a gradient
+    assert not y.requires_grad and not w.requires_grad
+    # a router that learns
+    a, b = low.clone().requires_grad_(True), low.clone().requires_grad_(True)
+    y, w = run(a, bias, rows)
+    y.backward(dout)
+    z, _ = f(b, bias.detach(), rows)
+    z.backward(dout)
+    assert bias.grad is None and torch.equal(y, z) and torch.equal(a.grad, b.grad)
