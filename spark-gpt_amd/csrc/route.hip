@@ -330,11 +330,11 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
 // from 2^23 on as the integer; what is below low has rank 0 and is not taken.  Each
 // step to it keeps the order, so ranks that differ are in the order of the
 // 32-bit values.  Without groups and with more lanes than slots the low value
-// is the smallest of the lanes' largest: L values are no smaller, so the
-// top_k + 1 first are among them.  The next key below `top` is max(key - top)
-// + top in wrapping arithmetic (keys below top wrap to 2^31 and above, those
-// from top on stay below), a subtraction and half a max3 for each value and
-// log2(L) lane steps, with nothing to clear.
+// is the smallest of the lanes' largest, less the errors of biased scores: L
+// values are no smaller, so the top_k + 1 first are among them.  The next key
+// below `top` is max(key - top) + top in wrapping arithmetic (keys below top wrap
+// to 2^31 and above, those from top on stay below), a subtraction and half a max3
+// for each value and log2(L) lane steps, with nothing to clear.
 //
 // Its limits.  Where two neighbours of the top_k + 1 first are closer than
 // their errors, the first few are put in order again by their values in 64 bits,
@@ -529,16 +529,21 @@ __global__ __launch_bounds__(256, 4) void moe_route_kernel(const RouteArgs a, in
       }
   } else {
     least = 1u << idx_bits;
-    float lo;
-    if (a.groups == 1 && L > a.k) lo = lanes_min<L>(mine_max);
-    else lo = ninf;
+    const float hi = lanes_max<L>(mine_max);
+    float lo = ninf;
+    if (a.groups == 1 && L > a.k) {
+      lo = lanes_min<L>(mine_max);
+      // What is below it by no more than two values' errors has a rank too, so
+      // that it is found among the near neighbours (3: and the steps to here).
+      if constexpr (BIAS) lo -= 3.0f * (err + 0x1p-23f * fmaxf(fabsf(lo), fabsf(hi)));
+    }
     if (__any(lo == ninf)) {  // a lane without an expert, a group that is out: the row's smallest
       float least_o = __builtin_inff();
 #pragma unroll
       for (int j = 0; j < V; ++j) least_o = fminf(least_o, o[j] == ninf ? least_o : o[j]);
-      lo = lanes_min<L>(least_o);
+      least_o = lanes_min<L>(least_o);
+      lo = lo == ninf ? least_o : lo;  // each token its own
     }
-    const float hi = lanes_max<L>(mine_max);
     const float range = hi - lo;
     // below 2^(31 - idx_bits) at the largest value, by two steps and the quotient's 2^-22
     const float steps = (float)(1u << (31 - idx_bits)) * (1.0f - 0x1p-19f) - 4.0f;

@@ -221,6 +221,43 @@ def test_route_close_scores(dev):
     _run(far, 8, score="sigmoid")
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,k", [(64, 2), (60, 3), (256, 8), (1000, 10)])
+@pytest.mark.parametrize("mixed", [False, True])
+def test_route_neighbours_of_many_equal_experts(dev, score, E, k, mixed):
+    """k - 1 clear winners, many experts with one logit and bias, and one whose
+    other logit and bias give the same biased score but for about 1e-9 either
+    way: fewer than 32 bits hold, a hundred times what 64 bits do and more.  `mixed`:
+    between the rows are some with hardly an expert."""
+    g = torch.Generator().manual_seed(E + k)
+    T, win = 96, [7 + 2 * j for j in range(k - 1)]
+    down = 0.19 if score == "sigmoid" else 0.25 / E
+    for at in (0, 1, E // 2, E - 1):
+        x = (0.8 + 0.2 * torch.rand(T, generator=g)).float()
+        low = x[:, None].repeat(1, E)
+        low[:, win] = 3.0 + 0.02 * torch.arange(k - 1)
+        bias = torch.full((E,), -0.037174962)
+        bias[at] = bias[at] + down
+        b = bias.double()
+        drop = b[at] - b[at - 1]
+        xd = x.double()
+        if score == "sigmoid":
+            p = torch.sigmoid(xd) - drop
+            y = torch.log(p / (1 - p))
+        else:
+            y = xd.clone()
+            top = float(low[0, win].max())
+            fixed = torch.exp(low[0, win].double() - top).sum()
+            for _ in range(60):  # e^(y - top) = e^(x - top) - drop * z, z the row's sum
+                z = fixed + (E - k) * torch.exp(xd - top) + torch.exp(y - top)
+                y = top + torch.log(torch.exp(xd - top) - drop * z)
+        low[:, at] = y.float()
+        if mixed:
+            low[::3] = -INF
+            low[::3, E - 2] = 1.0
+        _run(low.to(dev), k, torch.ones(T, k, device=dev), bias=bias.to(dev), score=score)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_route_strides(dev, dtype):
     """Any row stride and offset, a transposed view, an expanded row, no tokens."""
