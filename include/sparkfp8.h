@@ -512,13 +512,22 @@ int sfp8_moe_expert_order(const int64_t* selected, int64_t R, int64_t top_k, int
  * order and rounded once; slots whose row is outside [0, R) add nothing.
  * Backward: drows[inverse[t, j]] = weights[t, j] * dout[t] and dweights[t, j]
  * = the dot product of dout[t] and that row (0 for slots without one); either
- * may be NULL.  Each row below offsets[E - 1] is named by one slot; rows from
- * there on get zeros.  top_k <= 64, T <= 2^25. */
+ * may be NULL.  sfp8_moe_combine_bwd takes slots in an order as
+ * sfp8_moe_expert_order makes it: each row below offsets[E - 1] is named by one
+ * slot, and rows from there on get zeros.  sfp8_moe_combine_bwd_any takes any
+ * slots: a row that none names gets zeros, one that several name the sum of
+ * theirs, in slot order (a pass over the slots for each such row); ws of
+ * sfp8_moe_combine_bwd_any_workspace_ints(R, T, top_k) ints where drows is not
+ * NULL, whose contents do not matter.  top_k <= 64, T <= 2^25. */
 int sfp8_moe_combine(const void* rows, int dtype, int64_t R, int64_t D, const float* weights, const int64_t* inverse,
                      int64_t T, int64_t top_k, void* out, void* stream);
 int sfp8_moe_combine_bwd(const void* dout, const void* rows, int dtype, int64_t R, int64_t D, const float* weights,
                          const int64_t* inverse, int64_t T, int64_t top_k, const int* offsets, int64_t E, void* drows,
                          float* dweights, void* stream);
+int64_t sfp8_moe_combine_bwd_any_workspace_ints(int64_t R, int64_t T, int64_t top_k);
+int sfp8_moe_combine_bwd_any(const void* dout, const void* rows, int dtype, int64_t R, int64_t D, const float* weights,
+                             const int64_t* inverse, int64_t T, int64_t top_k, void* drows, float* dweights, int* ws,
+                             int64_t ws_ints, void* stream);
 
 /* ---------------------------------------------------------------------------
  * The global norm of many gradients, and clipping to a largest norm.

@@ -85,6 +85,8 @@ SIGNATURES = {
     "sfp8_moe_expert_order": (_INT, [_P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
     "sfp8_moe_combine": (_INT, [_P, _INT, _I64, _I64, _P, _P, _I64, _I64, _P, _P]),
     "sfp8_moe_combine_bwd": (_INT, [_P, _P, _INT, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _P]),
+    "sfp8_moe_combine_bwd_any_workspace_ints": (_I64, [_I64, _I64, _I64]),
+    "sfp8_moe_combine_bwd_any": (_INT, [_P, _P, _INT, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P, _I64, _P]),
     # the global gradient norm and clipping
     "sfp8_grad_norm_workspace_doubles": (_I64, [_I64]),
     "sfp8_grad_norm": (_INT, [_I64, _P, _P, _P, _P, _P, _I64, _P]),

@@ -516,9 +516,12 @@ std::tuple<OptTensor, OptTensor> moe_combine_bwd(const Tensor& dout, const Tenso
   OptTensor drows, dweights;
   if (need_rows) drows = empty(rows.sizes(), rows.scalar_type(), rows);
   if (need_weights) dweights = empty(weights.sizes(), kF32, rows);
-  CALL(sfp8_moe_combine_bwd, ptr(dout), ptr(rows), dtype, rows.size(0), rows.size(1), fptr(weights),
-       lptr(inverse_permutation), weights.size(0), weights.size(1), iptr(offsets), offsets.size(0), ptr(drows),
-       fptr(dweights), stream_of(rows));
+  const int64_t R = rows.size(0), T = weights.size(0), k = weights.size(1);
+  OptTensor ws;  // which slots name each row
+  const int64_t nws = need_rows ? sfp8_moe_combine_bwd_any_workspace_ints(R, T, k) : 0;
+  if (nws > 0) ws = empty({nws}, ScalarType::Int, rows);
+  CALL(sfp8_moe_combine_bwd_any, ptr(dout), ptr(rows), dtype, R, rows.size(1), fptr(weights), lptr(inverse_permutation), T,
+       k, ptr(drows), fptr(dweights), iptr(ws), nws, stream_of(rows));
   return {drows, dweights};
 }
 
@@ -892,7 +895,7 @@ PYBIND11_MODULE(_native, m) {
         "out[t] = sum of weights[t, j] * rows[inverse_permutation[t, j]] over the slots, summed in 32 bits in order.");
   m.def("moe_combine_bwd", &moe_combine_bwd, arg("dout"), arg("rows"), arg("weights"), arg("inverse_permutation"),
         arg("offsets"), arg("need_rows") = true, arg("need_weights") = true,
-        "(drows, dweights) of moe_combine; rows from offsets[-1] on get zeros.");
+        "(drows, dweights) of moe_combine; a row that no slot names gets zeros, one that several name the sum of theirs.");
   m.def("route_tokens", &route_tokens, arg("logits"), arg("bias"), arg("mask"), arg("score"), arg("groups"),
         arg("top_groups"), arg("group_best"), arg("top_k"), arg("renormalize"), arg("scale"),
         "(weights, selected) of moe_route, differentiable in the logits.");

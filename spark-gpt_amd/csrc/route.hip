@@ -1056,17 +1056,66 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const void* __restrict
   }
 }
 
+// ---------------------------------------------------------------------------
+// Which slots name a row, from the slots alone: the combine's backward pass must
+// write every row once, whatever the slots name.  of_row[r] becomes a slot that
+// names row r, and many[s] says of that slot whether there are others.  Neither
+// is cleared first, since what is left in of_row[r] proves itself: a number s
+// there is right if slot s names row r.  The slot that wrote last took the one
+// before it out of of_row[r], if there was one; a stale number can only pass for
+// another slot of the row where it is one.  Which of a row's slots comes last
+// changes from run to run, the gradients do not: one slot is the row's own, and
+// of several any one adds up all of them, in order.  4 bytes a slot, scattered,
+// and 9 in a row: 131072 slots 5 us.
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void moe_row_slots_kernel(const int64_t* __restrict__ inv, int64_t slots, int64_t R,
+                                                            uint32_t* __restrict__ of_row, uint8_t* __restrict__ many) {
+  const int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (s >= slots) return;
+  const int64_t r = inv[s];
+  if (r < 0 || r >= R) return;
+  const uint32_t before = atomicExch(of_row + r, (uint32_t)s);
+  many[s] = before < slots && before != (uint32_t)s && inv[before] == r;
+}
+
+// drows[r] = the sum over the slots of row r, in order, of w dout: a whole wave.
+template <int DT>
+SFP8_DEV void sum_slots(const void* dout, int64_t D, const float* weights, const int64_t* inv, int64_t slots, int k,
+                        int64_t r, void* drows) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t d0 = lane; d0 - lane < D; d0 += 256) {
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t b = 0; b < slots; b += 64) {
+      uint64_t found = __ballot(b + lane < slots && inv[b + lane] == r);
+      for (; found; found &= found - 1) {
+        const int64_t s = b + __builtin_ctzll(found);
+        const float w = weights[s];
+        const int64_t at = (int64_t)((uint32_t)s / (uint32_t)k) * D;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (d0 + 64 * q < D) acc[q] = __builtin_fmaf(w, load_as_f32(dout, DT, at + d0 + 64 * q), acc[q]);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (d0 + 64 * q < D) store_f32_as(drows, DT, r * D + d0 + 64 * q, acc[q]);
+  }
+}
+
 // drows[inv[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], rows[inv[t, j]]>
-// (either may be null); rows from offsets[E - 1] on, which no slot names, get
-// zeros.  One wave a slot, or `lanes` lanes (a power of two) where a row has
-// fewer units: the lanes of a token's slots share its gradient through the
+// (either may be null).  With of_row and many (moe_row_slots_kernel) a row that
+// several slots name gets the sum of theirs and one that none names zeros;
+// without them each row below offsets[E - 1] is one slot's, and those from there
+// on get zeros.  One wave a slot, or `lanes` lanes (a power of two) where a row
+// has fewer units: the lanes of a token's slots share its gradient through the
 // caches.  Bound by the rows' bytes, read and written (65536 tokens of 2 rows of
-// 1024 99 us, 6.8 TB/s; 131072 of 2 of 128 28, in whole waves 53).
+// 1024 104 us; 131072 of 2 of 128 32, in whole waves 53).
 template <int DT, int CUT, bool NT, bool WIDE>
 __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
     const void* __restrict__ dout, const void* __restrict__ rows, int64_t R, int64_t D,
     const float* __restrict__ weights, const int64_t* __restrict__ inv, int64_t slots, int k,
-    const int* __restrict__ offsets, int E, void* __restrict__ drows, float* __restrict__ dweights, int lanes) {
+    const int* __restrict__ offsets, int E, const uint32_t* __restrict__ of_row, const uint8_t* __restrict__ many,
+    void* __restrict__ drows, float* __restrict__ dweights, int lanes) {
   using X = Unit<DT, CUT>;
   const int per = WIDE ? 1 : 64 / lanes;  // slots of a wave
   const int sub = WIDE ? threadIdx.x & 63 : threadIdx.x & (lanes - 1);
@@ -1077,8 +1126,11 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
     const bool in = s < slots;
     const int64_t t = (uint32_t)s / (uint32_t)k, r = in ? inv[s] : -1;
     float dot = 0.0f;
+    bool sum = false;
     if (r >= 0 && r < R) {
       const float w = weights[s];
+      // the slot that writes the row, and whether it alone names it
+      const uint32_t owner = of_row ? of_row[r] : (uint32_t)s, others = of_row ? many[s] : 0u;
 #pragma unroll 2
       for (int64_t at = (int64_t)sub * X::U; at < D; at += stride) {
         const int64_t d = X::first(at, D);
@@ -1092,12 +1144,15 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
           for (int q = 0; q < X::U; ++q)
             dot = CUT != kAny || q >= at - d ? __builtin_fmaf(g.x[q], v.x[q], dot) : dot;
         }
-        if (drows) {
+        uint32_t writes = owner == (uint32_t)s && !others && drows;
+        asm volatile("" : "+v"(writes));  // asked for here, with the rows' loads in flight (before them: 4 us of 100 more)
+        if (writes) {
 #pragma unroll
           for (int q = 0; q < X::U; ++q) g.x[q] *= w;
           g.template store<NT>(drows, r * D + d);
         }
       }
+      sum = owner == (uint32_t)s && others;
     }
     if (dweights) {
       if constexpr (WIDE) dot = lanes_sum<64>(dot);
@@ -1105,13 +1160,30 @@ __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
         for (int o = 1; o < lanes; o <<= 1) dot += __shfl_xor(dot, o, 64);
       if (in && sub == 0) dweights[s] = dot;
     }
+    for (uint64_t left = __ballot(sum && sub == 0); left; left &= left - 1)  // seldom any
+      sum_slots<DT>(dout, D, weights, inv, slots, k, __shfl(r, __builtin_ctzll(left), 64), drows);
   }
   if (!drows) return;
-  int64_t used = offsets[E - 1];
-  used = used < 0 ? 0 : used;
   X zero;
 #pragma unroll
   for (int q = 0; q < X::U; ++q) zero.x[q] = 0.0f;
+  if (of_row) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t b = wave * 64; b < R; b += (int64_t)gridDim.x * 256) {  // 64 rows a wave
+      bool none = false;
+      if (b + lane < R) {
+        const uint32_t s = of_row[b + lane];
+        none = !(s < slots && inv[s] == b + lane);
+      }
+      for (uint64_t left = __ballot(none); left; left &= left - 1) {
+        const int64_t r = b + __builtin_ctzll(left);
+        for (int64_t d = (int64_t)lane * X::U; d < D; d += 64 * X::U) zero.store(drows, r * D + X::first(d, D));
+      }
+    }
+    return;
+  }
+  int64_t used = offsets[E - 1];
+  used = used < 0 ? 0 : used;
   for (int64_t r = used + first; r < R; r += step)
     for (int64_t d = (int64_t)sub * X::U; d < D; d += stride) zero.store(drows, r * D + X::first(d, D));
 }
@@ -1254,7 +1326,8 @@ struct Combine {
 template <int DT, int CUT>
 struct CombineBwd {
   static void run(const void* dout, const void* rows, int64_t R, int64_t D, const float* w, const int64_t* inv,
-                  int64_t T, int k, const int* offsets, int E, void* drows, float* dw, hipStream_t st) {
+                  int64_t T, int k, const int* offsets, int E, const uint32_t* of_row, const uint8_t* many,
+                  void* drows, float* dw, hipStream_t st) {
     constexpr int U = Unit<DT, CUT>::U;
     int lanes = 64;
     while (lanes > 1 && (int64_t)(lanes / 2) * U >= D) lanes /= 2;
@@ -1262,7 +1335,7 @@ struct CombineBwd {
     const int64_t per = 4 * (64 / lanes), need = (work + per - 1) / per, nb = need < most ? need : most;
     const auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)nb), dim3(256), 0, st, dout, rows, R, D, w, inv, slots, k, offsets, E,
-                         drows, dw, lanes);
+                         of_row, many, drows, dw, lanes);
     };
     constexpr bool kPast = CUT != kSingle;
     const bool past = kPast && (2 * R + T) * D * (DT == kF32 ? 4 : 2) > kLastLevelCache;
@@ -1275,6 +1348,14 @@ struct CombineBwd {
     }
   }
 };
+
+int combine_bwd_check(const void* dout, const void* rows, int dtype, int64_t R, int64_t D, const float* weights,
+                      const int64_t* inverse, int64_t T, int64_t top_k, const float* dweights) {
+  if ((T > 0 && (!dout || !weights || !inverse)) || (R > 0 && dweights && T > 0 && !rows)) return kErrNullPointer;
+  if (R < 0 || T < 0 || T > kMaxTokens || D <= 0 || top_k <= 0 || top_k > kRouteMaxK || bad_dtype(dtype))
+    return kErrBadShape;
+  return kOk;
+}
 }  // namespace
 
 extern "C" {
@@ -1349,13 +1430,43 @@ int sfp8_moe_combine(const void* rows, int dtype, int64_t R, int64_t D, const fl
 int sfp8_moe_combine_bwd(const void* dout, const void* rows, int dtype, int64_t R, int64_t D, const float* weights,
                          const int64_t* inverse, int64_t T, int64_t top_k, const int* offsets, int64_t E, void* drows,
                          float* dweights, void* stream) {
-  if ((T > 0 && (!dout || !weights || !inverse)) || (R > 0 && dweights && T > 0 && !rows) || (drows && !offsets))
-    return kErrNullPointer;
-  if (R < 0 || T < 0 || T > kMaxTokens || D <= 0 || top_k <= 0 || top_k > kRouteMaxK || bad_dtype(dtype) || E <= 0)
-    return kErrBadShape;
+  if (const int rc = combine_bwd_check(dout, rows, dtype, R, D, weights, inverse, T, top_k, dweights)) return rc;
+  if (drows && !offsets) return kErrNullPointer;
+  if (E <= 0) return kErrBadShape;
   if ((T == 0 && R == 0) || (!drows && !dweights)) return kOk;
   const int cut = row_cut(dtype, D, al16(rows) && al16(dout) && al16(drows));
-  by_type<CombineBwd>(dtype, cut, dout, rows, R, D, weights, inverse, T, (int)top_k, offsets, (int)E, drows, dweights,
+  by_type<CombineBwd>(dtype, cut, dout, rows, R, D, weights, inverse, T, (int)top_k, offsets, (int)E,
+                      (const uint32_t*)nullptr, (const uint8_t*)nullptr, drows, dweights, (hipStream_t)stream);
+  return route_status();
+}
+
+// of_row of every row, then a byte of many for every slot
+int64_t sfp8_moe_combine_bwd_any_workspace_ints(int64_t R, int64_t T, int64_t top_k) {
+  if (R < 0 || T < 0 || T > kMaxTokens || top_k <= 0 || top_k > kRouteMaxK) return -1;
+  return R + (T * top_k + 3) / 4;
+}
+
+int sfp8_moe_combine_bwd_any(const void* dout, const void* rows, int dtype, int64_t R, int64_t D, const float* weights,
+                             const int64_t* inverse, int64_t T, int64_t top_k, void* drows, float* dweights, int* ws,
+                             int64_t ws_ints, void* stream) {
+  if (const int rc = combine_bwd_check(dout, rows, dtype, R, D, weights, inverse, T, top_k, dweights)) return rc;
+  if ((T == 0 && R == 0) || (!drows && !dweights)) return kOk;
+  uint32_t* of_row = nullptr;
+  uint8_t* many = nullptr;
+  if (drows && R > 0) {
+    if (!ws || ws_ints < sfp8_moe_combine_bwd_any_workspace_ints(R, T, top_k)) return kErrWorkspaceTooSmall;
+    of_row = (uint32_t*)ws;
+    many = (uint8_t*)(ws + R);
+    const int64_t slots = T * top_k;
+    if (slots > 0)
+      hipLaunchKernelGGL(moe_row_slots_kernel, dim3((unsigned)((slots + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
+                         inverse, slots, R, of_row, many);
+  } else if (!dweights) {
+    return kOk;  // no rows
+  }
+  const int cut = row_cut(dtype, D, al16(rows) && al16(dout) && al16(drows));
+  by_type<CombineBwd>(dtype, cut, dout, rows, R, D, weights, inverse, T, (int)top_k, (const int*)nullptr, 0,
+                      (const uint32_t*)of_row, (const uint8_t*)many, R > 0 ? drows : nullptr, dweights,
                       (hipStream_t)stream);
   return route_status();
 }

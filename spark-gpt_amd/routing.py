@@ -112,10 +112,9 @@ def combine_experts(rows: torch.Tensor, weights: torch.Tensor, inverse_permutati
     [T, D]: rows [R, D] bf16, fp16 or fp32 in expert order, weights [T, k]
     (k <= 64), ``inverse_permutation`` and ``offsets`` of ``expert_order``.  The
     sum is taken in 32 bits in slot order and rounded once; slots without a row
-    add nothing.  In the backward pass rows from ``offsets[-1]`` on get zeros, and
-    each row before is expected to be the row of one slot, as in what
-    ``expert_order`` returns: a slot is left out by its -1 in ``selected``, before
-    the order is made, not by a change to ``inverse_permutation``."""
+    (-1, or anything outside [0, R)) add nothing.  In the backward pass a row that
+    no slot names gets zeros and one that several name the sum of theirs, in 32
+    bits and slot order; the latter costs a pass over the slots for each such row."""
     if torch.compiler.is_compiling():
         return _CombineExperts.apply(rows, weights.float(), inverse_permutation, offsets)
     return ops.combine_experts(rows, weights, inverse_permutation, offsets)

@@ -17,6 +17,7 @@ import torch
 
 import spark_gpt_amd as sg
 from oracle import routing as O
+from spark_gpt_amd import _lib
 
 pytestmark = pytest.mark.gpu
 DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
@@ -430,6 +431,140 @@ def test_combine_layouts(dev):
     assert ((got - want).abs() <= 3 * 2.0 ** -24 * size + 2.0 ** -8 * 1.01 * want.abs()).all()
     empty = sg.combine_experts(odd[:0], w[:0], inv[:0], torch.zeros(E, dtype=torch.int32, device=dev))
     assert empty.shape == (0, D)
+
+
+def _any_slots(T, k, how, g):
+    """inverse_permutation of T * k slots over T * k rows, changed after the order was made."""
+    R = T * k
+    inv = torch.randperm(R, generator=g)
+    if how == "dropped":
+        inv[torch.rand(R, generator=g) < 0.3] = -1
+    elif how == "out of range":
+        inv[torch.rand(R, generator=g) < 0.3] = R + 2
+        inv[torch.rand(R, generator=g) < 0.1] = -(2 ** 40)
+    elif how == "shared":
+        inv[torch.rand(R, generator=g) < 0.4] = inv[0].clone()
+        inv[torch.rand(R, generator=g) < 0.2] = inv[-1].clone()
+        inv[torch.rand(R, generator=g) < 0.2] = -1
+    elif how == "two each":
+        inv //= 2
+    elif how == "one row":
+        inv[:] = R - 1
+    elif how == "none":
+        inv[:] = -1
+    return inv
+
+
+def _any_slots_reference(dout, rows, weights, inv):
+    """(drows, sum of the absolute products, most slots of a row) in float64."""
+    R, (T, k) = rows.shape[0], weights.shape
+    live = ((inv >= 0) & (inv < R)).nonzero()[:, 0]
+    part = weights.double().view(-1)[live, None] * dout.double()[live // k]
+    zero = torch.zeros(rows.shape, dtype=torch.float64)
+    n = int(torch.bincount(inv[live], minlength=1).max())
+    return zero.index_add(0, inv[live], part), zero.index_add(0, inv[live], part.abs()), n
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("how", ["dropped", "out of range", "shared", "two each", "one row", "none"])
+@pytest.mark.parametrize("T,k,D", [(1, 2, 1), (40, 3, 5), (200, 1, 24), (33, 64, 8), (70, 6, 130), (300, 4, 64), (21, 2, 1500)])
+def test_combine_gradients_of_any_slots(dev, dtype, how, T, k, D):
+    """Whatever rows the slots name: a row that no slot names gets zeros, one that
+    several name the sum of theirs in slot order (n products and sums in 32 bits,
+    2^-24 each, rounded once), the same bits from call to call."""
+    dt, R = DTYPES[dtype], T * k
+    g = torch.Generator().manual_seed(R + D)
+    inv = _any_slots(T, k, how, g)
+    rows, dout = torch.randn(R, D, generator=g).to(dt), torch.randn(T, D, generator=g).to(dt)
+    w = torch.rand(T, k, generator=g)
+    off = torch.full((4,), R, dtype=torch.int32, device=dev)
+    args = [x.to(dev) for x in (dout, rows, w, inv)]
+    want, size, n = _any_slots_reference(dout, rows, w, inv)
+    step, tiny = _half_step(dt), torch.finfo(dt).tiny * torch.finfo(dt).eps
+    first = None
+    for _ in range(3):
+        stale = torch.full((R, D), NAN, device=dev, dtype=dt)  # what a gradient's memory may hold
+        del stale
+        leaf = args[1].clone().requires_grad_(True)
+        y = sg.combine_experts(leaf, args[2], args[3], off)
+        got, = torch.autograd.grad(y, leaf, args[0])
+        bound = n * 2.0 ** -24 * size + step * (1 + 2.0 ** -8) * want.abs() + tiny
+        assert ((got.cpu().double() - want).abs() <= bound).all()
+        first = got if first is None else first
+        assert torch.equal(got, first)
+    _, dw = sg.ops.moe_combine_bwd(*args, off, False, True)
+    there = (inv >= 0) & (inv < R)
+    dots = torch.where(there[:, None], rows.double()[inv.where(there, torch.zeros_like(inv))], 0.0) \
+        * dout.double().repeat_interleave(k, 0)
+    assert ((dw.cpu().double().view(-1) - dots.sum(1)).abs()
+            <= _sum_steps(D) * 2.0 ** -24 * dots.abs().sum(1) + 2.0 ** -120).all()
+
+
+def test_combine_gradients_whatever_the_workspace_holds(dev):
+    """The C entries: the workspace's contents do not matter, slots in a proper
+    order get the same bits from both, and what lies behind the workspace stays."""
+    T, k, D = 150, 4, 72
+    R, g = T * k, torch.Generator().manual_seed(5)
+    rows, dout = torch.randn(R, D, generator=g).to(dev), torch.randn(T, D, generator=g).to(dev)
+    w = torch.rand(T, k, generator=g).to(dev)
+    ints = _lib.query("sfp8_moe_combine_bwd_any_workspace_ints", R, T, k)
+    st = torch.cuda.current_stream().cuda_stream
+
+    def any_slots(inv, ws):
+        dr, dw = torch.full_like(rows, NAN), torch.full_like(w, NAN)
+        _lib.call("sfp8_moe_combine_bwd_any", dout.data_ptr(), rows.data_ptr(), 0, R, D, w.data_ptr(), inv.data_ptr(), T,
+                  k, dr.data_ptr(), dw.data_ptr(), ws.data_ptr(), ints, st)
+        assert bool((ws[ints:] == 77).all())
+        return dr, dw
+
+    for how in ("order", "dropped", "shared", "two each", "one row", "none"):
+        if how == "order":
+            sel = torch.randint(-1, 8, (T, k), generator=g).to(dev)
+            _, inv, off = sg.expert_order(sel, 8)
+        else:
+            inv = _any_slots(T, k, how, g).to(dev)
+        outs = []
+        for fill in ("zeros", "ones", "stale", "slots", "again"):
+            if fill != "again":
+                ws = torch.full((ints + 8,), 77, dtype=torch.int32, device=dev)
+                ws[:ints] = {"zeros": 0, "ones": -1}.get(fill, 0)
+            if fill == "stale":
+                ws[:ints] = torch.randint(-2 ** 31, 2 ** 31 - 1, (ints,), generator=g).to(dev)
+            elif fill == "slots":  # each row's first slot, where it has one
+                for s in reversed(range(R)):
+                    r = int(inv[s])
+                    if 0 <= r < R:
+                        ws[r] = s
+            outs.append(any_slots(inv, ws))
+        assert all(torch.equal(a, b) for o in outs[1:] for a, b in zip(o, outs[0])), how
+        if how == "order":
+            dr, dw = torch.full_like(rows, NAN), torch.full_like(w, NAN)
+            _lib.call("sfp8_moe_combine_bwd", dout.data_ptr(), rows.data_ptr(), 0, R, D, w.data_ptr(), inv.data_ptr(), T,
+                      k, off.data_ptr(), 8, dr.data_ptr(), dw.data_ptr(), st)
+            assert torch.equal(dr, outs[0][0]) and torch.equal(dw, outs[0][1])
+        want, size, n = _any_slots_reference(dout.cpu(), rows.cpu(), w.cpu(), inv.cpu())
+        assert ((outs[0][0].cpu().double() - want).abs() <= (n + 1) * 2.0 ** -24 * size).all()
+
+
+def test_combine_gradients_of_any_slots_captured(dev):
+    """Captured with slots of one kind and replayed with those of others: the
+    workspace then holds what the replay before left."""
+    T, k, D = 90, 3, 136
+    R, g = T * k, torch.Generator().manual_seed(6)
+    rows, dout = torch.randn(R, D, generator=g).to(dev), torch.randn(T, D, generator=g).to(dev)
+    w, off = torch.rand(T, k, generator=g).to(dev), torch.full((1,), R, dtype=torch.int32, device=dev)
+    inv = _any_slots(T, k, "dropped", g).to(dev)
+    sg.ops.moe_combine_bwd(dout, rows, w, inv, off)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = sg.ops.moe_combine_bwd(dout, rows, w, inv, off)
+    for how in ("shared", "none", "one row", "two each", "dropped", "shared", "dropped"):
+        inv.copy_(_any_slots(T, k, how, g))
+        graph.replay()
+        want = sg.ops.moe_combine_bwd(dout, rows, w, inv, off)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), how
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])

@@ -174,3 +174,19 @@ def test_fake_shapes():
         dr, dw = torch.ops.sparkfp8.combine_bwd(out, rows, w, inv, off)
         assert dr.shape == rows.shape and dr.dtype == rows.dtype and dw.shape == w.shape and dw.dtype == torch.float32
     assert torch_ops.route_fwd is not None
+
+
+def test_combine_of_any_slots_refuses_before_launch():
+    q = lambda *a: _lib.query("sfp8_moe_combine_bwd_any_workspace_ints", *a)
+    assert q(8, 4, 2) == 8 + 2 and q(9, 3, 3) == 9 + 3 and q(0, 0, 1) == 0 and q(5, 0, 2) == 5
+    assert q(-1, 4, 2) == q(8, -1, 2) == q(8, 2 ** 25 + 1, 2) == q(8, 4, 0) == q(8, 4, 65) == -1
+    cb = _lib.load().sfp8_moe_combine_bwd_any
+
+    def call(dout=16, rows=16, dtype=1, R=8, D=64, w=16, inv=16, T=4, k=2, dr=16, dw=16, ws=16, ints=10):
+        return cb(dout, rows, dtype, R, D, w, inv, T, k, dr, dw, ws, ints, None)
+
+    assert call(dout=None) == call(rows=None) == call(w=None) == call(inv=None) == -1
+    for bad in (dict(dtype=3), dict(R=-1), dict(D=0), dict(T=-1), dict(T=2 ** 25 + 1), dict(k=0), dict(k=65)):
+        assert call(**bad) == -2, bad
+    assert call(ws=None) == call(ints=9) == call(ws=None, dw=None) == -4
+    assert call(dr=None, dw=None) == call(T=0, R=0) == call(R=0, dw=None, T=4) == 0  # nothing to write
