@@ -534,7 +534,7 @@ int sfp8_moe_combine_bwd_any(const void* dout, const void* rows, int dtype, int6
  * ------------------------------------------------------------------------- */
 
 /* norm = sqrt(sum of squares over all elements of count gradients) (fp32 at a
- * device pointer; summed in 64 bits, in an order that the sizes alone give).
+ * device pointer; summed in 64 bits, in an order that sizes and types alone give).
  * grads, n (elements) and dtype are host arrays, read before the call
  * returns; ws: sfp8_grad_norm_workspace_doubles(count) doubles.
  * sfp8_grad_clip also writes out[i] = grads[i] * min(1, max_norm / (norm +

@@ -10,9 +10,10 @@ step does between the backward pass and the optimizer (whose momentum stage is
 
 Gradients are fp32, bf16 or fp16, mixed as they come, on one device, each
 dense in some order of its dimensions.  The squares are summed in 64 bits, in
-an order that the sizes alone give: the same gradients give the same norm, bit
-for bit.  A norm that is infinite or NaN goes into the factor as it is, as in
-torch.  Nothing synchronises the device unless ``error_if_nonfinite`` asks.
+an order that sizes and types alone give: the same gradients give the same norm,
+bit for bit, wherever they lie.  A norm that is infinite or NaN goes into the
+factor as it is, as in torch.  Nothing synchronises the device unless
+``error_if_nonfinite`` asks.
 """
 from __future__ import annotations
 

@@ -7,11 +7,14 @@
 //
 // The squares are summed in 64 bits (a square of a 32-bit number cannot
 // overflow there, and 64-bit FMAs cost a few percent of the time the bytes
-// take), in an order that depends on the sizes alone: every work-group sums
-// its own chunks, then the sums are added in order.  Bound by HBM: each
+// take), in an order that depends on the sizes and types alone, not on the
+// addresses: every work-group sums its own chunks, each thread the same elements
+// of them, then the sums are added in order.  Bound by HBM: each
 // gradient is read once for the norm and, where c != 1 or the result goes
 // elsewhere, read again and written.
 #include "common.h"
+
+#include <type_traits>
 
 namespace sfp8 {
 
@@ -85,16 +88,21 @@ struct Pack {
   }
 };
 
+// 16 bytes at any element's address: global memory takes them there in one access.
+typedef int intx4_any __attribute__((ext_vector_type(4), aligned(2)));
+
 // The elements [e0, e1) of a chunk: those before the first 16-byte boundary,
 // whole 16-byte vectors, and the rest.  one(i) takes element i, vec(i, v) the
-// vector v that starts at element i.  ONCE: loads that pass the caches by.
-template <int DT, bool ONCE, typename One, typename Vec>
+// vector v that starts at element i.  ONCE: loads that pass the caches by.  ANY:
+// vectors from e0 on, wherever that lies in its 16 bytes.
+template <int DT, bool ONCE, bool ANY, typename One, typename Vec>
 SFP8_DEV void clip_walk(const void* p, int64_t e0, int64_t e1, One one, Vec vec) {
   using P = Pack<DT>;
+  using V = std::conditional_t<ANY, intx4_any, intx4>;
   constexpr int kStep = kClipThreads * P::U;
   const char* at = reinterpret_cast<const char*>(p) + e0 * P::kSize;
   const int n = (int)(e1 - e0);
-  const int lead = (int)((16 - ((uintptr_t)at & 15)) & 15) / P::kSize;
+  const int lead = ANY ? 0 : (int)((16 - ((uintptr_t)at & 15)) & 15) / P::kSize;
   const int v0 = lead < n ? lead : n, v1 = v0 + (n - v0) / P::U * P::U;
   if ((int)threadIdx.x < v0) one(e0 + threadIdx.x);
   int i = v0 + (int)threadIdx.x * P::U;
@@ -102,13 +110,16 @@ SFP8_DEV void clip_walk(const void* p, int64_t e0, int64_t e1, One one, Vec vec)
     intx4 v[kClipUnroll];
 #pragma unroll
     for (int q = 0; q < kClipUnroll; ++q) {
-      const intx4* x = reinterpret_cast<const intx4*>(at + (i + q * kStep) * P::kSize);
+      const V* x = reinterpret_cast<const V*>(at + (i + q * kStep) * P::kSize);
       v[q] = ONCE ? __builtin_nontemporal_load(x) : *x;
     }
 #pragma unroll
     for (int q = 0; q < kClipUnroll; ++q) vec(e0 + i + q * kStep, v[q]);
   }
-  for (; i < v1; i += kStep) vec(e0 + i, *reinterpret_cast<const intx4*>(at + i * P::kSize));
+  for (; i < v1; i += kStep) {
+    const intx4 v = *reinterpret_cast<const V*>(at + i * P::kSize);
+    vec(e0 + i, v);
+  }
   if (v1 + (int)threadIdx.x < n) one(e0 + v1 + threadIdx.x);
 }
 
@@ -116,7 +127,7 @@ template <int DT, bool ONCE>
 SFP8_DEV double clip_squares(const void* p, int64_t e0, int64_t e1) {
   using P = Pack<DT>;
   double s = 0.0;
-  clip_walk<DT, ONCE>(
+  clip_walk<DT, ONCE, true>(
       p, e0, e1,
       [&](int64_t i) {
         const double x = P::load(p, i);
@@ -140,7 +151,7 @@ SFP8_DEV void clip_scale(const void* p, void* o, int64_t e0, int64_t e1, float c
     for (int64_t i = e0 + threadIdx.x; i < e1; i += kClipThreads) one(i);
     return;
   }
-  clip_walk<DT, ONCE>(p, e0, e1, one, [&](int64_t i, const intx4& v) {
+  clip_walk<DT, ONCE, false>(p, e0, e1, one, [&](int64_t i, const intx4& v) {
     __builtin_nontemporal_store(P::scaled(v, c), reinterpret_cast<intx4*>(reinterpret_cast<char*>(o) + i * P::kSize));
   });
 }

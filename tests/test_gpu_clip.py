@@ -4,6 +4,9 @@ The squares are summed in 64 bits, so the norm is off by its rounding to fp32,
 2^-24 relative (and 1e-9 for up to 10^7 additions of 2^-53).  The factor adds
 that, the sum with 1e-6 and the quotient, 2^-24 each; a scaled gradient its
 product and half a step of its type."""
+import math
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -112,6 +115,47 @@ def test_extremes(dev):
         sg.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)
     p.grad = torch.ones(4, device=dev)
     assert abs(float(sg.clip_grad_norm_([p], 1.0, error_if_nonfinite=True)) - 2.0) < 1e-6
+
+
+def _at_a_border(n, dtype, seed):
+    """n values whose exact norm lies halfway between two fp32 numbers to 2^-56:
+    the last bits of the 64-bit sum, and so its order, decide the result."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, generator=g).to(dtype)
+    x[:40] = 0
+    exact = sum((Fraction(v) ** 2 for v in x.tolist()), Fraction(0))
+    low = torch.tensor(math.sqrt(exact) * 1.001, dtype=torch.float32)
+    half = (Fraction(float(low)) + Fraction(float(torch.nextafter(low, low + 1)))) / 2
+    left, i = half ** 2 - exact, 0
+    while i < 40 and left > half ** 2 / 2 ** 56:  # each takes most of what is left
+        v = torch.tensor(math.sqrt(left) * (1 - 2.0 ** -12), dtype=torch.float64).to(dtype)
+        while Fraction(float(v)) ** 2 > left:
+            v = torch.nextafter(v, torch.zeros_like(v))
+        x[i] = v
+        left -= Fraction(float(v)) ** 2
+        i += 1
+    assert 0 <= left <= half ** 2 / 2 ** 56
+    return x[torch.randperm(n, generator=g)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_does_not_depend_on_the_address(dev, dtype):
+    """The same values at every offset in 16 bytes: the same sum, bit for bit,
+    alone and among others, read only and clipped."""
+    size = torch.empty((), dtype=dtype).element_size()
+    for n, seed in ((1003, 1), (1003, 2), (20001, 3), (20001, 4), (70000, 5), (70000, 6)):
+        x = _at_a_border(n, dtype, seed).to(dev)
+        one, two = set(), set()
+        for off in range(16 // size + 1):
+            store = torch.zeros(n + 32, device=dev, dtype=dtype)
+            v = store[off:off + n]
+            v.copy_(x)
+            assert v.data_ptr() % 16 == off * size % 16
+            one.add(float(sg.grad_norm([v])))
+            one.add(float(sg.clip_grads([v], 1e9, out=[torch.empty_like(v)])))
+            a, b = v[:n // 3], v[n // 3:]
+            two.add(float(sg.grad_norm([a, b])))
+        assert len(one) == 1 and len(two) == 1, (n, one, two)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
