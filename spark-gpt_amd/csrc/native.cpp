@@ -438,28 +438,38 @@ std::tuple<Tensor, Tensor, OptTensor> moe_route(const Tensor& logits_, const Opt
   return {w, sel, picked};
 }
 
-Tensor moe_route_bwd(const Tensor& dweights_, const Tensor& selected, const Tensor& picked, const Tensor& logits_,
-                     const std::string& score, bool renormalize, double scale) {
-  const int dtype = float_code("logits", logits_), sc = score_code(score);
-  const c10::DeviceGuard guard(logits_.device());
-  const Tensor logits = logit_rows(logits_);
-  const int64_t T = logits.size(0), E = logits.size(1);
+// Of the logits only the plain softmax reads the values; the others take their type and number of experts.
+Tensor route_gradient(const Tensor& dweights_, const Tensor& selected, const Tensor& picked, const OptTensor& logits_,
+                      ScalarType type, int64_t E, int score, bool renormalize, double scale) {
+  const c10::DeviceGuard guard(selected.device());
+  OptTensor logits;
+  if (logits_) logits = logit_rows(*logits_);
   contig("selected", selected, kI64, 2);
-  const int64_t k = selected.size(1);
+  const int64_t T = selected.size(0), k = selected.size(1);
   const Tensor dweights = dweights_.contiguous();
   for (const auto& [n, t] : {std::pair<const char*, const Tensor&>{"dweights", dweights}, {"picked", picked}}) {
     contig(n, t, kF32, 2);
     if (!(t.sizes() == selected.sizes())) refuse(std::string(n) + " must have the shape of selected");
+    same_device(n, t, selected);
   }
-  for (const auto& [n, t] : {std::pair<const char*, const Tensor&>{"dweights", dweights}, {"picked", picked},
-                             {"selected", selected}})
-    same_device(n, t, logits);
-  need(selected.size(0) == T, "selected must have one row per token");
   need(E <= 1024 && k >= 1 && k <= 64 && k <= E, "1 .. 64 slots of at most 1024 experts");
-  Tensor d = empty({T, E}, logits.scalar_type(), logits);
-  CALL(sfp8_moe_route_bwd, fptr(dweights), lptr(selected), fptr(picked), ptr(logits), dtype, T, E, logits.stride(0), sc,
-       k, (int)renormalize, (float)scale, ptr(d), stream_of(logits));
+  Tensor d = empty({T, E}, type, selected);
+  CALL(sfp8_moe_route_bwd, fptr(dweights), lptr(selected), fptr(picked), ptr(logits), dtype_code(type), T, E,
+       logits ? logits->stride(0) : E, score, k, (int)renormalize, (float)scale, ptr(d), stream_of(selected));
   return d;
+}
+
+Tensor moe_route_bwd(const Tensor& dweights, const Tensor& selected, const Tensor& picked, const Tensor& logits,
+                     const std::string& score, bool renormalize, double scale) {
+  float_code("logits", logits);
+  const int sc = score_code(score);
+  if (logits.dim() != 2) refuse("logits must be 2-D, got shape " + shape_of(logits));
+  need(logits.size(1) > 0, "logits need at least one expert");
+  contig("selected", selected, kI64, 2);
+  same_device("selected", selected, logits);
+  need(selected.size(0) == logits.size(0), "selected must have one row per token");
+  return route_gradient(dweights, selected, picked, sc == 0 && !renormalize ? OptTensor(logits) : OptTensor(),
+                        logits.scalar_type(), logits.size(1), sc, renormalize, scale);
 }
 
 std::tuple<Tensor, Tensor, Tensor> moe_expert_order(const Tensor& selected, int64_t E) {
@@ -548,10 +558,16 @@ struct RouteTokens : torch::autograd::Function<RouteTokens> {
                                int64_t top_k, bool renormalize, double scale, bool needs_grad) {
     auto [w, sel, picked] = moe_route(logits, bias, mask, score, groups, top_groups, group_best, top_k, renormalize,
                                       scale, needs_grad);
-    if (needs_grad) ctx->save_for_backward({logits, sel, *picked});
-    ctx->saved_data["score"] = score;
-    ctx->saved_data["renormalize"] = renormalize;
-    ctx->saved_data["scale"] = scale;
+    if (needs_grad) {
+      // the logits are kept for the plain softmax alone: else they may change or go
+      const bool dense = score == "softmax" && !renormalize;
+      ctx->save_for_backward(dense ? variable_list{sel, *picked, logits} : variable_list{sel, *picked});
+      ctx->saved_data["sigmoid"] = score == "sigmoid";
+      ctx->saved_data["renormalize"] = renormalize;
+      ctx->saved_data["scale"] = scale;
+      ctx->saved_data["type"] = (int64_t)logits.scalar_type();
+      ctx->saved_data["experts"] = logits.size(1);
+    }
     ctx->mark_non_differentiable({sel});
     ctx->set_materialize_grads(false);
     return {w, sel};
@@ -562,8 +578,10 @@ struct RouteTokens : torch::autograd::Function<RouteTokens> {
     const variable_list v = ctx->get_saved_variables();
     {
       const c10::AutoGradMode off(false);
-      out[0] = moe_route_bwd(grads[0], v[1], v[2], v[0], ctx->saved_data["score"].toStringRef(),
-                             ctx->saved_data["renormalize"].toBool(), ctx->saved_data["scale"].toDouble());
+      out[0] = route_gradient(grads[0], v[0], v[1], v.size() > 2 ? OptTensor(v[2]) : OptTensor(),
+                              (ScalarType)ctx->saved_data["type"].toInt(), ctx->saved_data["experts"].toInt(),
+                              ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renormalize"].toBool(),
+                              ctx->saved_data["scale"].toDouble());
     }
     return once(std::move(out), "route_tokens");
   }

@@ -898,3 +898,32 @@ def test_bias_that_requires_a_gradient(dev, score, compiled):
     z, _ = f(b, bias.detach(), rows)
     z.backward(dout)
     assert bias.grad is None and torch.equal(y, z) and torch.equal(a.grad, b.grad)
+
+
+@pytest.mark.parametrize("score,renorm", [("softmax", True), ("sigmoid", True), ("sigmoid", False), ("softmax", False)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_logits_after_routing(dev, score, renorm, dtype):
+    """The gradient needs the logits' values for the plain softmax alone: else
+    they may be written, and their memory is free, once the tokens are routed.
+    For the plain softmax a write is refused."""
+    T, E, k = 4096, 256, 4
+    leaf = _logits(dev, T, E, DTYPES[dtype], 31).requires_grad_(True)
+    dw = torch.randn(T, k, device=dev)
+    kw = dict(score=score, renormalize=renorm)
+    want, = torch.autograd.grad(sg.route_tokens(leaf * 1, k, **kw)[0], leaf, dw)
+    low = leaf * 1
+    w, sel = sg.route_tokens(low, k, **kw)
+    low.detach().zero_()
+    dense = score == "softmax" and not renorm
+    if dense:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(w, leaf, dw)
+    else:
+        assert torch.equal(torch.autograd.grad(w, leaf, dw)[0], want)
+    del low, w, sel
+    torch.cuda.synchronize()
+    start = torch.cuda.memory_allocated()
+    w, sel = sg.route_tokens(leaf * 1, k, **kw)
+    held = torch.cuda.memory_allocated() - start
+    assert (held >= T * E * leaf.element_size()) == dense
+    assert torch.equal(torch.autograd.grad(w, leaf, dw)[0], want)
