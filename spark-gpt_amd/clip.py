@@ -37,10 +37,14 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, out: Sequence[tor
     return ops.clip_grads(list(grads), float(max_norm), None if out is None else list(out))
 
 
-def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float,
-                    error_if_nonfinite: bool = False) -> torch.Tensor:
+def clip_grad_norm_(parameters: torch.Tensor | Iterable[torch.Tensor], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False, foreach: bool | None = None) -> torch.Tensor:
     """``clip_grads`` in place on the gradients of ``parameters`` (those that have
-    one); a zero when none has."""
+    one); a zero when none has.  The arguments are torch's: of the norms only the
+    2-norm is offered, ``foreach`` changes nothing.  Unlike there, a gradient that
+    is listed twice is refused, and all are on one device."""
+    if float(norm_type) != 2.0:
+        raise ValueError(f"clip_grad_norm_ offers the 2-norm alone, got norm_type {norm_type}")
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:

@@ -264,3 +264,34 @@ def test_captured_and_replayed(dev):
         wn = sg.clip_grads(new, 1.0, out=want)
         torch.cuda.synchronize()
         assert torch.equal(norm, wn) and all(torch.equal(a, b) for a, b in zip(out, want)), rep
+
+
+def test_parameters_called_as_torch_is(dev):
+    """The positions of torch.nn.utils.clip_grad_norm_: the third is the norm's
+    type, of which only 2 is offered, the fourth whether a norm that is not finite
+    raises, the fifth how torch goes about it."""
+    def params(*values):
+        out = []
+        for v in values:
+            out.append(torch.nn.Parameter(torch.zeros(50, device=dev)))
+            out[-1].grad = torch.full((50,), v, device=dev)
+        return out
+
+    for args in ((1.0,), (1.0, 2.0), (1.0, 2), (1.0, 2.0, False), (1.0, 2.0, True), (1.0, 2.0, False, None),
+                 (1.0, 2.0, True, True)):
+        ours, torchs = params(3.0, -0.5), params(3.0, -0.5)
+        norm, want = sg.clip_grad_norm_(ours, *args), torch.nn.utils.clip_grad_norm_(torchs, *args)
+        assert abs(float(norm) - float(want)) <= 1e-6 * float(want)
+        assert all(((a.grad - b.grad).abs() <= 1e-6 * b.grad.abs()).all() for a, b in zip(ours, torchs))
+    bad = params(3.0, float("nan"))
+    assert sg.clip_grad_norm_(bad, 1.0, 2.0).isnan()  # no error: none is asked for
+    bad = params(3.0, float("nan"))
+    with pytest.raises(RuntimeError, match="not clipped"):
+        sg.clip_grad_norm_(bad, 1.0, 2.0, True)
+    assert bool((bad[0].grad == 3).all())
+    for kind in (1.0, float("inf"), 0.0, 3, "inf"):
+        p = params(3.0)
+        for call in (lambda: sg.clip_grad_norm_(p, 1.0, kind), lambda: sg.clip_grad_norm_(p, 1.0, norm_type=kind)):
+            with pytest.raises(ValueError, match="2-norm"):
+                call()
+        assert bool((p[0].grad == 3).all())
