@@ -512,27 +512,33 @@ Tensor moe_combine(const Tensor& rows, const Tensor& weights, const Tensor& inve
   return out;
 }
 
+// Of the rows [R, D] only the gradient of the weights reads the values: without them, theirs alone is computed.
+std::tuple<OptTensor, OptTensor> combine_gradient(const Tensor& dout, const OptTensor& rows, int64_t R,
+                                                  const Tensor& weights, const Tensor& inverse_permutation,
+                                                  bool need_rows, bool need_weights) {
+  const c10::DeviceGuard guard(dout.device());
+  const int64_t T = weights.size(0), k = weights.size(1), D = dout.size(1);
+  OptTensor drows, dweights, ws;  // ws: which slots name each row
+  if (need_rows) drows = empty({R, D}, dout.scalar_type(), dout);
+  if (need_weights) dweights = empty(weights.sizes(), kF32, dout);
+  const int64_t nws = need_rows ? sfp8_moe_combine_bwd_any_workspace_ints(R, T, k) : 0;
+  if (nws > 0) ws = empty({nws}, ScalarType::Int, dout);
+  CALL(sfp8_moe_combine_bwd_any, ptr(dout), ptr(rows), dtype_code(dout.scalar_type()), R, D, fptr(weights),
+       lptr(inverse_permutation), T, k, ptr(drows), fptr(dweights), iptr(ws), nws, stream_of(dout));
+  return {drows, dweights};
+}
+
 std::tuple<OptTensor, OptTensor> moe_combine_bwd(const Tensor& dout, const Tensor& rows, const Tensor& weights,
                                                  const Tensor& inverse_permutation, const Tensor& offsets,
                                                  bool need_rows, bool need_weights) {
-  const int dtype = combine_args(rows, weights, inverse_permutation);
+  combine_args(rows, weights, inverse_permutation);
   contig("dout", dout, rows.scalar_type(), 2);
   contig("offsets", offsets, ScalarType::Int, 1);
   same_device("dout", dout, rows);
   same_device("offsets", offsets, rows);
   need(offsets.size(0) >= 1, "offsets must have one entry per expert");
   need(dout.size(0) == weights.size(0) && dout.size(1) == rows.size(1), "dout must be [tokens, columns of rows]");
-  const c10::DeviceGuard guard(rows.device());
-  OptTensor drows, dweights;
-  if (need_rows) drows = empty(rows.sizes(), rows.scalar_type(), rows);
-  if (need_weights) dweights = empty(weights.sizes(), kF32, rows);
-  const int64_t R = rows.size(0), T = weights.size(0), k = weights.size(1);
-  OptTensor ws;  // which slots name each row
-  const int64_t nws = need_rows ? sfp8_moe_combine_bwd_any_workspace_ints(R, T, k) : 0;
-  if (nws > 0) ws = empty({nws}, ScalarType::Int, rows);
-  CALL(sfp8_moe_combine_bwd_any, ptr(dout), ptr(rows), dtype, R, rows.size(1), fptr(weights), lptr(inverse_permutation), T,
-       k, ptr(drows), fptr(dweights), iptr(ws), nws, stream_of(rows));
-  return {drows, dweights};
+  return combine_gradient(dout, rows, rows.size(0), weights, inverse_permutation, need_rows, need_weights);
 }
 
 // The autograd nodes of routing.py's eager calls: what _RouteTokens and
@@ -600,18 +606,22 @@ std::tuple<Tensor, Tensor> route_tokens(const Tensor& logits, const OptTensor& b
 
 struct CombineExperts : torch::autograd::Function<CombineExperts> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& inverse,
-                        const Tensor& offsets) {
-    ctx->save_for_backward({rows, weights, inverse, offsets});
-    return moe_combine(rows.contiguous(), weights.contiguous(), inverse.contiguous());
+                        const Tensor& offsets, bool weights_grad) {
+    const Tensor out = moe_combine(rows.contiguous(), weights.contiguous(), inverse.contiguous());
+    // the rows are kept for the gradient of the weights alone: else they may change or go
+    ctx->save_for_backward(weights_grad ? variable_list{weights, inverse, rows} : variable_list{weights, inverse});
+    ctx->saved_data["rows"] = rows.size(0);
+    return out;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list v = ctx->get_saved_variables();
-    variable_list out(4);
+    variable_list out(5);
     {
       const c10::AutoGradMode off(false);
-      auto [drows, dweights] = moe_combine_bwd(grads[0].contiguous(), v[0].contiguous(), v[1].contiguous(),
-                                               v[2].contiguous(), v[3].contiguous(), ctx->needs_input_grad(0),
-                                               ctx->needs_input_grad(1));
+      const OptTensor rows = v.size() > 2 ? OptTensor(v[2].contiguous()) : OptTensor();
+      auto [drows, dweights] =
+          combine_gradient(grads[0].contiguous(), rows, ctx->saved_data["rows"].toInt(), v[0].contiguous(),
+                           v[1].contiguous(), ctx->needs_input_grad(0), rows && ctx->needs_input_grad(1));
       if (drows) out[0] = *drows;
       if (dweights) out[1] = *dweights;
     }
@@ -621,8 +631,8 @@ struct CombineExperts : torch::autograd::Function<CombineExperts> {
 
 Tensor combine_experts(const Tensor& rows, const Tensor& weights, const Tensor& inverse_permutation,
                        const Tensor& offsets) {
-  return CombineExperts::apply(rows, weights.scalar_type() == kF32 ? weights : weights.to(kF32), inverse_permutation,
-                               offsets);
+  const Tensor w = weights.scalar_type() == kF32 ? weights : weights.to(kF32);
+  return CombineExperts::apply(rows, w, inverse_permutation, offsets, c10::GradMode::is_enabled() && w.requires_grad());
 }
 
 // ------------------------------------------------------------------ gradient norm and clipping

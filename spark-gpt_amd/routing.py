@@ -110,7 +110,8 @@ def combine_experts(rows: torch.Tensor, weights: torch.Tensor, inverse_permutati
                     offsets: torch.Tensor) -> torch.Tensor:
     """``out[t] = sum over j of weights[t, j] * rows[inverse_permutation[t * k + j]]``
     [T, D]: rows [R, D] bf16, fp16 or fp32 in expert order, weights [T, k]
-    (k <= 64), ``inverse_permutation`` and ``offsets`` of ``expert_order``.  The
+    (k <= 64), ``inverse_permutation`` and ``offsets`` of ``expert_order`` (the
+    latter is not read: the slots say which rows there are).  The
     sum is taken in 32 bits in slot order and rounded once; slots without a row
     (-1, or anything outside [0, R)) add nothing.  In the backward pass a row that
     no slot names gets zeros and one that several name the sum of theirs, in 32

@@ -927,3 +927,36 @@ def test_logits_after_routing(dev, score, renorm, dtype):
     held = torch.cuda.memory_allocated() - start
     assert (held >= T * E * leaf.element_size()) == dense
     assert torch.equal(torch.autograd.grad(w, leaf, dw)[0], want)
+
+
+def test_rows_after_the_combine(dev):
+    """The rows' values are needed for the gradient of the weights alone: with
+    weights that need none the rows may be written, and their memory is free,
+    once they are combined.  Else a write is refused."""
+    T, k, D = 1000, 4, 256
+    sel = torch.randint(-1, 8, (T, k), device=dev)
+    _, inv, off = sg.expert_order(sel, 8)
+    leaf = torch.randn(T * k, D, device=dev, requires_grad=True)
+    dout = torch.randn(T, D, device=dev)
+    for learns in (False, True):
+        w = torch.rand(T, k, device=dev, requires_grad=learns)
+        want, = torch.autograd.grad(sg.combine_experts(leaf * 1, w, inv, off), leaf, dout)
+        rows = leaf * 1
+        y = sg.combine_experts(rows, w, inv, off)
+        rows.detach().zero_()
+        if learns:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(y, leaf, dout)
+        else:
+            assert torch.equal(torch.autograd.grad(y, leaf, dout)[0], want)
+        del rows, y
+        torch.cuda.synchronize()
+        start = torch.cuda.memory_allocated()
+        y = sg.combine_experts(leaf * 1, w, inv, off)
+        held = torch.cuda.memory_allocated() - start
+        assert (held >= T * k * D * 4) == learns
+        assert torch.equal(torch.autograd.grad(y, leaf, dout)[0], want)
+        del y
+    w = torch.rand(T, k, device=dev, requires_grad=True)
+    got, = torch.autograd.grad(sg.combine_experts(leaf.detach(), w, inv, off), w, dout)
+    assert torch.equal(got, sg.ops.moe_combine_bwd(dout, leaf.detach(), w.detach(), inv, off, False, True)[1])
