@@ -14,6 +14,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -548,14 +549,23 @@ std::tuple<OptTensor, OptTensor> moe_combine_bwd(const Tensor& dout, const Tenso
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Gradients that can be taken once: a second derivative raises.
-variable_list once(variable_list grads, const char* what) {
+// Gradients that can be taken once: a second derivative raises.  The node that
+// raises leads on to what the gradients depend on, the operator's inputs and the
+// upstream gradients, so that a derivative in one of these alone
+// (torch.autograd.grad) passes it too.
+variable_list once(variable_list grads, const variable_list& upstream, const char* what) {
   if (!c10::GradMode::is_enabled()) return grads;
+  torch::autograd::edge_list edges = torch::autograd::get_current_node()->next_edges();
+  for (const auto& e : torch::autograd::collect_next_edges(upstream)) edges.push_back(e);
+  const std::shared_ptr<torch::autograd::Node> raise(
+      new torch::autograd::Error(std::string(what) + " is differentiable once", std::move(edges)),
+      torch::autograd::deleteNode);
   for (Tensor& g : grads)
-    if (g.defined()) g = g.detach().set_requires_grad(true);
-  const int64_t n = (int64_t)grads.size();
-  return std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", n)
-      ->apply(std::move(grads));
+    if (g.defined()) {
+      g = g.detach();
+      torch::autograd::set_history(g, raise);
+    }
+  return grads;
 }
 
 struct RouteTokens : torch::autograd::Function<RouteTokens> {
@@ -589,7 +599,7 @@ struct RouteTokens : torch::autograd::Function<RouteTokens> {
                               ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["renormalize"].toBool(),
                               ctx->saved_data["scale"].toDouble());
     }
-    return once(std::move(out), "route_tokens");
+    return once(std::move(out), grads, "route_tokens");
   }
 };
 
@@ -625,7 +635,7 @@ struct CombineExperts : torch::autograd::Function<CombineExperts> {
       if (drows) out[0] = *drows;
       if (dweights) out[1] = *dweights;
     }
-    return once(std::move(out), "combine_experts");
+    return once(std::move(out), grads, "combine_experts");
   }
 };
 

@@ -960,3 +960,30 @@ def test_rows_after_the_combine(dev):
     w = torch.rand(T, k, device=dev, requires_grad=True)
     got, = torch.autograd.grad(sg.combine_experts(leaf.detach(), w, inv, off), w, dout)
     assert torch.equal(got, sg.ops.moe_combine_bwd(dout, leaf.detach(), w.detach(), inv, off, False, True)[1])
+
+
+def test_second_derivatives_are_refused(dev):
+    """The first gradient with create_graph is the plain one; a derivative of it
+    raises, whole or in one leaf, and alone or in a sum where its part would
+    otherwise be missing."""
+    T, E, k, D = 12, 8, 2, 24
+    sel = torch.randint(0, E, (T, k), device=dev)
+    _, inv, off = sg.expert_order(sel, E)
+    low, rows, w = (torch.randn(s, device=dev, requires_grad=True) for s in ((T, E), (T * k, D), (T, k)))
+    calls = [(lambda kw=kw: sg.route_tokens(low, k, **kw)[0], (low,), (T, k))
+             for kw in (dict(), dict(renormalize=False), dict(score="sigmoid"))]
+    calls.append((lambda: sg.combine_experts(rows, w, inv, off), (rows, w), (T, D)))
+    for call, leaves, shape in calls:
+        for upstream_learns in (False, True):
+            dy = torch.randn(shape, device=dev, requires_grad=upstream_learns)
+            want = torch.autograd.grad(call(), leaves, dy.detach())
+            got = torch.autograd.grad(call(), leaves, dy, create_graph=True)
+            for d, x in zip(got, want):
+                assert d.requires_grad and torch.equal(d, x)
+                with pytest.raises(RuntimeError, match="differentiable once"):
+                    d.square().sum().backward(retain_graph=True)
+                for leaf in leaves + ((dy,) if upstream_learns else ()):
+                    loss = (leaf * 3).sum() + d.square().sum()
+                    with pytest.raises(RuntimeError, match="differentiable once"):
+                        torch.autograd.grad(loss, leaf, retain_graph=True)
+        assert all(leaf.grad is None for leaf in leaves)
