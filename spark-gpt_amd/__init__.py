@@ -1,6 +1,6 @@
 """MI355X-native SwiGLU MLP paths of spark-gpt: the FP8 block and experts, and the
-bf16 fused SwiGLU, the routing of tokens to experts around the latter, and the
-clipping of their gradients (gfx950 HIP kernels behind a C ABI).
+bf16 fused SwiGLU, the routing of tokens around the FP8 experts, and the clipping
+of gradients (gfx950 HIP kernels behind a C ABI).
 
 Import as ``spark_gpt_amd`` (the repository-root module of that name loads
 this directory as the package).

@@ -544,8 +544,9 @@ std::tuple<OptTensor, OptTensor> moe_combine_bwd(const Tensor& dout, const Tenso
 
 // The autograd nodes of routing.py's eager calls: what _RouteTokens and
 // _CombineExperts do there, without Python's share of a node (a training pass
-// of a few tokens, bound by host time: 77 us with the Python nodes, 56 with
-// these, 49 for a torch product and its gradient).
+// of a few tokens, bound by host time, in one run on one clock: 74 us with the
+// Python nodes, 54 with these, 61 for the combine, 47 for a torch product and its
+// gradient).
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 

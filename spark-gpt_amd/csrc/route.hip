@@ -350,13 +350,24 @@ SFP8_DEV int route_exact(const RouteArgs& a, int64_t t, uint64_t* v) {
 // mean |d| is at most log(1024)) and up to 37 additions in a row, and the quotient: by
 // less than 64 2^-24 of the row's largest probability, 1 / z, in all (|d| e^-|d| <
 // 0.4).  A sigmoid is off by less than 2^-21.  The sums with the bias round once more.
+// The sums of two groups that 64 bits do not tell apart either come as they are
+// rounded there.
+//
+// What that costs goes by the values, since the bounds are those of the row's
+// largest (kernel us, 65536 tokens): a bias of 0 and 8 of 256 normal logits of
+// standard deviation 1, 3, 5, 8 take 36, 39, 57 and 104 with softmax, 28, 30, 38
+// and 146 with sigmoid (scores near 1 differ by less than 2^-21); with biases of
+// 0.05 33-37 and 28-29.  A large finite value in a row (-1e9 for what is masked)
+// takes all steps of the scale where the low value is the row's smallest: with
+// groups, or no more lanes than slots (8 of 64 experts 9 -> 108, 2 of 8 3.6 ->
+// 58, 8 of 256 19 as without); -inf costs nothing.
 //
 // A token's result depends on its row and on E, top_k and the groups alone,
 // not on the batch it comes in.
 //
-// Bound by its vector instructions: 65536 tokens, 8 of 256 experts, fp32 19.5 us
-// (15 for the bytes), 545 instructions a wave of four tokens, 300 of them in the
-// selection; bf16 17.5; with sigmoid scores, a bias and groups 34 (998).  16
+// Bound by its vector instructions: 65536 tokens, 8 of 256 experts, fp32 19-20 us
+// (15 for the bytes), 546 instructions a wave of four tokens, 300 of them in the
+// selection; bf16 17.2; with sigmoid scores, a bias and groups 35 (1003).  16
 // lanes of 16 logits take fewer of them a token than 64 of 4 (the lane steps are
 // shared by four tokens).
 // ---------------------------------------------------------------------------
@@ -693,7 +704,8 @@ struct RouteBwdArgs {
 // its expert, from the chosen logits alone; the plain softmax also reads the
 // row again, for p of every expert.  The row is put together in LDS (zeros or
 // the dense part, then the slots' values) and written whole, once: bound by
-// those bytes (65536 x 256 fp32 13.3 us, 5.0 TB/s; 65536 x 8 bf16 3.2).
+// those bytes (65536 x 256 fp32 13.5 us, 5.0 TB/s, the plain softmax 22.6, 5.9 read
+// and written; 65536 x 8 bf16 3.4).
 template <int L, int V>
 __global__ __launch_bounds__(256) void moe_route_bwd_kernel(const RouteBwdArgs a) {
   __shared__ __align__(16) float rows[256 * V];
@@ -1109,7 +1121,7 @@ SFP8_DEV void sum_slots(const void* dout, int64_t D, const float* weights, const
 // on get zeros.  One wave a slot, or `lanes` lanes (a power of two) where a row
 // has fewer units: the lanes of a token's slots share its gradient through the
 // caches.  Bound by the rows' bytes, read and written (65536 tokens of 2 rows of
-// 1024 104 us; 131072 of 2 of 128 32, in whole waves 53).
+// 1024 103 us, 6.5 TB/s; 131072 of 2 of 128 32, in whole waves 53).
 template <int DT, int CUT, bool NT, bool WIDE>
 __global__ __launch_bounds__(256) void moe_combine_bwd_kernel(
     const void* __restrict__ dout, const void* __restrict__ rows, int64_t R, int64_t D,

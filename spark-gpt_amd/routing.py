@@ -64,7 +64,8 @@ def route_tokens(logits: torch.Tensor, top_k: int, *, score: str = "softmax", bi
     * ``groups``, ``top_groups``, ``group_best``: the experts are ``groups``
       groups of E / groups in a row, and only the ``top_groups`` best take
       part (default: all).  A group's value is the best order value in it
-      (``group_best=1``) or the sum of its two best scores, biases included (2).
+      (``group_best=1``) or the sum of its two best scores, biases included (2);
+      two sums that 64 bits do not tell apart may come either way.
     * ``renormalize``: weights are scores over the sum of the chosen ones;
       ``scale`` multiplies the weights.
     * ``mask`` (bool [T]): tokens that are False are not routed.
