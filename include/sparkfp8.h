@@ -548,6 +548,45 @@ int sfp8_grad_clip(int64_t count, const void* const* grads, void* const* out, co
                    float max_norm, float* norm, double* ws, int64_t ws_doubles, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (MXFP4): quantisation and products.  No
+ * counterpart in the reference.
+ *
+ * 32 values of a row share one power of two, 2^(floor(log2(largest |value|)) -
+ * 2), not below 2^-127 (8-bit exponent, bias 127); each is held as the e2m1
+ * code (0 0.5 1 1.5 2 3 4 6, a sign) nearest to value / scale, ties to the even
+ * code, +-6 past that.  A block with an infinity or a NaN has scale 255: all
+ * its values are NaN.  A matrix [R, C] is
+ *   codes  [ceil(C / 128)][ceil(R / 16) * 16][64] bytes, the lower value in
+ *          the lower half of a byte,
+ *   scales [ceil(C / 128)][ceil(R / 16) * 16][4] bytes,
+ * padding zero; a batch is that many times this.  sfp8_mxfp4_code_bytes(R, C)
+ * is the size of one matrix' codes (its scales take a sixteenth of it).
+ * dtype: 0 fp32, 1 bf16, 2 fp16.  Codes and products are 16-byte aligned,
+ * scales 4; dimensions are at most 2^31.
+ * ------------------------------------------------------------------------- */
+int64_t sfp8_mxfp4_code_bytes(int64_t R, int64_t C);
+
+/* Codes and scales of batch matrices x [R, C] (rows ld apart, matrices
+ * batch_stride), and those of their transposes [C, R] (blocks along the
+ * columns of x); either pair may be NULL. */
+int sfp8_mxfp4_quantize(const void* x, int dtype, int64_t batch, int64_t R, int64_t C, int64_t ld,
+                        int64_t batch_stride, void* codes, void* scales, void* codes_t, void* scales_t, void* stream);
+
+/* out [batch, R, C] = the values that codes and scales stand for, rounded to dtype. */
+int sfp8_mxfp4_dequantize(const void* codes, const void* scales, int64_t batch, int64_t R, int64_t C, void* out,
+                          int dtype, void* stream);
+
+/* out [M, N] = A B^T over the values of A [M, K] and B [N, K], summed in fp32
+ * and rounded once to dtype. */
+int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t M, int64_t N,
+                    int64_t K, void* out, int dtype, void* stream);
+
+/* The same for up to 16 rows x [M, K] (x_type, rows ldx apart) that are
+ * quantised on the way, bit for bit as sfp8_mxfp4_quantize does. */
+int sfp8_mxfp4_gemm_rows(const void* x, int x_type, int64_t ldx, const void* b, const void* b_scales, int64_t M,
+                         int64_t N, int64_t K, void* out, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
  * The consumer of the fp32 weight gradients: the Muon optimizer's momentum
  * stage (train.py:2805-2839), alone and fused into the weight gradient.
  * ------------------------------------------------------------------------- */

@@ -91,6 +91,12 @@ SIGNATURES = {
     "sfp8_grad_norm_workspace_doubles": (_I64, [_I64]),
     "sfp8_grad_norm": (_INT, [_I64, _P, _P, _P, _P, _P, _I64, _P]),
     "sfp8_grad_clip": (_INT, [_I64, _P, _P, _P, _P, _F32, _P, _P, _I64, _P]),
+    # microscaled 4-bit floating point
+    "sfp8_mxfp4_code_bytes": (_I64, [_I64, _I64]),
+    "sfp8_mxfp4_quantize": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
+    "sfp8_mxfp4_dequantize": (_INT, [_P, _P, _I64, _I64, _I64, _P, _INT, _P]),
+    "sfp8_mxfp4_gemm": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _INT, _P]),
+    "sfp8_mxfp4_gemm_rows": (_INT, [_P, _INT, _I64, _P, _P, _I64, _I64, _I64, _P, _INT, _P]),
     # the optimizer's momentum stage, and the weight gradient fused with it
     "sfp8_momentum_stage": (_INT, [_P, _P, _P, _I64, _F32, _F32, _P]),
     "sfp8_wgrad_momentum_workspace_floats": (_I64, [_I64, _I64, _I64]),

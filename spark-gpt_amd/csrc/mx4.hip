@@ -1,0 +1,439 @@
+// MXFP4 (mx4.h): quantisation along rows and columns, the values back, and the
+// product of two quantised matrices (gfx950).
+//
+//  * mx_quantize: codes and scales of a matrix, of its transpose, or of both
+//    from one read.  Bound by the bytes it reads and writes.
+//  * mx_dequantize: the values that codes and scales stand for.
+//  * mx_gemm: C = A B^T over the values, v_mfma_scale_f32_*_f8f6f4 with fp4
+//    operands (the matrix cores multiply by the two blocks' scales), sums in
+//    fp32, one rounding at the end.
+#include "mx4.h"
+
+namespace sfp8 {
+
+// ---------------------------------------------------------------------------
+// Quantisation
+// ---------------------------------------------------------------------------
+SFP8_DEV uint32_t max_u(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <int CTRL>
+SFP8_DEV uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true);
+}
+
+struct MxQuantArgs {
+  const void* x;
+  int64_t R, C, ld, batch_stride;  // elements
+  uint8_t *codes, *scales;         // of x, or NULL
+  uint8_t *codes_t, *scales_t;     // of its transpose, or NULL
+};
+
+// One work-group takes 128 x 128 values.  Sixteen lanes hold 128 values of a
+// row (four lanes a block: its maximum is two lane exchanges away), so the row
+// codes leave straight from the registers, four rows of 64 bytes in one run.
+// For the columns the values pass through LDS as they are: a lane then holds
+// 32 values of one column (16-bit types: of two), so neither its maximum nor
+// its codes need another lane; the codes go back through LDS so that each
+// column's 64 bytes and the tile's 8 KiB are written in one run.
+template <int DT, bool ROWS, bool COLS>
+__global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
+  constexpr int kSize = DT == kMxF32 ? 4 : 2;
+  __shared__ __align__(16) uint8_t raw[COLS ? 128 * 128 * kSize : 16];
+  __shared__ __align__(16) uint8_t out[COLS ? 128 * 64 : 16];
+  __shared__ __align__(16) uint8_t out_scale[COLS ? 512 : 16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t nx = mx_slabs(a.C), ny = (a.R + 127) / 128;
+  const int64_t id = blockIdx.x, cs = id % nx, rs = id / nx % ny, z = id / nx / ny;
+  const int64_t c0 = cs * 128, r0 = rs * 128, rows = mx_rows(a.R), cols = mx_rows(a.C);
+  const uint8_t* x = reinterpret_cast<const uint8_t*>(a.x) + z * a.batch_stride * kSize;
+  const int col = 8 * (lane & 15), sub = 4 * wave + (lane >> 4);
+
+  Eight<DT> v[8];
+  if (c0 + 128 <= a.C && r0 + 128 <= a.R) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = load8<DT>(x, (r0 + 16 * i + sub) * a.ld + c0 + col);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t r = r0 + 16 * i + sub;
+      v[i] = Eight<DT>{};
+      if (r < a.R && c0 + col < a.C) v[i] = load8_upto<DT>(x, r * a.ld + c0 + col, a.C - c0 - col);
+    }
+  }
+  if constexpr (ROWS) {
+    uint8_t* codes = a.codes + (z * nx + cs) * rows * 64;
+    uint8_t* scales = a.scales + (z * nx + cs) * rows * 4;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m = abs_max8<DT>(v[i]);
+      m = max_u(m, dpp<0xB1>(m));
+      m = max_u(m, dpp<0x4E>(m));
+      const uint32_t e = mx_scale_code(abs_bits_to_f32<DT>(m));
+      const uint32_t c = codes8<DT>(v[i], mx_scale_value(e));
+      uint32_t s = e << (8 * ((lane >> 2) & 3));  // the row's four scales in one word
+      s |= dpp<0x141>(s);
+      s |= dpp<0x140>(s);
+      const int64_t r = r0 + 16 * i + sub;
+      if (r < rows) {
+        *reinterpret_cast<uint32_t*>(codes + r * 64 + 4 * (lane & 15)) = c;
+        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + r * 4) = s;
+      }
+    }
+  }
+  if constexpr (COLS) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t* p = reinterpret_cast<uint32_t*>(raw + ((16 * i + sub) * 128 + col) * kSize);
+      *reinterpret_cast<intx4*>(p) = intx4{(int)v[i].w[0], (int)v[i].w[1], (int)v[i].w[2], (int)v[i].w[3]};
+      if constexpr (DT == kMxF32)
+        *reinterpret_cast<intx4*>(p + 4) = intx4{(int)v[i].w[4], (int)v[i].w[5], (int)v[i].w[6], (int)v[i].w[7]};
+    }
+    __syncthreads();
+    // 64 words of a row; this lane's word holds one column (fp32) or two
+    constexpr int kHalves = DT == kMxF32 ? 2 : 1;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(raw) + 32 * wave * (64 * kHalves) + 64 * h + lane;
+      uint32_t w[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) w[i] = p[i * 64 * kHalves];
+      constexpr int kCols = DT == kMxF32 ? 1 : 2;
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) {
+        Eight<DT> q[4];
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (DT == kMxF32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[j].w[i] = w[8 * j + i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t lo = w[8 * j + 2 * i], hi = w[8 * j + 2 * i + 1];
+              q[j].w[i] = k ? (lo >> 16) | (hi & 0xffff0000u) : (lo & 0xffffu) | (hi << 16);
+            }
+          }
+          m = max_u(m, abs_max8<DT>(q[j]));
+        }
+        const uint32_t e = mx_scale_code(abs_bits_to_f32<DT>(m));
+        const float s = mx_scale_value(e);
+        const int c = DT == kMxF32 ? 64 * h + lane : 2 * lane + k;
+        // 16-byte chunk `wave` of column c, at chunk wave ^ (c / 2) % 4: the lanes of a store spread over the banks
+        *reinterpret_cast<intx4*>(out + c * 64 + 16 * (wave ^ ((c >> 1) & 3))) =
+            intx4{(int)codes8<DT>(q[0], s), (int)codes8<DT>(q[1], s), (int)codes8<DT>(q[2], s),
+                  (int)codes8<DT>(q[3], s)};
+        out_scale[c * 4 + wave] = (uint8_t)e;
+      }
+    }
+    __syncthreads();
+    uint8_t* codes = a.codes_t + (z * ny + rs) * cols * 64;
+    uint8_t* scales = a.scales_t + (z * ny + rs) * cols * 4;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int u = tid + 256 * j, c = u >> 2, ch = u & 3;
+      if (c0 + c < cols)
+        *reinterpret_cast<intx4*>(codes + (c0 + c) * 64 + 16 * ch) =
+            *reinterpret_cast<const intx4*>(out + c * 64 + 16 * (ch ^ ((c >> 1) & 3)));
+    }
+    if (tid < 128 && c0 + tid < cols)
+      *reinterpret_cast<uint32_t*>(scales + (c0 + tid) * 4) = reinterpret_cast<const uint32_t*>(out_scale)[tid];
+  }
+}
+
+template <int DT>
+void launch_quantize(const MxQuantArgs& a, unsigned grid, hipStream_t stream) {
+  if (a.codes && a.codes_t) mx_quantize_kernel<DT, true, true><<<grid, 256, 0, stream>>>(a);
+  else if (a.codes) mx_quantize_kernel<DT, true, false><<<grid, 256, 0, stream>>>(a);
+  else mx_quantize_kernel<DT, false, true><<<grid, 256, 0, stream>>>(a);
+}
+
+// ---------------------------------------------------------------------------
+// The values back
+// ---------------------------------------------------------------------------
+struct MxDequantArgs {
+  const uint8_t *codes, *scales;
+  int64_t R, C;
+  void* out;  // [R, C]
+};
+
+template <int DT>
+__global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantArgs a) {
+  constexpr int kSize = DT == kMxF32 ? 4 : 2;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t nx = mx_slabs(a.C), ny = (a.R + 127) / 128;
+  const int64_t id = blockIdx.x, cs = id % nx, rs = id / nx % ny, z = id / nx / ny;
+  const int64_t rows = mx_rows(a.R), c = cs * 128 + 8 * (lane & 15), r0 = rs * 128 + 4 * wave + (lane >> 4);
+  const uint8_t* codes = a.codes + (z * nx + cs) * rows * 64;
+  const uint8_t* scales = a.scales + (z * nx + cs) * rows * 4;
+  uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + z * a.R * a.C * kSize;
+  if (c >= a.C) return;
+  uint32_t q[8], e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + 16 * i, rr = r < a.R ? r : 0;
+    q[i] = *reinterpret_cast<const uint32_t*>(codes + rr * 64 + 4 * (lane & 15));
+    e[i] = scales[rr * 4 + ((lane >> 2) & 3)];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t r = r0 + 16 * i;
+    if (r >= a.R) break;
+    const float s = mx_scale_value(e[i]);
+    Eight<DT> v;
+    if constexpr (DT == kMxF32) {
+      const floatx2 f0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], s, 0);
+      const floatx2 f1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], s, 1);
+      const floatx2 f2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], s, 2);
+      const floatx2 f3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[i], s, 3);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        v.w[j] = __float_as_uint(f0[j]);
+        v.w[2 + j] = __float_as_uint(f1[j]);
+        v.w[4 + j] = __float_as_uint(f2[j]);
+        v.w[6 + j] = __float_as_uint(f3[j]);
+      }
+    } else if constexpr (DT == kMxBf16) {
+      const intx4 w = __builtin_bit_cast(intx4, bf16_of_codes8(q[i], s));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v.w[j] = (uint32_t)w[j];
+    } else {
+      v.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q[i], s, 0));
+      v.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q[i], s, 1));
+      v.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q[i], s, 2));
+      v.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q[i], s, 3));
+    }
+    uint8_t* p = out + (r * a.C + c) * kSize;
+    if (c + 8 <= a.C) {
+      *reinterpret_cast<mx_intx4_any*>(p) = mx_intx4_any{(int)v.w[0], (int)v.w[1], (int)v.w[2], (int)v.w[3]};
+      if constexpr (DT == kMxF32)
+        *reinterpret_cast<mx_intx4_any*>(p + 16) = mx_intx4_any{(int)v.w[4], (int)v.w[5], (int)v.w[6], (int)v.w[7]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (c + j < a.C) {
+          if constexpr (DT == kMxF32) reinterpret_cast<uint32_t*>(p)[j] = v.w[j];
+          else reinterpret_cast<uint16_t*>(p)[j] = (uint16_t)(v.w[j / 2] >> (16 * (j & 1)));
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The product, few rows
+// ---------------------------------------------------------------------------
+struct MxGemmArgs {
+  const uint8_t *a, *as;  // [M, K] codes and scales
+  const uint8_t *b, *bs;  // [N, K]
+  const void* x;          // or the first operand's values, rows ldx apart, quantised on the way
+  int64_t ldx;
+  int64_t M, N, K;
+  void* out;  // [M, N]
+  int out_type;
+};
+
+SFP8_DEV void store4(void* out, int type, int64_t i, const float (&v)[4], int n) {
+  if (type == kMxF32) {
+    float* p = reinterpret_cast<float*>(out) + i;
+    if (n == 4 && ((uintptr_t)p & 15) == 0) *reinterpret_cast<floatx4*>(p) = floatx4{v[0], v[1], v[2], v[3]};
+    else
+      for (int j = 0; j < n; ++j) p[j] = v[j];
+    return;
+  }
+  uint16_t* p = reinterpret_cast<uint16_t*>(out) + i;
+  uint32_t w[2];
+  if (type == kMxBf16) {
+    w[0] = pack2_bf16(v[0], v[1]);
+    w[1] = pack2_bf16(v[2], v[3]);
+  } else {
+    w[0] = __builtin_bit_cast(uint32_t, halfx2{(_Float16)v[0], (_Float16)v[1]});
+    w[1] = __builtin_bit_cast(uint32_t, halfx2{(_Float16)v[2], (_Float16)v[3]});
+  }
+  if (n == 4 && ((uintptr_t)p & 7) == 0) *reinterpret_cast<intx2*>(p) = intx2{(int)w[0], (int)w[1]};
+  else
+    for (int j = 0; j < n; ++j) p[j] = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+}
+
+SFP8_DEV intx8 fp4_operand(intx4 v) { return intx8{v[0], v[1], v[2], v[3], 0, 0, 0, 0}; }
+
+// 16 MB rows of A times 16 NB rows of B by WV waves that share the K slabs (a
+// wave takes every WV-th): the operands go from memory to registers, 16 bytes
+// a lane and 1 KiB in a run, each read once in the work-group, and the waves'
+// sums meet in LDS in the order of the waves.  v_mfma_scale_f32_16x16x128:
+// lane l holds row l % 16, block l / 16 of a slab, and its scale; B is the
+// first operand, so a lane's four sums are neighbours in a row of the output.
+// XT >= 0: A is quantised here; a lane's 32 values are one block.
+template <int MB, int NB, int WV, int XT>
+__global__ __launch_bounds__(64 * WV) void mx_few_kernel(MxGemmArgs g) {
+  __shared__ __align__(16) float red[WV][MB * 16][NB * 16 + 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * NB), m0 = (int64_t)blockIdx.y * (16 * MB);
+  const int64_t np = mx_rows(g.N), mp = mx_rows(g.M), S = mx_slabs(g.K);
+  int64_t brow[NB], arow[MB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) brow[j] = (n0 + 16 * j < np ? n0 + 16 * j : np - 16) + r;
+#pragma unroll
+  for (int i = 0; i < MB; ++i) arow[i] = (m0 + 16 * i < mp ? m0 + 16 * i : mp - 16) + r;
+  floatx4 acc[MB][NB];
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int64_t s = wave; s < S; s += WV) {
+    intx4 bv[NB], av[MB];
+    int bsc[NB], asc[MB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      bv[j] = *reinterpret_cast<const intx4*>(g.b + (s * np + brow[j]) * 64 + 16 * q);
+      bsc[j] = (int)(*reinterpret_cast<const uint32_t*>(g.bs + (s * np + brow[j]) * 4) >> (8 * q));
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i) {
+      if constexpr (XT < 0) {
+        av[i] = *reinterpret_cast<const intx4*>(g.a + (s * mp + arow[i]) * 64 + 16 * q);
+        asc[i] = (int)(*reinterpret_cast<const uint32_t*>(g.as + (s * mp + arow[i]) * 4) >> (8 * q));
+      } else {
+        constexpr int DT = XT < 0 ? 0 : XT;
+        const int64_t k = s * 128 + 32 * q, left = arow[i] < g.M ? g.K - k : 0, at = arow[i] * g.ldx + k;
+        Eight<DT> v[4];
+        if (left >= 32) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = load8<DT>(g.x, at + 8 * c);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            v[c] = Eight<DT>{};
+            if (left > 8 * c) v[c] = load8_upto<DT>(g.x, at + 8 * c, left - 8 * c);
+          }
+        }
+        uint32_t m = abs_max8<DT>(v[0]);
+#pragma unroll
+        for (int c = 1; c < 4; ++c) {
+          const uint32_t o = abs_max8<DT>(v[c]);
+          m = o > m ? o : m;
+        }
+        asc[i] = (int)mx_scale_code(abs_bits_to_f32<DT>(m));
+        const float sv = mx_scale_value((uint32_t)asc[i]);
+        av[i] = intx4{(int)codes8<DT>(v[0], sv), (int)codes8<DT>(v[1], sv), (int)codes8<DT>(v[2], sv),
+                      (int)codes8<DT>(v[3], sv)};
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(bv[j]), fp4_operand(av[i]), acc[i][j],
+                                                                     4, 4, 0, bsc[j], 0, asc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) *reinterpret_cast<floatx4*>(&red[wave][16 * i + r][16 * j + 4 * q]) = acc[i][j];
+  __syncthreads();
+  for (int u = tid; u < MB * 16 * NB * 4; u += 64 * WV) {
+    const int m = u / (NB * 4), n = 4 * (u % (NB * 4));
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WV; ++w) {
+      const floatx4 p = *reinterpret_cast<const floatx4*>(&red[w][m][n]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += p[j];
+    }
+    const int64_t left = g.N - (n0 + n);
+    if (m0 + m < g.M && left > 0) store4(g.out, g.out_type, (m0 + m) * g.N + n0 + n, v, left < 4 ? (int)left : 4);
+  }
+}
+
+inline int launched() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? kOk : (int)e;
+}
+inline bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+inline bool type_ok(int dtype) { return dtype >= kMxF32 && dtype <= kMxF16; }
+constexpr int64_t kMxMaxDim = (int64_t)1 << 31;
+
+}  // namespace sfp8
+
+using namespace sfp8;
+
+extern "C" {
+
+int64_t sfp8_mxfp4_code_bytes(int64_t R, int64_t C) {
+  return R < 0 || C < 0 || R > kMxMaxDim || C > kMxMaxDim ? -1 : mx_slabs(C) * mx_rows(R) * 64;
+}
+
+int sfp8_mxfp4_quantize(const void* x, int dtype, int64_t batch, int64_t R, int64_t C, int64_t ld,
+                        int64_t batch_stride, void* codes, void* scales, void* codes_t, void* scales_t, void* stream) {
+  if (!type_ok(dtype) || batch < 0 || R < 0 || C < 0 || R > kMxMaxDim || C > kMxMaxDim || ld < 0 || batch_stride < 0)
+    return kErrBadShape;
+  if (!codes != !scales || !codes_t != !scales_t) return kErrNullPointer;
+  if (batch == 0 || R == 0 || C == 0 || (!codes && !codes_t)) return kOk;
+  if (!x) return kErrNullPointer;
+  if (!aligned(x, dtype == kMxF32 ? 4 : 2) || !aligned(codes, 16) || !aligned(codes_t, 16) || !aligned(scales, 4) ||
+      !aligned(scales_t, 4))
+    return kErrBadAlignment;
+  const int64_t tiles = mx_slabs(C) * ((R + 127) / 128);
+  if (tiles > 0x7fffffff / batch) return kErrBadShape;
+  const MxQuantArgs a{x, R, C, ld, batch_stride, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)codes_t,
+                      (uint8_t*)scales_t};
+  const unsigned grid = (unsigned)(tiles * batch);
+  const hipStream_t s = (hipStream_t)stream;
+  if (dtype == kMxF32) launch_quantize<kMxF32>(a, grid, s);
+  else if (dtype == kMxBf16) launch_quantize<kMxBf16>(a, grid, s);
+  else launch_quantize<kMxF16>(a, grid, s);
+  return launched();
+}
+
+int sfp8_mxfp4_dequantize(const void* codes, const void* scales, int64_t batch, int64_t R, int64_t C, void* out,
+                          int dtype, void* stream) {
+  if (!type_ok(dtype) || batch < 0 || R < 0 || C < 0 || R > kMxMaxDim || C > kMxMaxDim) return kErrBadShape;
+  if (batch == 0 || R == 0 || C == 0) return kOk;
+  if (!codes || !scales || !out) return kErrNullPointer;
+  if (!aligned(codes, 16) || !aligned(scales, 4) || !aligned(out, 16)) return kErrBadAlignment;
+  const int64_t tiles = mx_slabs(C) * ((R + 127) / 128);
+  if (tiles > 0x7fffffff / batch) return kErrBadShape;
+  const MxDequantArgs a{(const uint8_t*)codes, (const uint8_t*)scales, R, C, out};
+  const unsigned grid = (unsigned)(tiles * batch);
+  const hipStream_t s = (hipStream_t)stream;
+  if (dtype == kMxF32) mx_dequantize_kernel<kMxF32><<<grid, 256, 0, s>>>(a);
+  else if (dtype == kMxBf16) mx_dequantize_kernel<kMxBf16><<<grid, 256, 0, s>>>(a);
+  else mx_dequantize_kernel<kMxF16><<<grid, 256, 0, s>>>(a);
+  return launched();
+}
+
+int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t M, int64_t N,
+                    int64_t K, void* out, int dtype, void* stream) {
+  if (!type_ok(dtype) || M < 0 || N < 0 || K < 0 || M > kMxMaxDim || N > kMxMaxDim || K > kMxMaxDim)
+    return kErrBadShape;
+  if (M == 0 || N == 0) return kOk;
+  if (!out || (K && (!a || !a_scales || !b || !b_scales))) return kErrNullPointer;
+  if (!aligned(a, 16) || !aligned(b, 16) || !aligned(a_scales, 4) || !aligned(b_scales, 4) || !aligned(out, 16))
+    return kErrBadAlignment;
+  const MxGemmArgs g{(const uint8_t*)a, (const uint8_t*)a_scales, (const uint8_t*)b, (const uint8_t*)b_scales,
+                     nullptr, 0, M, N, K, out, dtype};
+  const int64_t gx = (N + 63) / 64, gy = (M + 63) / 64;
+  if (gy > 65535) return kErrBadShape;
+  mx_few_kernel<4, 4, 4, -1><<<dim3((unsigned)gx, (unsigned)gy), 256, 0, (hipStream_t)stream>>>(g);
+  return launched();
+}
+
+int sfp8_mxfp4_gemm_rows(const void* x, int x_type, int64_t ldx, const void* b, const void* b_scales, int64_t M,
+                         int64_t N, int64_t K, void* out, int dtype, void* stream) {
+  if (!type_ok(dtype) || !type_ok(x_type) || M < 0 || M > 16 || N < 0 || K < 0 || N > kMxMaxDim || K > kMxMaxDim ||
+      ldx < 0)
+    return kErrBadShape;
+  if (M == 0 || N == 0) return kOk;
+  if (!out || (K && (!x || !b || !b_scales))) return kErrNullPointer;
+  if (!aligned(x, x_type == kMxF32 ? 4 : 2) || !aligned(b, 16) || !aligned(b_scales, 4) || !aligned(out, 16))
+    return kErrBadAlignment;
+  const MxGemmArgs g{nullptr, nullptr, (const uint8_t*)b, (const uint8_t*)b_scales, x, ldx, M, N, K, out, dtype};
+  const unsigned gx = (unsigned)((N + 15) / 16);
+  const hipStream_t s = (hipStream_t)stream;
+  if (x_type == kMxF32) mx_few_kernel<1, 1, 8, kMxF32><<<gx, 512, 0, s>>>(g);
+  else if (x_type == kMxBf16) mx_few_kernel<1, 1, 8, kMxBf16><<<gx, 512, 0, s>>>(g);
+  else mx_few_kernel<1, 1, 8, kMxF16><<<gx, 512, 0, s>>>(g);
+  return launched();
+}
+
+}  // extern "C"

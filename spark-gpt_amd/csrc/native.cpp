@@ -720,6 +720,104 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
   return norm;
 }
 
+// ------------------------------------------------------------------ microscaled 4-bit floating point
+constexpr auto kU8 = ScalarType::Byte;
+constexpr int64_t kMxDim = (int64_t)1 << 31;
+inline int64_t mx_slabs(int64_t C) { return (C + 127) / 128; }
+inline int64_t mx_rows(int64_t R) { return (R + 15) / 16 * 16; }
+
+// Codes and scales of [R, C], or of a batch of E of them.
+void is_mxfp4(const char* name, const Tensor& codes, const Tensor& scales, std::optional<int64_t> E, int64_t R,
+              int64_t C) {
+  need(R >= 0 && C >= 0 && R <= kMxDim && C <= kMxDim, "dimensions must be 0 .. 2^31");
+  const std::string n(name);
+  const int64_t lead = E ? 1 : 0;
+  for (const auto& [what, t, last] :
+       {std::tuple<const char*, const Tensor&, int64_t>{"codes", codes, 64}, {"scales", scales, 4}}) {
+    contig((n + what).c_str(), t, kU8, 3 + lead);
+    if ((E && t.size(0) != *E) || t.size(lead) != mx_slabs(C) || t.size(lead + 1) != mx_rows(R) ||
+        t.size(lead + 2) != last)
+      refuse(n + what + " do not fit the matrix: got " + shape_of(t) + " for [" + std::to_string(R) + ", " +
+             std::to_string(C) + "]");
+    if ((uintptr_t)t.data_ptr() % (last == 64 ? 16 : 4)) refuse(n + what + " must be aligned to 16 bytes, scales to 4");
+  }
+  same_device((n + "scales").c_str(), scales, codes);
+}
+
+ScalarType float_type(const py::object& dtype) {
+  need(THPDtype_Check(dtype.ptr()), "dtype must be a torch.dtype");
+  const ScalarType type = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+  need(dtype_code(type) >= 0, "dtype must be float32, bfloat16 or float16");
+  return type;
+}
+
+using Codes = std::tuple<OptTensor, OptTensor, OptTensor, OptTensor>;
+
+Codes mxfp4_quantize(const Tensor& x_, bool rows, bool columns) {
+  const int dtype = float_code("x", x_);
+  if (x_.dim() != 2 && x_.dim() != 3) refuse("x must be 2-D or 3-D, got shape " + shape_of(x_));
+  need(x_.layout() == at::kStrided, "x must be dense");
+  need(rows || columns, "rows, columns or both");
+  const c10::DeviceGuard guard(x_.device());
+  const int64_t b = x_.dim() - 2;
+  const Tensor x = x_.size(b + 1) <= 1 || x_.stride(b + 1) == 1 ? x_ : x_.contiguous();
+  const int64_t E = b ? x.size(0) : 1, R = x.size(b), C = x.size(b + 1);
+  need(R <= kMxDim && C <= kMxDim, "dimensions must be at most 2^31");
+  const auto make = [&](int64_t r, int64_t c, int64_t last) {
+    const int64_t s = mx_slabs(c), p = mx_rows(r);
+    return b ? empty({E, s, p, last}, kU8, x) : empty({s, p, last}, kU8, x);
+  };
+  Codes out;
+  auto& [codes, scales, codes_t, scales_t] = out;
+  if (rows) codes = make(R, C, 64), scales = make(R, C, 4);
+  if (columns) codes_t = make(C, R, 64), scales_t = make(C, R, 4);
+  CALL(sfp8_mxfp4_quantize, ptr(x), dtype, E, R, C, x.stride(b), b ? x.stride(0) : 0, ptr(codes), ptr(scales),
+       ptr(codes_t), ptr(scales_t), stream_of(x));
+  return out;
+}
+
+Tensor mxfp4_dequantize(const Tensor& codes, const Tensor& scales, int64_t R, int64_t C, const py::object& dtype) {
+  const ScalarType type = float_type(dtype);
+  const int code = dtype_code(type);
+  const bool batch = codes.dim() == 4;
+  const int64_t E = batch ? codes.size(0) : 1;
+  is_mxfp4("", codes, scales, batch ? std::optional<int64_t>(E) : std::nullopt, R, C);
+  const c10::DeviceGuard guard(codes.device());
+  Tensor out = batch ? empty({E, R, C}, type, codes) : empty({R, C}, type, codes);
+  CALL(sfp8_mxfp4_dequantize, ptr(codes), ptr(scales), E, R, C, ptr(out), code, stream_of(codes));
+  return out;
+}
+
+Tensor mxfp4_matmul(const Tensor& a, const Tensor& a_scales, const Tensor& b, const Tensor& b_scales, int64_t M,
+                    int64_t N, int64_t K, const py::object& dtype) {
+  const ScalarType type = float_type(dtype);
+  is_mxfp4("a: ", a, a_scales, std::nullopt, M, K);
+  is_mxfp4("b: ", b, b_scales, std::nullopt, N, K);
+  same_device("b", b, a);
+  const c10::DeviceGuard guard(a.device());
+  Tensor out = empty({M, N}, type, a);
+  CALL(sfp8_mxfp4_gemm, ptr(a), ptr(a_scales), ptr(b), ptr(b_scales), M, N, K, ptr(out), dtype_code(type),
+       stream_of(a));
+  return out;
+}
+
+Tensor mxfp4_rows_matmul(const Tensor& x_, const Tensor& b, const Tensor& b_scales, int64_t N,
+                         const py::object& dtype) {
+  const ScalarType type = float_type(dtype);
+  const int code = float_code("x", x_);
+  if (x_.dim() != 2) refuse("x must be 2-D, got shape " + shape_of(x_));
+  const int64_t M = x_.size(0), K = x_.size(1);
+  need(M <= 16, "at most 16 rows");
+  is_mxfp4("w: ", b, b_scales, std::nullopt, N, K);
+  same_device("w", b, x_);
+  const c10::DeviceGuard guard(x_.device());
+  const Tensor x = K <= 1 || x_.stride(1) == 1 ? x_ : x_.contiguous();
+  Tensor out = empty({M, N}, type, x);
+  CALL(sfp8_mxfp4_gemm_rows, ptr(x), code, x.stride(0), ptr(b), ptr(b_scales), M, N, K, ptr(out), dtype_code(type),
+       stream_of(x));
+  return out;
+}
+
 // ------------------------------------------------------------------ bf16 SwiGLU path
 std::tuple<OptTensor, OptTensor> bf16_weight_slabs(const Tensor& w, const OptTensor& norm_w, bool rows,
                                                    bool transposed) {
@@ -943,6 +1041,15 @@ PYBIND11_MODULE(_native, m) {
   m.def("grad_norm", &grad_norm, arg("grads"), "The 2-norm over all elements of all gradients (fp32 scalar tensor).");
   m.def("clip_grads", &clip_grads, arg("grads"), arg("max_norm"), arg("out") = py::none(),
         "grad_norm(grads); every gradient times min(1, max_norm / (norm + 1e-6)), in place or into out.");
+  m.def("mxfp4_quantize", &mxfp4_quantize, arg("x"), arg("rows") = true, arg("columns") = false,
+        "(codes, scales, codes_t, scales_t) of x [R, C] or [E, R, C], blocks along rows, and of its transpose; None "
+        "where not asked for.");
+  m.def("mxfp4_dequantize", &mxfp4_dequantize, arg("codes"), arg("scales"), arg("R"), arg("C"), arg("dtype"),
+        "The values [R, C] (or [E, R, C]) that codes and scales stand for.");
+  m.def("mxfp4_matmul", &mxfp4_matmul, arg("a"), arg("a_scales"), arg("b"), arg("b_scales"), arg("M"), arg("N"),
+        arg("K"), arg("dtype"), "out [M, N] = A B^T over the values of two quantised matrices.");
+  m.def("mxfp4_rows_matmul", &mxfp4_rows_matmul, arg("x"), arg("w"), arg("w_scales"), arg("N"), arg("dtype"),
+        "mxfp4_matmul of at most 16 rows x [M, K] that are quantised on the way.");
   m.def("bf16_weight_slabs", &bf16_weight_slabs, arg("w"), arg("norm_w") = py::none(), kw, arg("rows") = true,
         arg("transposed") = true,
         "bf16 K-slabs of W [E, R, C] (fp32, times norm_w[c] when given, or bf16): (ws: stacked K-slabs of W[e] [R, C] "

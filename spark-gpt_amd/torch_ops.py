@@ -28,7 +28,7 @@ from __future__ import annotations
 
 import threading
 import weakref
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
@@ -513,3 +513,62 @@ combine_bwd = torch.library.custom_op("sparkfp8::combine_bwd", combine_bwd_impl,
 @combine_bwd.register_fake
 def _combine_bwd_fake(dout, rows, weights, inverse_permutation, offsets):
     return rows.new_empty(tuple(rows.shape)), weights.new_empty(tuple(weights.shape))
+
+
+# ------------------------------------------------------------------ microscaled 4-bit floating point
+def mxfp4_quantize_impl(x: Tensor, rows: bool, columns: bool) -> List[Tensor]:
+    """codes and scales of x, then those of its transpose; a direction that is not asked for is left out."""
+    return [t for t in ops.mxfp4_quantize(x, rows, columns) if t is not None]
+
+
+mxfp4_quantize = torch.library.custom_op("sparkfp8::mxfp4_quantize", mxfp4_quantize_impl, mutates_args=())
+
+
+@mxfp4_quantize.register_fake
+def _mxfp4_quantize_fake(x, rows, columns):
+    R, C = x.shape[-2:]
+    out = []
+    for wanted, r, c in ((rows, R, C), (columns, C, R)):
+        if wanted:
+            out += [x.new_empty((*x.shape[:-2], -(-c // 128), -(-r // 16) * 16, n), dtype=torch.uint8) for n in (64, 4)]
+    return out
+
+
+def mxfp4_dequantize_impl(codes: Tensor, scales: Tensor, R: int, C: int, dtype: torch.dtype) -> Tensor:
+    """The values of codes and scales."""
+    return ops.mxfp4_dequantize(codes, scales, R, C, dtype)
+
+
+mxfp4_dequantize = torch.library.custom_op("sparkfp8::mxfp4_dequantize", mxfp4_dequantize_impl, mutates_args=())
+
+
+@mxfp4_dequantize.register_fake
+def _mxfp4_dequantize_fake(codes, scales, R, C, dtype):
+    return codes.new_empty((*codes.shape[:-3], R, C), dtype=dtype)
+
+
+def mxfp4_matmul_impl(a: Tensor, a_scales: Tensor, b: Tensor, b_scales: Tensor, M: int, N: int, K: int,
+                      dtype: torch.dtype) -> Tensor:
+    """a b^T over the values of two quantised matrices."""
+    return ops.mxfp4_matmul(a, a_scales, b, b_scales, M, N, K, dtype)
+
+
+mxfp4_matmul = torch.library.custom_op("sparkfp8::mxfp4_matmul", mxfp4_matmul_impl, mutates_args=())
+
+
+@mxfp4_matmul.register_fake
+def _mxfp4_matmul_fake(a, a_scales, b, b_scales, M, N, K, dtype):
+    return a.new_empty((M, N), dtype=dtype)
+
+
+def mxfp4_rows_matmul_impl(x: Tensor, w: Tensor, w_scales: Tensor, N: int, dtype: torch.dtype) -> Tensor:
+    """x w^T for at most 16 rows, quantised within the kernel."""
+    return ops.mxfp4_rows_matmul(x, w, w_scales, N, dtype)
+
+
+mxfp4_rows_matmul = torch.library.custom_op("sparkfp8::mxfp4_rows_matmul", mxfp4_rows_matmul_impl, mutates_args=())
+
+
+@mxfp4_rows_matmul.register_fake
+def _mxfp4_rows_matmul_fake(x, w, w_scales, N, dtype):
+    return x.new_empty((x.shape[0], N), dtype=dtype)
