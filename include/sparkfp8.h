@@ -587,6 +587,28 @@ int sfp8_mxfp4_gemm_rows(const void* x, int x_type, int64_t ldx, const void* b, 
                          int64_t N, int64_t K, void* out, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * A mixture-of-experts layer for a few tokens (T <= 64).  No counterpart in
+ * the reference, whose experts run as one grouped path (train.py:2262-2299).
+ * ------------------------------------------------------------------------- */
+
+/* x [T, D] bf16 (rows ldx apart); logits = x router^T (router [E, D] fp32 or
+ * bf16: router_type 0 or 1), summed in 64 bits; experts and weights as
+ * sfp8_moe_route's (the same bias, mask, score, groups, top_groups,
+ * group_best, top_k, renorm, scale), ordered by the 64-bit values; h = silu(x
+ * Wg^T) * (x Wu^T) and out[t] = sum over the slots of weight * h Wd^T (bf16).
+ * gate_up [E, 2I, D] (gate rows first) and down [E, D, I]: bf16 with NULL
+ * scales, or both MXFP4 codes and scales.  selected int64 [T, top_k].  D and I
+ * are multiples of 8, at most 2^20.  ws: sfp8_moe_decode_workspace_bytes(T, E,
+ * top_k, I) bytes, whose contents do not matter; 16-byte aligned, as are the
+ * weights and out. */
+int64_t sfp8_moe_decode_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t I);
+int sfp8_moe_decode(const void* x, int64_t ldx, int64_t T, int64_t D, const void* router, int router_type, int64_t E,
+                    const void* gate_up, const void* gate_up_scales, const void* down, const void* down_scales,
+                    int64_t I, const float* bias, const void* mask, int score, int64_t groups, int64_t top_groups,
+                    int64_t group_best, int64_t top_k, int renorm, float scale, int64_t* selected, void* out, void* ws,
+                    int64_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * The consumer of the fp32 weight gradients: the Muon optimizer's momentum
  * stage (train.py:2805-2839), alone and fused into the weight gradient.
  * ------------------------------------------------------------------------- */

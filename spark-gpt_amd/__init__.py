@@ -13,8 +13,9 @@ from .swiglu import (_FusedSwiGLU, _NormSwiGLU, _use_fused_norm_mlp, _use_fused_
 from .muon import _momentum_stage, _momentum_stage_supported
 from .routing import combine_experts, expert_order, fp8_routed_experts, route_tokens
 from .mxfp4 import MXFP4, mxfp4_dequantize, mxfp4_linear, mxfp4_matmul, mxfp4_quantize
+from .decode import decode_routed_experts
 from .clip import clip_grad_norm_, clip_grads, grad_norm
-from . import clip, mlp, moe, muon, mxfp4, ops, routing, swiglu, torch_ops
+from . import clip, decode, mlp, moe, muon, mxfp4, ops, routing, swiglu, torch_ops
 
 __all__ = [
     "FP8_HEADROOM_BINADES", "FP8_SITE_MAX", "MLP", "_FP8MLPBlock", "_use_fp8_mlp",
@@ -23,7 +24,7 @@ __all__ = [
     "_FusedSwiGLU", "_NormSwiGLU", "_use_fused_norm_mlp", "_use_fused_swiglu", "make_fused_norm_mlp_guard",
     "make_fused_swiglu_guard", "swiglu", "_momentum_stage", "_momentum_stage_supported", "muon",
     "combine_experts", "expert_order", "fp8_routed_experts", "route_tokens", "routing",
-    "MXFP4", "mxfp4", "mxfp4_dequantize", "mxfp4_linear", "mxfp4_matmul", "mxfp4_quantize",
+    "decode", "decode_routed_experts", "MXFP4", "mxfp4", "mxfp4_dequantize", "mxfp4_linear", "mxfp4_matmul", "mxfp4_quantize",
     "clip", "clip_grad_norm_", "clip_grads", "grad_norm",
 ]
 

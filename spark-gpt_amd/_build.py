@@ -14,7 +14,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libsparkfp8.so")
-SOURCES = ("quant.hip", "gemm.hip", "moe.hip", "bf16.hip", "optim.hip", "route.hip", "clip.hip", "mx4.hip")
+SOURCES = ("quant.hip", "gemm.hip", "moe.hip", "bf16.hip", "optim.hip", "route.hip", "clip.hip", "mx4.hip",
+           "decode.hip")
 NATIVE = os.path.join(HERE, "_native.so")
 NATIVE_SOURCE = "native.cpp"
 ARCH = "gfx950"

@@ -818,6 +818,66 @@ Tensor mxfp4_rows_matmul(const Tensor& x_, const Tensor& b, const Tensor& b_scal
   return out;
 }
 
+// ------------------------------------------------------------------ the experts' layer for a few tokens
+std::tuple<Tensor, Tensor> moe_decode(const Tensor& x_, const Tensor& router, const Tensor& w_gu,
+                                      const OptTensor& gu_scales, const Tensor& w_down, const OptTensor& down_scales,
+                                      int64_t I, const OptTensor& bias, const OptTensor& mask, const std::string& score,
+                                      int64_t groups, int64_t top_groups, int64_t group_best, int64_t top_k,
+                                      bool renormalize, double scale) {
+  const int sc = score_code(score);
+  need(x_.is_cuda(), "x must be a ROCm device tensor");
+  need(x_.scalar_type() == kBF16, "x must be BFloat16");
+  if (x_.dim() != 2) refuse("x must be 2-D, got shape " + shape_of(x_));
+  const int64_t T = x_.size(0), D = x_.size(1);
+  if (T > 64) refuse("at most 64 tokens, got " + std::to_string(T) + ": more run through the grouped experts");
+  const bool wide = router.scalar_type() == kF32;
+  contig("router", router, wide ? kF32 : kBF16, 2);
+  const int64_t E = router.size(0);
+  need(router.size(1) == D, "router must be [experts, columns of x]");
+  need(E >= 1 && E <= 1024, "1 .. 1024 experts");
+  if (D < 8 || D % 8 || I < 8 || I % 8 || D > 1 << 20 || I > 1 << 20)
+    refuse("the widths must be multiples of 8 and at most 2^20, got " + std::to_string(D) + " and " +
+           std::to_string(I));
+  need(gu_scales.has_value() == down_scales.has_value(), "both weights bf16 or both MXFP4");
+  if (gu_scales) {
+    is_mxfp4("w_gu: ", w_gu, *gu_scales, E, 2 * I, D);
+    is_mxfp4("w_down: ", w_down, *down_scales, E, D, I);
+  } else {
+    contig("w_gu", w_gu, kBF16, 3);
+    contig("w_down", w_down, kBF16, 3);
+    need(w_gu.size(0) == E && w_gu.size(1) == 2 * I && w_gu.size(2) == D, "w_gu must be [experts, 2I, D]");
+    need(w_down.size(0) == E && w_down.size(1) == D && w_down.size(2) == I, "w_down must be [experts, D, I]");
+  }
+  for (const auto& [n, t] :
+       {std::pair<const char*, const Tensor&>{"router", router}, {"w_gu", w_gu}, {"w_down", w_down}})
+    same_device(n, t, x_);
+  if (bias) {
+    contig("bias", *bias, kF32, 1);
+    same_device("bias", *bias, x_);
+    need(bias->size(0) == E, "bias must have one entry per expert");
+  }
+  if (mask) {
+    contig("mask", *mask, ScalarType::Bool, 1);
+    same_device("mask", *mask, x_);
+    need(mask->size(0) == T, "mask must have one entry per token");
+  }
+  if (groups < 1 || groups > 64 || E % groups)
+    refuse("groups must be 1 .. 64 and divide the " + std::to_string(E) + " experts, got " + std::to_string(groups));
+  need(top_groups >= 1 && top_groups <= groups, "top_groups must be 1 .. groups");
+  need(group_best == 1 || group_best == 2, "group_best must be 1 or 2");
+  if (top_k < 1 || top_k > 64 || top_k > top_groups * (E / groups))
+    refuse("top_k must be 1 .. 64 and no more than the experts of the kept groups, got " + std::to_string(top_k));
+  const c10::DeviceGuard guard(x_.device());
+  const Tensor x = x_.stride(1) == 1 ? x_ : x_.contiguous();
+  Tensor out = empty({T, D}, kBF16, x), selected = empty({T, top_k}, kI64, x);
+  const int64_t n = sfp8_moe_decode_workspace_bytes(T, E, top_k, I);
+  Tensor ws = empty({n > 1 ? n : 1}, kU8, x);
+  CALL(sfp8_moe_decode, ptr(x), x.stride(0), T, D, ptr(router), wide ? 0 : 1, E, ptr(w_gu), ptr(gu_scales),
+       ptr(w_down), ptr(down_scales), I, fptr(bias), ptr(mask), sc, groups, top_groups, group_best, top_k,
+       (int)renormalize, (float)scale, lptr(selected), ptr(out), ptr(ws), n, stream_of(x));
+  return {out, selected};
+}
+
 // ------------------------------------------------------------------ bf16 SwiGLU path
 std::tuple<OptTensor, OptTensor> bf16_weight_slabs(const Tensor& w, const OptTensor& norm_w, bool rows,
                                                    bool transposed) {
@@ -1050,6 +1110,11 @@ PYBIND11_MODULE(_native, m) {
         arg("K"), arg("dtype"), "out [M, N] = A B^T over the values of two quantised matrices.");
   m.def("mxfp4_rows_matmul", &mxfp4_rows_matmul, arg("x"), arg("w"), arg("w_scales"), arg("N"), arg("dtype"),
         "mxfp4_matmul of at most 16 rows x [M, K] that are quantised on the way.");
+  m.def("moe_decode", &moe_decode, arg("x"), arg("router"), arg("w_gu"), arg("gu_scales"), arg("w_down"),
+        arg("down_scales"), arg("I"), arg("bias"), arg("mask"), arg("score"), arg("groups"), arg("top_groups"),
+        arg("group_best"), arg("top_k"), arg("renormalize"), arg("scale"),
+        "(out [T, D] bf16, selected int64 [T, top_k]) of the experts' layer for at most 64 tokens; the weights bf16 "
+        "(scales None) or MXFP4 codes and scales.");
   m.def("bf16_weight_slabs", &bf16_weight_slabs, arg("w"), arg("norm_w") = py::none(), kw, arg("rows") = true,
         arg("transposed") = true,
         "bf16 K-slabs of W [E, R, C] (fp32, times norm_w[c] when given, or bf16): (ws: stacked K-slabs of W[e] [R, C] "

@@ -25,8 +25,8 @@ _NATIVE = ("norm_quant", "block_weight_quant", "weight_quant_experts", "gateup_s
 # those around the experts and between the backward pass and the optimizer
 _NATIVE_STEP = ("moe_route", "moe_route_bwd", "moe_expert_order", "moe_combine", "moe_combine_bwd", "grad_norm",
                 "clip_grads")
-# microscaled 4-bit floating point
-_NATIVE_MX = ("mxfp4_quantize", "mxfp4_dequantize", "mxfp4_matmul", "mxfp4_rows_matmul")
+# microscaled 4-bit floating point, and the experts' layer for a few tokens
+_NATIVE_MX = ("mxfp4_quantize", "mxfp4_dequantize", "mxfp4_matmul", "mxfp4_rows_matmul", "moe_decode")
 # differentiable as they are: the eager calls of routing.py
 _NATIVE_AUTOGRAD = ("route_tokens", "combine_experts")
 

@@ -572,3 +572,22 @@ mxfp4_rows_matmul = torch.library.custom_op("sparkfp8::mxfp4_rows_matmul", mxfp4
 @mxfp4_rows_matmul.register_fake
 def _mxfp4_rows_matmul_fake(x, w, w_scales, N, dtype):
     return x.new_empty((x.shape[0], N), dtype=dtype)
+
+
+# ------------------------------------------------------------------ the experts' layer for a few tokens
+def moe_decode_impl(x: Tensor, router: Tensor, w_gu: Tensor, gu_scales: Optional[Tensor], w_down: Tensor,
+                    down_scales: Optional[Tensor], I: int, bias: Optional[Tensor], mask: Optional[Tensor], score: str,
+                    groups: int, top_groups: int, group_best: int, top_k: int, renormalize: bool,
+                    scale: float) -> Tuple[Tensor, Tensor]:
+    """(out [T, D] bf16, selected int64 [T, top_k])."""
+    return ops.moe_decode(x, router, w_gu, gu_scales, w_down, down_scales, I, bias, mask, score, groups, top_groups,
+                          group_best, top_k, renormalize, scale)
+
+
+moe_decode = torch.library.custom_op("sparkfp8::moe_decode", moe_decode_impl, mutates_args=())
+
+
+@moe_decode.register_fake
+def _moe_decode_fake(x, router, w_gu, gu_scales, w_down, down_scales, I, bias, mask, score, groups, top_groups,
+                     group_best, top_k, renormalize, scale):
+    return x.new_empty(tuple(x.shape)), x.new_empty((x.shape[0], top_k), dtype=torch.int64)
