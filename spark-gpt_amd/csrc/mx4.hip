@@ -345,6 +345,328 @@ __global__ __launch_bounds__(64 * WV) void mx_few_kernel(MxGemmArgs g) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// The product, tiles
+// ---------------------------------------------------------------------------
+// TM x TM outputs of one work-group: 8 waves of 128 x 64 (TM = 256) or 4 of 64 x
+// 64 (TM = 128, two work-groups a CU).  K advances a slab (128 values, 64 bytes
+// of a row) at a time through a ring of four LDS stages: codes of TM rows of A
+// and of B, and their four scales a row.  Everything comes by DMA
+// (buffer_load .. lds, 1 KiB of codes or 256 bytes of scales a wave and
+// instruction), three stages ahead; rows past the operand's end read as zeros.
+// Row r keeps its 16-byte chunk c at c ^ (r / 4) % 4: the 16 rows that a lane
+// group reads lie in different banks.
+//
+// v_mfma_scale_f32_32x32x64: lane l holds row l % 32 and 32 values, which are
+// one block of the row: half g = l / 32 takes chunk 2 g + h in step h of the two
+// of a slab, and its scale is byte 2 g + h of the row's four.  B is the first
+// operand, and its rows are permuted as they are fetched so that a lane's 16
+// sums of a block are neighbours: columns 32 g + 16 nb + v of the wave's 64.
+//
+// A stage's MFMAs run in a fixed order with the next stage's LDS reads and the
+// DMA between them; the first two go ahead of the stage's wait and barrier.
+template <int TM>
+struct MxTile {
+  static constexpr int TB = TM == 256 ? 4 : 2, NB = 2, WN = TM / 64, kWaves = 2 * WN, kStages = 4;
+  static constexpr int kSide = TM * 64, kScaleSide = TM * 4;        // bytes of a stage, one operand
+  static constexpr int kStage = 2 * kSide + 2 * kScaleSide, kLds = kStages * kStage;
+  static constexpr int kCodeDma = TM / 16 / kWaves;                  // of A, and of B, a wave and stage: 2
+  static constexpr int kDma = 2 * kCodeDma + 1;                      // and one of scales: 64 rows a wave
+  static constexpr int kMfma = 2 * TB * NB;
+  static_assert(kCodeDma == 2 && kWaves * 64 == 2 * TM, "one scale instruction a wave");
+  using Rsrc = __amdgpu_buffer_rsrc_t;
+  using Lds = __attribute__((address_space(3))) void*;
+
+  struct Frag {
+    intx4 a[TB][2], b[NB][2];
+    uint32_t as[TB], bs[NB];
+  };
+  typedef floatx16 Acc[TB][NB];
+
+  struct Operands {
+    const uint8_t *a, *b, *scales;       // this tile's first rows of the first slab; scales of A or of B by wave
+    int64_t a_step, b_step, scale_step;  // bytes from slab to slab
+    int a_bytes, b_bytes, scale_bytes;   // of the tile's rows that there are
+    int stages;
+  };
+  uint8_t* lds;
+  Operands op;
+  uint32_t va[2], vb[2], vs;      // DMA lane offsets
+  uint32_t da[2], db[2], ds;      // and where in a stage they land
+  uint32_t ra[2], rb[2], rs, rt;  // LDS read offsets: chunk 2 g + h of A and B, scales of A and B
+
+  static SFP8_DEV Rsrc rsrc(const uint8_t* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), (short)0, bytes, 0x00020000);
+  }
+  // column of the wave's 64 that row i of block nb stands for
+  static SFP8_DEV int column(int p) {
+    const int nb = (p >> 5) & 1, i = p & 31;
+    return (p & ~63) + 32 * ((i >> 2) & 1) + 16 * nb + 4 * (i >> 3) + (i & 3);
+  }
+
+  SFP8_DEV MxTile(uint8_t* l, const Operands& o) : lds(l), op(o) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave % 2, wn = wave / 2;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = 32 * wave + 16 * j + (lane >> 2);
+      const uint32_t chunk = (uint32_t)(((lane & 3) ^ ((r >> 2) & 3)) << 4);
+      va[j] = (uint32_t)r * 64 + chunk;
+      vb[j] = (uint32_t)column(r) * 64 + chunk;
+      da[j] = (uint32_t)(32 * wave + 16 * j) * 64;
+      db[j] = kSide + da[j];
+    }
+    const bool of_b = wave >= WN;
+    const int r = 64 * (of_b ? wave - WN : wave) + lane;
+    vs = (uint32_t)(of_b ? column(r) : r) * 4;
+    ds = 2 * kSide + (uint32_t)wave * 256;
+    const int fr = lane & 31, g = lane >> 5, sw = (fr >> 2) & 3;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t chunk = (uint32_t)(((2 * g + h) ^ sw) << 4);
+      ra[h] = (uint32_t)(32 * TB * wm + fr) * 64 + chunk;
+      rb[h] = kSide + (uint32_t)(64 * wn + fr) * 64 + chunk;
+    }
+    rs = 2 * kSide + (uint32_t)(32 * TB * wm + fr) * 4 + 2 * g;
+    rt = 2 * kSide + kScaleSide + (uint32_t)(64 * wn + fr) * 4 + 2 * g;
+  }
+
+  // DMA instruction j of stage s into ring slot `slot`; past the last stage nothing is read
+  SFP8_DEV void dma(int j, int s, int slot) const {
+    const bool live = s < op.stages;
+    uint8_t* at = lds + slot * kStage;
+    if (j < 2)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(op.a + s * op.a_step, live ? op.a_bytes : 0), (Lds)(at + da[j]), 16,
+                                               va[j], 0, 0, 0);
+    else if (j < 4)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(op.b + s * op.b_step, live ? op.b_bytes : 0),
+                                               (Lds)(at + db[j - 2]), 16, vb[j - 2], 0, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc(op.scales + s * op.scale_step, live ? op.scale_bytes : 0),
+                                               (Lds)(at + ds), 4, vs, 0, 0, 0);
+  }
+  // Fragment i: A block i, or B block i - TB, with its scales
+  template <int I>
+  SFP8_DEV void read(int slot, Frag& f) const {
+    const uint8_t* at = lds + slot * kStage;
+    if constexpr (I < TB) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f.a[I][h] = *reinterpret_cast<const intx4*>(at + ra[h] + I * 32 * 64);
+      f.as[I] = *reinterpret_cast<const uint16_t*>(at + rs + I * 32 * 4);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f.b[I - TB][h] = *reinterpret_cast<const intx4*>(at + rb[h] + (I - TB) * 32 * 64);
+      f.bs[I - TB] = *reinterpret_cast<const uint16_t*>(at + rt + (I - TB) * 32 * 4);
+    }
+  }
+  template <int I = 0>
+  SFP8_DEV void read_all(int slot, Frag& f) const {
+    if constexpr (I < TB + NB) {
+      read<I>(slot, f);
+      read_all<I + 1>(slot, f);
+    }
+  }
+  template <int I>
+  static SFP8_DEV void mfma(const Frag& f, Acc& acc) {
+    constexpr int h = I / (TB * NB), tb = I / NB % TB, nb = I % NB;
+    acc[tb][nb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fp4_operand(f.b[nb][h]), fp4_operand(f.a[tb][h]),
+                                                                  acc[tb][nb], 4, 4, h, (int)f.bs[nb], h,
+                                                                  (int)f.as[tb]);
+  }
+  template <int LO, int HI>
+  static SFP8_DEV void mfmas(const Frag& f, Acc& acc) {
+    if constexpr (LO < HI) {
+      mfma<LO>(f, acc);
+      mfmas<LO + 1, HI>(f, acc);
+    }
+  }
+  // MFMA I, then a fragment of the next stage and DMA instruction D (either may be -1)
+  template <int I, int R, int D>
+  SFP8_DEV void slot(const Frag& cur, Frag& nxt, Acc& acc, int s, int read_slot, int dma_slot) const {
+    mfma<I>(cur, acc);
+    if constexpr (R >= 0) read<R>(read_slot, nxt);
+    if constexpr (D >= 0) dma(D, s + kStages - 1, dma_slot);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // Stage s on `cur`: reads stage s + 1 into `nxt`, fetches stage s + 3 into the slot of stage s - 1.
+  SFP8_DEV void stage(const Frag& cur, Frag& nxt, Acc& acc, int s) const {
+    const int rd = (s + 1) % kStages, wr = (s + kStages - 1) % kStages;
+    mfmas<0, 2>(cur, acc);
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kDma * (kStages - 3)) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (TB == 4) {
+      slot<2, 0, -1>(cur, nxt, acc, s, rd, wr);
+      slot<3, -1, 0>(cur, nxt, acc, s, rd, wr);
+      slot<4, 4, -1>(cur, nxt, acc, s, rd, wr);
+      slot<5, -1, 1>(cur, nxt, acc, s, rd, wr);
+      slot<6, 5, -1>(cur, nxt, acc, s, rd, wr);
+      slot<7, -1, 2>(cur, nxt, acc, s, rd, wr);
+      slot<8, 1, -1>(cur, nxt, acc, s, rd, wr);
+      slot<9, -1, 3>(cur, nxt, acc, s, rd, wr);
+      slot<10, 2, -1>(cur, nxt, acc, s, rd, wr);
+      slot<11, -1, 4>(cur, nxt, acc, s, rd, wr);
+      slot<12, 3, -1>(cur, nxt, acc, s, rd, wr);
+      mfmas<13, 16>(cur, acc);
+    } else {
+      slot<2, 0, 0>(cur, nxt, acc, s, rd, wr);
+      slot<3, 2, 1>(cur, nxt, acc, s, rd, wr);
+      slot<4, 3, 2>(cur, nxt, acc, s, rd, wr);
+      slot<5, 1, 3>(cur, nxt, acc, s, rd, wr);
+      slot<6, -1, 4>(cur, nxt, acc, s, rd, wr);
+      mfmas<7, 8>(cur, acc);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  SFP8_DEV void run(Acc& acc) const {
+#pragma unroll
+    for (int i = 0; i < TB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+        acc[i][j] = floatx16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s)
+#pragma unroll
+      for (int j = 0; j < kDma; ++j) dma(j, s, s);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(kDma * (kStages - 2)) : "memory");
+    Frag f0, f1;
+    read_all(0, f0);
+    // two stages a turn, so that the fragments alternate by name; an odd count runs one more on zeros
+    for (int s = 0; s < op.stages; s += 2) {
+      stage(f0, f1, acc, s);
+      stage(f1, f0, acc, s + 1);
+    }
+    // nothing in flight into the ring, and nobody reads it any more
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  }
+};
+
+// Tiles in the order in which work-groups take them: the 8 XCDs own runs of
+// them, each 8 tile rows high, so that an XCD's L2 serves the columns again.
+SFP8_DEV bool mx_tile_of(int id, int rows, int cols, int& r, int& c) {
+  const int n = rows * cols, per = (n + 7) / 8;
+  const int t = (id & 7) * per + (id >> 3);
+  if ((id >> 3) >= per || t >= n) return false;
+  const int group = t / (8 * cols), first = 8 * group, high = rows - first < 8 ? rows - first : 8, in = t - first * cols;
+  r = first + in % high;
+  c = in / high;
+  return true;
+}
+
+// 8 neighbours of an output row from element i on, `left` of them in the matrix.
+template <int OUT>
+SFP8_DEV void store8(void* out, int64_t i, const Eight<OUT>& v, int64_t left) {
+  if constexpr (OUT == kMxF32) {
+    typedef int any4 __attribute__((ext_vector_type(4), aligned(4)));
+    float* p = reinterpret_cast<float*>(out) + i;
+    if (left >= 8) {
+      *reinterpret_cast<any4*>(p) = any4{(int)v.w[0], (int)v.w[1], (int)v.w[2], (int)v.w[3]};
+      *reinterpret_cast<any4*>(p + 4) = any4{(int)v.w[4], (int)v.w[5], (int)v.w[6], (int)v.w[7]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 7; ++j)
+        if (j < left) p[j] = __uint_as_float(v.w[j]);
+    }
+  } else {
+    uint16_t* p = reinterpret_cast<uint16_t*>(out) + i;
+    if (left >= 8) {
+      *reinterpret_cast<mx_intx4_any*>(p) = mx_intx4_any{(int)v.w[0], (int)v.w[1], (int)v.w[2], (int)v.w[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 7; ++j)
+        if (j < left) p[j] = (uint16_t)(v.w[j / 2] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// A wave's 32 TB x 64 sums to memory: through its own part of the LDS (the ring
+// is done with), so that each store writes whole 128-byte lines: eight lanes a
+// row.  16-byte chunk c of row r lies at c ^ (r / 2) % 8.  ROWS of them at a time.
+template <int OUT, int TB, int ROWS>
+SFP8_DEV void store_wave(uint8_t* lds, void* out, int64_t m, int64_t n, int64_t M, int64_t N,
+                         const floatx16 (&acc)[TB][2]) {
+  constexpr int kSize = OUT == kMxF32 ? 4 : 2, kRow = 64 * kSize, kChunks = kRow / 16;
+  const int lane = threadIdx.x & 63, g = lane >> 5;
+#pragma unroll
+  for (int b0 = 0; b0 < TB; b0 += ROWS / 32) {
+#pragma unroll
+    for (int b = 0; b < ROWS / 32; ++b) {
+      const int r = 32 * b + (lane & 31);
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        const floatx16& v = acc[b0 + b][nb];
+#pragma unroll
+        for (int c = 0; c < kSize; ++c) {  // 16 values are kSize chunks
+          intx4 w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (OUT == kMxF32) w[j] = (int)__float_as_uint(v[4 * c + j]);
+            else if constexpr (OUT == kMxBf16) w[j] = (int)pack2_bf16(v[8 * c + 2 * j], v[8 * c + 2 * j + 1]);
+            else
+              w[j] = __builtin_bit_cast(int, halfx2{(_Float16)v[8 * c + 2 * j], (_Float16)v[8 * c + 2 * j + 1]});
+          }
+          const int chunk = (32 * g + 16 * nb) * kSize / 16 + c;
+          *reinterpret_cast<intx4*>(lds + r * kRow + 16 * ((chunk & ~7) | ((chunk ^ (r >> 1)) & 7))) = w;
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < ROWS / 8; ++i) {
+      const int r = 8 * i + (lane >> 3), c = lane & 7;  // eight values a lane
+      Eight<OUT> v;
+#pragma unroll
+      for (int j = 0; j < kChunks / 8; ++j) {
+        const int chunk = c * (kChunks / 8) + j;
+        const intx4 w =
+            *reinterpret_cast<const intx4*>(lds + r * kRow + 16 * ((chunk & ~7) | ((chunk ^ (r >> 1)) & 7)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v.w[4 * j + k] = (uint32_t)w[k];
+      }
+      const int64_t row = m + 32 * b0 + r;
+      if (row < M) store8<OUT>(out, row * N + n + 8 * c, v, N - n - 8 * c);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+template <int TM, int OUT>
+__global__ __launch_bounds__(2 * TM, 2) void mx_tile_kernel(MxGemmArgs g) {
+  using Tile = MxTile<TM>;
+  __shared__ __align__(1024) uint8_t lds[Tile::kLds];
+  const int64_t mp = mx_rows(g.M), np = mx_rows(g.N);
+  int tr, tc;
+  if (!mx_tile_of(blockIdx.x, (int)((mp + TM - 1) / TM), (int)((np + TM - 1) / TM), tr, tc)) return;
+  const int64_t m0 = (int64_t)tr * TM, n0 = (int64_t)tc * TM;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int arows = (int)(mp - m0 < TM ? mp - m0 : TM), brows = (int)(np - n0 < TM ? np - n0 : TM);
+  const bool of_b = wave >= Tile::WN;
+  const typename Tile::Operands op{
+      g.a + m0 * 64, g.b + n0 * 64, of_b ? g.bs + n0 * 4 : g.as + m0 * 4, mp * 64, np * 64, (of_b ? np : mp) * 4,
+      arows * 64, brows * 64, (of_b ? brows : arows) * 4, (int)mx_slabs(g.K)};
+  typename Tile::Acc acc;
+  Tile(lds, op).run(acc);
+  constexpr int kPart = Tile::kLds / Tile::kWaves & ~1023, kRow = 64 * (OUT == kMxF32 ? 4 : 2);
+  constexpr int kRows = kPart / kRow / 32 * 32 < 32 * Tile::TB ? (kPart / kRow >= 64 ? 64 : 32) : 32 * Tile::TB;
+  store_wave<OUT, Tile::TB, kRows>(lds + wave * kPart, g.out, m0 + 32 * Tile::TB * (wave % 2), n0 + 64 * (wave / 2),
+                                   g.M, g.N, acc);
+}
+
+template <int TM>
+void launch_tiles(const MxGemmArgs& g, int64_t tiles, hipStream_t s) {
+  const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);
+  if (g.out_type == kMxF32) mx_tile_kernel<TM, kMxF32><<<grid, 2 * TM, 0, s>>>(g);
+  else if (g.out_type == kMxBf16) mx_tile_kernel<TM, kMxBf16><<<grid, 2 * TM, 0, s>>>(g);
+  else mx_tile_kernel<TM, kMxF16><<<grid, 2 * TM, 0, s>>>(g);
+}
+
+template <int MB, int NB, int WV, int XT>
+void launch_few(const MxGemmArgs& g, hipStream_t s) {
+  const dim3 grid((unsigned)((g.N + 16 * NB - 1) / (16 * NB)), (unsigned)((g.M + 16 * MB - 1) / (16 * MB)));
+  mx_few_kernel<MB, NB, WV, XT><<<grid, 64 * WV, 0, s>>>(g);
+}
+
 inline int launched() {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? kOk : (int)e;
@@ -352,6 +674,7 @@ inline int launched() {
 inline bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 inline bool type_ok(int dtype) { return dtype >= kMxF32 && dtype <= kMxF16; }
 constexpr int64_t kMxMaxDim = (int64_t)1 << 31;
+constexpr int64_t kMxMaxTiles = ((int64_t)1 << 24) - 8;  // of 256 threads: a grid has less than 2^32
 
 }  // namespace sfp8
 
@@ -374,7 +697,7 @@ int sfp8_mxfp4_quantize(const void* x, int dtype, int64_t batch, int64_t R, int6
       !aligned(scales_t, 4))
     return kErrBadAlignment;
   const int64_t tiles = mx_slabs(C) * ((R + 127) / 128);
-  if (tiles > 0x7fffffff / batch) return kErrBadShape;
+  if (tiles > kMxMaxTiles / batch) return kErrBadShape;
   const MxQuantArgs a{x, R, C, ld, batch_stride, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)codes_t,
                       (uint8_t*)scales_t};
   const unsigned grid = (unsigned)(tiles * batch);
@@ -392,7 +715,7 @@ int sfp8_mxfp4_dequantize(const void* codes, const void* scales, int64_t batch, 
   if (!codes || !scales || !out) return kErrNullPointer;
   if (!aligned(codes, 16) || !aligned(scales, 4) || !aligned(out, 16)) return kErrBadAlignment;
   const int64_t tiles = mx_slabs(C) * ((R + 127) / 128);
-  if (tiles > 0x7fffffff / batch) return kErrBadShape;
+  if (tiles > kMxMaxTiles / batch) return kErrBadShape;
   const MxDequantArgs a{(const uint8_t*)codes, (const uint8_t*)scales, R, C, out};
   const unsigned grid = (unsigned)(tiles * batch);
   const hipStream_t s = (hipStream_t)stream;
@@ -412,27 +735,40 @@ int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const vo
     return kErrBadAlignment;
   const MxGemmArgs g{(const uint8_t*)a, (const uint8_t*)a_scales, (const uint8_t*)b, (const uint8_t*)b_scales,
                      nullptr, 0, M, N, K, out, dtype};
-  const int64_t gx = (N + 63) / 64, gy = (M + 63) / 64;
-  if (gy > 65535) return kErrBadShape;
-  mx_few_kernel<4, 4, 4, -1><<<dim3((unsigned)gx, (unsigned)gy), 256, 0, (hipStream_t)stream>>>(g);
+  const hipStream_t st = (hipStream_t)stream;
+  // By the number of tiles (us; M, N, K):
+  //  256 x 256 where they fill the CUs and K is long: its loop fetches half of what that of 128 x 128 does for a
+  //  product, which hides its stores behind a second work-group: 16384, 8192, 4096 281 against 362; 4096, 4096, 4096
+  //  40.5 against 43.6; but 16384, 4096, 2048 96.5 against 88.8 and 65536, 1024, 1024 72.0 against 55.5.
+  //  128 x 128 from half a tile a CU on (1003, 2050, 1000 6.1 against 10.6; 512, 4096, 4096 11.1 against 13.2);
+  //  below that the waves share K (1024, 1024, 4096 9.3 against 10.6), in the largest tile of which there are 256:
+  //  64, 4096, 4096 32 x 32 4.7, 16 x 16 6.7, 64 x 64 8.5; 128, 1024, 8192 16 x 32 5.4, 64 x 64 12.4.
+  const auto tiles = [&](int64_t m, int64_t n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
+  if (tiles(128, 128) > kMxMaxTiles) return kErrBadShape;
+  if (tiles(256, 256) >= 256 && K >= 4096) launch_tiles<256>(g, tiles(256, 256), st);
+  else if (tiles(128, 128) >= 128) launch_tiles<128>(g, tiles(128, 128), st);
+  else if (tiles(64, 64) >= 256) launch_few<4, 4, 4, -1>(g, st);
+  else if (M > 32 && tiles(64, 32) >= 256) launch_few<4, 2, 8, -1>(g, st);
+  else if (M > 16 && tiles(32, 32) >= 256) launch_few<2, 2, 8, -1>(g, st);
+  else if (tiles(16, 32) >= 256) launch_few<1, 2, 8, -1>(g, st);
+  else launch_few<1, 1, 8, -1>(g, st);
   return launched();
 }
 
 int sfp8_mxfp4_gemm_rows(const void* x, int x_type, int64_t ldx, const void* b, const void* b_scales, int64_t M,
                          int64_t N, int64_t K, void* out, int dtype, void* stream) {
-  if (!type_ok(dtype) || !type_ok(x_type) || M < 0 || M > 16 || N < 0 || K < 0 || N > kMxMaxDim || K > kMxMaxDim ||
-      ldx < 0)
+  if (!type_ok(dtype) || !type_ok(x_type) || M < 0 || M > 16 || N < 0 || K < 0 || N >= (int64_t)1 << 27 ||
+      K > kMxMaxDim || ldx < 0)
     return kErrBadShape;
   if (M == 0 || N == 0) return kOk;
   if (!out || (K && (!x || !b || !b_scales))) return kErrNullPointer;
   if (!aligned(x, x_type == kMxF32 ? 4 : 2) || !aligned(b, 16) || !aligned(b_scales, 4) || !aligned(out, 16))
     return kErrBadAlignment;
   const MxGemmArgs g{nullptr, nullptr, (const uint8_t*)b, (const uint8_t*)b_scales, x, ldx, M, N, K, out, dtype};
-  const unsigned gx = (unsigned)((N + 15) / 16);
   const hipStream_t s = (hipStream_t)stream;
-  if (x_type == kMxF32) mx_few_kernel<1, 1, 8, kMxF32><<<gx, 512, 0, s>>>(g);
-  else if (x_type == kMxBf16) mx_few_kernel<1, 1, 8, kMxBf16><<<gx, 512, 0, s>>>(g);
-  else mx_few_kernel<1, 1, 8, kMxF16><<<gx, 512, 0, s>>>(g);
+  if (x_type == kMxF32) launch_few<1, 1, 8, kMxF32>(g, s);
+  else if (x_type == kMxBf16) launch_few<1, 1, 8, kMxBf16>(g, s);
+  else launch_few<1, 1, 8, kMxF16>(g, s);
   return launched();
 }
 

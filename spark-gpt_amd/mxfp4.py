@@ -116,7 +116,8 @@ def mxfp4_matmul(a: MXFP4, b: MXFP4, dtype: torch.dtype = torch.bfloat16) -> tor
 
 
 class _MXFP4Linear(torch.autograd.Function):
-    """x w^T on quantised operands.  Each of the three products quantises its
+    """x w^T on quantised operands in a compiled graph (an eager call makes the
+    same node in C++).  Each of the three products quantises its
     operands along the dimension that it sums over; gradients pass the
     quantisation as if it were not there.  What is kept for the backward pass is
     in 4 bits: the codes of x along its rows' dimension and of w along its."""
@@ -174,10 +175,10 @@ def mxfp4_linear(x: torch.Tensor, w) -> torch.Tensor:
     if torch.is_grad_enabled() and (x.requires_grad or (not kept and w.requires_grad)):
         if kept:
             raise ValueError("weights kept as MXFP4 give no gradient of x: pass the master, or call without gradients")
-        y = _MXFP4Linear.apply(flat, w)
+        y = (_MXFP4Linear.apply if torch.compiler.is_compiling() else ops.mxfp4_linear)(flat, w)
     else:
         q = w if kept else _quantized(w, True, False)[0]
-        if flat.shape[0] <= ROW_ALIGN:
+        if flat.shape[0] <= ROW_ALIGN and N < 1 << 27:
             y = torch_ops.op("mxfp4_rows_matmul")(flat, q.codes, q.scales, N, x.dtype)
         else:
             y = mxfp4_matmul(_quantized(flat, True, False)[0], q, x.dtype)

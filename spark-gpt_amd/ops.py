@@ -27,8 +27,8 @@ _NATIVE_STEP = ("moe_route", "moe_route_bwd", "moe_expert_order", "moe_combine",
                 "clip_grads")
 # microscaled 4-bit floating point, and the experts' layer for a few tokens
 _NATIVE_MX = ("mxfp4_quantize", "mxfp4_dequantize", "mxfp4_matmul", "mxfp4_rows_matmul", "moe_decode")
-# differentiable as they are: the eager calls of routing.py
-_NATIVE_AUTOGRAD = ("route_tokens", "combine_experts")
+# differentiable as they are: the eager calls of routing.py and mxfp4.py
+_NATIVE_AUTOGRAD = ("route_tokens", "combine_experts", "mxfp4_linear")
 
 
 def _missing(name: str, why: str):

@@ -118,7 +118,9 @@ def _operand(dev, R, K, seed, exponents=(0, 0)):
 SHAPES = [(1, 1, 1), (1, 16, 32), (3, 17, 129), (16, 64, 128), (8, 4096, 512), (17, 33, 4096), (64, 64, 640),
           (65, 130, 200), (128, 128, 256), (100, 1000, 1000), (256, 256, 384), (257, 255, 1024), (300, 700, 130),
           (513, 511, 2304), (1003, 2050, 1000), (2048, 1536, 256), (40, 3, 8192), (2, 20000, 96), (4100, 24, 4096),
-          (2300, 2304, 2048)]
+          (2300, 2304, 2048),
+          # every tile shape: 256 x 256 with an odd number of slabs, 64 x 64, 64 x 32, 32 x 32, 16 x 32 and 16 x 16
+          (4100, 4100, 4100), (1030, 1000, 2003), (100, 4100, 300), (20, 8200, 130), (7, 8200, 520), (9, 300, 5000)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -275,7 +277,7 @@ def test_linear_gradients_one_at_a_time(dev):
     assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, [xl, wl], dy), (dx, dw)))
     y = sg.mxfp4_linear(xl, wl)
     g, = torch.autograd.grad(y, [xl], dy.clone().requires_grad_(True), create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable|differentiat"):
+    with pytest.raises(RuntimeError, match="differentiable once"):
         g.sum().backward()
 
 
