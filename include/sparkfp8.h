@@ -598,10 +598,10 @@ int sfp8_mxfp4_gemm_rows(const void* x, int x_type, int64_t ldx, const void* b, 
  * Wg^T) * (x Wu^T) and out[t] = sum over the slots of weight * h Wd^T (bf16).
  * gate_up [E, 2I, D] (gate rows first) and down [E, D, I]: bf16 with NULL
  * scales, or both MXFP4 codes and scales.  selected int64 [T, top_k].  D and I
- * are multiples of 8, at most 2^20.  ws: sfp8_moe_decode_workspace_bytes(T, E,
- * top_k, I) bytes, whose contents do not matter; 16-byte aligned, as are the
+ * are multiples of 8, at most 2^20, D * I at most 2^29.  ws: sfp8_moe_decode_workspace_bytes(T, E,
+ * top_k, D, I) bytes, whose contents do not matter; 16-byte aligned, as are the
  * weights and out. */
-int64_t sfp8_moe_decode_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t I);
+int64_t sfp8_moe_decode_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t D, int64_t I);
 int sfp8_moe_decode(const void* x, int64_t ldx, int64_t T, int64_t D, const void* router, int router_type, int64_t E,
                     const void* gate_up, const void* gate_up_scales, const void* down, const void* down_scales,
                     int64_t I, const float* bias, const void* mask, int score, int64_t groups, int64_t top_groups,

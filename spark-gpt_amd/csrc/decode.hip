@@ -11,8 +11,9 @@
 // cores with the weights as first operand and up to 16 tokens as second.
 // Weights are bf16, or MXFP4 codes (mx4.h) that become bf16 values in
 // registers, which hold them exactly; x stays bf16 in both.
-// Four launches: logits; one work-group that selects and sorts the slots by
-// expert; gate and up; down and the sum.
+// Four launches: logits; the selection, a wave a token; gate and up, whose
+// work-groups find their expert's slots among all; down and the sum.  For up to
+// kFused tokens the selection is part of gate and up: three.
 #include <type_traits>
 
 #include "mx4.h"
@@ -20,7 +21,7 @@
 namespace sfp8 {
 
 constexpr int kMaxTokens = 64, kMaxExperts = 1024, kMaxTopK = 64;
-constexpr int kSlots = kMaxTokens * kMaxTopK;
+constexpr int kSlots = kMaxTokens * kMaxTopK;  // at most
 
 struct DecodeArgs {
   const uint16_t* x;
@@ -38,20 +39,20 @@ struct DecodeArgs {
   // workspace
   double* low;      // [T, E]
   float* weights;   // [T, k]
-  int* plan;        // number of experts taken; their index, first slot; the slots by expert
-  uint16_t* h;      // [T * k][2][I]: h and what its rounding to bf16 left
+  int* plan;        // per candidate: number of slots (0: not taken); its expert; its slots, 64 each
+  uint16_t* h;      // [T * k][2][ldh]: h and what its rounding to bf16 left, zeros from I on
+  int ldh;          // I up to a whole number of down's steps
+  float* partial;   // [shares of the steps][T, D]
+  int* done;        // per column block of down: work-groups that have finished
+  int done_count;
 };
 
-// plan: [0] experts taken; [1 + a] expert; [1 + n + a] begin (one past the last too); then the slots
-__host__ __device__ inline int plan_most(int T, int E, int k) { return T * k < E ? T * k : E; }
-struct Plan {
-  const int* p;
-  int most;
-  SFP8_DEV int count() const { return p[0]; }
-  SFP8_DEV int expert(int a) const { return p[1 + a]; }
-  SFP8_DEV int begin(int a) const { return p[1 + most + a]; }
-  SFP8_DEV const int* slots() const { return p + 2 + 2 * most; }
-};
+// Candidates are what may be an expert that is taken: the slots, where they are
+// fewer than the experts (a slot stands for its expert if it is the first that
+// names it), else the experts.
+__host__ __device__ inline int candidates(int T, int E, int k) { return T * k < E ? T * k : E; }
+// where the candidates' slots begin in the plan: from 16 bytes on
+__host__ __device__ inline int plan_slots(int most) { return (2 * most + 3) / 4 * 4; }
 
 SFP8_DEV double wave_sum(double v) { return wave_sum_f64(v); }
 SFP8_DEV double wave_max_or_nan(double v) {
@@ -64,47 +65,56 @@ SFP8_DEV double wave_max_or_nan(double v) {
 }
 
 // ---------------------------------------------------------------------------
-// Logits: a work-group takes one expert and up to 8 tokens, its four waves a
-// quarter of the width each.  Sums in 64 bits, so that the order of two experts
-// is that of the exact sums but for 2^-50 of their size.
+// Logits: a work-group takes one expert and TOK tokens, its four waves a quarter
+// of the width each.  Sums in 64 bits, so that the order of two experts is that
+// of the exact sums but for 2^-50 of their size.
 // ---------------------------------------------------------------------------
-constexpr int kLogitTokens = 8;
+SFP8_DEV double bf16_at(const Eight<kMxBf16>& v, int j) {
+  return (double)__uint_as_float(j & 1 ? v.w[j / 2] & 0xffff0000u : v.w[j / 2] << 16);
+}
 
+template <int TOK>
 __global__ __launch_bounds__(256) void decode_logits_kernel(DecodeArgs a) {
-  __shared__ double part[4][kLogitTokens];
+  __shared__ double part[4][TOK];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int e = blockIdx.x, t0 = blockIdx.y * kLogitTokens, n = min(kLogitTokens, a.T - t0);
-  double acc[kLogitTokens];
+  const int e = blockIdx.x, t0 = blockIdx.y * TOK, n = min(TOK, a.T - t0);
+  if (e == 0 && t0 == 0)
+    for (int i = threadIdx.x; i < a.done_count; i += 256) a.done[i] = 0;
+  double acc[TOK];
 #pragma unroll
-  for (int t = 0; t < kLogitTokens; ++t) acc[t] = 0.0;
+  for (int t = 0; t < TOK; ++t) acc[t] = 0.0;
   for (int d = 8 * threadIdx.x; d < a.D; d += 8 * 256) {
+    Eight<kMxBf16> x[TOK];
+#pragma unroll
+    for (int t = 0; t < TOK; ++t) x[t] = load8<kMxBf16>(a.x, (t0 + min(t, n - 1)) * a.ldx + d);
     double w[8];
     if (a.router_f32) {
-      const float* p = reinterpret_cast<const float*>(a.router) + (int64_t)e * a.D + d;
+      const Eight<kMxF32> v = load8<kMxF32>(a.router, (int64_t)e * a.D + d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = (double)p[j];
+      for (int j = 0; j < 8; ++j) w[j] = (double)__uint_as_float(v.w[j]);
     } else {
       const Eight<kMxBf16> v = load8<kMxBf16>(a.router, (int64_t)e * a.D + d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = (double)__uint_as_float(j & 1 ? v.w[j / 2] & 0xffff0000u : v.w[j / 2] << 16);
+      for (int j = 0; j < 8; ++j) w[j] = bf16_at(v, j);
     }
 #pragma unroll
-    for (int t = 0; t < kLogitTokens; ++t) {
-      if (t < n) {
-        const Eight<kMxBf16> v = load8<kMxBf16>(a.x, (t0 + t) * a.ldx + d);
+    for (int t = 0; t < TOK; ++t)
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          acc[t] = fma((double)__uint_as_float(j & 1 ? v.w[j / 2] & 0xffff0000u : v.w[j / 2] << 16), w[j], acc[t]);
-      }
+      for (int j = 0; j < 8; ++j) acc[t] = fma(bf16_at(x[t], j), w[j], acc[t]);
+  }
+  // TOK sums over 64 lanes: a lane hands half of its sums to the lane o away and keeps the other half's
+#pragma unroll
+  for (int h = TOK / 2, o = 32; h > 0; h >>= 1, o >>= 1) {
+#pragma unroll
+    for (int j = 0; j < h; ++j) {
+      const double keep = lane & o ? acc[j + h] : acc[j], give = lane & o ? acc[j] : acc[j + h];
+      acc[j] = keep + __shfl_xor(give, o, 64);
     }
   }
 #pragma unroll
-  for (int t = 0; t < kLogitTokens; ++t) {
-    if (t < n) {
-      const double s = wave_sum(acc[t]);
-      if (lane == 0) part[wave][t] = s;
-    }
-  }
+  for (int o = 32 / TOK; o > 0; o >>= 1) acc[0] += __shfl_xor(acc[0], o, 64);
+  static_assert(TOK == 1 || TOK == 4, "the lanes that hold token t");
+  if (lane % (64 / TOK) == 0) part[wave][TOK == 4 ? 2 * (lane >> 5) + (lane >> 4 & 1) : 0] = acc[0];
   __syncthreads();
   if ((int)threadIdx.x < n)
     a.low[(int64_t)(t0 + threadIdx.x) * a.E + e] =
@@ -144,72 +154,86 @@ struct Scores {  // of one token
   const double* low;
   int score;
   double top, sum;  // softmax: the largest logit (NaN if there is one), the sum of exp(l - top)
-  SFP8_DEV double operator()(int e) const {
-    return score == 0 ? exp(low[e] - top) / sum : 1.0 / (1.0 + exp(-low[e]));
-  }
+  SFP8_DEV double operator()(int e) const { return of(low[e]); }
+  SFP8_DEV double of(double l) const { return score == 0 ? exp(l - top) / sum : 1.0 / (1.0 + exp(-l)); }
 };
 
-// One wave selects for one token; keys: E of LDS.  chosen[j] = expert or -1, w[j] its weight (lane j).
-SFP8_DEV void select_token(const DecodeArgs& a, int t, uint64_t* keys, int& chosen, float& weight) {
-  const int lane = threadIdx.x & 63;
-  const double* low = a.low + (int64_t)t * a.E;
-  chosen = -1;
-  weight = 0.f;
-  if (a.mask && !a.mask[t]) return;
-  Scores s{low, a.score, 0.0, 1.0};
-  const bool all_scores = a.bias || (a.groups > 1 && a.group_best == 2) || !a.renorm;
-  if (a.score == 0 && all_scores) {
-    double m = -__builtin_inf(), z = 0.0;
-    for (int e = lane; e < a.E; e += 64) m = (low[e] > m || low[e] != low[e]) ? low[e] : m;
+// A wave's choice for token t.  A lane holds the keys of experts lane, lane +
+// 64, .. in registers (P of them), so a choice is the maximum of the lanes' best
+// (its high words first: seldom do two lanes agree in them) and one lane's
+// update.  `shared`: 64 P keys of LDS, read where there are groups.  Afterwards
+// lane j has expert and logit of slot j; -1 where nobody is left, and for all
+// slots of a masked token.
+struct Choice {
+  int expert;
+  double logit;
+};
+
+template <int P>
+SFP8_DEV Choice choose(const DecodeArgs& a, int t, Scores& s, uint64_t* shared) {
+  const int lane = threadIdx.x & 63, E = a.E;
+  Choice mine{-1, 0.0};
+  s = Scores{a.low + (int64_t)t * E, a.score, 0.0, 1.0};
+  if (a.mask && !a.mask[t]) return mine;
+  double l[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) l[i] = lane + 64 * i < E ? s.low[lane + 64 * i] : -__builtin_inf();
+  if (a.score == 0 && (a.bias || (a.groups > 1 && a.group_best == 2) || !a.renorm)) {
+    double m = l[0], z = 0.0;
+#pragma unroll
+    for (int i = 1; i < P; ++i) m = (l[i] > m || l[i] != l[i]) ? l[i] : m;
     s.top = wave_max_or_nan(m);
-    for (int e = lane; e < a.E; e += 64) z += exp(low[e] - s.top);
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (lane + 64 * i < E) z += exp(l[i] - s.top);
     s.sum = wave_sum(z);
   }
-  for (int e = lane; e < a.E; e += 64) {
-    const double l = low[e];
-    keys[e] = l == -__builtin_inf() ? 0 : order_key(a.bias ? s(e) + (double)a.bias[e] : l);
+  uint64_t key[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int e = lane + 64 * i;
+    key[i] = e >= E || l[i] == -__builtin_inf() ? 0 : order_key(a.bias ? s.of(l[i]) + (double)a.bias[e] : l[i]);
   }
-  __builtin_amdgcn_wave_barrier();
-  __threadfence_block();
   if (a.groups > 1) {
-    const int size = a.E / a.groups;
-    uint64_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < P; ++i) shared[lane + 64 * i] = key[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int size = E / a.groups;
+    uint64_t best = 0;
     if (lane < a.groups) {
       uint64_t k1 = 0, k2 = 0;
       int e1 = -1, e2 = -1;
       for (int e = lane * size; e < (lane + 1) * size; ++e) {
-        const uint64_t key = keys[e];
-        if (key > k1) k2 = k1, e2 = e1, k1 = key, e1 = e;
-        else if (key > k2) k2 = key, e2 = e;
+        const uint64_t x = shared[e];
+        if (x > k1) k2 = k1, e2 = e1, k1 = x, e1 = e;
+        else if (x > k2) k2 = x, e2 = e;
       }
-      mine = k1;
+      best = k1;
       if (a.group_best == 2 && e1 >= 0) {
         double v = s(e1) + (a.bias ? (double)a.bias[e1] : 0.0);
         if (e2 >= 0) v += s(e2) + (a.bias ? (double)a.bias[e2] : 0.0);
-        mine = order_key(v);
+        best = order_key(v);
       }
     }
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
-      const uint64_t other = __shfl(mine, g, 64);
-      rank += other > mine || (other == mine && g < lane);
+      const uint64_t other = __shfl(best, g, 64);
+      rank += other > best || (other == best && g < lane);
     }
-    const uint64_t kept = __ballot(lane < a.groups && mine != 0 && rank < a.top_groups);
-    for (int e = lane; e < a.E; e += 64)
-      if (!(kept >> (e / size) & 1)) keys[e] = 0;
-    __builtin_amdgcn_wave_barrier();
-    __threadfence_block();
+    const uint64_t kept = __ballot(lane < a.groups && best != 0 && rank < a.top_groups);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int e = lane + 64 * i;
+      if (e < E && !(kept >> (e / size) & 1)) key[i] = 0;
+    }
   }
-  // lane's own best among e = lane, lane + 64, ..: the lowest of equals
-  uint64_t best = 0;
-  int at = 0;
-  const auto rescan = [&]() {
-    best = 0, at = lane;
-    for (int e = lane; e < a.E; e += 64)
-      if (keys[e] > best) best = keys[e], at = e;
-  };
-  rescan();
   for (int j = 0; j < a.k; ++j) {
+    uint64_t best = key[0];
+    int at = lane;
+    double low = l[0];
+#pragma unroll
+    for (int i = 1; i < P; ++i)
+      if (key[i] > best) best = key[i], at = lane + 64 * i, low = l[i];
     const uint32_t hi = wave_max_u((uint32_t)(best >> 32));
     bool in = (uint32_t)(best >> 32) == hi;
     uint64_t who = __ballot(in);
@@ -217,92 +241,60 @@ SFP8_DEV void select_token(const DecodeArgs& a, int t, uint64_t* keys, int& chos
       const uint32_t lo = wave_max_u(in ? (uint32_t)best : 0u);
       in = in && (uint32_t)best == lo;
       who = __ballot(in);
-      if (who & (who - 1)) {
+      if (who & (who - 1)) {  // equals: the lowest index
         const uint32_t first = ~wave_max_u(in ? ~(uint32_t)at : 0u);
         who = __ballot(in && (uint32_t)at == first);
       }
     }
     const int win = __builtin_ctzll(who);
-    const uint32_t top_hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), win);
-    const uint32_t top_lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, win);
-    if ((top_hi | top_lo) == 0) break;  // nobody is left
+    if (hi == 0 && __builtin_amdgcn_readlane((int)(uint32_t)best, win) == 0) break;  // nobody is left
     const int e = __builtin_amdgcn_readlane(at, win);
-    if (lane == j) chosen = e;
-    if (lane == win) {
-      keys[e] = 0;
-      rescan();
-    }
+    const uint64_t bits = (uint64_t)__double_as_longlong(low);
+    const uint32_t b0 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, win);
+    const uint32_t b1 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), win);
+    if (lane == j) mine = Choice{e, __longlong_as_double((long long)((uint64_t)b1 << 32 | b0))};
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+      if (lane + 64 * i == e) key[i] = 0;
   }
-  // weights: shares of the chosen, in 64 bits
-  const bool there = chosen >= 0;
-  const double l = there ? low[chosen] : 0.0;
-  double share;
-  if (!a.renorm) {
-    share = there ? s(chosen) : 0.0;
-  } else {
-    // sigmoid(l) = exp(min(l, 0)) / (1 + exp(-|l|)): over exp of the largest min(l, 0) it cannot vanish for all
-    const double low_part = a.score == 0 ? l : (l > 0.0 ? 0.0 : l);
-    const double m = wave_max_or_nan(there ? low_part : -__builtin_inf());
-    const double v = exp(low_part - m);
-    const double part = there ? (a.score == 0 ? v : v / (1.0 + exp(-fabs(l)))) : 0.0;
-    share = part / wave_sum(part);
-  }
-  weight = there ? (float)((double)a.scale * share) : 0.f;
+  return mine;
 }
 
-// One work-group: a wave a token, then a thread an expert for the plan.
-__global__ __launch_bounds__(1024) void decode_select_kernel(DecodeArgs a) {
-  extern __shared__ __align__(16) uint64_t keys[];  // [waves][E]
-  __shared__ short sel[kSlots];
-  __shared__ int wave_slots[16], wave_experts[16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, waves = blockDim.x >> 6;
-  for (int t = wave; t < a.T; t += waves) {
-    int chosen;
-    float w;
-    select_token(a, t, keys + (int64_t)wave * a.E, chosen, w);
-    if (lane < a.k) {
-      sel[t * a.k + lane] = (short)chosen;
-      a.selected[t * a.k + lane] = chosen;
-      a.weights[t * a.k + lane] = w;
+// The weights of a wave's choice, shares of the chosen in 64 bits, written with the selection.
+SFP8_DEV void write_choice(const DecodeArgs& a, int t, const Scores& s, const Choice& c) {
+  const int lane = threadIdx.x & 63;
+  const bool there = c.expert >= 0;
+  double share;
+  if (!a.renorm) {
+    share = there ? s.of(c.logit) : 0.0;
+  } else {
+    // sigmoid(l) = exp(min(l, 0)) / (1 + exp(-|l|)): over exp of the largest min(l, 0) it cannot vanish for all
+    const double part = a.score == 0 ? c.logit : (c.logit > 0.0 ? 0.0 : c.logit);
+    int width = 1;
+    while (width < a.k) width *= 2;
+    double m = there ? part : -__builtin_inf();
+    for (int o = width / 2; o > 0; o >>= 1) {
+      const double w = __shfl_xor(m, o, 64);
+      m = (w > m || w != w) ? w : m;
     }
+    const double v = exp(part - m);
+    share = there ? (a.score == 0 ? v : v / (1.0 + exp(-fabs(c.logit)))) : 0.0;
+    double z = share;
+    for (int o = width / 2; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
+    share /= z;
   }
-  __syncthreads();
-  // experts in blocks of the work-group's threads; slots and experts before each
-  const int slots = a.T * a.k, most = plan_most(a.T, a.E, a.k);
-  int* out = a.plan + 2 + 2 * most;
-  int base_slots = 0, base_experts = 0;
-  for (int e0 = 0; e0 < a.E; e0 += blockDim.x) {
-    const int e = e0 + tid;
-    int n = 0;
-    for (int s = 0; s < slots; ++s) n += sel[s] == e;
-    int before = n, live = n > 0;  // inclusive sums over the lanes
-    int upto = live;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int p = __shfl_up(before, o, 64), q = __shfl_up(upto, o, 64);
-      if (lane >= o) before += p, upto += q;
-    }
-    if (lane == 63) wave_slots[wave] = before, wave_experts[wave] = upto;
-    __syncthreads();
-    int first = base_slots, rank = base_experts, all_slots = 0, all_experts = 0;
-    for (int w = 0; w < waves; ++w) {
-      if (w < wave) first += wave_slots[w], rank += wave_experts[w];
-      all_slots += wave_slots[w], all_experts += wave_experts[w];
-    }
-    first += before - n, rank += upto - live;
-    if (live) {
-      a.plan[1 + rank] = e;
-      a.plan[1 + most + rank] = first;
-      for (int s = 0, i = first; s < slots; ++s)
-        if (sel[s] == e) out[i++] = s;
-    }
-    base_slots += all_slots, base_experts += all_experts;
-    __syncthreads();
+  if (lane < a.k) {
+    a.selected[(int64_t)t * a.k + lane] = c.expert;
+    a.weights[t * a.k + lane] = there ? (float)((double)a.scale * share) : 0.f;
   }
-  if (tid == 0) {
-    a.plan[0] = base_experts;
-    a.plan[1 + most + base_experts] = base_slots;
-  }
+}
+
+template <int P>
+__global__ __launch_bounds__(64) void decode_select_kernel(DecodeArgs a) {
+  __shared__ uint64_t shared[64 * P];
+  Scores s;
+  const Choice c = choose<P>(a, blockIdx.x, s, shared);
+  write_choice(a, blockIdx.x, s, c);
 }
 
 // ---------------------------------------------------------------------------
@@ -320,236 +312,522 @@ SFP8_DEV floatx4 mfma16(bf16x8 w, bf16x8 x, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x, c, 0, 0, 0);
 }
 
-// How a lane (row r of 16, quarter q) reads a stretch of K of its weight row:
-// kStep values a wave and step, kPieces pieces of 8 a lane, piece j at value
-// at(q, j) of the stretch.
+// How a lane (row r of 16, quarter q) holds a stretch of K: kStep values of its
+// row, of which it has kPieces pieces of 8, piece j at value at(q, j) of the
+// stretch.  The four quarters' pieces are neighbours, so that a load's 64 lanes
+// read 64 bytes in a run from each of 16 rows; with a lane's own pieces as
+// neighbours the first-level cache serves two to four times as many lines.
 template <bool W4>
 struct Stretch {
   static constexpr int kStep = W4 ? 128 : 64, kPieces = W4 ? 4 : 2;
-  static SFP8_DEV int at(int q, int j) { return kPieces * 8 * q + 8 * j; }
+  static SFP8_DEV int at(int q, int j) { return 32 * j + 8 * q; }
   bf16x8 w[kPieces];
 };
 
-// Rows of one expert's matrix.
+// One expert's matrix: at() is a lane's place in row n, `part` stretches further
+// on; read() has what the lane holds s stretches from there in flight, values()
+// makes bf16 values of it.  Buffer loads: 32-bit offsets from a base in scalar
+// registers (a matrix is below 4 GiB), and zeros for what is past its end.
+SFP8_DEV __amdgpu_buffer_rsrc_t matrix_rsrc(const uint8_t* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), (short)0, (int)(uint32_t)bytes, 0x00020000);
+}
+typedef unsigned int uintx4 __attribute__((ext_vector_type(4)));
+
 template <bool W4>
 struct WeightRows;
 template <>
 struct WeightRows<false> {
-  const uint16_t* p;  // [rows, K]
-  int64_t K;
+  using Raw = Stretch<false>;
+  struct At {
+    uint32_t off;
+  };
+  __amdgpu_buffer_rsrc_t r;
+  uint32_t bytes;  // of a row
   SFP8_DEV WeightRows(const uint8_t* base, const uint8_t*, int64_t e, int64_t rows, int64_t k)
-      : p(reinterpret_cast<const uint16_t*>(base) + e * rows * k), K(k) {}
-  // step s of row n; past K (a multiple of 8) the last piece again, whose product the caller zeroes
-  template <bool TAIL>
-  SFP8_DEV void read(int64_t n, int s, int q, Stretch<false>& f) const {
+      : r(matrix_rsrc(base + e * rows * k * 2, rows * k * 2)), bytes((uint32_t)k * 2) {}
+  SFP8_DEV At at(int n, int part, int q) const { return At{(uint32_t)n * bytes + 128u * part + 16u * q}; }
+  SFP8_DEV void read(At at, int s, Raw& f) const {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      int64_t k = (int64_t)s * 64 + Stretch<false>::at(q, j);
-      bool ok = true;
-      if (TAIL) ok = k < K, k = ok ? k : K - 8;
-      f.w[j] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const intx4*>(p + n * K + k));
-      if (TAIL) f.w[j] = zero_unless(ok, f.w[j]);
-    }
+    for (int j = 0; j < 2; ++j)
+      f.w[j] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, at.off + 128u * s + 64u * j, 0, 0));
+  }
+  SFP8_DEV void values(const Raw& raw, Stretch<false>& f) const { f = raw; }
+  // what is past column K, the next row's, as zeros; k: the stretch's first column
+  static SFP8_DEV void zero_past(Stretch<false>& f, int K, int k, int q) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) f.w[j] = zero_unless(k + Stretch<false>::at(q, j) < K, f.w[j]);
   }
 };
 template <>
 struct WeightRows<true> {
-  const uint8_t *codes, *scales;  // [slabs][rows rounded up][64], [..][4]
-  int64_t rows;
-  SFP8_DEV WeightRows(const uint8_t* c, const uint8_t* s, int64_t e, int64_t r, int64_t k) : rows(mx_rows(r)) {
-    codes = c + e * mx_slabs(k) * rows * 64;
-    scales = s + e * mx_slabs(k) * rows * 4;
+  struct Raw {
+    uintx4 codes;
+    uint32_t scales;
+  };
+  struct At {
+    uint32_t row;
+    uint32_t q;
+  };
+  __amdgpu_buffer_rsrc_t r, rs;  // [slabs][rows rounded up][64], [..][4]
+  uint32_t rows;
+  SFP8_DEV WeightRows(const uint8_t* c, const uint8_t* s, int64_t e, int64_t n, int64_t k)
+      : r(matrix_rsrc(c + e * mx_slabs(k) * mx_rows(n) * 64, mx_slabs(k) * mx_rows(n) * 64)),
+        rs(matrix_rsrc(s + e * mx_slabs(k) * mx_rows(n) * 4, mx_slabs(k) * mx_rows(n) * 4)), rows((uint32_t)mx_rows(n)) {}
+  SFP8_DEV At at(int n, int part, int q) const { return At{(uint32_t)part * rows + n, 16u * q}; }
+  SFP8_DEV void read(At at, int s, Raw& f) const {
+    const uint32_t row = at.row + (uint32_t)s * rows;
+    f.codes = __builtin_amdgcn_raw_buffer_load_b128(r, row * 64 + at.q, 0, 0);
+    f.scales = __builtin_amdgcn_raw_buffer_load_b32(rs, row * 4, 0, 0);
   }
-  template <bool TAIL>
-  SFP8_DEV void read(int64_t n, int s, int q, Stretch<true>& f) const {
-    const intx4 c = *reinterpret_cast<const intx4*>(codes + (s * rows + n) * 64 + 16 * q);
-    const uint32_t e = *reinterpret_cast<const uint32_t*>(scales + (s * rows + n) * 4) >> (8 * q) & 255u;
-    const float v = mx_scale_value(e);
+  // A lane has read block q of the row; piece j is a quarter of block j: a transpose of the quarters' words.
+  SFP8_DEV void values(const Raw& raw, Stretch<true>& f) const {
+    const auto a = __builtin_amdgcn_permlane32_swap(raw.codes[0], raw.codes[2], false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(raw.codes[1], raw.codes[3], false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+    const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    const uint32_t word[4] = {c[0], c[1], d[0], d[1]};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f.w[j] = bf16_of_codes8((uint32_t)c[j], v);
+    for (int j = 0; j < 4; ++j) f.w[j] = bf16_of_codes8(word[j], mx_scale_value(raw.scales >> (8 * j) & 255u));
   }
+  static SFP8_DEV void zero_past(Stretch<true>&, int, int, int) {}  // padding has zero codes, past the end are zeros
 };
 
-// A token's (or slot's) values beside them.
-template <bool W4, bool TAIL>
-SFP8_DEV void read_values(const uint16_t* row, int K, int s, int q, Stretch<W4>& f) {
+// A token's (or slot's) values beside them; `row` is the lane's own place, 8 q values into the row.
+template <bool W4>
+SFP8_DEV void read_values(const uint16_t* row, int k, Stretch<W4>& f) {
+#pragma unroll
+  for (int j = 0; j < Stretch<W4>::kPieces; ++j) f.w[j] = load_bf16x8(row + k + 32 * j);
+}
+// ... of a stretch that the row ends in: zeros from column K (a multiple of 8) on.
+template <bool W4>
+SFP8_DEV void read_last(const uint16_t* row, int K, int k, int q, Stretch<W4>& f) {
 #pragma unroll
   for (int j = 0; j < Stretch<W4>::kPieces; ++j) {
-    int k = s * Stretch<W4>::kStep + Stretch<W4>::at(q, j);
-    bool ok = true;
-    if (TAIL) ok = k < K, k = ok ? k : K - 8;
-    f.w[j] = load_bf16x8(row + k);
-    if (TAIL) f.w[j] = zero_unless(ok, f.w[j]);
+    const int at = k + Stretch<W4>::at(q, j);
+    f.w[j] = zero_unless(at < K, load_bf16x8(row + (at < K ? at : K - 8) - 8 * q));
   }
 }
 
-// Gate and up of 16 columns of h for all slots of one expert: eight waves share
-// the width, their sums meet in LDS in the order of the waves.  NB: blocks of
+// n steps as calls of f(size, first) with sizes U, U / 2, .., 1 (compile-time).
+template <int U, class F>
+SFP8_DEV void in_batches(int n, F f, int i = 0) {
+  for (; i + U <= n; i += U) f(std::integral_constant<int, U>{}, i);
+  if constexpr (U > 1) in_batches<U / 2>(n, f, i);
+}
+
+// Up to this many tokens are selected by the waves of every work-group of gate
+// and up (P keys a lane): 3 us that it waits longer against 6 of a launch and a
+// kernel of its own.
+constexpr int kFused = 4, kFusedKeys = 4, kFusedGroups = 1024;
+
+// Gate and up of 8 columns of h for all slots of one expert: a product's 16 rows
+// are the 8 gate rows and the 8 up rows.  Four waves share the width, up to four
+// steps of each in flight, and their sums meet in LDS in the order of the waves.
+// Small work-groups, several a CU: with one token and eight experts of 768
+// columns there are three for each CU, and their waits overlap.  NB: blocks of
 // 16 slots that an expert can have.
-template <bool W4, int NB>
-__global__ __launch_bounds__(512) void decode_gateup_kernel(DecodeArgs a) {
-  constexpr int W = 8;
-  __shared__ __align__(16) float red[W][2][NB * 16][20];
-  const Plan plan{a.plan, plan_most(a.T, a.E, a.k)};
-  const int which = blockIdx.y;
-  if (which >= plan.count()) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
-  const int e = plan.expert(which), begin = plan.begin(which), n = plan.begin(which + 1) - begin;
-  const int* slots = plan.slots() + begin;
-  const int i0 = 16 * blockIdx.x, D = a.D, I = a.I;
+template <bool W4, int NB, int SETS>
+__global__ __launch_bounds__(256, W4 && NB > 1 ? 3 : 4) void decode_gateup_kernel(DecodeArgs a) {
+  constexpr int W = 4, kStep = Stretch<W4>::kStep, kPieces = Stretch<W4>::kPieces;
+  constexpr bool FUSED = SETS == 1;
+  static_assert(!FUSED || (kFused <= W && NB == 1), "a wave a token");
+  __shared__ __align__(16) float red[W][SETS][16][20];
+  __shared__ int list[kMaxTokens], count[W], own;
+  __shared__ uint64_t keys[FUSED ? W * 64 * kFusedKeys : 1];
+  __shared__ short chosen[FUSED ? kFused * kMaxTopK : 1];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // the expert of this candidate, and its slots in order
+  const int slots = a.T * a.k, most = candidates(a.T, a.E, a.k), c = blockIdx.y;
+  if constexpr (FUSED) {
+    if (c == most && blockIdx.x) return;  // one work-group more writes the selection and the weights
+    if (wave < a.T) {
+      Scores s;
+      const Choice x = choose<kFusedKeys>(a, wave, s, keys + wave * 64 * kFusedKeys);
+      if (c == most) write_choice(a, wave, s, x);
+      else if (lane < a.k) chosen[wave * a.k + lane] = (short)x.expert;
+    }
+    if (c == most) return;
+    __syncthreads();
+  }
+  const auto expert_of = [&](int s) { return FUSED ? (int)chosen[FUSED ? s : 0] : (int)a.selected[s]; };
+  const bool by_slot = slots < a.E;
+  int e = c, n = 0;
+  for (int s0 = 0; s0 < slots; s0 += 64 * W) {
+    const int s = s0 + tid, x = s < slots ? expert_of(s) : -1;
+    if (by_slot && s0 == 0) {
+      if (c < 64 * W ? s == c : tid == 0) own = c < 64 * W ? x : expert_of(c);
+      __syncthreads();
+      e = own;
+    }
+    const bool match = e >= 0 && x == e;
+    const uint64_t who = __ballot(match);
+    if (lane == 0) count[wave] = __builtin_popcountll(who);
+    __syncthreads();
+    int before = n;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) before += count[w];
+      n += count[w];
+    }
+    if (match) list[before + __builtin_popcountll(who & ((1ull << lane) - 1))] = s;
+    __syncthreads();
+  }
+  if (by_slot && n > 0 && list[0] != c) n = 0;  // an earlier slot stands for this expert
+  if (blockIdx.x == 0) {
+    if (tid == 0) a.plan[c] = n, a.plan[most + c] = e;
+    if (tid < n) a.plan[plan_slots(most) + 64 * c + tid] = list[tid];
+  }
+  if (n == 0) return;
+
+  e = __builtin_amdgcn_readfirstlane(e);
+  n = __builtin_amdgcn_readfirstlane(n);
+  const int i0 = 8 * SETS * blockIdx.x, D = a.D, I = a.I;  // I is a multiple of 8
   const WeightRows<W4> w(a.gu, a.gu_scales, e, 2 * (int64_t)I, D);
-  const int64_t grow = min(i0 + r, I - 1), urow = I + grow;
+  typename WeightRows<W4>::At row[SETS];
+#pragma unroll
+  for (int z = 0; z < SETS; ++z) row[z] = w.at((r < 8 ? 0 : I - 8) + r + min(i0 + 8 * z, I - 8), 0, q);
   const uint16_t* xrow[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int s = 16 * b + r;  // a lane without a slot goes along with the first
-    xrow[b] = a.x + (slots[s < n ? s : 0] / a.k) * a.ldx;
+    xrow[b] = a.x + (list[s < n ? s : 0] / a.k) * a.ldx + 8 * q;
   }
-  floatx4 g[NB], u[NB];
+  floatx4 acc[NB][SETS];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) g[b] = u[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const auto step = [&](auto tail, int s) {
-    constexpr bool TAIL = decltype(tail)::value;
-    Stretch<W4> fg, fu, fx;
-    w.template read<TAIL>(grow, s, q, fg);
-    w.template read<TAIL>(urow, s, q, fu);
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      if (b == 0 || 16 * b < n) {
-        read_values<W4, TAIL>(xrow[b], D, s, q, fx);
+    for (int z = 0; z < SETS; ++z) acc[b][z] = floatx4{0.f, 0.f, 0.f, 0.f};
+  const auto multiply = [&](const Stretch<W4> (&fw)[SETS], const Stretch<W4>& fx, int b) {
 #pragma unroll
-        for (int j = 0; j < Stretch<W4>::kPieces; ++j) {
-          g[b] = mfma16(fg.w[j], fx.w[j], g[b]);
-          u[b] = mfma16(fu.w[j], fx.w[j], u[b]);
+    for (int z = 0; z < SETS; ++z)
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) acc[b][z] = mfma16(fw[z].w[j], fx.w[j], acc[b][z]);
+  };
+  const int full = D / kStep;
+  const auto batch = [&](auto size, int s) {  // steps s, s + W, ..: all of their bytes in flight at once
+    constexpr int U = decltype(size)::value;
+    typename WeightRows<W4>::Raw raw[U][SETS];
+    Stretch<W4> fx[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int z = 0; z < SETS; ++z) w.read(row[z], s + i * W, raw[i][z]);
+      read_values<W4>(xrow[0], (s + i * W) * kStep, fx[i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead of the products
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      Stretch<W4> fw[SETS];
+#pragma unroll
+      for (int z = 0; z < SETS; ++z) w.values(raw[i][z], fw[z]);
+      multiply(fw, fx[i], 0);
+#pragma unroll
+      for (int b = 1; b < NB; ++b) {
+        if (16 * b < n) {
+          Stretch<W4> more;
+          read_values<W4>(xrow[b], (s + i * W) * kStep, more);
+          multiply(fw, more, b);
         }
       }
     }
   };
-  const int full = D / Stretch<W4>::kStep;
-  for (int s = wave; s < full; s += W) step(std::false_type{}, s);
-  if (D % Stretch<W4>::kStep && wave == full % W) step(std::true_type{}, full);
+  constexpr int kMost = SETS > 1 && (W4 || NB > 1) ? 2 : 4;  // what the registers of four waves a SIMD hold
+  in_batches<kMost>((full - wave + W - 1) / W, [&](auto size, int i) { batch(size, wave + i * W); });
+  if (D % kStep && wave == full % W) {
+    typename WeightRows<W4>::Raw raw;
+    Stretch<W4> fw[SETS], fx;
+#pragma unroll
+    for (int z = 0; z < SETS; ++z) {
+      w.read(row[z], full, raw);
+      w.values(raw, fw[z]);
+      w.zero_past(fw[z], D, full * kStep, q);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if (16 * b < n) {
+        read_last<W4>(xrow[b], D, full * kStep, q, fx);
+        multiply(fw, fx, b);
+      }
+    }
+  }
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    *reinterpret_cast<floatx4*>(&red[wave][0][16 * b + r][4 * q]) = g[b];
-    *reinterpret_cast<floatx4*>(&red[wave][1][16 * b + r][4 * q]) = u[b];
-  }
-  __syncthreads();
-  for (int i = tid; i < n * 16; i += 64 * W) {
-    const int s = i >> 4, c = i & 15;
-    float gs = 0.f, us = 0.f;
+    if (16 * b >= n) break;
+    if (b) __syncthreads();
 #pragma unroll
-    for (int v = 0; v < W; ++v) gs += red[v][0][s][c], us += red[v][1][s][c];
-    if (i0 + c < I) {
-      const float h = gs * sigmoid_fast(gs) * us, hi = round_bf16(h);
-      uint16_t* p = a.h + (int64_t)slots[s] * 2 * I + i0 + c;
+    for (int z = 0; z < SETS; ++z) *reinterpret_cast<floatx4*>(&red[wave][z][r][4 * q]) = acc[b][z];
+    __syncthreads();
+    const int s = tid / (8 * SETS), col = tid % (8 * SETS), z = col >> 3;
+    if (s < 16 && 16 * b + s < n && i0 + col < I) {
+      float g = 0.f, u = 0.f;
+#pragma unroll
+      for (int v = 0; v < W; ++v) g += red[v][z][s][col & 7], u += red[v][z][s][8 + (col & 7)];
+      const float h = g * sigmoid_fast(g) * u, hi = round_bf16(h);
+      uint16_t* p = a.h + (int64_t)list[16 * b + s] * 2 * a.ldh + i0 + col;
       p[0] = (uint16_t)f32_to_bf16_bits(h);
       // an infinity or a NaN leaves nothing to be added
-      p[I] = (uint16_t)f32_to_bf16_bits(__builtin_isfinite(hi) ? h - hi : 0.f);
+      p[a.ldh] = (uint16_t)f32_to_bf16_bits(__builtin_isfinite(hi) ? h - hi : 0.f);
+    }
+  }
+  if (i0 + 8 * SETS >= I && a.ldh > I) {  // zeros up to the end of down's last stretch
+    const int pad = a.ldh - I;
+    for (int i = tid; i < 2 * n * pad; i += 64 * W) {
+      const int row2 = i / pad;
+      a.h[((int64_t)list[row2 >> 1] * 2 + (row2 & 1)) * a.ldh + I + i % pad] = 0;
     }
   }
 }
 
-// Down and the weighted sum for 16 columns of the output: the steps of all
-// experts that are taken, in their order, are dealt out to the waves in even
-// runs.  A wave adds each expert's sums times the slots' weights to its own
-// totals of all tokens (LDS), and the waves' totals meet in their order: every
-// weight is read once, and no sum depends on the order of arrival.
-template <bool W4, int NB>
+// Down and the weighted sum for C SETS columns of the output: the steps of all
+// experts that are taken are dealt out to the waves in even runs.  A wave adds
+// each expert's sums times the slots' weights to its own totals of all tokens
+// (LDS), and the waves' totals meet in their order: every weight is read once,
+// and no sum depends on the order of arrival.
+// A product's 16 rows are C columns in P = 16 / C parts of K, its 16 columns C
+// slots in the same parts, and of the result the blocks where the parts agree
+// are kept: a CU takes no more than about 20 bytes a nanosecond from memory, so
+// all of them have to have a work-group.  An expert of more than 2 C slots is
+// read again for each 2 C of them.  RAGGED: I is no multiple of a step.
+// With many slots an expert, h is what the CUs take most of (two parts of each
+// slot beside C rows of weights): then SETS = 2 sets of 16 columns share it, and
+// gridDim.y work-groups share the steps of a column block; the last of them to
+// finish (counters that the logits' launch has zeroed) adds their sums in order.
+template <bool W4, int C, int SETS, bool RAGGED>
 __global__ __launch_bounds__(512) void decode_down_kernel(DecodeArgs a) {
-  constexpr int W = 8;
-  extern __shared__ __align__(16) float totals[];  // [W][T][16]
-  const Plan plan{a.plan, plan_most(a.T, a.E, a.k)};
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, q = lane >> 4;
-  const int n0 = 16 * blockIdx.x, D = a.D, I = a.I, T = a.T;
-  float* mine = totals + wave * T * 16;
-  for (int i = lane; i < T * 4; i += 64) reinterpret_cast<floatx4*>(mine)[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  const int steps = (I + Stretch<W4>::kStep - 1) / Stretch<W4>::kStep;
-  const int64_t all = (int64_t)plan.count() * steps;
-  const int lo = (int)(all * wave / W), hi = (int)(all * (wave + 1) / W);
-  const int64_t row = min(n0 + r, D - 1);
+  static_assert(SETS == 1 || C == 16, "");
+  constexpr int W = 8, P = 16 / C, CB = C * SETS, NB = 2, kPieces = Stretch<W4>::kPieces, kStep = P * Stretch<W4>::kStep;
+  extern __shared__ __align__(16) float totals[];  // [W][T][CB]
+  __shared__ short expert_of[kMaxExperts], slot_of[kSlots];
+  __shared__ int begin[kMaxExperts + 1], count[W], slots_before[W], last;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = CB * blockIdx.x, D = a.D, I = a.I, T = a.T, most = candidates(T, a.E, a.k);
+  float* mine = totals + wave * T * CB;
+  for (int i = lane; i < T * CB / 4; i += 64) reinterpret_cast<floatx4*>(mine)[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  // the experts that are taken, in the candidates' order, and their slots
+  int live = 0, taken = 0;
+  for (int c0 = 0; c0 < most; c0 += 64 * W) {
+    const int c = c0 + tid;
+    const int* list = a.plan + plan_slots(most) + 64 * c;
+    int n = 0, e = 0, some[4];
+    if (c < most) {  // all at once: the list's first slots whether there or not
+      n = a.plan[c], e = a.plan[most + c];
+      const intx4 v = *reinterpret_cast<const intx4*>(list);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) some[i] = v[i];
+    }
+    const uint64_t who = __ballot(n > 0);
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int p = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += p;
+    }
+    if (lane == 63) count[wave] = __builtin_popcountll(who), slots_before[wave] = upto;
+    __syncthreads();
+    int at = live + __builtin_popcountll(who & ((1ull << lane) - 1)), first = taken + upto - n;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) at += count[w], first += slots_before[w];
+      live += count[w], taken += slots_before[w];
+    }
+    if (n > 0) {
+      expert_of[at] = (short)e;
+      begin[at] = first;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < n) slot_of[first + i] = (short)some[i];
+      for (int i = 4; i < n; ++i) slot_of[first + i] = (short)list[i];
+    }
+    __syncthreads();
+  }
+  if (tid == 0) begin[live] = taken;
+  __syncthreads();
+  const int steps = (I + kStep - 1) / kStep;
+  const int64_t all = (int64_t)live * steps;
+  const int turn = blockIdx.y * W + wave, turns = gridDim.y * W;
+  const int lo = (int)(all * turn / turns), hi = (int)(all * (turn + 1) / turns);
+  const int part = r / C;
   for (int at = lo; at < hi;) {
     const int which = at / steps, s0 = at - which * steps, s1 = min(steps, s0 + hi - at);
     at += s1 - s0;
-    const int e = plan.expert(which), begin = plan.begin(which), n = plan.begin(which + 1) - begin;
-    const int* slots = plan.slots() + begin;
-    const WeightRows<W4> w(a.down, a.down_scales, e, D, I);
-    const uint16_t* hrow[NB];
+    const int end = __builtin_amdgcn_readfirstlane(begin[which + 1]);
+    const WeightRows<W4> w(a.down, a.down_scales, __builtin_amdgcn_readfirstlane(expert_of[which]), D, I);
+    typename WeightRows<W4>::At place[SETS];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int s = 16 * b + r;
-      hrow[b] = a.h + (int64_t)slots[s < n ? s : 0] * 2 * I;
-    }
-    floatx4 acc[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = floatx4{0.f, 0.f, 0.f, 0.f};
-    const auto step = [&](auto tail, int s) {
-      constexpr bool TAIL = decltype(tail)::value;
-      Stretch<W4> fw, f0, f1;
-      w.template read<TAIL>(row, s, q, fw);
+    for (int z = 0; z < SETS; ++z) place[z] = w.at(min(n0 + C * z + r % C, D - 1), part, q);
+    for (int first = __builtin_amdgcn_readfirstlane(begin[which]); first < end; first += NB * C) {
+      const int n = min(end - first, NB * C);
+      const uint16_t* hrow[NB];
+      float weight[NB];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        if (b == 0 || 16 * b < n) {
-          read_values<W4, TAIL>(hrow[b], I, s, q, f0);
-          read_values<W4, TAIL>(hrow[b] + I, I, s, q, f1);
+        const int i = C * b + r % C, s = slot_of[first + (i < n ? i : 0)];
+        hrow[b] = a.h + (int64_t)s * 2 * a.ldh + part * Stretch<W4>::kStep + 8 * q;
+        weight[b] = a.weights[s];
+      }
+      floatx4 acc[NB][SETS];
 #pragma unroll
-          for (int j = 0; j < Stretch<W4>::kPieces; ++j) {
-            acc[b] = mfma16(fw.w[j], f0.w[j], acc[b]);
-            acc[b] = mfma16(fw.w[j], f1.w[j], acc[b]);
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int z = 0; z < SETS; ++z) acc[b][z] = floatx4{0.f, 0.f, 0.f, 0.f};
+      const auto batch = [&](auto blocks, auto size, int s) {
+        constexpr int B = decltype(blocks)::value, U = decltype(size)::value;
+        typename WeightRows<W4>::Raw rw[U][SETS];
+        Stretch<W4> f[U][B][2];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+#pragma unroll
+          for (int z = 0; z < SETS; ++z) w.read(place[z], P * (s + i), rw[i][z]);
+#pragma unroll
+          for (int b = 0; b < B; ++b) {
+            read_values<W4>(hrow[b], (s + i) * kStep, f[i][b][0]);
+            read_values<W4>(hrow[b] + a.ldh, (s + i) * kStep, f[i][b][1]);
           }
         }
-      }
-    };
-    const int full = I / Stretch<W4>::kStep;
-    for (int s = s0; s < min(s1, full); ++s) step(std::false_type{}, s);
-    if (s1 > full) step(std::true_type{}, full);
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead of the products
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int s = 16 * b + r;
-      if (s < n) {
-        const int slot = slots[s];
-        const float wt = a.weights[slot];
-        floatx4* p = reinterpret_cast<floatx4*>(mine + (slot / a.k) * 16 + 4 * q);
-        floatx4 t = *p;
+        for (int i = 0; i < U; ++i)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) t[v] = __builtin_fmaf(wt, acc[b][v], t[v]);
-        *p = t;
-      }
+          for (int z = 0; z < SETS; ++z) {
+            Stretch<W4> fw;
+            w.values(rw[i][z], fw);
+            if (RAGGED && s + i == steps - 1) w.zero_past(fw, I, (s + i) * kStep + part * Stretch<W4>::kStep, q);
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) acc[b][z] = mfma16(fw.w[j], f[i][b][half].w[j], acc[b][z]);
+          }
+      };
+      // as many steps in flight as 256 registers hold
+      constexpr int kOne = (W4 ? 3 : 6) - (SETS > 1 ? W4 ? 1 : 2 : 0), kTwo = (W4 ? 2 : 4) - (SETS > 1 ? 1 : 0);
+      if (n <= C)
+        in_batches<kOne>(s1 - s0, [&](auto u, int i) { batch(std::integral_constant<int, 1>{}, u, s0 + i); });
+      else
+        in_batches<kTwo>(s1 - s0, [&](auto u, int i) { batch(std::integral_constant<int, 2>{}, u, s0 + i); });
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int z = 0; z < SETS; ++z) {
+          floatx4 v = acc[b][z];
+          // a part's columns are 4 q' .. + 3 of slot r % C: the next part's lie 256 / P + C lanes on (rows, columns)
+          if constexpr (P > 1) {
+            floatx4 sum = v;
+#pragma unroll
+            for (int o = 1; o < P; ++o)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) sum[j] += __shfl(v[j], (lane + o * (64 / P + C)) & 63, 64);
+            v = sum;
+          }
+          const int i = C * b + r % C;
+          if (i < n && r < C && q < C / 4) {
+            const int token = slot_of[first + i] / a.k;
+            floatx4* p = reinterpret_cast<floatx4*>(mine + token * CB + C * z + 4 * q);
+            floatx4 t = *p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = __builtin_fmaf(weight[b], v[j], t[j]);
+            *p = t;
+          }
+        }
     }
   }
   __syncthreads();
-  for (int i = tid; i < T * 8; i += 64 * W) {
-    const int t = i >> 3, c = 2 * (i & 7);
+  const bool shared = gridDim.y > 1;
+  for (int i = tid; i < T * CB / 2; i += 64 * W) {
+    const int t = i / (CB / 2), col = 2 * (i % (CB / 2));
     float v0 = 0.f, v1 = 0.f;
 #pragma unroll
-    for (int v = 0; v < W; ++v) v0 += totals[(v * T + t) * 16 + c], v1 += totals[(v * T + t) * 16 + c + 1];
-    if (n0 + c < D) *reinterpret_cast<uint32_t*>(a.out + (int64_t)t * D + n0 + c) = pack2_bf16(v0, v1);
+    for (int v = 0; v < W; ++v) v0 += totals[(v * T + t) * CB + col], v1 += totals[(v * T + t) * CB + col + 1];
+    if (n0 + col < D) {
+      const int64_t at = (int64_t)t * D + n0 + col;
+      if (shared) *reinterpret_cast<floatx2*>(a.partial + (int64_t)blockIdx.y * T * D + at) = floatx2{v0, v1};
+      else *reinterpret_cast<uint32_t*>(a.out + at) = pack2_bf16(v0, v1);
+    }
+  }
+  if (!shared) return;
+  // The barriers order the work-group's accesses with thread 0's, whose release and acquire work on the whole L2 and
+  // this CU's cache: done by every wave they took as long as the products.
+  __syncthreads();
+  if (tid == 0)
+    last = __hip_atomic_fetch_add(a.done + blockIdx.x, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+           (int)gridDim.y - 1;
+  __syncthreads();
+  if (!last) return;
+  for (int i = tid; i < T * CB / 2; i += 64 * W) {
+    const int t = i / (CB / 2), col = 2 * (i % (CB / 2));
+    if (n0 + col < D) {
+      const int64_t at = (int64_t)t * D + n0 + col;
+      floatx2 v = {0.f, 0.f};
+      for (int y = 0; y < (int)gridDim.y; ++y) {
+        const floatx2 p = *reinterpret_cast<const floatx2*>(a.partial + (int64_t)y * T * D + at);
+        v[0] += p[0], v[1] += p[1];
+      }
+      *reinterpret_cast<uint32_t*>(a.out + at) = pack2_bf16(v[0], v[1]);
+    }
   }
 }
 
 inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
+// work-groups that share the steps of a block of 32 columns (T > 16): about one for each CU in all
+inline int down_shares(int64_t T, int64_t D) {
+  const int64_t blocks = (D + 31) / 32;
+  return T <= 16 || blocks >= 256 ? 1 : (int)(blocks <= 16 ? 16 : 256 / blocks);
+}
+
 struct DecodeSpace {
-  int64_t low, weights, plan, h, all;
-  DecodeSpace(int64_t T, int64_t E, int64_t k, int64_t I) {
+  int64_t low, weights, plan, done, partial, h, all;
+  DecodeSpace(int64_t T, int64_t E, int64_t k, int64_t D, int64_t I) {
+    const int64_t most = candidates((int)T, (int)E, (int)k), shares = down_shares(T, D);
     low = 0;
     weights = low + up256(T * E * 8);
     plan = weights + up256(T * k * 4);
-    h = plan + up256((2 + 2 * plan_most((int)T, (int)E, (int)k) + T * k) * 4);
-    all = h + T * k * 2 * I * 2;
+    done = plan + up256((plan_slots((int)most) + 64 * most) * 4);
+    partial = done + up256(shares > 1 ? (D + 31) / 32 * 4 : 0);
+    h = partial + up256(shares > 1 ? shares * T * D * 4 : 0);
+    all = h + T * k * 2 * ((I + 511) / 512 * 512) * 2;  // a step of down has at most 512 columns
   }
 };
 
 inline bool decode_sizes_ok(int64_t T, int64_t E, int64_t k, int64_t D, int64_t I) {
   return T >= 0 && T <= kMaxTokens && E >= 1 && E <= kMaxExperts && k >= 1 && k <= kMaxTopK && k <= E && D >= 8 &&
-         D % 8 == 0 && D <= 1 << 20 && I >= 8 && I % 8 == 0 && I <= 1 << 20;
+         D % 8 == 0 && D <= 1 << 20 && I >= 8 && I % 8 == 0 && I <= 1 << 20 && D * I <= (int64_t)1 << 29;
 }
 
-template <bool W4, int NB>
-int launch_experts(const DecodeArgs& a, hipStream_t s) {
-  decode_gateup_kernel<W4, NB><<<dim3((a.I + 15) / 16, plan_most(a.T, a.E, a.k)), 512, 0, s>>>(a);
-  decode_down_kernel<W4, NB><<<(a.D + 15) / 16, 512, (size_t)8 * a.T * 16 * 4, s>>>(a);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? kOk : (int)e;
+template <bool W4, int C, int SETS>
+void launch_down(const DecodeArgs& a, int shares, hipStream_t s) {
+  const dim3 grid((unsigned)((a.D + C * SETS - 1) / (C * SETS)), (unsigned)shares);
+  const size_t totals = (size_t)8 * a.T * C * SETS * 4;
+  if (a.I != a.ldh) decode_down_kernel<W4, C, SETS, true><<<grid, 512, totals, s>>>(a);
+  else decode_down_kernel<W4, C, SETS, false><<<grid, 512, totals, s>>>(a);
+}
+
+template <bool W4>
+void launch_experts(DecodeArgs a, hipStream_t s) {
+  // Columns a work-group of down: such that there is one for each CU (T = 16, D = 1024, 8 experts of 1536: 4 columns
+  // 32.7 us a layer, 8 35.9, 16 43.2; T = 1, D = 2048, 8 of 768: 30.5, 27.5, 30.8; steps of 4-bit weights are twice as
+  // long, and 4 columns 44.6 against 36.9 with 8).  Beyond 16 tokens 32 columns, whose steps are shared (T = 64, D =
+  // 2048, 64 of 1032: 196 against 203; with 16 tokens 36.2 against 32.7).
+  const int C = a.T > 16 ? 32 : a.D >= 4096 ? 16 : !W4 && a.D < 2048 ? 4 : 8;
+  const int step = (C < 16 ? 16 / C : 1) * Stretch<W4>::kStep;
+  a.ldh = (a.I + step - 1) / step * step;
+  const unsigned most = (unsigned)candidates(a.T, a.E, a.k);
+  if (a.T <= kFused && a.E <= 64 * kFusedKeys && most * (unsigned)(a.I / 8) <= kFusedGroups) {
+    decode_gateup_kernel<W4, 1, 1><<<dim3((unsigned)(a.I / 8), most + 1), 256, 0, s>>>(a);
+  } else {
+    if (a.E <= 256) decode_select_kernel<4><<<a.T, 64, 0, s>>>(a);
+    else decode_select_kernel<16><<<a.T, 64, 0, s>>>(a);
+    const dim3 grid((unsigned)((a.I + 15) / 16), most);
+    if (a.T <= 16) decode_gateup_kernel<W4, 1, 2><<<grid, 256, 0, s>>>(a);
+    else decode_gateup_kernel<W4, 4, 2><<<grid, 256, 0, s>>>(a);
+  }
+  if (C == 32) launch_down<W4, 16, 2>(a, down_shares(a.T, a.D), s);
+  else if (C == 16) launch_down<W4, 16, 1>(a, 1, s);
+  else if (C == 8) launch_down<W4, 8, 1>(a, 1, s);
+  else launch_down<W4, 4, 1>(a, 1, s);
 }
 
 }  // namespace sfp8
@@ -558,8 +836,8 @@ using namespace sfp8;
 
 extern "C" {
 
-int64_t sfp8_moe_decode_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t I) {
-  return decode_sizes_ok(T, E, top_k, 8, I) ? DecodeSpace(T, E, top_k, I).all : -1;
+int64_t sfp8_moe_decode_workspace_bytes(int64_t T, int64_t E, int64_t top_k, int64_t D, int64_t I) {
+  return decode_sizes_ok(T, E, top_k, D, I) ? DecodeSpace(T, E, top_k, D, I).all : -1;
 }
 
 int sfp8_moe_decode(const void* x, int64_t ldx, int64_t T, int64_t D, const void* router, int router_type, int64_t E,
@@ -578,25 +856,22 @@ int sfp8_moe_decode(const void* x, int64_t ldx, int64_t T, int64_t D, const void
   if (off(x, 2) || off(router, router_type == kMxF32 ? 4 : 2) || off(gate_up, 16) || off(down, 16) ||
       off(gate_up_scales, 4) || off(down_scales, 4) || off(out, 16) || off(ws, 16) || off(selected, 8) || off(bias, 4))
     return kErrBadAlignment;
-  const DecodeSpace at(T, E, top_k, I);
+  const DecodeSpace at(T, E, top_k, D, I);
   if (ws_bytes < at.all) return kErrWorkspaceTooSmall;
   uint8_t* w = reinterpret_cast<uint8_t*>(ws);
   const DecodeArgs a{(const uint16_t*)x, ldx, (int)T, (int)E, (int)top_k, (int)D, (int)I, router,
                      (int)(router_type == kMxF32), (const uint8_t*)gate_up, (const uint8_t*)gate_up_scales,
                      (const uint8_t*)down, (const uint8_t*)down_scales, bias, (const uint8_t*)mask, score, (int)groups,
                      (int)top_groups, (int)group_best, renorm, scale, selected, (uint16_t*)out, (double*)(w + at.low),
-                     (float*)(w + at.weights), (int*)(w + at.plan), (uint16_t*)(w + at.h)};
+                     (float*)(w + at.weights), (int*)(w + at.plan), (uint16_t*)(w + at.h), 0, (float*)(w + at.partial), (int*)(w + at.done),
+                     down_shares(T, D) > 1 ? (int)((D + 31) / 32) : 0};
   const hipStream_t s = (hipStream_t)stream;
-  decode_logits_kernel<<<dim3((unsigned)E, (unsigned)((T + kLogitTokens - 1) / kLogitTokens)), 256, 0, s>>>(a);
-  // a wave a token, as many as 48 KiB of keys hold
-  int waves = T < 16 ? (int)T : 16;
-  if (waves > 6144 / E) waves = (int)(6144 / E);
-  decode_select_kernel<<<1, 64 * waves, (size_t)waves * E * 8, s>>>(a);
+  if (T == 1) decode_logits_kernel<1><<<dim3((unsigned)E, 1), 256, 0, s>>>(a);
+  else decode_logits_kernel<4><<<dim3((unsigned)E, (unsigned)((T + 3) / 4)), 256, 0, s>>>(a);
+  if (gate_up_scales) launch_experts<true>(a, s);
+  else launch_experts<false>(a, s);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return (int)e;
-  const bool one = T <= 16;
-  if (gate_up_scales) return one ? launch_experts<true, 1>(a, s) : launch_experts<true, 4>(a, s);
-  return one ? launch_experts<false, 1>(a, s) : launch_experts<false, 4>(a, s);
+  return e == hipSuccess ? kOk : (int)e;
 }
 
 }  // extern "C"

@@ -886,8 +886,8 @@ std::tuple<Tensor, Tensor> moe_decode(const Tensor& x_, const Tensor& router, co
   const int64_t E = router.size(0);
   need(router.size(1) == D, "router must be [experts, columns of x]");
   need(E >= 1 && E <= 1024, "1 .. 1024 experts");
-  if (D < 8 || D % 8 || I < 8 || I % 8 || D > 1 << 20 || I > 1 << 20)
-    refuse("the widths must be multiples of 8 and at most 2^20, got " + std::to_string(D) + " and " +
+  if (D < 8 || D % 8 || I < 8 || I % 8 || D > 1 << 20 || I > 1 << 20 || D * I > (int64_t)1 << 29)
+    refuse("the widths must be multiples of 8, at most 2^20 and 2^29 in product, got " + std::to_string(D) + " and " +
            std::to_string(I));
   need(gu_scales.has_value() == down_scales.has_value(), "both weights bf16 or both MXFP4");
   if (gu_scales) {
@@ -921,7 +921,7 @@ std::tuple<Tensor, Tensor> moe_decode(const Tensor& x_, const Tensor& router, co
   const c10::DeviceGuard guard(x_.device());
   const Tensor x = x_.stride(1) == 1 ? x_ : x_.contiguous();
   Tensor out = empty({T, D}, kBF16, x), selected = empty({T, top_k}, kI64, x);
-  const int64_t n = sfp8_moe_decode_workspace_bytes(T, E, top_k, I);
+  const int64_t n = sfp8_moe_decode_workspace_bytes(T, E, top_k, D, I);
   Tensor ws = empty({n > 1 ? n : 1}, kU8, x);
   CALL(sfp8_moe_decode, ptr(x), x.stride(0), T, D, ptr(router), wide ? 0 : 1, E, ptr(w_gu), ptr(gu_scales),
        ptr(w_down), ptr(down_scales), I, fptr(bias), ptr(mask), sc, groups, top_groups, group_best, top_k,

@@ -10,12 +10,15 @@ from spark_gpt_amd import _lib
 
 def test_workspace_sizes():
     q = lambda *a: _lib.query("sfp8_moe_decode_workspace_bytes", *a)
-    # logits [T, E] in 64 bits, weights [T, k], the plan, h in two parts; each from a 256-byte boundary
-    assert q(4, 128, 8, 768) == 4096 + 256 + 512 + 32 * 2 * 768 * 2
-    assert q(64, 8, 2, 16) == 4096 + 512 + 768 + 128 * 2 * 16 * 2
-    assert q(0, 8, 2, 16) >= 0
-    for bad in ((65, 8, 2, 16), (-1, 8, 2, 16), (4, 0, 1, 16), (4, 1025, 2, 16), (4, 8, 0, 16), (4, 8, 9, 16),
-                (4, 100, 65, 16), (4, 8, 2, 12), (4, 8, 2, 0), (4, 8, 2, (1 << 20) + 8)):
+    # logits [T, E] in 64 bits, weights [T, k], the plan, beyond 16 tokens a counter for each 32 columns and sums in 32
+    # bits for each share of the work, h in two parts of whole 512s; each from a 256-byte boundary
+    assert q(4, 128, 8, 2048, 768) == 4096 + 256 + 8448 + 32 * 2 * 1024 * 2
+    assert q(64, 8, 2, 1024, 16) == 4096 + 512 + 2304 + 256 + 8 * 64 * 1024 * 4 + 128 * 2 * 512 * 2
+    assert q(64, 8, 2, 8192, 16) == 4096 + 512 + 2304 + 128 * 2 * 512 * 2  # 256 column blocks: no sharing
+    assert q(0, 8, 2, 64, 16) >= 0
+    for bad in ((65, 8, 2, 64, 16), (-1, 8, 2, 64, 16), (4, 0, 1, 64, 16), (4, 1025, 2, 64, 16), (4, 8, 0, 64, 16),
+                (4, 8, 9, 64, 16), (4, 100, 65, 64, 16), (4, 8, 2, 64, 12), (4, 8, 2, 64, 0), (4, 8, 2, 60, 16),
+                (4, 8, 2, 8, (1 << 20) + 8), (4, 8, 2, 1 << 16, 1 << 14)):
         assert q(*bad) == -1, bad
 
 
@@ -32,7 +35,8 @@ def test_c_abi_refuses_before_launch():
     for bad in (dict(T=65), dict(T=-1), dict(D=60), dict(D=0), dict(I=12), dict(I=0), dict(E=0), dict(E=1025), dict(k=0),
                 dict(k=9), dict(rt=2), dict(rt=-1), dict(ldx=-1), dict(score=2), dict(groups=3), dict(groups=0),
                 dict(groups=4, top_groups=5), dict(groups=4, top_groups=0), dict(groups=4, top_groups=1, k=3),
-                dict(best=0), dict(gs=16), dict(ds=16), dict(E=65, groups=65)):
+                dict(best=0), dict(gs=16), dict(ds=16), dict(E=65, groups=65),
+                dict(D=1 << 16, I=1 << 14)):
         assert call(**bad) == -2, bad
     for bad in (dict(x=17), dict(router=17), dict(rt=0, router=18), dict(gu=8), dict(down=24), dict(gs=18, ds=16),
                 dict(out=8), dict(ws=8), dict(sel=4), dict(bias=18)):

@@ -67,7 +67,7 @@ def _check(x, router, w_gu, w_down, k, values=None, **kw):
 
 SIZES = [(1, 1, 1, 8, 8), (1, 8, 2, 64, 24), (2, 4, 4, 40, 16), (1, 128, 8, 512, 96), (3, 16, 3, 264, 72),
          (16, 8, 2, 128, 200), (17, 8, 2, 128, 64), (33, 60, 4, 96, 136), (64, 64, 6, 256, 88), (64, 4, 1, 72, 40),
-         (64, 2, 2, 200, 64), (5, 300, 10, 64, 32), (2, 1024, 64, 64, 16), (64, 70, 64, 32, 8), (8, 8, 2, 1024, 1536)]
+         (64, 2, 2, 200, 64), (20, 8, 2, 4096, 40), (10, 8, 2, 4104, 16), (40, 3, 2, 8200, 8), (5, 300, 10, 64, 32), (2, 1024, 64, 64, 16), (64, 70, 64, 32, 8), (8, 8, 2, 1024, 1536)]
 
 
 @pytest.mark.parametrize("four", [False, True])
