@@ -27,33 +27,36 @@ struct MxQuantArgs {
   uint8_t *codes_t, *scales_t;     // of its transpose, or NULL
 };
 
-// One work-group takes 128 x 128 values.  Sixteen lanes hold 128 values of a
+// One work-group takes 16 ITER x 128 values.  Sixteen lanes hold 128 values of a
 // row (four lanes a block: its maximum is two lane exchanges away), so the row
 // codes leave straight from the registers, four rows of 64 bytes in one run.
 // For the columns the values pass through LDS as they are: a lane then holds
 // 32 values of one column (16-bit types: of two), so neither its maximum nor
 // its codes need another lane; the codes go back through LDS so that each
 // column's 64 bytes and the tile's 8 KiB are written in one run.
-template <int DT, bool ROWS, bool COLS>
+// ITER = 8 where there are columns; along rows alone 2 where a taller tile would
+// leave CUs without one.
+template <int DT, bool ROWS, bool COLS, int ITER>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
+  static_assert(ITER == 8 || !COLS, "a slab of the transpose");
   constexpr int kSize = DT == kMxF32 ? 4 : 2;
   __shared__ __align__(16) uint8_t raw[COLS ? 128 * 128 * kSize : 16];
   __shared__ __align__(16) uint8_t out[COLS ? 128 * 64 : 16];
   __shared__ __align__(16) uint8_t out_scale[COLS ? 512 : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t nx = mx_slabs(a.C), ny = (a.R + 127) / 128;
+  const int64_t nx = mx_slabs(a.C), ny = (a.R + 16 * ITER - 1) / (16 * ITER);
   const int64_t id = blockIdx.x, cs = id % nx, rs = id / nx % ny, z = id / nx / ny;
-  const int64_t c0 = cs * 128, r0 = rs * 128, rows = mx_rows(a.R), cols = mx_rows(a.C);
+  const int64_t c0 = cs * 128, r0 = rs * (16 * ITER), rows = mx_rows(a.R), cols = mx_rows(a.C);
   const uint8_t* x = reinterpret_cast<const uint8_t*>(a.x) + z * a.batch_stride * kSize;
   const int col = 8 * (lane & 15), sub = 4 * wave + (lane >> 4);
 
-  Eight<DT> v[8];
-  if (c0 + 128 <= a.C && r0 + 128 <= a.R) {
+  Eight<DT> v[ITER];
+  if (c0 + 128 <= a.C && r0 + 16 * ITER <= a.R) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = load8<DT>(x, (r0 + 16 * i + sub) * a.ld + c0 + col);
+    for (int i = 0; i < ITER; ++i) v[i] = load8<DT>(x, (r0 + 16 * i + sub) * a.ld + c0 + col);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < ITER; ++i) {
       const int64_t r = r0 + 16 * i + sub;
       v[i] = Eight<DT>{};
       if (r < a.R && c0 + col < a.C) v[i] = load8_upto<DT>(x, r * a.ld + c0 + col, a.C - c0 - col);
@@ -63,7 +66,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
     uint8_t* codes = a.codes + (z * nx + cs) * rows * 64;
     uint8_t* scales = a.scales + (z * nx + cs) * rows * 4;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < ITER; ++i) {
       uint32_t m = abs_max8<DT>(v[i]);
       m = max_u(m, dpp<0xB1>(m));
       m = max_u(m, dpp<0x4E>(m));
@@ -140,11 +143,22 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
   }
 }
 
+// Work-groups for tiles of 128 rows and, where those would not be two for each
+// CU, of 32 (rows of 5003 x 1001: 4.2 us against 5.2; of 65536 x 1024 27.9 against
+// 26.1).
+struct MxGrid {
+  unsigned tall, low;
+  MxGrid(int64_t batch, int64_t R, int64_t C)
+      : tall((unsigned)(batch * mx_slabs(C) * ((R + 127) / 128))),
+        low(tall >= 512 ? 0 : (unsigned)(batch * mx_slabs(C) * ((R + 31) / 32))) {}
+};
+
 template <int DT>
-void launch_quantize(const MxQuantArgs& a, unsigned grid, hipStream_t stream) {
-  if (a.codes && a.codes_t) mx_quantize_kernel<DT, true, true><<<grid, 256, 0, stream>>>(a);
-  else if (a.codes) mx_quantize_kernel<DT, true, false><<<grid, 256, 0, stream>>>(a);
-  else mx_quantize_kernel<DT, false, true><<<grid, 256, 0, stream>>>(a);
+void launch_quantize(const MxQuantArgs& a, const MxGrid& grid, hipStream_t stream) {
+  if (a.codes && a.codes_t) mx_quantize_kernel<DT, true, true, 8><<<grid.tall, 256, 0, stream>>>(a);
+  else if (a.codes_t) mx_quantize_kernel<DT, false, true, 8><<<grid.tall, 256, 0, stream>>>(a);
+  else if (grid.low) mx_quantize_kernel<DT, true, false, 2><<<grid.low, 256, 0, stream>>>(a);
+  else mx_quantize_kernel<DT, true, false, 8><<<grid.tall, 256, 0, stream>>>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -156,26 +170,26 @@ struct MxDequantArgs {
   void* out;  // [R, C]
 };
 
-template <int DT>
+template <int DT, int ITER>
 __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantArgs a) {
   constexpr int kSize = DT == kMxF32 ? 4 : 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t nx = mx_slabs(a.C), ny = (a.R + 127) / 128;
+  const int64_t nx = mx_slabs(a.C), ny = (a.R + 16 * ITER - 1) / (16 * ITER);
   const int64_t id = blockIdx.x, cs = id % nx, rs = id / nx % ny, z = id / nx / ny;
-  const int64_t rows = mx_rows(a.R), c = cs * 128 + 8 * (lane & 15), r0 = rs * 128 + 4 * wave + (lane >> 4);
+  const int64_t rows = mx_rows(a.R), c = cs * 128 + 8 * (lane & 15), r0 = rs * (16 * ITER) + 4 * wave + (lane >> 4);
   const uint8_t* codes = a.codes + (z * nx + cs) * rows * 64;
   const uint8_t* scales = a.scales + (z * nx + cs) * rows * 4;
   uint8_t* out = reinterpret_cast<uint8_t*>(a.out) + z * a.R * a.C * kSize;
   if (c >= a.C) return;
-  uint32_t q[8], e[8];
+  uint32_t q[ITER], e[ITER];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < ITER; ++i) {
     const int64_t r = r0 + 16 * i, rr = r < a.R ? r : 0;
     q[i] = *reinterpret_cast<const uint32_t*>(codes + rr * 64 + 4 * (lane & 15));
     e[i] = scales[rr * 4 + ((lane >> 2) & 3)];
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < ITER; ++i) {
     const int64_t r = r0 + 16 * i;
     if (r >= a.R) break;
     const float s = mx_scale_value(e[i]);
@@ -217,6 +231,12 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(MxDequantArgs a) {
       }
     }
   }
+}
+
+template <int DT>
+void launch_dequantize(const MxDequantArgs& a, const MxGrid& grid, hipStream_t s) {
+  if (grid.low) mx_dequantize_kernel<DT, 2><<<grid.low, 256, 0, s>>>(a);
+  else mx_dequantize_kernel<DT, 8><<<grid.tall, 256, 0, s>>>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -700,7 +720,7 @@ int sfp8_mxfp4_quantize(const void* x, int dtype, int64_t batch, int64_t R, int6
   if (tiles > kMxMaxTiles / batch) return kErrBadShape;
   const MxQuantArgs a{x, R, C, ld, batch_stride, (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)codes_t,
                       (uint8_t*)scales_t};
-  const unsigned grid = (unsigned)(tiles * batch);
+  const MxGrid grid(batch, R, C);
   const hipStream_t s = (hipStream_t)stream;
   if (dtype == kMxF32) launch_quantize<kMxF32>(a, grid, s);
   else if (dtype == kMxBf16) launch_quantize<kMxBf16>(a, grid, s);
@@ -717,11 +737,11 @@ int sfp8_mxfp4_dequantize(const void* codes, const void* scales, int64_t batch, 
   const int64_t tiles = mx_slabs(C) * ((R + 127) / 128);
   if (tiles > kMxMaxTiles / batch) return kErrBadShape;
   const MxDequantArgs a{(const uint8_t*)codes, (const uint8_t*)scales, R, C, out};
-  const unsigned grid = (unsigned)(tiles * batch);
+  const MxGrid grid(batch, R, C);
   const hipStream_t s = (hipStream_t)stream;
-  if (dtype == kMxF32) mx_dequantize_kernel<kMxF32><<<grid, 256, 0, s>>>(a);
-  else if (dtype == kMxBf16) mx_dequantize_kernel<kMxBf16><<<grid, 256, 0, s>>>(a);
-  else mx_dequantize_kernel<kMxF16><<<grid, 256, 0, s>>>(a);
+  if (dtype == kMxF32) launch_dequantize<kMxF32>(a, grid, s);
+  else if (dtype == kMxBf16) launch_dequantize<kMxBf16>(a, grid, s);
+  else launch_dequantize<kMxF16>(a, grid, s);
   return launched();
 }
 
@@ -738,14 +758,14 @@ int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const vo
   const hipStream_t st = (hipStream_t)stream;
   // By the number of tiles (us; M, N, K):
   //  256 x 256 where they fill the CUs and K is long: its loop fetches half of what that of 128 x 128 does for a
-  //  product, which hides its stores behind a second work-group: 16384, 8192, 4096 281 against 362; 4096, 4096, 4096
-  //  40.5 against 43.6; but 16384, 4096, 2048 96.5 against 88.8 and 65536, 1024, 1024 72.0 against 55.5.
+  //  product, which hides its stores behind a second work-group: 16384, 8192, 4096 281 against 362; 4096, 4096, 2560
+  //  26.3 against 28.3; but 16384, 4096, 2048 96.5 against 88.8 and 65536, 1024, 1024 72.0 against 55.5.
   //  128 x 128 from half a tile a CU on (1003, 2050, 1000 6.1 against 10.6; 512, 4096, 4096 11.1 against 13.2);
   //  below that the waves share K (1024, 1024, 4096 9.3 against 10.6), in the largest tile of which there are 256:
   //  64, 4096, 4096 32 x 32 4.7, 16 x 16 6.7, 64 x 64 8.5; 128, 1024, 8192 16 x 32 5.4, 64 x 64 12.4.
   const auto tiles = [&](int64_t m, int64_t n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
   if (tiles(128, 128) > kMxMaxTiles) return kErrBadShape;
-  if (tiles(256, 256) >= 256 && K >= 4096) launch_tiles<256>(g, tiles(256, 256), st);
+  if (tiles(256, 256) >= 256 && K >= 2560) launch_tiles<256>(g, tiles(256, 256), st);
   else if (tiles(128, 128) >= 128) launch_tiles<128>(g, tiles(128, 128), st);
   else if (tiles(64, 64) >= 256) launch_few<4, 4, 4, -1>(g, st);
   else if (M > 32 && tiles(64, 32) >= 256) launch_few<4, 2, 8, -1>(g, st);

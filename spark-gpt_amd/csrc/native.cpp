@@ -822,38 +822,66 @@ Tensor mxfp4_rows_matmul(const Tensor& x_, const Tensor& b, const Tensor& b_scal
   return out;
 }
 
+// Codes and scales in one buffer: half the allocations of a step that is bound by host time.
+struct Packed {
+  Tensor buf;
+  int64_t codes_bytes;
+  uint8_t* codes() const { return static_cast<uint8_t*>(buf.data_ptr()); }
+  uint8_t* scales() const { return codes() + codes_bytes; }
+};
+Packed packed(int64_t R, int64_t C, const Tensor& like) {
+  const int64_t n = mx_slabs(C) * mx_rows(R) * 64;
+  return {empty({n / 16 * 17}, kU8, like), n};
+}
+Packed packed(const Tensor& buf) { return {buf, buf.numel() / 17 * 16}; }
+
+// x along its rows and along its columns, where asked for.
+std::pair<Packed, Packed> packed_quantize(const Tensor& x_, bool rows, bool columns) {
+  const Tensor x = x_.size(1) <= 1 || x_.stride(1) == 1 ? x_ : x_.contiguous();
+  const int64_t R = x.size(0), C = x.size(1);
+  Packed r{}, c{};
+  if (rows) r = packed(R, C, x);
+  if (columns) c = packed(C, R, x);
+  CALL(sfp8_mxfp4_quantize, ptr(x), dtype_code(x.scalar_type()), 1, R, C, x.stride(0), 0, rows ? r.codes() : nullptr,
+       rows ? r.scales() : nullptr, columns ? c.codes() : nullptr, columns ? c.scales() : nullptr, stream_of(x));
+  return {r, c};
+}
+Tensor packed_product(const Packed& a, const Packed& b, int64_t M, int64_t N, int64_t K, ScalarType type) {
+  Tensor out = empty({M, N}, type, a.buf);
+  CALL(sfp8_mxfp4_gemm, a.codes(), a.scales(), b.codes(), b.scales(), M, N, K, ptr(out), dtype_code(type),
+       stream_of(a.buf));
+  return out;
+}
+
 // The eager node of mxfp4.py's linear layer: what _MXFP4Linear does there (a
 // training pass of 2003 x 1000 x 1030, bound by host time: 126 us with the
 // Python node).  Kept for the backward pass are codes alone, those of x along
 // the tokens and of w along its rows.
 struct Mxfp4Linear : torch::autograd::Function<Mxfp4Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, bool need_x, bool need_w) {
-    const auto [xr, xrs, xc, xcs] = mxfp4_quantize(x, true, need_w);
-    const auto [wr, wrs, wc, wcs] = mxfp4_quantize(w, true, need_x);
+    const c10::DeviceGuard guard(x.device());
+    const auto [xr, xc] = packed_quantize(x, true, need_w);
+    const auto [wr, wc] = packed_quantize(w, true, need_x);
     variable_list kept;
-    if (need_w) kept.insert(kept.end(), {*xc, *xcs});
-    if (need_x) kept.insert(kept.end(), {*wc, *wcs});
-    ctx->save_for_backward(kept);
-    ctx->saved_data["T"] = x.size(0);
-    ctx->saved_data["K"] = x.size(1);
-    ctx->saved_data["N"] = w.size(0);
-    ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
-    ctx->saved_data["w_type"] = (int64_t)w.scalar_type();
-    return mx_product(*xr, *xrs, *wr, *wrs, x.size(0), w.size(0), x.size(1), x.scalar_type());
+    if (need_w) kept.push_back(xc.buf);
+    if (need_x) kept.push_back(wc.buf);
+    ctx->save_for_backward(std::move(kept));
+    ctx->saved_data["size"] = std::vector<int64_t>{x.size(0), x.size(1), w.size(0), (int64_t)x.scalar_type(),
+                                                   (int64_t)w.scalar_type()};
+    return packed_product(xr, wr, x.size(0), w.size(0), x.size(1), x.scalar_type());
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     const variable_list kept = ctx->get_saved_variables();
-    const int64_t T = ctx->saved_data["T"].toInt(), K = ctx->saved_data["K"].toInt(), N = ctx->saved_data["N"].toInt();
+    const std::vector<int64_t> size = ctx->saved_data["size"].toIntVector();
+    const int64_t T = size[0], K = size[1], N = size[2];
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     variable_list out(4);
     {
       const c10::AutoGradMode off(false);
-      const auto [dr, drs, dc, dcs] = mxfp4_quantize(grads[0], need_x, need_w);
-      if (need_x)
-        out[0] = mx_product(*dr, *drs, kept[kept.size() - 2], kept[kept.size() - 1], T, K, N,
-                            (ScalarType)ctx->saved_data["x_type"].toInt());
-      if (need_w)
-        out[1] = mx_product(*dc, *dcs, kept[0], kept[1], N, K, T, (ScalarType)ctx->saved_data["w_type"].toInt());
+      const c10::DeviceGuard guard(grads[0].device());
+      const auto [dr, dc] = packed_quantize(grads[0], need_x, need_w);
+      if (need_x) out[0] = packed_product(dr, packed(kept.back()), T, K, N, (ScalarType)size[3]);
+      if (need_w) out[1] = packed_product(dc, packed(kept.front()), N, K, T, (ScalarType)size[4]);
     }
     return once(std::move(out), grads, "mxfp4_linear");
   }
@@ -866,6 +894,7 @@ Tensor mxfp4_linear(const Tensor& x, const Tensor& w) {
   if (x.dim() != 2 || w.dim() != 2 || x.size(1) != w.size(1))
     refuse("x must be [T, K] and w [N, K], got " + shape_of(x) + " and " + shape_of(w));
   same_device("w", w, x);
+  need(x.size(0) <= kMxDim && x.size(1) <= kMxDim && w.size(0) <= kMxDim, "dimensions must be at most 2^31");
   return Mxfp4Linear::apply(x, w, x.requires_grad(), w.requires_grad());
 }
 
