@@ -7,6 +7,8 @@
 //  * mx_gemm: C = A B^T over the values, v_mfma_scale_f32_*_f8f6f4 with fp4
 //    operands (the matrix cores multiply by the two blocks' scales), sums in
 //    fp32, one rounding at the end.
+#include <type_traits>
+
 #include "mx4.h"
 
 namespace sfp8 {
@@ -299,52 +301,73 @@ __global__ __launch_bounds__(64 * WV) void mx_few_kernel(MxGemmArgs g) {
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int64_t s = wave; s < S; s += WV) {
-    intx4 bv[NB], av[MB];
-    int bsc[NB], asc[MB];
+  const auto batch = [&](auto size, int64_t s0) {  // slabs s0 and s0 + WV, or s0
+    constexpr int U = decltype(size)::value, DT = XT < 0 ? 0 : XT;
+    intx4 bv[U][NB], av[U][MB];
+    uint32_t bsc[U][NB], asc[U][MB];
+    Eight<DT> xv[U][MB][XT < 0 ? 1 : 4];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      bv[j] = *reinterpret_cast<const intx4*>(g.b + (s * np + brow[j]) * 64 + 16 * q);
-      bsc[j] = (int)(*reinterpret_cast<const uint32_t*>(g.bs + (s * np + brow[j]) * 4) >> (8 * q));
-    }
+    for (int u = 0; u < U; ++u) {
+      const int64_t s = s0 + u * WV;
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-      if constexpr (XT < 0) {
-        av[i] = *reinterpret_cast<const intx4*>(g.a + (s * mp + arow[i]) * 64 + 16 * q);
-        asc[i] = (int)(*reinterpret_cast<const uint32_t*>(g.as + (s * mp + arow[i]) * 4) >> (8 * q));
-      } else {
-        constexpr int DT = XT < 0 ? 0 : XT;
-        const int64_t k = s * 128 + 32 * q, left = arow[i] < g.M ? g.K - k : 0, at = arow[i] * g.ldx + k;
-        Eight<DT> v[4];
-        if (left >= 32) {
+      for (int j = 0; j < NB; ++j) {
+        bv[u][j] = *reinterpret_cast<const intx4*>(g.b + (s * np + brow[j]) * 64 + 16 * q);
+        bsc[u][j] = *reinterpret_cast<const uint32_t*>(g.bs + (s * np + brow[j]) * 4);
+      }
 #pragma unroll
-          for (int c = 0; c < 4; ++c) v[c] = load8<DT>(g.x, at + 8 * c);
+      for (int i = 0; i < MB; ++i) {
+        if constexpr (XT < 0) {
+          av[u][i] = *reinterpret_cast<const intx4*>(g.a + (s * mp + arow[i]) * 64 + 16 * q);
+          asc[u][i] = *reinterpret_cast<const uint32_t*>(g.as + (s * mp + arow[i]) * 4);
         } else {
+          const int64_t k = s * 128 + 32 * q, left = arow[i] < g.M ? g.K - k : 0, at = arow[i] * g.ldx + k;
+          if (left >= 32) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            v[c] = Eight<DT>{};
-            if (left > 8 * c) v[c] = load8_upto<DT>(g.x, at + 8 * c, left - 8 * c);
+            for (int c = 0; c < 4; ++c) xv[u][i][c] = load8<DT>(g.x, at + 8 * c);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              xv[u][i][c] = Eight<DT>{};
+              if (left > 8 * c) xv[u][i][c] = load8_upto<DT>(g.x, at + 8 * c, left - 8 * c);
+            }
           }
         }
-        uint32_t m = abs_max8<DT>(v[0]);
-#pragma unroll
-        for (int c = 1; c < 4; ++c) {
-          const uint32_t o = abs_max8<DT>(v[c]);
-          m = o > m ? o : m;
-        }
-        asc[i] = (int)mx_scale_code(abs_bits_to_f32<DT>(m));
-        const float sv = mx_scale_value((uint32_t)asc[i]);
-        av[i] = intx4{(int)codes8<DT>(v[0], sv), (int)codes8<DT>(v[1], sv), (int)codes8<DT>(v[2], sv),
-                      (int)codes8<DT>(v[3], sv)};
       }
     }
+    if constexpr (U > 1) __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead of the products
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(bv[j]), fp4_operand(av[i]), acc[i][j],
-                                                                     4, 4, 0, bsc[j], 0, asc[i]);
+      for (int i = 0; i < MB; ++i) {
+        if constexpr (XT >= 0) {
+          uint32_t m = abs_max8<DT>(xv[u][i][0]);
+#pragma unroll
+          for (int c = 1; c < 4; ++c) m = max_u(m, abs_max8<DT>(xv[u][i][c]));
+          asc[u][i] = mx_scale_code(abs_bits_to_f32<DT>(m)) << (8 * q);
+          const float sv = mx_scale_value(asc[u][i] >> (8 * q));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) av[u][i][c] = (int)codes8<DT>(xv[u][i][c], sv);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              fp4_operand(bv[u][j]), fp4_operand(av[u][i]), acc[i][j], 4, 4, 0, (int)(bsc[u][j] >> (8 * q)), 0,
+              (int)(asc[u][i] >> (8 * q)));
+    }
+  };
+  // Two slabs at once pay with many operands a slab, whose loads the compiler otherwise spreads over the products
+  // (1024 x 1024 x 4096 9.4 -> 8.1 us); the small variants lose by it (8 x 8192 x 2048 from bf16 rows 5.4 against 5.7).
+  const int64_t n = (S - wave + WV - 1) / WV;  // this wave's slabs
+  int64_t i = 0;
+  if constexpr (MB * NB >= 8) {
+    for (; i + 2 <= n; i += 2) batch(std::integral_constant<int, 2>{}, wave + i * WV);
+    for (; i < n; ++i) batch(std::integral_constant<int, 1>{}, wave + i * WV);
+  } else {
+#pragma unroll 2
+    for (; i < n; ++i) batch(std::integral_constant<int, 1>{}, wave + i * WV);
   }
 #pragma unroll
   for (int i = 0; i < MB; ++i)
