@@ -12,8 +12,9 @@
 // Weights are bf16, or MXFP4 codes (mx4.h) that become bf16 values in
 // registers, which hold them exactly; x stays bf16 in both.
 // Four launches: logits; the selection, a wave a token; gate and up, whose
-// work-groups find their expert's slots among all; down and the sum.  For up to
-// kFused tokens the selection is part of gate and up: three.
+// work-groups find their expert's slots among all; down and the sum.  Three where
+// the router is small (logits and selection in one) and for up to kFused tokens
+// (the selection is part of gate and up).
 #include <type_traits>
 
 #include "mx4.h"
@@ -73,6 +74,25 @@ SFP8_DEV double bf16_at(const Eight<kMxBf16>& v, int j) {
   return (double)__uint_as_float(j & 1 ? v.w[j / 2] & 0xffff0000u : v.w[j / 2] << 16);
 }
 
+// N sums over the 64 lanes: a lane hands half of its sums to the lane o away and
+// keeps the other half's, then adds over the lanes that hold the same one.  Sum
+// n is in the lanes of 64 / N from n on (N = 4: lanes 16 n ..).
+template <int N>
+SFP8_DEV double lane_sums(double (&v)[N]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int h = N / 2, o = 32; h > 0; h >>= 1, o >>= 1) {
+#pragma unroll
+    for (int j = 0; j < h; ++j) {
+      const double keep = lane & o ? v[j + h] : v[j], give = lane & o ? v[j] : v[j + h];
+      v[j] = keep + __shfl_xor(give, o, 64);
+    }
+  }
+#pragma unroll
+  for (int o = 32 / N; o > 0; o >>= 1) v[0] += __shfl_xor(v[0], o, 64);
+  return v[0];
+}
+
 template <int TOK>
 __global__ __launch_bounds__(256) void decode_logits_kernel(DecodeArgs a) {
   __shared__ double part[4][TOK];
@@ -102,19 +122,8 @@ __global__ __launch_bounds__(256) void decode_logits_kernel(DecodeArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[t] = fma(bf16_at(x[t], j), w[j], acc[t]);
   }
-  // TOK sums over 64 lanes: a lane hands half of its sums to the lane o away and keeps the other half's
-#pragma unroll
-  for (int h = TOK / 2, o = 32; h > 0; h >>= 1, o >>= 1) {
-#pragma unroll
-    for (int j = 0; j < h; ++j) {
-      const double keep = lane & o ? acc[j + h] : acc[j], give = lane & o ? acc[j] : acc[j + h];
-      acc[j] = keep + __shfl_xor(give, o, 64);
-    }
-  }
-#pragma unroll
-  for (int o = 32 / TOK; o > 0; o >>= 1) acc[0] += __shfl_xor(acc[0], o, 64);
-  static_assert(TOK == 1 || TOK == 4, "the lanes that hold token t");
-  if (lane % (64 / TOK) == 0) part[wave][TOK == 4 ? 2 * (lane >> 5) + (lane >> 4 & 1) : 0] = acc[0];
+  acc[0] = lane_sums<TOK>(acc);
+  if (lane % (64 / TOK) == 0) part[wave][lane / (64 / TOK)] = acc[0];
   __syncthreads();
   if ((int)threadIdx.x < n)
     a.low[(int64_t)(t0 + threadIdx.x) * a.E + e] =
@@ -170,10 +179,10 @@ struct Choice {
 };
 
 template <int P>
-SFP8_DEV Choice choose(const DecodeArgs& a, int t, Scores& s, uint64_t* shared) {
+SFP8_DEV Choice choose(const DecodeArgs& a, int t, const double* low, Scores& s, uint64_t* shared) {
   const int lane = threadIdx.x & 63, E = a.E;
   Choice mine{-1, 0.0};
-  s = Scores{a.low + (int64_t)t * E, a.score, 0.0, 1.0};
+  s = Scores{low, a.score, 0.0, 1.0};
   if (a.mask && !a.mask[t]) return mine;
   double l[P];
 #pragma unroll
@@ -230,10 +239,10 @@ SFP8_DEV Choice choose(const DecodeArgs& a, int t, Scores& s, uint64_t* shared) 
   for (int j = 0; j < a.k; ++j) {
     uint64_t best = key[0];
     int at = lane;
-    double low = l[0];
+    double logit = l[0];
 #pragma unroll
     for (int i = 1; i < P; ++i)
-      if (key[i] > best) best = key[i], at = lane + 64 * i, low = l[i];
+      if (key[i] > best) best = key[i], at = lane + 64 * i, logit = l[i];
     const uint32_t hi = wave_max_u((uint32_t)(best >> 32));
     bool in = (uint32_t)(best >> 32) == hi;
     uint64_t who = __ballot(in);
@@ -249,7 +258,7 @@ SFP8_DEV Choice choose(const DecodeArgs& a, int t, Scores& s, uint64_t* shared) 
     const int win = __builtin_ctzll(who);
     if (hi == 0 && __builtin_amdgcn_readlane((int)(uint32_t)best, win) == 0) break;  // nobody is left
     const int e = __builtin_amdgcn_readlane(at, win);
-    const uint64_t bits = (uint64_t)__double_as_longlong(low);
+    const uint64_t bits = (uint64_t)__double_as_longlong(logit);
     const uint32_t b0 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, win);
     const uint32_t b1 = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), win);
     if (lane == j) mine = Choice{e, __longlong_as_double((long long)((uint64_t)b1 << 32 | b0))};
@@ -293,8 +302,60 @@ template <int P>
 __global__ __launch_bounds__(64) void decode_select_kernel(DecodeArgs a) {
   __shared__ uint64_t shared[64 * P];
   Scores s;
-  const Choice c = choose<P>(a, blockIdx.x, s, shared);
+  const Choice c = choose<P>(a, blockIdx.x, a.low + (int64_t)blockIdx.x * a.E, s, shared);
   write_choice(a, blockIdx.x, s, c);
+}
+
+// A small router: a work-group a token has all logits and the selection.  A wave
+// takes four experts at a time; where there are fewer than four for each of the
+// eight waves, several share the width.  A layer of 16 tokens and 8 experts of
+// width 1024 takes 31.0 us with it and 32.7 with two kernels; with 16 experts as
+// long, and with 64 of 512 26.0 against 24.2: one CU reads slowly.
+constexpr int kSmallRouter = 8192, kSmallExperts = 64;
+
+__global__ __launch_bounds__(512) void decode_router_kernel(DecodeArgs a) {
+  constexpr int W = 8;
+  __shared__ double part[4 * W], low[kSmallExperts];
+  __shared__ uint64_t shared[kSmallExperts];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = blockIdx.x;
+  if (t == 0)
+    for (int i = threadIdx.x; i < a.done_count; i += 64 * W) a.done[i] = 0;
+  const int sets = (a.E + 3) / 4, parts = sets >= W ? 1 : W / sets;
+  for (int u = wave; u < sets * parts; u += W) {
+    const int e0 = 4 * (u / parts), p = u % parts;
+    double acc[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int d = 8 * (64 * p + lane); d < a.D; d += 512 * parts) {
+      const Eight<kMxBf16> x = load8<kMxBf16>(a.x, t * a.ldx + d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t at = (int64_t)min(e0 + i, a.E - 1) * a.D + d;
+        if (a.router_f32) {
+          const Eight<kMxF32> w = load8<kMxF32>(a.router, at);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[i] = fma(bf16_at(x, j), (double)__uint_as_float(w.w[j]), acc[i]);
+        } else {
+          const Eight<kMxBf16> w = load8<kMxBf16>(a.router, at);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[i] = fma(bf16_at(x, j), bf16_at(w, j), acc[i]);
+        }
+      }
+    }
+    const double sum = lane_sums<4>(acc);
+    if (lane % 16 == 0 && e0 + lane / 16 < a.E) (parts == 1 ? low[e0 + lane / 16] : part[4 * u + lane / 16]) = sum;
+  }
+  __syncthreads();
+  if (parts > 1) {
+    for (int e = threadIdx.x; e < a.E; e += 64 * W) {
+      double sum = 0.0;
+      for (int p = 0; p < parts; ++p) sum += part[4 * (e / 4 * parts + p) + e % 4];
+      low[e] = sum;
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+  Scores s;
+  const Choice c = choose<1>(a, t, low, s, shared);
+  write_choice(a, t, s, c);
 }
 
 // ---------------------------------------------------------------------------
@@ -443,7 +504,7 @@ __global__ __launch_bounds__(256, W4 && NB > 1 ? 3 : 4) void decode_gateup_kerne
     if (c == most && blockIdx.x) return;  // one work-group more writes the selection and the weights
     if (wave < a.T) {
       Scores s;
-      const Choice x = choose<kFusedKeys>(a, wave, s, keys + wave * 64 * kFusedKeys);
+      const Choice x = choose<kFusedKeys>(a, wave, a.low + (int64_t)wave * a.E, s, keys + wave * 64 * kFusedKeys);
       if (c == most) write_choice(a, wave, s, x);
       else if (lane < a.k) chosen[wave * a.k + lane] = (short)x.expert;
     }
@@ -748,8 +809,9 @@ __global__ __launch_bounds__(512) void decode_down_kernel(DecodeArgs a) {
     }
   }
   if (!shared) return;
-  // The barriers order the work-group's accesses with thread 0's, whose release and acquire work on the whole L2 and
-  // this CU's cache: done by every wave they took as long as the products.
+  // Every wave's sums are in the L2 before the barrier (which by itself waits for none); thread 0's release and acquire
+  // then work on the whole L2 and on this CU's cache.  Done by every wave they took as long as the products.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0)
     last = __hip_atomic_fetch_add(a.done + blockIdx.x, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
@@ -815,11 +877,18 @@ void launch_experts(DecodeArgs a, hipStream_t s) {
   const int step = (C < 16 ? 16 / C : 1) * Stretch<W4>::kStep;
   a.ldh = (a.I + step - 1) / step * step;
   const unsigned most = (unsigned)candidates(a.T, a.E, a.k);
-  if (a.T <= kFused && a.E <= 64 * kFusedKeys && most * (unsigned)(a.I / 8) <= kFusedGroups) {
+  const bool fused = a.T <= kFused && a.E <= 64 * kFusedKeys && most * (unsigned)(a.I / 8) <= kFusedGroups;
+  const bool small = !fused && a.E <= kSmallExperts && a.E * a.D <= kSmallRouter;
+  if (small) decode_router_kernel<<<a.T, 512, 0, s>>>(a);
+  else if (a.T == 1) decode_logits_kernel<1><<<dim3(a.E, 1), 256, 0, s>>>(a);
+  else decode_logits_kernel<4><<<dim3(a.E, (a.T + 3) / 4), 256, 0, s>>>(a);
+  if (fused) {
     decode_gateup_kernel<W4, 1, 1><<<dim3((unsigned)(a.I / 8), most + 1), 256, 0, s>>>(a);
   } else {
-    if (a.E <= 256) decode_select_kernel<4><<<a.T, 64, 0, s>>>(a);
-    else decode_select_kernel<16><<<a.T, 64, 0, s>>>(a);
+    if (!small) {
+      if (a.E <= 256) decode_select_kernel<4><<<a.T, 64, 0, s>>>(a);
+      else decode_select_kernel<16><<<a.T, 64, 0, s>>>(a);
+    }
     const dim3 grid((unsigned)((a.I + 15) / 16), most);
     if (a.T <= 16) decode_gateup_kernel<W4, 1, 2><<<grid, 256, 0, s>>>(a);
     else decode_gateup_kernel<W4, 4, 2><<<grid, 256, 0, s>>>(a);
@@ -866,8 +935,6 @@ int sfp8_moe_decode(const void* x, int64_t ldx, int64_t T, int64_t D, const void
                      (float*)(w + at.weights), (int*)(w + at.plan), (uint16_t*)(w + at.h), 0, (float*)(w + at.partial), (int*)(w + at.done),
                      down_shares(T, D) > 1 ? (int)((D + 31) / 32) : 0};
   const hipStream_t s = (hipStream_t)stream;
-  if (T == 1) decode_logits_kernel<1><<<dim3((unsigned)E, 1), 256, 0, s>>>(a);
-  else decode_logits_kernel<4><<<dim3((unsigned)E, (unsigned)((T + 3) / 4)), 256, 0, s>>>(a);
   if (gate_up_scales) launch_experts<true>(a, s);
   else launch_experts<false>(a, s);
   const hipError_t e = hipGetLastError();
