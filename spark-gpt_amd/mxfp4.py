@@ -74,6 +74,8 @@ def _is_mxfp4(name: str, q, dims=(2,)) -> None:
         raise TypeError(f"{name} must be an MXFP4, got {type(q).__name__}")
     if len(q.shape) not in dims:
         raise ValueError(f"{name} must be {' or '.join(f'{d}-D' for d in dims)}, got shape {tuple(q.shape)}")
+    if q.codes.dim() != len(q.shape) + 1 or (len(q.shape) == 3 and q.codes.shape[0] != q.shape[0]):
+        raise ValueError(f"{name}: codes {tuple(q.codes.shape)} do not fit the shape {tuple(q.shape)}")
 
 
 def _quantized(x: torch.Tensor, rows: bool, columns: bool):
@@ -171,7 +173,7 @@ def mxfp4_linear(x: torch.Tensor, w) -> torch.Tensor:
     N, K = w.shape
     if x.shape[-1] != K:
         raise ValueError(f"x must be [..., {K}], got shape {tuple(x.shape)}")
-    flat = x.reshape(-1, K) if x.dim() != 2 else x
+    flat = x if x.dim() == 2 else x[None] if x.dim() == 1 else x.flatten(0, -2)
     if torch.is_grad_enabled() and (x.requires_grad or (not kept and w.requires_grad)):
         if kept:
             raise ValueError("weights kept as MXFP4 give no gradient of x: pass the master, or call without gradients")

@@ -281,6 +281,26 @@ def test_linear_gradients_one_at_a_time(dev):
         g.sum().backward()
 
 
+def test_linear_of_no_tokens_and_no_width(dev):
+    """A gradient over no tokens is zero at sizes of every kernel; no width gives zeros; leading dimensions of any kind."""
+    for N, K in ((24, 40), (700, 700), (2100, 2000)):
+        w = _randn(dev, N, K, seed=1).requires_grad_(True)
+        x = torch.zeros(0, 3, K, device=dev, dtype=torch.bfloat16, requires_grad=True)
+        y = sg.mxfp4_linear(x, w)
+        dx, dw = torch.autograd.grad(y, [x, w], torch.zeros_like(y))
+        assert y.shape == (0, 3, N) and dx.shape == x.shape and torch.equal(dw, torch.zeros_like(w))
+    w = torch.zeros(5, 0, device=dev)
+    for shape in ((4, 0), (2, 3, 0), (0,)):
+        y = sg.mxfp4_linear(torch.zeros(shape, device=dev), w)
+        assert torch.equal(y, torch.zeros(*shape[:-1], 5, device=dev))
+    w = _randn(dev, 30, 64, seed=2).requires_grad_(True)
+    x = _randn(dev, 64, seed=3).requires_grad_(True)
+    y = sg.mxfp4_linear(x, w)
+    assert y.shape == (30,)
+    dx, dw = torch.autograd.grad(y, [x, w], torch.ones_like(y))
+    assert dx.shape == (64,) and dw.shape == (30, 64)
+
+
 def test_weights_kept_refuse_a_gradient(dev):
     q = sg.mxfp4_quantize(_randn(dev, 16, 64))
     with pytest.raises(ValueError, match="no gradient"):

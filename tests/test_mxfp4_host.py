@@ -73,7 +73,7 @@ def test_c_abi_refuses_before_launch():
     rows = lambda x=16, xt=1, ld=64, b=16, sb=16, M=4, N=4, K=64, out=16, dtype=1: \
         lib.sfp8_mxfp4_gemm_rows(x, xt, ld, b, sb, M, N, K, out, dtype, None)
     assert rows(x=None) == rows(b=None) == rows(sb=None) == rows(out=None) == -1
-    for bad in (dict(M=17), dict(M=-1), dict(xt=3), dict(dtype=-1), dict(ld=-1), dict(N=-1)):
+    for bad in (dict(M=17), dict(M=-1), dict(N=1 << 27), dict(xt=3), dict(dtype=-1), dict(ld=-1), dict(N=-1)):
         assert rows(**bad) == -2, bad
     assert rows(x=17) == rows(b=8) == rows(sb=2) == rows(out=8) == -3
     assert rows(M=0) == 0
@@ -96,6 +96,10 @@ def test_wrappers_refuse_host_tensors_and_misfits():
         sg.mxfp4_dequantize((q.codes, q.scales))
     with pytest.raises(ValueError, match="2-D"):
         sg.mxfp4_matmul(q, sg.MXFP4(q.codes[None], q.scales[None], (1, 4, 64)))
+    for other in (sg.MXFP4(q.codes, q.scales, (1, 4, 64)), sg.MXFP4(q.codes[None], q.scales[None], (4, 64)),
+                  sg.MXFP4(q.codes[None], q.scales[None], (2, 4, 64))):
+        with pytest.raises(ValueError, match="do not fit"):
+            sg.mxfp4_dequantize(other)
     with pytest.raises(ValueError, match=r"\[\.\.\., 64\]"):
         sg.mxfp4_linear(x[:, :32], q)
     with pytest.raises(ValueError, match=r"\[N, K\]"):
