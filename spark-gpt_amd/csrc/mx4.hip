@@ -784,7 +784,7 @@ int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const vo
   //  product, which hides its stores behind a second work-group: 16384, 8192, 4096 281 against 362; 4096, 4096, 2560
   //  26.3 against 28.3; but 16384, 4096, 2048 96.5 against 88.8 and 65536, 1024, 1024 72.0 against 55.5.
   //  128 x 128 from half a tile a CU on (1003, 2050, 1000 6.1 against 10.6; 512, 4096, 4096 11.1 against 13.2);
-  //  below that the waves share K (1024, 1024, 4096 9.3 against 10.6), in the largest tile of which there are 256:
+  //  below that the waves share K (1024, 1024, 4096 8.1 against 10.6), in the largest tile of which there are 256:
   //  64, 4096, 4096 32 x 32 4.7, 16 x 16 6.7, 64 x 64 8.5; 128, 1024, 8192 16 x 32 5.4, 64 x 64 12.4.
   const auto tiles = [&](int64_t m, int64_t n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
   if (tiles(128, 128) > kMxMaxTiles) return kErrBadShape;
