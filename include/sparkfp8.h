@@ -577,9 +577,11 @@ int sfp8_mxfp4_dequantize(const void* codes, const void* scales, int64_t batch, 
                           int dtype, void* stream);
 
 /* out [M, N] = A B^T over the values of A [M, K] and B [N, K], summed in fp32
- * and rounded once to dtype. */
+ * and rounded once to dtype.  ws (16-byte aligned) holds the sums of products
+ * whose K several work-groups share: none (and NULL) for most sizes. */
+int64_t sfp8_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t M, int64_t N,
-                    int64_t K, void* out, int dtype, void* stream);
+                    int64_t K, void* out, int dtype, void* ws, int64_t ws_bytes, void* stream);
 
 /* The same for up to 16 rows x [M, K] (x_type, rows ldx apart) that are
  * quantised on the way, bit for bit as sfp8_mxfp4_quantize does; N < 2^27. */

@@ -95,7 +95,8 @@ SIGNATURES = {
     "sfp8_mxfp4_code_bytes": (_I64, [_I64, _I64]),
     "sfp8_mxfp4_quantize": (_INT, [_P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     "sfp8_mxfp4_dequantize": (_INT, [_P, _P, _I64, _I64, _I64, _P, _INT, _P]),
-    "sfp8_mxfp4_gemm": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _INT, _P]),
+    "sfp8_mxfp4_gemm_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "sfp8_mxfp4_gemm": (_INT, [_P, _P, _P, _P, _I64, _I64, _I64, _P, _INT, _P, _I64, _P]),
     "sfp8_mxfp4_gemm_rows": (_INT, [_P, _INT, _I64, _P, _P, _I64, _I64, _I64, _P, _INT, _P]),
     # the experts' layer for a few tokens
     "sfp8_moe_decode_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),

@@ -674,6 +674,10 @@ SFP8_DEV void store_wave(uint8_t* lds, void* out, int64_t m, int64_t n, int64_t 
   }
 }
 
+// Sums of a share of K, [M, N] fp32, so many values after those of the share before
+inline __host__ __device__ int64_t mx_part(int64_t M, int64_t N) { return (M * N + 3) / 4 * 4; }
+
+// gridDim.y work-groups share the slabs of a tile; with more than one the results are their sums alone (fp32).
 template <int TM, int OUT>
 __global__ __launch_bounds__(2 * TM, 2) void mx_tile_kernel(MxGemmArgs g) {
   using Tile = MxTile<TM>;
@@ -685,21 +689,46 @@ __global__ __launch_bounds__(2 * TM, 2) void mx_tile_kernel(MxGemmArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int arows = (int)(mp - m0 < TM ? mp - m0 : TM), brows = (int)(np - n0 < TM ? np - n0 : TM);
   const bool of_b = wave >= Tile::WN;
+  const int64_t slabs = mx_slabs(g.K), sp = of_b ? np : mp;
+  const int lo = (int)(slabs * blockIdx.y / gridDim.y), hi = (int)(slabs * (blockIdx.y + 1) / gridDim.y);
   const typename Tile::Operands op{
-      g.a + m0 * 64, g.b + n0 * 64, of_b ? g.bs + n0 * 4 : g.as + m0 * 4, mp * 64, np * 64, (of_b ? np : mp) * 4,
-      arows * 64, brows * 64, (of_b ? brows : arows) * 4, (int)mx_slabs(g.K)};
+      g.a + (lo * mp + m0) * 64, g.b + (lo * np + n0) * 64, (of_b ? g.bs + (lo * np + n0) * 4 : g.as + (lo * mp + m0) * 4),
+      mp * 64, np * 64, sp * 4,
+      arows * 64, brows * 64, (of_b ? brows : arows) * 4, hi - lo};
   typename Tile::Acc acc;
   Tile(lds, op).run(acc);
   constexpr int kPart = Tile::kLds / Tile::kWaves & ~1023, kRow = 64 * (OUT == kMxF32 ? 4 : 2);
   constexpr int kRows = kPart / kRow / 32 * 32 < 32 * Tile::TB ? (kPart / kRow >= 64 ? 64 : 32) : 32 * Tile::TB;
-  store_wave<OUT, Tile::TB, kRows>(lds + wave * kPart, g.out, m0 + 32 * Tile::TB * (wave % 2), n0 + 64 * (wave / 2),
+  void* out = g.out;
+  if constexpr (OUT == kMxF32) out = reinterpret_cast<float*>(g.out) + blockIdx.y * mx_part(g.M, g.N);
+  store_wave<OUT, Tile::TB, kRows>(lds + wave * kPart, out, m0 + 32 * Tile::TB * (wave % 2), n0 + 64 * (wave / 2),
                                    g.M, g.N, acc);
 }
 
+// The shares' sums in order, and the one rounding.
+__global__ __launch_bounds__(256) void mx_sum_kernel(const float* parts, int shares, int64_t n, void* out, int type) {
+  const int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x), step = (n + 3) / 4 * 4;
+  if (i >= n) return;
+  floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int y = 0; y < shares; ++y) {
+    const floatx4 p = *reinterpret_cast<const floatx4*>(parts + y * step + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += p[j];
+  }
+  store4(out, type, i, {v[0], v[1], v[2], v[3]}, n - i < 4 ? (int)(n - i) : 4);
+}
+
 template <int TM>
-void launch_tiles(const MxGemmArgs& g, int64_t tiles, hipStream_t s) {
-  const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);
-  if (g.out_type == kMxF32) mx_tile_kernel<TM, kMxF32><<<grid, 2 * TM, 0, s>>>(g);
+void launch_tiles(const MxGemmArgs& g, int64_t tiles, int shares, void* ws, hipStream_t s) {
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)shares);
+  if (shares > 1) {
+    MxGemmArgs p = g;
+    p.out = ws;
+    mx_tile_kernel<TM, kMxF32><<<grid, 2 * TM, 0, s>>>(p);
+    mx_sum_kernel<<<(unsigned)((g.M * g.N + 1023) / 1024), 256, 0, s>>>((const float*)ws, shares, g.M * g.N, g.out,
+                                                                        g.out_type);
+  } else if (g.out_type == kMxF32) mx_tile_kernel<TM, kMxF32><<<grid, 2 * TM, 0, s>>>(g);
   else if (g.out_type == kMxBf16) mx_tile_kernel<TM, kMxBf16><<<grid, 2 * TM, 0, s>>>(g);
   else mx_tile_kernel<TM, kMxF16><<<grid, 2 * TM, 0, s>>>(g);
 }
@@ -717,6 +746,33 @@ inline int launched() {
 inline bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 inline bool type_ok(int dtype) { return dtype >= kMxF32 && dtype <= kMxF16; }
 constexpr int64_t kMxMaxDim = (int64_t)1 << 31;
+
+// By the number of tiles (us; M, N, K):
+//  256 x 256 where they fill the CUs and K is long: its loop fetches half of what that of 128 x 128 does for a
+//  product, which hides its stores behind a second work-group: 16384, 8192, 4096 281 against 362; 4096, 4096, 2560
+//  26.3 against 28.3; but 16384, 4096, 2048 96.5 against 88.8 and 65536, 1024, 1024 72.0 against 55.5.
+//  128 x 128 from half a tile a CU on (1003, 2050, 1000 6.1 against 10.6; 512, 4096, 4096 11.1 against 13.2);
+//  below that the waves share K (1024, 1024, 4096 8.1 against 10.6).
+//  Where K is very long (the weight gradients of many tokens) work-groups share it, 128 x 128 each, until there is
+//  one a CU with at least 4096 of K: 1024, 1024, 65536 74 -> 54; 1000, 1030, 16384 40 -> 25; 512, 1536, 49152 77 -> 34;
+//  the sums' way through memory costs more than it gives at 1024, 1024, 12288 (18.0, shared 20.6; 16384 23.0, 24.0),
+//  512, 512, 24576 (15.8, 17.2) and 256, 256, 32768 (13.6, 15.4), but not at 128, 128, 65536 (24.2, 16.9).
+struct MxPlan {
+  int tile = 0, shares = 1;  // 0: by waves that share K
+  MxPlan(int64_t M, int64_t N, int64_t K) {
+    const auto tiles = [&](int64_t n) { return ((M + n - 1) / n) * ((N + n - 1) / n); };
+    if (tiles(256) >= 256 && K >= 2560) {
+      tile = 256;
+    } else if (tiles(128) <= 128 && K >= 16384 && (K >= 49152 || M * N >= ((int64_t)1 << 33) / K)) {
+      const int64_t fill = 256 / tiles(128), most = K / 4096;
+      tile = 128, shares = (int)(fill < most ? fill : most);
+    } else if (tiles(128) >= 128) {
+      tile = 128;
+    }
+  }
+  int64_t workspace(int64_t M, int64_t N) const { return shares > 1 ? shares * mx_part(M, N) * 4 : 0; }
+};
+
 constexpr int64_t kMxMaxTiles = ((int64_t)1 << 24) - 8;  // of 256 threads: a grid has less than 2^32
 
 }  // namespace sfp8
@@ -768,8 +824,13 @@ int sfp8_mxfp4_dequantize(const void* codes, const void* scales, int64_t batch, 
   return launched();
 }
 
+int64_t sfp8_mxfp4_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 0 || M > kMxMaxDim || N > kMxMaxDim || K > kMxMaxDim) return -1;
+  return M == 0 || N == 0 ? 0 : MxPlan(M, N, K).workspace(M, N);
+}
+
 int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const void* b_scales, int64_t M, int64_t N,
-                    int64_t K, void* out, int dtype, void* stream) {
+                    int64_t K, void* out, int dtype, void* ws, int64_t ws_bytes, void* stream) {
   if (!type_ok(dtype) || M < 0 || N < 0 || K < 0 || M > kMxMaxDim || N > kMxMaxDim || K > kMxMaxDim)
     return kErrBadShape;
   if (M == 0 || N == 0) return kOk;
@@ -779,17 +840,18 @@ int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const vo
   const MxGemmArgs g{(const uint8_t*)a, (const uint8_t*)a_scales, (const uint8_t*)b, (const uint8_t*)b_scales,
                      nullptr, 0, M, N, K, out, dtype};
   const hipStream_t st = (hipStream_t)stream;
-  // By the number of tiles (us; M, N, K):
-  //  256 x 256 where they fill the CUs and K is long: its loop fetches half of what that of 128 x 128 does for a
-  //  product, which hides its stores behind a second work-group: 16384, 8192, 4096 281 against 362; 4096, 4096, 2560
-  //  26.3 against 28.3; but 16384, 4096, 2048 96.5 against 88.8 and 65536, 1024, 1024 72.0 against 55.5.
-  //  128 x 128 from half a tile a CU on (1003, 2050, 1000 6.1 against 10.6; 512, 4096, 4096 11.1 against 13.2);
-  //  below that the waves share K (1024, 1024, 4096 8.1 against 10.6), in the largest tile of which there are 256:
-  //  64, 4096, 4096 32 x 32 4.7, 16 x 16 6.7, 64 x 64 8.5; 128, 1024, 8192 16 x 32 5.4, 64 x 64 12.4.
+  // Without tiles, in the largest block of which there are 256 (us): 64, 4096, 4096 32 x 32 4.7, 16 x 16 6.7, 64 x 64
+  // 8.5; 128, 1024, 8192 16 x 32 5.4, 64 x 64 12.4.
   const auto tiles = [&](int64_t m, int64_t n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
   if (tiles(128, 128) > kMxMaxTiles) return kErrBadShape;
-  if (tiles(256, 256) >= 256 && K >= 2560) launch_tiles<256>(g, tiles(256, 256), st);
-  else if (tiles(128, 128) >= 128) launch_tiles<128>(g, tiles(128, 128), st);
+  const MxPlan plan(M, N, K);
+  if (plan.shares > 1) {
+    if (!ws) return kErrNullPointer;
+    if (!aligned(ws, 16)) return kErrBadAlignment;
+    if (ws_bytes < plan.workspace(M, N)) return kErrWorkspaceTooSmall;
+  }
+  if (plan.tile == 256) launch_tiles<256>(g, tiles(256, 256), plan.shares, ws, st);
+  else if (plan.tile == 128) launch_tiles<128>(g, tiles(128, 128), plan.shares, ws, st);
   else if (tiles(64, 64) >= 256) launch_few<4, 4, 4, -1>(g, st);
   else if (M > 32 && tiles(64, 32) >= 256) launch_few<4, 2, 8, -1>(g, st);
   else if (M > 16 && tiles(32, 32) >= 256) launch_few<2, 2, 8, -1>(g, st);

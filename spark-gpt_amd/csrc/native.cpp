@@ -788,6 +788,16 @@ Tensor mxfp4_dequantize(const Tensor& codes, const Tensor& scales, int64_t R, in
   return out;
 }
 
+// The space of a product whose K is shared; none for most sizes.
+struct Shares {
+  int64_t bytes;
+  Tensor ws;
+  Shares(int64_t M, int64_t N, int64_t K, const Tensor& like) : bytes(sfp8_mxfp4_gemm_workspace_bytes(M, N, K)) {
+    if (bytes > 0) ws = empty({bytes}, kU8, like);
+  }
+  void* at() const { return bytes > 0 ? ws.data_ptr() : nullptr; }
+};
+
 Tensor mx_product(const Tensor& a, const Tensor& a_scales, const Tensor& b, const Tensor& b_scales, int64_t M,
                   int64_t N, int64_t K, ScalarType type) {
   is_mxfp4("a: ", a, a_scales, std::nullopt, M, K);
@@ -795,8 +805,9 @@ Tensor mx_product(const Tensor& a, const Tensor& a_scales, const Tensor& b, cons
   same_device("b", b, a);
   const c10::DeviceGuard guard(a.device());
   Tensor out = empty({M, N}, type, a);
-  CALL(sfp8_mxfp4_gemm, ptr(a), ptr(a_scales), ptr(b), ptr(b_scales), M, N, K, ptr(out), dtype_code(type),
-       stream_of(a));
+  const Shares shares(M, N, K, a);
+  CALL(sfp8_mxfp4_gemm, ptr(a), ptr(a_scales), ptr(b), ptr(b_scales), M, N, K, ptr(out), dtype_code(type), shares.at(),
+       shares.bytes, stream_of(a));
   return out;
 }
 
@@ -848,8 +859,9 @@ std::pair<Packed, Packed> packed_quantize(const Tensor& x_, bool rows, bool colu
 }
 Tensor packed_product(const Packed& a, const Packed& b, int64_t M, int64_t N, int64_t K, ScalarType type) {
   Tensor out = empty({M, N}, type, a.buf);
-  CALL(sfp8_mxfp4_gemm, a.codes(), a.scales(), b.codes(), b.scales(), M, N, K, ptr(out), dtype_code(type),
-       stream_of(a.buf));
+  const Shares shares(M, N, K, a.buf);
+  CALL(sfp8_mxfp4_gemm, a.codes(), a.scales(), b.codes(), b.scales(), M, N, K, ptr(out), dtype_code(type), shares.at(),
+       shares.bytes, stream_of(a.buf));
   return out;
 }
 

@@ -162,6 +162,42 @@ def test_matmul_extreme_scales(dev):
             assert torch.equal(got, ref * 2.0 ** (low + high - 254))
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 8, 49153), (130, 70, 49183), (3, 5, 65536), (700, 768, 16500), (128, 257, 70000)])
+def test_matmul_shared(dev, M, N, K):
+    """Work-groups that share K: exact sums where every one is exact, again and again and from a graph, a NaN where it is
+    one, and the bound of one sum (the shares' sums are as many additions fewer)."""
+    assert sg._lib.load().sfp8_mxfp4_gemm_workspace_bytes(M, N, K) > 0
+    (a, av), (b, bv) = _operand(dev, M, K, 3), _operand(dev, N, K, 4)
+    ref = av.to(dev) @ bv.to(dev).T
+    assert torch.equal(sg.mxfp4_matmul(a, b, torch.float32).double(), ref)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = sg.mxfp4_matmul(a, b, torch.float32)
+    for dtype in DTYPES.values():
+        got = sg.mxfp4_matmul(a, b, dtype)
+        assert got.shape == (M, N) and torch.equal(got, ref.to(dtype))
+        graph.replay()
+        assert torch.equal(replayed.double(), ref)
+    a.scales[-1, 0, 0] = 255
+    got = sg.mxfp4_matmul(a, b, torch.float32)
+    assert got[0].isnan().all() and torch.equal(got[1:].double(), ref[1:])
+    (a, av), (b, bv) = _operand(dev, M, K, 7, (-9, 9)), _operand(dev, N, K, 8, (-14, 3))
+    av, bv = av.to(dev), bv.to(dev)
+    ref, size = av @ bv.T, av.abs() @ bv.abs().T
+    got = sg.mxfp4_matmul(a, b, torch.float32)
+    assert ((got.double() - ref).abs() <= K * 2.0 ** -23 * size + 2.0 ** -24 * ref.abs()).all()
+    assert torch.equal(got, sg.mxfp4_matmul(a, b, torch.float32))
+
+
+def test_linear_of_many_tokens(dev):
+    """The weight gradient of a small weight over many tokens is the product of the two quantised transposes."""
+    x, dy = _randn(dev, 50000, 96, seed=1).bfloat16().requires_grad_(True), _randn(dev, 50000, 40, seed=2).bfloat16()
+    w = _randn(dev, 40, 96, seed=3).requires_grad_(True)
+    dw, = torch.autograd.grad(sg.mxfp4_linear(x, w), [w], dy)
+    columns = lambda t: sg.mxfp4_quantize(t.detach(), along="columns")
+    assert torch.equal(dw, sg.mxfp4_matmul(columns(dy), columns(x), torch.float32))
+
+
 def test_matmul_of_nothing(dev):
     empty = lambda r, c: sg.mxfp4_quantize(torch.zeros(r, c, device=dev))
     assert sg.mxfp4_matmul(empty(0, 64), empty(5, 64)).shape == (0, 5)

@@ -62,13 +62,21 @@ def test_c_abi_refuses_before_launch():
     assert deq(codes=8) == deq(scales=2) == deq(out=8) == -3
     assert deq(R=0) == deq(C=0) == 0
 
-    gemm = lambda a=16, sa=16, b=16, sb=16, M=4, N=4, K=64, out=16, dtype=1: \
-        lib.sfp8_mxfp4_gemm(a, sa, b, sb, M, N, K, out, dtype, None)
+    gemm = lambda a=16, sa=16, b=16, sb=16, M=4, N=4, K=64, out=16, dtype=1, ws=None, bytes=0: \
+        lib.sfp8_mxfp4_gemm(a, sa, b, sb, M, N, K, out, dtype, ws, bytes, None)
     assert gemm(a=None) == gemm(sa=None) == gemm(b=None) == gemm(sb=None) == gemm(out=None) == -1
     for bad in (dict(M=-1), dict(N=-1), dict(K=-1), dict(dtype=3), dict(M=2 ** 31 + 1)):
         assert gemm(**bad) == -2, bad
     assert gemm(a=8) == gemm(sb=2) == gemm(out=8) == -3
     assert gemm(M=0) == gemm(N=0) == 0
+
+    space = lib.sfp8_mxfp4_gemm_workspace_bytes
+    assert space(4, 4, 64) == space(0, 4, 1 << 20) == space(4, 0, 1 << 20) == space(16384, 4096, 65536) == 0
+    assert space(128, 128, 65536) == 16 * 128 * 128 * 4 and space(3, 3, 49152) == 12 * 12 * 4
+    assert space(-1, 4, 4) == space(4, 2 ** 31 + 1, 4) == -1
+    shared = dict(M=128, N=128, K=65536)
+    assert gemm(**shared) == -1 and gemm(**shared, ws=8, bytes=1 << 30) == -3
+    assert gemm(**shared, ws=16, bytes=space(128, 128, 65536) - 1) == -4
 
     rows = lambda x=16, xt=1, ld=64, b=16, sb=16, M=4, N=4, K=64, out=16, dtype=1: \
         lib.sfp8_mxfp4_gemm_rows(x, xt, ld, b, sb, M, N, K, out, dtype, None)
