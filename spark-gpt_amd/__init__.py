@@ -25,7 +25,8 @@ __all__ = [
     "_FusedSwiGLU", "_NormSwiGLU", "_use_fused_norm_mlp", "_use_fused_swiglu", "make_fused_norm_mlp_guard",
     "make_fused_swiglu_guard", "swiglu", "_momentum_stage", "_momentum_stage_supported", "muon",
     "combine_experts", "expert_order", "fp8_routed_experts", "route_tokens", "routing",
-    "decode", "decode_routed_experts", "MXFP4", "mxfp4", "mxfp4_dequantize", "mxfp4_linear", "mxfp4_matmul", "mxfp4_quantize",
+    "decode", "decode_routed_experts",
+    "MXFP4", "mxfp4", "mxfp4_dequantize", "mxfp4_linear", "mxfp4_matmul", "mxfp4_quantize",
     "clip", "clip_grad_norm_", "clip_grads", "grad_norm",
 ]
 

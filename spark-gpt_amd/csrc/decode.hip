@@ -433,7 +433,8 @@ struct WeightRows<true> {
   uint32_t rows;
   SFP8_DEV WeightRows(const uint8_t* c, const uint8_t* s, int64_t e, int64_t n, int64_t k)
       : r(matrix_rsrc(c + e * mx_slabs(k) * mx_rows(n) * 64, mx_slabs(k) * mx_rows(n) * 64)),
-        rs(matrix_rsrc(s + e * mx_slabs(k) * mx_rows(n) * 4, mx_slabs(k) * mx_rows(n) * 4)), rows((uint32_t)mx_rows(n)) {}
+        rs(matrix_rsrc(s + e * mx_slabs(k) * mx_rows(n) * 4, mx_slabs(k) * mx_rows(n) * 4)),
+        rows((uint32_t)mx_rows(n)) {}
   SFP8_DEV At at(int n, int part, int q) const { return At{(uint32_t)part * rows + n, 16u * q}; }
   SFP8_DEV void read(At at, int s, Raw& f) const {
     const uint32_t row = at.row + (uint32_t)s * rows;
@@ -657,7 +658,8 @@ __global__ __launch_bounds__(256, W4 && NB > 1 ? 3 : 4) void decode_gateup_kerne
 template <bool W4, int C, int SETS, bool RAGGED>
 __global__ __launch_bounds__(512) void decode_down_kernel(DecodeArgs a) {
   static_assert(SETS == 1 || C == 16, "");
-  constexpr int W = 8, P = 16 / C, CB = C * SETS, NB = 2, kPieces = Stretch<W4>::kPieces, kStep = P * Stretch<W4>::kStep;
+  constexpr int W = 8, P = 16 / C, CB = C * SETS, NB = 2;
+  constexpr int kPieces = Stretch<W4>::kPieces, kStep = P * Stretch<W4>::kStep;
   extern __shared__ __align__(16) float totals[];  // [W][T][CB]
   __shared__ short expert_of[kMaxExperts], slot_of[kSlots];
   __shared__ int begin[kMaxExperts + 1], count[W], slots_before[W], last;
@@ -932,7 +934,8 @@ int sfp8_moe_decode(const void* x, int64_t ldx, int64_t T, int64_t D, const void
                      (int)(router_type == kMxF32), (const uint8_t*)gate_up, (const uint8_t*)gate_up_scales,
                      (const uint8_t*)down, (const uint8_t*)down_scales, bias, (const uint8_t*)mask, score, (int)groups,
                      (int)top_groups, (int)group_best, renorm, scale, selected, (uint16_t*)out, (double*)(w + at.low),
-                     (float*)(w + at.weights), (int*)(w + at.plan), (uint16_t*)(w + at.h), 0, (float*)(w + at.partial), (int*)(w + at.done),
+                     (float*)(w + at.weights), (int*)(w + at.plan), (uint16_t*)(w + at.h), 0,
+                     (float*)(w + at.partial), (int*)(w + at.done),
                      down_shares(T, D) > 1 ? (int)((D + 31) / 32) : 0};
   const hipStream_t s = (hipStream_t)stream;
   if (gate_up_scales) launch_experts<true>(a, s);

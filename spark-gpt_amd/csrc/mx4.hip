@@ -591,7 +591,7 @@ SFP8_DEV bool mx_tile_of(int id, int rows, int cols, int& r, int& c) {
   const int n = rows * cols, per = (n + 7) / 8;
   const int t = (id & 7) * per + (id >> 3);
   if ((id >> 3) >= per || t >= n) return false;
-  const int group = t / (8 * cols), first = 8 * group, high = rows - first < 8 ? rows - first : 8, in = t - first * cols;
+  const int first = t / (8 * cols) * 8, high = rows - first < 8 ? rows - first : 8, in = t - first * cols;
   r = first + in % high;
   c = in / high;
   return true;
@@ -692,8 +692,8 @@ __global__ __launch_bounds__(2 * TM, 2) void mx_tile_kernel(MxGemmArgs g) {
   const int64_t slabs = mx_slabs(g.K), sp = of_b ? np : mp;
   const int lo = (int)(slabs * blockIdx.y / gridDim.y), hi = (int)(slabs * (blockIdx.y + 1) / gridDim.y);
   const typename Tile::Operands op{
-      g.a + (lo * mp + m0) * 64, g.b + (lo * np + n0) * 64, (of_b ? g.bs + (lo * np + n0) * 4 : g.as + (lo * mp + m0) * 4),
-      mp * 64, np * 64, sp * 4,
+      g.a + (lo * mp + m0) * 64, g.b + (lo * np + n0) * 64,
+      of_b ? g.bs + (lo * np + n0) * 4 : g.as + (lo * mp + m0) * 4, mp * 64, np * 64, sp * 4,
       arows * 64, brows * 64, (of_b ? brows : arows) * 4, hi - lo};
   typename Tile::Acc acc;
   Tile(lds, op).run(acc);

@@ -67,7 +67,8 @@ def _check(x, router, w_gu, w_down, k, values=None, **kw):
 
 SIZES = [(1, 1, 1, 8, 8), (1, 8, 2, 64, 24), (2, 4, 4, 40, 16), (1, 128, 8, 512, 96), (3, 16, 3, 264, 72),
          (16, 8, 2, 128, 200), (17, 8, 2, 128, 64), (33, 60, 4, 96, 136), (64, 64, 6, 256, 88), (64, 4, 1, 72, 40),
-         (64, 2, 2, 200, 64), (20, 8, 2, 4096, 40), (10, 8, 2, 4104, 16), (40, 3, 2, 8200, 8), (5, 300, 10, 64, 32), (2, 1024, 64, 64, 16), (64, 70, 64, 32, 8), (8, 8, 2, 1024, 1536)]
+         (64, 2, 2, 200, 64), (20, 8, 2, 4096, 40), (10, 8, 2, 4104, 16), (40, 3, 2, 8200, 8),
+         (5, 300, 10, 64, 32), (2, 1024, 64, 64, 16), (64, 70, 64, 32, 8), (8, 8, 2, 1024, 1536)]
 
 
 @pytest.mark.parametrize("four", [False, True])
@@ -80,6 +81,24 @@ def test_layer(dev, T, E, k, D, I, four):
     q_gu, q_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
     values = (Q.quantized(w_gu).to(dev), Q.quantized(w_down).to(dev))
     _check(x, router, q_gu, q_down, k, values=values)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("T,E,k,D,I", [(2, 1, 1, 16384, 32768), (18, 40, 1, 4096, 8192)])
+def test_largest_matrices_and_offsets(dev, T, E, k, D, I, four):
+    """A matrix of the largest size (2 GiB in bf16), and experts that lie past 4 GiB."""
+    x, router, w_gu, w_down = _layer(dev, T, E, D, I, seed=3)
+    if E > 1:  # token t takes expert 39 - t
+        x[:, :E] = torch.eye(E, device=dev)[E - 1 - torch.arange(T, device=dev)].bfloat16()
+        router.zero_()[:, :E] = 4 * torch.eye(E, device=dev)
+    if four:
+        q_gu, q_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
+        del w_gu, w_down
+        values = (sg.mxfp4_dequantize(q_gu), sg.mxfp4_dequantize(q_down))
+        _, selected = _check(x, router, q_gu, q_down, k, values=values)
+    else:
+        _, selected = _check(x, router, w_gu, w_down, k)
+    assert selected[:, 0].tolist() == ([39 - t for t in range(T)] if E > 1 else [0, 0])
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
