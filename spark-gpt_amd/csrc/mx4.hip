@@ -29,44 +29,46 @@ struct MxQuantArgs {
   uint8_t *codes_t, *scales_t;     // of its transpose, or NULL
 };
 
-// One work-group takes 16 ITER x 128 values.  Sixteen lanes hold 128 values of a
-// row (four lanes a block: its maximum is two lane exchanges away), so the row
-// codes leave straight from the registers, four rows of 64 bytes in one run.
+// One work-group takes ITER times 2048 values in rows of WIDE.  WIDE / 8 lanes hold
+// those of a row (four lanes a block: its maximum is two lane exchanges away), so
+// the row codes leave straight from the registers, four rows of 64 bytes in one run.
 // For the columns the values pass through LDS as they are: a lane then holds
-// 32 values of one column (16-bit types: of two), so neither its maximum nor
-// its codes need another lane; the codes go back through LDS so that each
-// column's 64 bytes and the tile's 8 KiB are written in one run.
-// ITER = 8 where there are columns; along rows alone 2 where a taller tile would
-// leave CUs without one.
-template <int DT, bool ROWS, bool COLS, int ITER>
+// 32 values of one column (16-bit types in the wide tile: of two), so neither its
+// maximum nor its codes need another lane; the codes go back through LDS so that
+// each column's 64 bytes and the tile's 8 KiB are written in one run.
+// 128 x 128 values where there are columns, half as wide where those tiles would
+// leave CUs without one; along rows alone 32 x 128 there.
+template <int DT, bool ROWS, bool COLS, int ITER, int WIDE>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
-  static_assert(ITER == 8 || !COLS, "a slab of the transpose");
-  constexpr int kSize = DT == kMxF32 ? 4 : 2;
-  __shared__ __align__(16) uint8_t raw[COLS ? 128 * 128 * kSize : 16];
-  __shared__ __align__(16) uint8_t out[COLS ? 128 * 64 : 16];
-  __shared__ __align__(16) uint8_t out_scale[COLS ? 512 : 16];
+  constexpr int kSize = DT == kMxF32 ? 4 : 2, kLanes = WIDE / 8, kRows = 256 / kLanes, kTall = kRows * ITER;
+  static_assert(kTall == 128 || !COLS, "a slab of the transpose");
+  __shared__ __align__(16) uint8_t raw[COLS ? 128 * WIDE * kSize : 16];
+  __shared__ __align__(16) uint8_t out[COLS ? WIDE * 64 : 16];
+  __shared__ __align__(16) uint8_t out_scale[COLS ? WIDE * 4 : 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t nx = mx_slabs(a.C), ny = (a.R + 16 * ITER - 1) / (16 * ITER);
+  const int64_t slabs = mx_slabs(a.C), nx = slabs * (128 / WIDE), ny = (a.R + kTall - 1) / kTall;
   const int64_t id = blockIdx.x, cs = id % nx, rs = id / nx % ny, z = id / nx / ny;
-  const int64_t c0 = cs * 128, r0 = rs * (16 * ITER), rows = mx_rows(a.R), cols = mx_rows(a.C);
+  const int64_t c0 = cs * WIDE, r0 = rs * kTall, rows = mx_rows(a.R), cols = mx_rows(a.C);
   const uint8_t* x = reinterpret_cast<const uint8_t*>(a.x) + z * a.batch_stride * kSize;
-  const int col = 8 * (lane & 15), sub = 4 * wave + (lane >> 4);
+  const int col = 8 * (tid % kLanes), sub = tid / kLanes;
 
   Eight<DT> v[ITER];
-  if (c0 + 128 <= a.C && r0 + 16 * ITER <= a.R) {
+  if (c0 + WIDE <= a.C && r0 + kTall <= a.R) {
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) v[i] = load8<DT>(x, (r0 + 16 * i + sub) * a.ld + c0 + col);
+    for (int i = 0; i < ITER; ++i) v[i] = load8<DT>(x, (r0 + kRows * i + sub) * a.ld + c0 + col);
   } else {
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
-      const int64_t r = r0 + 16 * i + sub;
+      const int64_t r = r0 + kRows * i + sub;
       v[i] = Eight<DT>{};
       if (r < a.R && c0 + col < a.C) v[i] = load8_upto<DT>(x, r * a.ld + c0 + col, a.C - c0 - col);
     }
   }
   if constexpr (ROWS) {
-    uint8_t* codes = a.codes + (z * nx + cs) * rows * 64;
-    uint8_t* scales = a.scales + (z * nx + cs) * rows * 4;
+    const int64_t slab = z * slabs + cs / (128 / WIDE);
+    const int in = (int)(cs % (128 / WIDE)) * WIDE;  // the tile's first column in its slab
+    uint8_t* codes = a.codes + slab * rows * 64 + in / 2;
+    uint8_t* scales = a.scales + slab * rows * 4 + in / 32;
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       uint32_t m = abs_max8<DT>(v[i]);
@@ -74,36 +76,40 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
       m = max_u(m, dpp<0x4E>(m));
       const uint32_t e = mx_scale_code(abs_bits_to_f32<DT>(m));
       const uint32_t c = codes8<DT>(v[i], mx_scale_value(e));
-      uint32_t s = e << (8 * ((lane >> 2) & 3));  // the row's four scales in one word
+      uint32_t s = e << (8 * (tid % kLanes / 4));  // the row's four scales (or two) in one word
       s |= dpp<0x141>(s);
-      s |= dpp<0x140>(s);
-      const int64_t r = r0 + 16 * i + sub;
+      if constexpr (WIDE == 128) s |= dpp<0x140>(s);
+      const int64_t r = r0 + kRows * i + sub;
       if (r < rows) {
-        *reinterpret_cast<uint32_t*>(codes + r * 64 + 4 * (lane & 15)) = c;
-        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + r * 4) = s;
+        *reinterpret_cast<uint32_t*>(codes + r * 64 + col / 2) = c;
+        if (col == 0) {
+          if constexpr (WIDE == 128) *reinterpret_cast<uint32_t*>(scales + r * 4) = s;
+          else *reinterpret_cast<uint16_t*>(scales + r * 4) = (uint16_t)s;
+        }
       }
     }
   }
   if constexpr (COLS) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t* p = reinterpret_cast<uint32_t*>(raw + ((16 * i + sub) * 128 + col) * kSize);
+    for (int i = 0; i < ITER; ++i) {
+      uint32_t* p = reinterpret_cast<uint32_t*>(raw + ((kRows * i + sub) * WIDE + col) * kSize);
       *reinterpret_cast<intx4*>(p) = intx4{(int)v[i].w[0], (int)v[i].w[1], (int)v[i].w[2], (int)v[i].w[3]};
       if constexpr (DT == kMxF32)
         *reinterpret_cast<intx4*>(p + 4) = intx4{(int)v[i].w[4], (int)v[i].w[5], (int)v[i].w[6], (int)v[i].w[7]};
     }
     __syncthreads();
-    // 64 words of a row; this lane's word holds one column (fp32) or two
-    constexpr int kHalves = DT == kMxF32 ? 2 : 1;
+    // 64 columns of the wave's 32 rows a turn, one a lane; or 128 where a lane's word holds two
+    constexpr int kWords = WIDE * kSize / 4, kCols = kWords * 2 == WIDE && WIDE == 128 ? 2 : 1;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const uint32_t* p = reinterpret_cast<const uint32_t*>(raw) + 32 * wave * (64 * kHalves) + 64 * h + lane;
+    for (int h = 0; h < WIDE / 64 / kCols; ++h) {
+      const int first = 64 * h + kCols * lane;  // this lane's column
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(raw) + 32 * wave * kWords + first * kSize / 4;
       uint32_t w[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) w[i] = p[i * 64 * kHalves];
-      constexpr int kCols = DT == kMxF32 ? 1 : 2;
+      for (int i = 0; i < 32; ++i) w[i] = p[i * kWords];
 #pragma unroll
-      for (int k = 0; k < kCols; ++k) {
+      for (int half = 0; half < kCols; ++half) {
+        const int k = kCols == 2 ? half : first & 1;  // the column's half of the word
         Eight<DT> q[4];
         uint32_t m = 0;
 #pragma unroll
@@ -122,7 +128,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
         }
         const uint32_t e = mx_scale_code(abs_bits_to_f32<DT>(m));
         const float s = mx_scale_value(e);
-        const int c = DT == kMxF32 ? 64 * h + lane : 2 * lane + k;
+        const int c = first + half;
         // 16-byte chunk `wave` of column c, at chunk wave ^ (c / 2) % 4: the lanes of a store spread over the banks
         *reinterpret_cast<intx4*>(out + c * 64 + 16 * (wave ^ ((c >> 1) & 3))) =
             intx4{(int)codes8<DT>(q[0], s), (int)codes8<DT>(q[1], s), (int)codes8<DT>(q[2], s),
@@ -134,20 +140,22 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
     uint8_t* codes = a.codes_t + (z * ny + rs) * cols * 64;
     uint8_t* scales = a.scales_t + (z * ny + rs) * cols * 4;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < WIDE / 64; ++j) {
       const int u = tid + 256 * j, c = u >> 2, ch = u & 3;
       if (c0 + c < cols)
         *reinterpret_cast<intx4*>(codes + (c0 + c) * 64 + 16 * ch) =
             *reinterpret_cast<const intx4*>(out + c * 64 + 16 * (ch ^ ((c >> 1) & 3)));
     }
-    if (tid < 128 && c0 + tid < cols)
+    if (tid < WIDE && c0 + tid < cols)
       *reinterpret_cast<uint32_t*>(scales + (c0 + tid) * 4) = reinterpret_cast<const uint32_t*>(out_scale)[tid];
   }
 }
 
-// Work-groups for tiles of 128 rows and, where those would not be two for each
-// CU, of 32 (rows of 5003 x 1001: 4.2 us against 5.2; of 65536 x 1024 27.9 against
-// 26.1).
+// Work-groups for tiles of 128 x 128 and, where those would not be two for each
+// CU, of 32 x 128 along rows (5003 x 1001: 4.2 us against 5.2; 65536 x 1024 27.9
+// against 26.1); where they would not be one, of 128 x 64 along columns (rows and
+// columns of 1030 x 1000 in fp32 4.1 against 5.4, of 2003 x 1030 in bf16 6.1 against
+// 7.5; of 4096 x 1024 in bf16 5.4 against 5.1).
 struct MxGrid {
   unsigned tall, low;
   MxGrid(int64_t batch, int64_t R, int64_t C)
@@ -157,10 +165,17 @@ struct MxGrid {
 
 template <int DT>
 void launch_quantize(const MxQuantArgs& a, const MxGrid& grid, hipStream_t stream) {
-  if (a.codes && a.codes_t) mx_quantize_kernel<DT, true, true, 8><<<grid.tall, 256, 0, stream>>>(a);
-  else if (a.codes_t) mx_quantize_kernel<DT, false, true, 8><<<grid.tall, 256, 0, stream>>>(a);
-  else if (grid.low) mx_quantize_kernel<DT, true, false, 2><<<grid.low, 256, 0, stream>>>(a);
-  else mx_quantize_kernel<DT, true, false, 8><<<grid.tall, 256, 0, stream>>>(a);
+  const unsigned narrow = grid.tall < 256 ? 2 * grid.tall : 0;
+  if (a.codes && a.codes_t) {
+    if (narrow) mx_quantize_kernel<DT, true, true, 4, 64><<<narrow, 256, 0, stream>>>(a);
+    else mx_quantize_kernel<DT, true, true, 8, 128><<<grid.tall, 256, 0, stream>>>(a);
+  } else if (a.codes_t) {
+    if (narrow) mx_quantize_kernel<DT, false, true, 4, 64><<<narrow, 256, 0, stream>>>(a);
+    else mx_quantize_kernel<DT, false, true, 8, 128><<<grid.tall, 256, 0, stream>>>(a);
+  } else {
+    if (grid.low) mx_quantize_kernel<DT, true, false, 2, 128><<<grid.low, 256, 0, stream>>>(a);
+    else mx_quantize_kernel<DT, true, false, 8, 128><<<grid.tall, 256, 0, stream>>>(a);
+  }
 }
 
 // ---------------------------------------------------------------------------

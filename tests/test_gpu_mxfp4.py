@@ -41,7 +41,7 @@ def _check_codes(q, x):
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("R,C", [(1, 1), (1, 32), (3, 31), (16, 128), (17, 129), (128, 128), (130, 260), (1, 1000),
-                                 (257, 40), (300, 1001), (64, 4096)])
+                                 (257, 40), (300, 1001), (64, 4096), (4100, 1000), (33000, 130)])
 def test_quantize(dev, R, C, dtype):
     x = _randn(dev, R, C, seed=R + C, dtype=DTYPES[dtype]) * torch.exp(2 * _randn(dev, C, seed=1)).to(DTYPES[dtype])
     rows, columns = sg.mxfp4_quantize(x, along="both")
