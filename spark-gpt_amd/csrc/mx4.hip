@@ -267,6 +267,7 @@ struct MxGemmArgs {
   int64_t M, N, K;
   void* out;  // [M, N]
   int out_type;
+  int share = 1 << 30;  // slabs of a work-group's share of K, where there are several
 };
 
 SFP8_DEV void store4(void* out, int type, int64_t i, const float (&v)[4], int n) {
@@ -704,8 +705,8 @@ __global__ __launch_bounds__(2 * TM, 2) void mx_tile_kernel(MxGemmArgs g) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int arows = (int)(mp - m0 < TM ? mp - m0 : TM), brows = (int)(np - n0 < TM ? np - n0 : TM);
   const bool of_b = wave >= Tile::WN;
-  const int64_t slabs = mx_slabs(g.K), sp = of_b ? np : mp;
-  const int lo = (int)(slabs * blockIdx.y / gridDim.y), hi = (int)(slabs * (blockIdx.y + 1) / gridDim.y);
+  const int64_t sp = of_b ? np : mp;
+  const int slabs = (int)mx_slabs(g.K), lo = min((int)blockIdx.y * g.share, slabs), hi = min(lo + g.share, slabs);
   const typename Tile::Operands op{
       g.a + (lo * mp + m0) * 64, g.b + (lo * np + n0) * 64,
       of_b ? g.bs + (lo * np + n0) * 4 : g.as + (lo * mp + m0) * 4, mp * 64, np * 64, sp * 4,
@@ -740,6 +741,7 @@ void launch_tiles(const MxGemmArgs& g, int64_t tiles, int shares, void* ws, hipS
   if (shares > 1) {
     MxGemmArgs p = g;
     p.out = ws;
+    p.share = (int)((mx_slabs(g.K) + shares - 1) / shares);
     mx_tile_kernel<TM, kMxF32><<<grid, 2 * TM, 0, s>>>(p);
     mx_sum_kernel<<<(unsigned)((g.M * g.N + 1023) / 1024), 256, 0, s>>>((const float*)ws, shares, g.M * g.N, g.out,
                                                                         g.out_type);

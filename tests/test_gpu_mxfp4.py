@@ -189,6 +189,15 @@ def test_matmul_shared(dev, M, N, K):
     assert torch.equal(got, sg.mxfp4_matmul(a, b, torch.float32))
 
 
+def test_matmul_shared_unevenly(dev):
+    """8300 slabs for 256 work-groups of 33: the last of them have none."""
+    K, g = 8300 * 128 - 5, torch.Generator().manual_seed(1)
+    signs = lambda rows: 1 - 2 * torch.randint(0, 2, (rows, K), generator=g)
+    a, b = signs(2), signs(3)
+    quantized = lambda t: sg.mxfp4_quantize(t.to(dev, torch.bfloat16))
+    assert torch.equal(sg.mxfp4_matmul(quantized(a), quantized(b), torch.float32).cpu(), (a @ b.T).float())
+
+
 def test_linear_of_many_tokens(dev):
     """The weight gradient of a small weight over many tokens is the product of the two quantised transposes."""
     x, dy = _randn(dev, 50000, 96, seed=1).bfloat16().requires_grad_(True), _randn(dev, 50000, 40, seed=2).bfloat16()
