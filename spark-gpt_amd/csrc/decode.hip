@@ -41,7 +41,7 @@ struct DecodeArgs {
   double* low;      // [T, E]
   float* weights;   // [T, k]
   int* plan;        // per candidate: number of slots (0: not taken); its expert; its slots, 64 each
-  uint16_t* h;      // [T * k][2][ldh]: h and what its rounding to bf16 left, zeros from I on
+  float* h;         // [T * k][ldh], zeros from I on
   int ldh;          // I up to a whole number of down's steps
   float* partial;   // [shares of the steps][T, D]
   int* done;        // per column block of down: work-groups that have finished
@@ -454,7 +454,7 @@ struct WeightRows<true> {
   static SFP8_DEV void zero_past(Stretch<true>&, int, int, int) {}  // padding has zero codes, past the end are zeros
 };
 
-// A token's (or slot's) values beside them; `row` is the lane's own place, 8 q values into the row.
+// A token's values beside them; `row` is the lane's own place, 8 q values into the row.
 template <bool W4>
 SFP8_DEV void read_values(const uint16_t* row, int k, Stretch<W4>& f) {
 #pragma unroll
@@ -467,6 +467,29 @@ SFP8_DEV void read_last(const uint16_t* row, int K, int k, int q, Stretch<W4>& f
   for (int j = 0; j < Stretch<W4>::kPieces; ++j) {
     const int at = k + Stretch<W4>::at(q, j);
     f.w[j] = zero_unless(at < K, load_bf16x8(row + (at < K ? at : K - 8) - 8 * q));
+  }
+}
+
+// Four values of h as three bf16 values each: the upper eight bits of what is
+// left, three times, are all 24 of a value (down to bf16's smallest), and the
+// products of bf16 values are exact, so the sums are those of h in 32 bits.  An
+// infinity leaves nothing.
+SFP8_DEV void three_parts(const intx4& v, intx2 (&part)[3]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t left[2] = {(uint32_t)v[2 * i], (uint32_t)v[2 * i + 1]};
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      part[p][i] = (int)__builtin_amdgcn_perm(left[1], left[0], 0x07060302u);
+      if (p < 2) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float f = __uint_as_float(left[j]);
+          const float rest = f - __uint_as_float(left[j] & 0xffff0000u);
+          left[j] = p == 0 && !__builtin_isfinite(f) ? 0u : __float_as_uint(rest);
+        }
+      }
+    }
   }
 }
 
@@ -625,19 +648,12 @@ __global__ __launch_bounds__(256, W4 && NB > 1 ? 3 : 4) void decode_gateup_kerne
       float g = 0.f, u = 0.f;
 #pragma unroll
       for (int v = 0; v < W; ++v) g += red[v][z][s][col & 7], u += red[v][z][s][8 + (col & 7)];
-      const float h = g * sigmoid_fast(g) * u, hi = round_bf16(h);
-      uint16_t* p = a.h + (int64_t)list[16 * b + s] * 2 * a.ldh + i0 + col;
-      p[0] = (uint16_t)f32_to_bf16_bits(h);
-      // an infinity or a NaN leaves nothing to be added
-      p[a.ldh] = (uint16_t)f32_to_bf16_bits(__builtin_isfinite(hi) ? h - hi : 0.f);
+      a.h[(int64_t)list[16 * b + s] * a.ldh + i0 + col] = g * sigmoid_fast(g) * u;
     }
   }
   if (i0 + 8 * SETS >= I && a.ldh > I) {  // zeros up to the end of down's last stretch
     const int pad = a.ldh - I;
-    for (int i = tid; i < 2 * n * pad; i += 64 * W) {
-      const int row2 = i / pad;
-      a.h[((int64_t)list[row2 >> 1] * 2 + (row2 & 1)) * a.ldh + I + i % pad] = 0;
-    }
+    for (int i = tid; i < n * pad; i += 64 * W) a.h[(int64_t)list[i / pad] * a.ldh + I + i % pad] = 0.f;
   }
 }
 
@@ -651,7 +667,16 @@ __global__ __launch_bounds__(256, W4 && NB > 1 ? 3 : 4) void decode_gateup_kerne
 // are kept: a CU takes no more than about 20 bytes a nanosecond from memory, so
 // all of them have to have a work-group.  An expert of more than 2 C slots is
 // read again for each 2 C of them.  RAGGED: I is no multiple of a step.
-// With many slots an expert, h is what the CUs take most of (two parts of each
+// h is in 32 bits.  A wave reads each value of a step once (16 lanes 64 columns
+// of a slot and part), splits it into three bf16 parts and hands them to the
+// matrix cores' lanes through its own LDS, 64 columns of K at a time.  Where the
+// slots take a quarter of the product's columns at most, their parts are columns
+// of their own: a third of the LDS reads and products, and the three sums meet
+// at the end.  (Layer of 2048 x 768, 8 of 128 experts, us: 4 tokens 4-bit 40.4, 16
+// tokens bf16 160; every lane splitting what it multiplies, without LDS, 46.6 and
+// 172; three products for few slots too 41.7 and 167; h in two bf16 parts as they
+// lie in memory, 17 bits of it, 38.6 and 168.)
+// With many slots an expert, h is what the CUs take most of (32 bits of each
 // slot beside C rows of weights): then SETS = 2 sets of 16 columns share it, and
 // gridDim.y work-groups share the steps of a column block; the last of them to
 // finish (counters that the logits' launch has zeroed) adds their sums in order.
@@ -659,14 +684,18 @@ template <bool W4, int C, int SETS, bool RAGGED>
 __global__ __launch_bounds__(512) void decode_down_kernel(DecodeArgs a) {
   static_assert(SETS == 1 || C == 16, "");
   constexpr int W = 8, P = 16 / C, CB = C * SETS, NB = 2;
-  constexpr int kPieces = Stretch<W4>::kPieces, kStep = P * Stretch<W4>::kStep;
+  constexpr int kStep = P * Stretch<W4>::kStep, kSubs = Stretch<W4>::kPieces / 2;
+  // rows of 64 bf16 values, 16 bytes further on by the banks from one to the next
+  constexpr int kHRow = 144, kMostTogether = SETS > 1 ? 1 : kSubs;
   extern __shared__ __align__(16) float totals[];  // [W][T][CB]
+  __shared__ __align__(16) uint8_t hparts[W][kMostTogether * 3 * 16 * kHRow];
   __shared__ short expert_of[kMaxExperts], slot_of[kSlots];
   __shared__ int begin[kMaxExperts + 1], count[W], slots_before[W], last;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = CB * blockIdx.x, D = a.D, I = a.I, T = a.T, most = candidates(T, a.E, a.k);
   float* mine = totals + wave * T * CB;
+  uint8_t* hs = hparts[wave];
   for (int i = lane; i < T * CB / 4; i += 64) reinterpret_cast<floatx4*>(mine)[i] = floatx4{0.f, 0.f, 0.f, 0.f};
   // the experts that are taken, in the candidates' order, and their slots
   int live = 0, taken = 0;
@@ -722,79 +751,132 @@ __global__ __launch_bounds__(512) void decode_down_kernel(DecodeArgs a) {
     for (int z = 0; z < SETS; ++z) place[z] = w.at(min(n0 + C * z + r % C, D - 1), part, q);
     for (int first = __builtin_amdgcn_readfirstlane(begin[which]); first < end; first += NB * C) {
       const int n = min(end - first, NB * C);
-      const uint16_t* hrow[NB];
-      float weight[NB];
+      const auto products = [&](auto blocks, auto loads) {
+        constexpr int B = decltype(blocks)::value, X = decltype(loads)::value;
+        constexpr int kRegs = SETS * (int)sizeof(typename WeightRows<W4>::Raw) / 4 + B * kSubs * X * 4;
+        // slots that are few enough have their parts in columns of their own: one product in the place of three
+        constexpr bool kApart = X == 1;
+        constexpr int kParts = kApart ? 1 : 3, kTogether = kApart ? 1 : kMostTogether;
+        // as many steps in flight as 256 registers hold
+        constexpr int kSpace = SETS > 1 ? 112 : kTogether > 1 ? 128 : 160;
+        constexpr int kInFlight = kSpace / kRegs < 8 ? kSpace / kRegs : 8;
+        const float* hrow[B][X];
+        uint32_t to[X];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int i = C * b + r % C, s = slot_of[first + (i < n ? i : 0)];
-        hrow[b] = a.h + (int64_t)s * 2 * a.ldh + part * Stretch<W4>::kStep + 8 * q;
-        weight[b] = a.weights[s];
-      }
-      floatx4 acc[NB][SETS];
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int z = 0; z < SETS; ++z) acc[b][z] = floatx4{0.f, 0.f, 0.f, 0.f};
-      const auto batch = [&](auto blocks, auto size, int s) {
-        constexpr int B = decltype(blocks)::value, U = decltype(size)::value;
-        typename WeightRows<W4>::Raw rw[U][SETS];
-        Stretch<W4> f[U][B][2];
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-#pragma unroll
-          for (int z = 0; z < SETS; ++z) w.read(place[z], P * (s + i), rw[i][z]);
+        for (int x = 0; x < X; ++x) {
+          const int u = 4 * x + q, slot = u / P, prt = u % P;
+          to[x] = (uint32_t)(prt * C + (kApart ? 3 * slot : slot)) * kHRow + 8 * r;
 #pragma unroll
           for (int b = 0; b < B; ++b) {
-            read_values<W4>(hrow[b], (s + i) * kStep, f[i][b][0]);
-            read_values<W4>(hrow[b] + a.ldh, (s + i) * kStep, f[i][b][1]);
+            const int i = C * b + slot;
+            hrow[b][x] = a.h + (int64_t)slot_of[first + (i < n ? i : 0)] * a.ldh + prt * Stretch<W4>::kStep + 4 * r;
           }
         }
-        __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead of the products
+        const auto slot_in = [&](int b) { return kApart ? r % C / 3 : C * b + r % C; };  // that this lane's sums are of
+        float weight[B];
 #pragma unroll
-        for (int i = 0; i < U; ++i)
+        for (int b = 0; b < B; ++b) weight[b] = a.weights[slot_of[first + (slot_in(b) < n ? slot_in(b) : 0)]];
+        floatx4 acc[B][SETS];
 #pragma unroll
-          for (int z = 0; z < SETS; ++z) {
-            Stretch<W4> fw;
-            w.values(rw[i][z], fw);
-            if (RAGGED && s + i == steps - 1) w.zero_past(fw, I, (s + i) * kStep + part * Stretch<W4>::kStep, q);
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+          for (int z = 0; z < SETS; ++z) acc[b][z] = floatx4{0.f, 0.f, 0.f, 0.f};
+        in_batches<kInFlight>(s1 - s0, [&](auto size, int from) {
+          constexpr int U = decltype(size)::value;
+          typename WeightRows<W4>::Raw rw[U][SETS];
+          intx4 f[U][B][kSubs][X];
+#pragma unroll
+          for (int i = 0; i < U; ++i) {
+            const int s = s0 + from + i;
+#pragma unroll
+            for (int z = 0; z < SETS; ++z) w.read(place[z], P * s, rw[i][z]);
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
-              for (int half = 0; half < 2; ++half)
+              for (int u = 0; u < kSubs; ++u)
 #pragma unroll
-                for (int j = 0; j < kPieces; ++j) acc[b][z] = mfma16(fw.w[j], f[i][b][half].w[j], acc[b][z]);
+                for (int x = 0; x < X; ++x)
+                  f[i][b][u][x] = *reinterpret_cast<const intx4*>(hrow[b][x] + s * kStep + 64 * u);
+          }
+          __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead of the products
+#pragma unroll
+          for (int i = 0; i < U; ++i) {
+            const int s = s0 + from + i;
+            Stretch<W4> fw[SETS];
+#pragma unroll
+            for (int z = 0; z < SETS; ++z) {
+              w.values(rw[i][z], fw[z]);
+              if (RAGGED && s == steps - 1) w.zero_past(fw[z], I, s * kStep + part * Stretch<W4>::kStep, q);
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+              for (int u0 = 0; u0 < kSubs; u0 += kTogether) {
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u)
+#pragma unroll
+                  for (int x = 0; x < X; ++x) {
+                    intx2 h[3];
+                    three_parts(f[i][b][u0 + u][x], h);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p)
+                      *reinterpret_cast<intx2*>(hs + (u * 48 + p * (kApart ? 1 : 16)) * kHRow + to[x]) = h[p];
+                  }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                bf16x8 h[kTogether][2][kParts];
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u)
+#pragma unroll
+                  for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)
+                      h[u][j][p] =
+                          *reinterpret_cast<const bf16x8*>(hs + (u * 48 + p * 16 + r) * kHRow + 64 * j + 16 * q);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int u = 0; u < kTogether; ++u)
+#pragma unroll
+                  for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                      for (int z = 0; z < SETS; ++z)
+                        acc[b][z] = mfma16(fw[z].w[2 * (u0 + u) + j], h[u][j][p], acc[b][z]);
+              }
+          }
+        });
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+          for (int z = 0; z < SETS; ++z) {
+            floatx4 v = acc[b][z];
+            // a part's columns are 4 q' .. + 3 of slot r % C: the next part's lie 256 / P + C lanes on (rows, columns)
+            if constexpr (P > 1) {
+              floatx4 sum = v;
+#pragma unroll
+              for (int o = 1; o < P; ++o)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] += __shfl(v[j], (lane + o * (64 / P + C)) & 63, 64);
+              v = sum;
+            }
+            if constexpr (kApart) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] += __shfl(v[j], (lane + 1) & 63, 64) + __shfl(v[j], (lane + 2) & 63, 64);
+            }
+            if (slot_in(b) < n && (!kApart || r % 3 == 0) && r < C && q < C / 4) {
+              floatx4* p = reinterpret_cast<floatx4*>(mine + slot_of[first + slot_in(b)] / a.k * CB + C * z + 4 * q);
+              floatx4 t = *p;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) t[j] = __builtin_fmaf(weight[b], v[j], t[j]);
+              *p = t;
+            }
           }
       };
-      // as many steps in flight as 256 registers hold
-      constexpr int kOne = (W4 ? 3 : 6) - (SETS > 1 ? W4 ? 1 : 2 : 0), kTwo = (W4 ? 2 : 4) - (SETS > 1 ? 1 : 0);
-      if (n <= C)
-        in_batches<kOne>(s1 - s0, [&](auto u, int i) { batch(std::integral_constant<int, 1>{}, u, s0 + i); });
-      else
-        in_batches<kTwo>(s1 - s0, [&](auto u, int i) { batch(std::integral_constant<int, 2>{}, u, s0 + i); });
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int z = 0; z < SETS; ++z) {
-          floatx4 v = acc[b][z];
-          // a part's columns are 4 q' .. + 3 of slot r % C: the next part's lie 256 / P + C lanes on (rows, columns)
-          if constexpr (P > 1) {
-            floatx4 sum = v;
-#pragma unroll
-            for (int o = 1; o < P; ++o)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) sum[j] += __shfl(v[j], (lane + o * (64 / P + C)) & 63, 64);
-            v = sum;
-          }
-          const int i = C * b + r % C;
-          if (i < n && r < C && q < C / 4) {
-            const int token = slot_of[first + i] / a.k;
-            floatx4* p = reinterpret_cast<floatx4*>(mine + token * CB + C * z + 4 * q);
-            floatx4 t = *p;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) t[j] = __builtin_fmaf(weight[b], v[j], t[j]);
-            *p = t;
-          }
-        }
+      const auto one = std::integral_constant<int, 1>{};
+      if (n > C) products(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+      else if (P * n > 8) products(one, std::integral_constant<int, 4>{});
+      else if (P * n > 4) products(one, std::integral_constant<int, 2>{});
+      else products(one, one);
     }
   }
   __syncthreads();
@@ -852,7 +934,7 @@ struct DecodeSpace {
     done = plan + up256((plan_slots((int)most) + 64 * most) * 4);
     partial = done + up256(shares > 1 ? (D + 31) / 32 * 4 : 0);
     h = partial + up256(shares > 1 ? shares * T * D * 4 : 0);
-    all = h + T * k * 2 * ((I + 511) / 512 * 512) * 2;  // a step of down has at most 512 columns
+    all = h + T * k * ((I + 511) / 512 * 512) * 4;  // a step of down has at most 512 columns
   }
 };
 
@@ -934,7 +1016,7 @@ int sfp8_moe_decode(const void* x, int64_t ldx, int64_t T, int64_t D, const void
                      (int)(router_type == kMxF32), (const uint8_t*)gate_up, (const uint8_t*)gate_up_scales,
                      (const uint8_t*)down, (const uint8_t*)down_scales, bias, (const uint8_t*)mask, score, (int)groups,
                      (int)top_groups, (int)group_best, renorm, scale, selected, (uint16_t*)out, (double*)(w + at.low),
-                     (float*)(w + at.weights), (int*)(w + at.plan), (uint16_t*)(w + at.h), 0,
+                     (float*)(w + at.weights), (int*)(w + at.plan), (float*)(w + at.h), 0,
                      (float*)(w + at.partial), (int*)(w + at.done),
                      down_shares(T, D) > 1 ? (int)((D + 31) / 32) : 0};
   const hipStream_t s = (hipStream_t)stream;

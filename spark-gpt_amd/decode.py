@@ -30,10 +30,11 @@ def decode_routed_experts(x: torch.Tensor, router: torch.Tensor, w_gu, w_down, t
     The logits are x router^T, summed in 64 bits; ``top_k`` and the keyword
     arguments are those of ``route_tokens``, and the experts are ordered by the
     64-bit values (not by logits rounded to 32).  h = silu(x Wg^T) * (x Wu^T), and
-    out is the sum over the chosen experts of weight * h Wd^T, with sums in 32
-    bits, h in two bf16 parts (17 bits of it) and one rounding at the end; 4-bit
-    weights multiply x in bf16 as the values they stand for.  Masked tokens give
-    rows of zeros and -1.
+    out is the sum over the chosen experts of weight * h Wd^T, with h and the sums
+    in 32 bits and one rounding at the end; 4-bit weights multiply x in bf16 as the
+    values they stand for.  Masked tokens give rows of zeros and -1.  An infinity
+    in w_down makes its column of its expert's tokens NaN (h meets it in parts,
+    some of them zero).
 
     No gradient is taken: with gradients enabled, inputs that require one are
     refused."""

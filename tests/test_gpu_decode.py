@@ -317,3 +317,45 @@ def test_same_layer_as_the_grouped_experts(dev):
     rows = (w_down[owner].float() @ h[:, :, None])[:, :, 0].to(torch.bfloat16)
     ref = sg.combine_experts(rows, weights, inverse, offsets)
     assert float((out.float() - ref.float()).norm() / ref.float().norm()) < 2.0 ** -7
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("T,D", [(1, 64), (1, 2048), (1, 4096), (9, 64), (9, 2048), (24, 64)])
+def test_h_keeps_its_32_bits(dev, T, D, four):
+    """Two columns of h, 64 (1 + 2^-8 + 2^-17) and 64 (1 + 2^-8), whose difference is the output: 2^-11, which the 17 bits
+    of two bf16 parts do not hold.  In steps of 2^-23 of 65, which h stays below: a sum of three products is off by 3, the
+    sigmoid by 1, the two products by 1 together; the difference of what two columns' three parts give, six products, by
+    12: 2 * 5 + 12 in all."""
+    x, router, w_gu, w_down = _layer(dev, T, 2, D, 16)
+    for t in (x, router, w_gu, w_down):
+        t.zero_()
+    x[:, :4] = torch.tensor([64.0, 1.0, 2.0 ** -8, 2.0 ** -17], device=dev).bfloat16()
+    w_gu[:, :2, 0] = 1  # the gate
+    w_gu[:, 16:18, 1:3] = 1
+    w_gu[:, 16, 3] = 1
+    w_down[:, :, 0], w_down[:, :, 1] = 1, -1
+    if four:
+        w_gu, w_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
+    out, _ = sg.decode_routed_experts(x, router, w_gu, w_down, 1)
+    off = (out.double() - 2.0 ** -11).abs().max()
+    assert float(off) <= 22 * 65 * 2.0 ** -23 + 2.0 ** -8 * 2.0 ** -11, float(off)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("T", [1, 9, 24])
+def test_infinities_in_h(dev, T, four):
+    """An infinity in one column of h is one in the output, of either sign; both, or a weight of zero beside it, are a NaN."""
+    def run(columns, zero_weight=False):
+        x, router, w_gu, w_down = (torch.zeros_like(t) for t in _layer(dev, T, 2, 64, 16))
+        x[:, 0] = 1
+        w_down.fill_(1)
+        if zero_weight:
+            w_down[:, :, 5] = 0
+        for column, sign in columns:
+            w_gu[:, column, 0], w_gu[:, 16 + column, 0] = 2.0 ** 100, sign * 2.0 ** 100
+        if four:
+            w_gu, w_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
+        return sg.decode_routed_experts(x, router, w_gu, w_down, 1)[0]
+
+    assert (run([(2, 1)]) == float("inf")).all() and (run([(3, -1)]) == -float("inf")).all()
+    assert run([(2, 1), (3, -1)]).isnan().all() and run([(5, 1)], zero_weight=True).isnan().all()
