@@ -648,7 +648,8 @@ __global__ __launch_bounds__(256, W4 && NB > 1 ? 3 : 4) void decode_gateup_kerne
       float g = 0.f, u = 0.f;
 #pragma unroll
       for (int v = 0; v < W; ++v) g += red[v][z][s][col & 7], u += red[v][z][s][8 + (col & 7)];
-      a.h[(int64_t)list[16 * b + s] * a.ldh + i0 + col] = g * sigmoid_fast(g) * u;
+      // exp's argument is not rounded first, as exp2 of g log2(e) would have it: that is off by |g| / 2 steps
+      a.h[(int64_t)list[16 * b + s] * a.ldh + i0 + col] = g / (1.f + expf(-g)) * u;
     }
   }
   if (i0 + 8 * SETS >= I && a.ldh > I) {  // zeros up to the end of down's last stretch

@@ -359,3 +359,31 @@ def test_infinities_in_h(dev, T, four):
 
     assert (run([(2, 1)]) == float("inf")).all() and (run([(3, -1)]) == -float("inf")).all()
     assert run([(2, 1), (3, -1)]).isnan().all() and run([(5, 1)], zero_weight=True).isnan().all()
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("T", [1, 6, 24])
+def test_silu_of_large_gates(dev, T, four):
+    """silu(g) less 64 v, v the fp32 value nearest to silu(g) / 64, for gates whose product with log2(e) rounds badly (off
+    by 26 steps of 2^-23 in the exponential).  In those steps of silu(g): the exponential is off by 1, the sum and the
+    quotient by 1 together, v's three parts by 2, the down sums' six products by 6: 10."""
+    x, router, w_gu, w_down = (torch.zeros_like(t) for t in _layer(dev, T, 2, 64, 16))
+    g = -torch.tensor([61.25, 58.0, 54.75, 51.5, 48.25, 45.0], dtype=torch.float64, device=dev)
+    g = g[torch.arange(T, device=dev) % 6]
+    silu = g / (1 + torch.exp(-g))
+    left = (silu / 64).float()
+    v = left.double()
+    x[:, 0], x[:, 1], x[:, 2] = g.bfloat16(), 64, 1
+    for part in range(3):
+        x[:, 3 + part] = left.bfloat16()
+        left = left - x[:, 3 + part].float()
+    assert not left.any()
+    w_gu[:, 0, 0] = w_gu[:, 1, 1] = w_gu[:, 16, 2] = 1
+    w_gu[:, 17, 3:6] = 1
+    w_down[:, :, 0], w_down[:, :, 1] = 1, -1
+    if four:
+        w_gu, w_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
+    out, _ = sg.decode_routed_experts(x, router, w_gu, w_down, 1)
+    ref, err = (silu - 64 * v)[:, None], (10 * 2.0 ** -23 * silu.abs())[:, None]
+    off = (out.double() - ref).abs()
+    assert (off <= err + 2.0 ** -8 * (ref.abs() + err)).all(), (off / silu.abs()[:, None]).max() * 2.0 ** 23
