@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import torch_ops
-from .mxfp4 import MXFP4, _is_mxfp4
+from .mxfp4 import MXFP4, _is_mxfp4, _no_tangent
 
 MAX_TOKENS = 64
 
@@ -37,7 +37,7 @@ def decode_routed_experts(x: torch.Tensor, router: torch.Tensor, w_gu, w_down, t
     some of them zero).
 
     No gradient is taken: with gradients enabled, inputs that require one are
-    refused."""
+    refused, and so are inputs with a forward-mode tangent."""
     quantized = isinstance(w_gu, MXFP4)
     if quantized != isinstance(w_down, MXFP4):
         raise TypeError("w_gu and w_down must be both bf16 tensors or both MXFP4")
@@ -45,6 +45,7 @@ def decode_routed_experts(x: torch.Tensor, router: torch.Tensor, w_gu, w_down, t
                                        + (() if quantized else (w_gu, w_down))):
         raise ValueError("decode_routed_experts takes no gradient: call it under torch.no_grad(), or train through "
                          "route_tokens and the grouped experts")
+    _no_tangent("decode_routed_experts", x, router, bias, w_gu, w_down)
     if quantized:
         _is_mxfp4("w_gu", w_gu, (3,))
         _is_mxfp4("w_down", w_down, (3,))

@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops, torch_ops
@@ -76,6 +77,14 @@ def _is_mxfp4(name: str, q, dims=(2,)) -> None:
         raise ValueError(f"{name} must be {' or '.join(f'{d}-D' for d in dims)}, got shape {tuple(q.shape)}")
     if q.codes.dim() != len(q.shape) + 1 or (len(q.shape) == 3 and q.codes.shape[0] != q.shape[0]):
         raise ValueError(f"{name}: codes {tuple(q.codes.shape)} do not fit the shape {tuple(q.shape)}")
+
+
+def _no_tangent(what: str, *tensors) -> None:
+    """Refuses inputs of forward-mode differentiation: a dual tensor needs no gradient, so the paths without a node
+    would drop its tangent."""
+    if not torch.compiler.is_compiling() and forward_ad._current_level >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _quantized(x: torch.Tensor, rows: bool, columns: bool):
@@ -162,7 +171,7 @@ def mxfp4_linear(x: torch.Tensor, w) -> torch.Tensor:
     to 16 tokens without a gradient are quantised within the product's kernel,
     with the same codes.
 
-    Differentiable once."""
+    Differentiable once, and not in forward mode."""
     if x.dim() < 1:
         raise ValueError("x must have at least one dimension")
     kept = isinstance(w, MXFP4)
@@ -173,6 +182,7 @@ def mxfp4_linear(x: torch.Tensor, w) -> torch.Tensor:
     N, K = w.shape
     if x.shape[-1] != K:
         raise ValueError(f"x must be [..., {K}], got shape {tuple(x.shape)}")
+    _no_tangent("mxfp4_linear", x, w)
     flat = x if x.dim() == 2 else x[None] if x.dim() == 1 else x.flatten(0, -2)
     if torch.is_grad_enabled() and (x.requires_grad or (not kept and w.requires_grad)):
         if kept:

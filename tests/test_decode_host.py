@@ -70,3 +70,21 @@ def test_fake_shapes():
                                                  torch.empty(8, 64, 16, dtype=torch.bfloat16), None, 16, None, None,
                                                  "softmax", 1, 1, 1, 2, True, 1.0)
         assert out.shape == (3, 64) and out.dtype == torch.bfloat16 and sel.shape == (3, 2) and sel.dtype == torch.int64
+
+
+def test_refuses_tangents():
+    """A dual tensor requires no gradient: its tangent is refused, not dropped."""
+    from torch.autograd import forward_ad
+
+    x, router = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(4, 64)
+    w_gu, w_down = torch.zeros(4, 32, 64, dtype=torch.bfloat16), torch.zeros(4, 64, 16, dtype=torch.bfloat16)
+    args, bias = [x, router, w_gu, w_down], torch.zeros(4)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for i in range(4):
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                sg.decode_routed_experts(*args[:i], dual(args[i]), *args[i + 1:], 2)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            sg.decode_routed_experts(*args, 2, bias=dual(bias))
+        with pytest.raises(ValueError, match="ROCm device"):
+            sg.decode_routed_experts(*args, 2, bias=bias)

@@ -445,3 +445,19 @@ def test_large_offsets(dev):
     del back
     small = sg.mxfp4_quantize(_randn(dev, 20, C, seed=2))
     assert torch.equal(sg.mxfp4_matmul(q, small)[-40:], sg.mxfp4_matmul(want, small))
+
+
+def test_no_forward_mode(dev):
+    """Tangents are refused on every path; tensors without one pass inside a level."""
+    from torch.autograd import forward_ad
+
+    x, w = torch.randn(20, 64, device=dev, dtype=torch.bfloat16), torch.randn(32, 64, device=dev)
+    q = sg.mxfp4_quantize(w)
+    plain = [sg.mxfp4_linear(v, q) for v in (x, x[:3])]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for v in (dual, dual[:3]):
+            for weights in (q, w, w.clone().requires_grad_(True)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    sg.mxfp4_linear(v, weights)
+        assert all(torch.equal(sg.mxfp4_linear(v, q), p) for v, p in zip((x, x[:3]), plain))

@@ -134,3 +134,21 @@ def test_fake_shapes():
         y = torch.ops.sparkfp8.mxfp4_matmul(a, s, a, s, 17, 17, 130, torch.float16)
         assert y.shape == (17, 17) and y.dtype == torch.float16
         assert torch.ops.sparkfp8.mxfp4_rows_matmul(x[0, :5], a, s, 17, torch.float32).shape == (5, 17)
+
+
+def test_linear_refuses_tangents():
+    """A dual tensor requires no gradient: its tangent is refused, not dropped."""
+    from torch.autograd import forward_ad
+
+    x = torch.zeros(4, 64)
+    q = sg.MXFP4.from_rows(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8), 64)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for args in ((dual, q), (dual, x), (x, dual)):
+            for on in (True, False):
+                with torch.set_grad_enabled(on), pytest.raises(NotImplementedError, match="forward-mode"):
+                    sg.mxfp4_linear(*args)
+        with pytest.raises(ValueError, match="ROCm device"):
+            sg.mxfp4_linear(x, q)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda v: sg.mxfp4_linear(v, q), (x,), (x,))
