@@ -584,7 +584,7 @@ int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const vo
                     int64_t K, void* out, int dtype, void* ws, int64_t ws_bytes, void* stream);
 
 /* The same for up to 16 rows x [M, K] (x_type, rows ldx apart) that are
- * quantised on the way, bit for bit as sfp8_mxfp4_quantize does; N < 2^27. */
+ * quantised on the way, bit for bit as sfp8_mxfp4_quantize does; N <= 2^27 - 16. */
 int sfp8_mxfp4_gemm_rows(const void* x, int x_type, int64_t ldx, const void* b, const void* b_scales, int64_t M,
                          int64_t N, int64_t K, void* out, int dtype, void* stream);
 

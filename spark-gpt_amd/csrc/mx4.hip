@@ -791,6 +791,7 @@ struct MxPlan {
 };
 
 constexpr int64_t kMxMaxTiles = ((int64_t)1 << 24) - 8;  // of 256 threads: a grid has less than 2^32
+constexpr int64_t kMxMaxRowsN = ((int64_t)1 << 27) - 16;  // 16 columns of 512 threads
 
 }  // namespace sfp8
 
@@ -879,7 +880,7 @@ int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const vo
 
 int sfp8_mxfp4_gemm_rows(const void* x, int x_type, int64_t ldx, const void* b, const void* b_scales, int64_t M,
                          int64_t N, int64_t K, void* out, int dtype, void* stream) {
-  if (!type_ok(dtype) || !type_ok(x_type) || M < 0 || M > 16 || N < 0 || K < 0 || N >= (int64_t)1 << 27 ||
+  if (!type_ok(dtype) || !type_ok(x_type) || M < 0 || M > 16 || N < 0 || K < 0 || N > kMxMaxRowsN ||
       K > kMxMaxDim || ldx < 0)
     return kErrBadShape;
   if (M == 0 || N == 0) return kOk;

@@ -26,6 +26,7 @@ from . import ops, torch_ops
 BLOCK = 32  # values that share a scale
 SLAB = 128  # values of a row that lie together
 ROW_ALIGN = 16
+ROWS_MAX_N = (1 << 27) - 16  # columns of a product whose rows are quantised on the way
 _DIRECTIONS = {"rows": (True, False), "columns": (False, True), "both": (True, True)}
 
 
@@ -190,7 +191,7 @@ def mxfp4_linear(x: torch.Tensor, w) -> torch.Tensor:
         y = (_MXFP4Linear.apply if torch.compiler.is_compiling() else ops.mxfp4_linear)(flat, w)
     else:
         q = w if kept else _quantized(w, True, False)[0]
-        if flat.shape[0] <= ROW_ALIGN and N < 1 << 27:
+        if flat.shape[0] <= ROW_ALIGN and N <= ROWS_MAX_N:
             y = torch_ops.op("mxfp4_rows_matmul")(flat, q.codes, q.scales, N, x.dtype)
         else:
             y = mxfp4_matmul(_quantized(flat, True, False)[0], q, x.dtype)

@@ -152,3 +152,10 @@ def test_linear_refuses_tangents():
             sg.mxfp4_linear(x, q)
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(lambda v: sg.mxfp4_linear(v, q), (x,), (x,))
+
+
+def test_rows_product_refuses_grids_past_the_limit():
+    """16 columns take 512 threads, and a grid has less than 2^32 of them."""
+    rows = lambda N: _lib.load().sfp8_mxfp4_gemm_rows(16, 1, 64, 16, 16, 4, N, 64, 16, 1, None)
+    assert rows((1 << 27) - 1) == rows((1 << 27) - 15) == -2
+    assert sg.mxfp4.ROWS_MAX_N == (1 << 27) - 16
