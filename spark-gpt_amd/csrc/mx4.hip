@@ -791,6 +791,7 @@ struct MxPlan {
 };
 
 constexpr int64_t kMxMaxTiles = ((int64_t)1 << 24) - 8;  // of 256 threads: a grid has less than 2^32
+constexpr int64_t kMxMaxTiles256 = ((int64_t)1 << 23) - 8;  // of 512
 constexpr int64_t kMxMaxRowsN = ((int64_t)1 << 27) - 16;  // 16 columns of 512 threads
 
 }  // namespace sfp8
@@ -863,6 +864,7 @@ int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const vo
   const auto tiles = [&](int64_t m, int64_t n) { return ((M + m - 1) / m) * ((N + n - 1) / n); };
   if (tiles(128, 128) > kMxMaxTiles) return kErrBadShape;
   const MxPlan plan(M, N, K);
+  if (plan.tile == 256 && tiles(256, 256) > kMxMaxTiles256) return kErrBadShape;
   if (plan.shares > 1) {
     if (!ws) return kErrNullPointer;
     if (!aligned(ws, 16)) return kErrBadAlignment;

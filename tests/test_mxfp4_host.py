@@ -159,3 +159,10 @@ def test_rows_product_refuses_grids_past_the_limit():
     rows = lambda N: _lib.load().sfp8_mxfp4_gemm_rows(16, 1, 64, 16, 16, 4, N, 64, 16, 1, None)
     assert rows((1 << 27) - 1) == rows((1 << 27) - 15) == -2
     assert sg.mxfp4.ROWS_MAX_N == (1 << 27) - 16
+
+
+def test_product_refuses_grids_past_the_limit():
+    """Tiles of 256 x 256 take 512 threads: one row of them reaches 2^32 before those of 128 x 128 are too many."""
+    gemm = lambda N, K: _lib.load().sfp8_mxfp4_gemm(16, 16, 16, 16, 1, N, K, 16, 1, None, 0, None)
+    assert gemm((1 << 31) - 1024, 2560) == gemm((1 << 31) - 2047, 2560) == -2
+    assert gemm((1 << 31) - 1023, 64) == -2
