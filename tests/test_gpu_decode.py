@@ -387,3 +387,88 @@ def test_silu_of_large_gates(dev, T, four):
     ref, err = (silu - 64 * v)[:, None], (10 * 2.0 ** -23 * silu.abs())[:, None]
     off = (out.double() - ref).abs()
     assert (off <= err + 2.0 ** -8 * (ref.abs() + err)).all(), (off / silu.abs()[:, None]).max() * 2.0 ** 23
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("with_bias", [True, False])
+@pytest.mark.parametrize("groups,top_groups,best", [(1, 1, 1), (4, 2, 1), (4, 2, 2), (12, 5, 2), (6, 6, 1)])
+def test_routing_options_of_one_to_four_tokens(dev, score, renorm, with_bias, groups, top_groups, best):
+    """Few enough tokens and candidates that gate and up selects by itself, up to 256 experts, bf16 and 4-bit."""
+    for T, E, k, router, four in ((1, 12, 3, torch.float32, False), (3, 12, 3, torch.bfloat16, True),
+                                  (4, 120, 8, torch.bfloat16, False), (4, 252, 6, torch.float32, True)):
+        k = min(k, top_groups * (E // groups))
+        x, r, w_gu, w_down = _layer(dev, T, E, 64, 24, seed=E + T, router=router)
+        bias = _randn(dev, E, seed=5, std=0.3, dtype=torch.float32) if with_bias else None
+        values = None
+        if four:
+            values = (Q.quantized(w_gu).to(dev), Q.quantized(w_down).to(dev))
+            w_gu, w_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
+        for masked in ((), (0,), tuple(range(T))) if T > 1 else ((), (0,)):
+            mask = torch.ones(T, dtype=torch.bool, device=dev)
+            mask[list(masked)] = False
+            out, sel = _check(x, r, w_gu, w_down, k, values=values, score=score, renormalize=renorm, bias=bias,
+                              groups=groups, top_groups=top_groups, group_best=best, mask=mask, scale=2.5)
+            assert not out[~mask].any() and (sel[~mask] == -1).all() and (sel[mask] >= 0).all()
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("E", [20, 150])
+def test_special_tokens_and_scores_of_four_tokens(dev, E, four):
+    """Ties, NaN and infinite tokens, experts that cannot be taken, masks, where gate and up selects by itself."""
+    T, k, D, I = 4, 4, 64, 24
+    x, router, w_gu, w_down = _layer(dev, T, E, D, I)
+    x.copy_((x.float() * 2).round().clamp(-4, 4) / 2)  # exact logits, multiples of a quarter
+    router.copy_((router.float() * 16).round().clamp(-4, 4) / 2)
+    router[7] = router[3]
+    router[11] = router[3]
+    x[3] = 0
+    values = None
+    if four:
+        values = (Q.quantized(w_gu).to(dev), Q.quantized(w_down).to(dev))
+        w_gu, w_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
+    clean, chosen = _check(x, router, w_gu, w_down, k, values=values)
+    assert chosen[3].tolist() == [0, 1, 2, 3]
+    for value in (float("nan"), float("inf")):
+        broken = x.clone()
+        broken[1, 9] = value
+        out, sel = sg.decode_routed_experts(broken, router, w_gu, w_down, k)
+        low = broken.double() @ router.double().T
+        assert torch.equal(sel.cpu(), O.route(low, k)[1]) and out[1].isnan().all()
+        assert torch.equal(out[[0, 2, 3]], clean[[0, 2, 3]])
+        some = torch.tensor([True, False, True, True], device=dev)
+        out, sel = sg.decode_routed_experts(broken, router, w_gu, w_down, k, mask=some)
+        assert torch.equal(out[some], clean[some]) and not out[1].any() and (sel[1] == -1).all()
+    for score in ("softmax", "sigmoid"):
+        bias = torch.full((E,), -float("inf"), device=dev)
+        bias[5], bias[13] = 0.0, 0.1
+        _, sel = _check(x, router, w_gu, w_down, k, values=values, bias=bias, score=score)
+        assert (sel[:, 2:] == -1).all() and (sel[:, :2] >= 0).all()
+        out, sel = sg.decode_routed_experts(x, router, w_gu, w_down, k, bias=bias.fill_(-float("inf")), score=score)
+        assert (sel == -1).all() and not out.any()
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("T,E,k,D,I", [(64, 1024, 16, 64, 16), (40, 1024, 12, 64, 16), (64, 600, 64, 32, 8),
+                                       (50, 1024, 20, 40, 24)])
+def test_many_candidates(dev, T, E, k, D, I, four):
+    """More candidates than down's work-groups take in a turn (512), as experts and as slots, and slots past 256."""
+    x, router, w_gu, w_down = _layer(dev, T, E, D, I, seed=T)
+    if not four:
+        _check(x, router, w_gu, w_down, k)
+        return
+    values = (Q.quantized(w_gu).to(dev), Q.quantized(w_down).to(dev))
+    _check(x, router, sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down), k, values=values)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [True, False])
+@pytest.mark.parametrize("groups,top_groups,best", [(1, 1, 1), (8, 3, 2), (64, 20, 1)])
+def test_routing_options_of_many_experts(dev, score, with_bias, groups, top_groups, best):
+    """Past 256 experts a lane of the selection holds sixteen of them."""
+    for T, E, k in ((3, 512, 8), (30, 960, 12)):
+        x, router, w_gu, w_down = _layer(dev, T, E, 64, 16, seed=E, router=torch.float32)
+        bias = _randn(dev, E, seed=5, std=0.3, dtype=torch.float32) if with_bias else None
+        mask = torch.rand(T, device=dev, generator=torch.Generator(device=dev).manual_seed(3)) > 0.25
+        _check(x, router, w_gu, w_down, k, score=score, renormalize=False, bias=bias, groups=groups,
+               top_groups=top_groups, group_best=best, mask=mask, scale=0.5)
