@@ -472,3 +472,20 @@ def test_routing_options_of_many_experts(dev, score, with_bias, groups, top_grou
         mask = torch.rand(T, device=dev, generator=torch.Generator(device=dev).manual_seed(3)) > 0.25
         _check(x, router, w_gu, w_down, k, score=score, renormalize=False, bias=bias, groups=groups,
                top_groups=top_groups, group_best=best, mask=mask, scale=0.5)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("D,I", [(64, 72), (2048, 136), (4096, 264)])
+def test_every_number_of_slots(dev, D, I, four):
+    """An expert of 1 .. 18 tokens, and of 33 and 64: each way that down has of putting slots in a product's columns."""
+    x, router, w_gu, w_down = _layer(dev, 64, 1, D, I, seed=D)
+    values = (w_gu, w_down)
+    if four:
+        values = (Q.quantized(w_gu).to(dev), Q.quantized(w_down).to(dev))
+        w_gu, w_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
+    one = torch.ones(64, 1, device=dev)
+    ref, bound = _reference(x, one, torch.zeros(64, 1, dtype=torch.int64), *values)
+    for T in (*range(1, 19), 33, 64):
+        out, sel = sg.decode_routed_experts(x[:T], router, w_gu, w_down, 1)
+        bad = ~((out.double() - ref[:T]).abs() <= bound[:T])
+        assert not bad.any() and not sel.any(), (T, int(bad.sum()), out[bad][:4], ref[:T][bad][:4])
