@@ -980,8 +980,8 @@ void launch_experts(DecodeArgs a, hipStream_t s) {
   }
   if (C == 32) launch_down<W4, 16, 2>(a, down_shares(a.T, a.D), s);
   else if (C == 16) launch_down<W4, 16, 1>(a, 1, s);
-  else if (C == 8) launch_down<W4, 8, 1>(a, 1, s);
-  else launch_down<W4, 4, 1>(a, 1, s);
+  else if (W4 || C == 8) launch_down<W4, 8, 1>(a, 1, s);
+  else if constexpr (!W4) launch_down<W4, 4, 1>(a, 1, s);
 }
 
 }  // namespace sfp8

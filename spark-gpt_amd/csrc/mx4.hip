@@ -735,17 +735,19 @@ __global__ __launch_bounds__(256) void mx_sum_kernel(const float* parts, int sha
   store4(out, type, i, {v[0], v[1], v[2], v[3]}, n - i < 4 ? (int)(n - i) : 4);
 }
 
+void launch_shares(const MxGemmArgs& g, int64_t tiles, int shares, void* ws, hipStream_t s) {
+  MxGemmArgs p = g;
+  p.out = ws;
+  p.share = (int)((mx_slabs(g.K) + shares - 1) / shares);
+  mx_tile_kernel<128, kMxF32><<<dim3((unsigned)((tiles + 7) / 8 * 8), (unsigned)shares), 256, 0, s>>>(p);
+  mx_sum_kernel<<<(unsigned)((g.M * g.N + 1023) / 1024), 256, 0, s>>>((const float*)ws, shares, g.M * g.N, g.out,
+                                                                      g.out_type);
+}
+
 template <int TM>
-void launch_tiles(const MxGemmArgs& g, int64_t tiles, int shares, void* ws, hipStream_t s) {
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)shares);
-  if (shares > 1) {
-    MxGemmArgs p = g;
-    p.out = ws;
-    p.share = (int)((mx_slabs(g.K) + shares - 1) / shares);
-    mx_tile_kernel<TM, kMxF32><<<grid, 2 * TM, 0, s>>>(p);
-    mx_sum_kernel<<<(unsigned)((g.M * g.N + 1023) / 1024), 256, 0, s>>>((const float*)ws, shares, g.M * g.N, g.out,
-                                                                        g.out_type);
-  } else if (g.out_type == kMxF32) mx_tile_kernel<TM, kMxF32><<<grid, 2 * TM, 0, s>>>(g);
+void launch_tiles(const MxGemmArgs& g, int64_t tiles, hipStream_t s) {
+  const unsigned grid = (unsigned)((tiles + 7) / 8 * 8);
+  if (g.out_type == kMxF32) mx_tile_kernel<TM, kMxF32><<<grid, 2 * TM, 0, s>>>(g);
   else if (g.out_type == kMxBf16) mx_tile_kernel<TM, kMxBf16><<<grid, 2 * TM, 0, s>>>(g);
   else mx_tile_kernel<TM, kMxF16><<<grid, 2 * TM, 0, s>>>(g);
 }
@@ -870,8 +872,9 @@ int sfp8_mxfp4_gemm(const void* a, const void* a_scales, const void* b, const vo
     if (!aligned(ws, 16)) return kErrBadAlignment;
     if (ws_bytes < plan.workspace(M, N)) return kErrWorkspaceTooSmall;
   }
-  if (plan.tile == 256) launch_tiles<256>(g, tiles(256, 256), plan.shares, ws, st);
-  else if (plan.tile == 128) launch_tiles<128>(g, tiles(128, 128), plan.shares, ws, st);
+  if (plan.tile == 256) launch_tiles<256>(g, tiles(256, 256), st);
+  else if (plan.shares > 1) launch_shares(g, tiles(128, 128), plan.shares, ws, st);
+  else if (plan.tile == 128) launch_tiles<128>(g, tiles(128, 128), st);
   else if (tiles(64, 64) >= 256) launch_few<4, 4, 4, -1>(g, st);
   else if (M > 32 && tiles(64, 32) >= 256) launch_few<4, 2, 8, -1>(g, st);
   else if (M > 16 && tiles(32, 32) >= 256) launch_few<2, 2, 8, -1>(g, st);
