@@ -6,9 +6,10 @@
 //   h_j = silu(x Wg_j^T) * (x Wu_j^T);  out = sum_j w_j h_j Wd_j^T
 //
 // With at most 64 tokens the layer is bound by the bytes of the experts that
-// are taken, so each of their weights is read once for all tokens and goes from
-// memory to registers (16 bytes a lane); the products run on the bf16 matrix
-// cores with the weights as first operand and up to 16 tokens as second.
+// are taken, so their weights are read for all of their tokens at once (down's
+// again for each 8 to 32 slots of an expert, from the caches) and go from memory to
+// registers (16 bytes a lane); the products run on the bf16 matrix cores with the
+// weights as first operand and up to 16 tokens as second.
 // Weights are bf16, or MXFP4 codes (mx4.h) that become bf16 values in
 // registers, which hold them exactly; x stays bf16 in both.
 // Four launches: logits; the selection, a wave a token; gate and up, whose
@@ -67,8 +68,11 @@ SFP8_DEV double wave_max_or_nan(double v) {
 
 // ---------------------------------------------------------------------------
 // Logits: a work-group takes one expert and TOK tokens, its four waves a quarter
-// of the width each.  Sums in 64 bits, so that the order of two experts is that
-// of the exact sums but for 2^-50 of their size.
+// of the width each.  Sums in 64 bits: products of bf16 with bf16 or fp32 are
+// exact in them, and a sum passes at most D / 256 + 8 roundings (a lane's in turn,
+// 6 over the lanes, 2 over the waves), so that the order of two experts is that of
+// the exact sums but for (D / 256 + 8) 2^-53 of the sum of the products' sizes: 2^-49
+// at D = 2048, 2^-41 at the largest.  (A small router's: at most 29 roundings.)
 // ---------------------------------------------------------------------------
 SFP8_DEV double bf16_at(const Eight<kMxBf16>& v, int j) {
   return (double)__uint_as_float(j & 1 ? v.w[j / 2] & 0xffff0000u : v.w[j / 2] << 16);
@@ -308,9 +312,9 @@ __global__ __launch_bounds__(64) void decode_select_kernel(DecodeArgs a) {
 
 // A small router: a work-group a token has all logits and the selection.  A wave
 // takes four experts at a time; where there are fewer than four for each of the
-// eight waves, several share the width.  A layer of 16 tokens and 8 experts of
-// width 1024 takes 31.0 us with it and 32.7 with two kernels; with 16 experts as
-// long, and with 64 of 512 26.0 against 24.2: one CU reads slowly.
+// eight waves, several share the width.  A layer of 16 tokens (us, in a graph): 8
+// experts of width 1024 32.5 with it and 33.8 with two kernels, 16 of 512 25.1 and
+// 26.1; 16 of 1024 41.0 and 42.0, but 64 of 512 45.1 and 43.9: one CU reads slowly.
 constexpr int kSmallRouter = 8192, kSmallExperts = 64;
 
 __global__ __launch_bounds__(512) void decode_router_kernel(DecodeArgs a) {
@@ -502,7 +506,8 @@ SFP8_DEV void in_batches(int n, F f, int i = 0) {
 
 // Up to this many tokens are selected by the waves of every work-group of gate
 // and up (P keys a lane): 3 us that it waits longer against 6 of a launch and a
-// kernel of its own.
+// kernel of its own.  (Layer in a graph, us: one token, 8 of 128 experts, bf16 28.3
+// against 32.3, 4-bit 19.9 against 22.2; four tokens, 2 of 128, 18.9 against 21.0.)
 constexpr int kFused = 4, kFusedKeys = 4, kFusedGroups = 1024;
 
 // Gate and up of 8 columns of h for all slots of one expert: a product's 16 rows
@@ -661,8 +666,8 @@ __global__ __launch_bounds__(256, W4 && NB > 1 ? 3 : 4) void decode_gateup_kerne
 // Down and the weighted sum for C SETS columns of the output: the steps of all
 // experts that are taken are dealt out to the waves in even runs.  A wave adds
 // each expert's sums times the slots' weights to its own totals of all tokens
-// (LDS), and the waves' totals meet in their order: every weight is read once,
-// and no sum depends on the order of arrival.
+// (LDS), and the waves' totals meet in their order: no sum depends on the order of
+// arrival.
 // A product's 16 rows are C columns in P = 16 / C parts of K, its 16 columns C
 // slots in the same parts, and of the result the blocks where the parts agree
 // are kept: a CU takes no more than about 20 bytes a nanosecond from memory, so
@@ -954,10 +959,14 @@ void launch_down(const DecodeArgs& a, int shares, hipStream_t s) {
 
 template <bool W4>
 void launch_experts(DecodeArgs a, hipStream_t s) {
-  // Columns a work-group of down: such that there is one for each CU (T = 16, D = 1024, 8 experts of 1536: 4 columns
-  // 32.7 us a layer, 8 35.9, 16 43.2; T = 1, D = 2048, 8 of 768: 30.5, 27.5, 30.8; steps of 4-bit weights are twice as
-  // long, and 4 columns 44.6 against 36.9 with 8).  Beyond 16 tokens 32 columns, whose steps are shared (T = 64, D =
-  // 2048, 64 of 1032: 196 against 203; with 16 tokens 36.2 against 32.7).
+  // Columns a work-group of down: such that at D = 1024 (bf16), 2048 and 4096 there is one for each CU; narrower layers
+  // leave CUs without one.  In a graph, us a layer with 4, 8 and 16 columns:
+  //  bf16  T = 16, D = 1024, 2 of 8 experts of 1536 32.9, 34.1, 37.9; T = 4, D = 512, the same experts 21.3, 22.7, 26.8;
+  //        T = 1, D = 2048, 8 of 128 of 768 31.5, 27.8, 30.6; T = 4, D = 4096, 2 of 16 of 1536 73.3, 63.8, 60.0
+  //  4-bit T = 4, 8 of 128 of 768, D = 512 30.0, 31.9, 37.3; 1024 34.1, 35.2, 40.3; 2048 50.8, 40.1, 45.3; D = 4096, 8
+  //        of 32 77.7, 55.9, 48.1
+  // Beyond 16 tokens 32 columns, whose steps are shared (T = 64, D = 2048, 6 of 64 of 1032: 185 against 227 with 16; T =
+  // 24, D = 1024, 2 of 8: 35.5 against 42.3; T = 16, the first of the layers above: 33.8).
   const int C = a.T > 16 ? 32 : a.D >= 4096 ? 16 : !W4 && a.D < 2048 ? 4 : 8;
   const int step = (C < 16 ? 16 / C : 1) * Stretch<W4>::kStep;
   a.ldh = (a.I + step - 1) / step * step;

@@ -155,7 +155,8 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(MxQuantArgs a) {
 // CU, of 32 x 128 along rows (5003 x 1001: 4.2 us against 5.2; 65536 x 1024 27.9
 // against 26.1); where they would not be one, of 128 x 64 along columns (rows and
 // columns of 1030 x 1000 in fp32 4.1 against 5.4, of 2003 x 1030 in bf16 6.1 against
-// 7.5; of 4096 x 1024 in bf16 5.4 against 5.1).
+// 7.5; of 4096 x 1024 in bf16 5.4 against 5.1).  One limit for all types: fp32 tiles
+// of 128 x 128 have 74 KB of LDS, two a CU, and were not timed against narrow ones past it.
 struct MxGrid {
   unsigned tall, low;
   MxGrid(int64_t batch, int64_t R, int64_t C)
@@ -776,6 +777,8 @@ constexpr int64_t kMxMaxDim = (int64_t)1 << 31;
 //  one a CU with at least 4096 of K: 1024, 1024, 65536 74 -> 54; 1000, 1030, 16384 40 -> 25; 512, 1536, 49152 77 -> 34;
 //  the sums' way through memory costs more than it gives at 1024, 1024, 12288 (18.0, shared 20.6; 16384 23.0, 24.0),
 //  512, 512, 24576 (15.8, 17.2) and 256, 256, 32768 (13.6, 15.4), but not at 128, 128, 65536 (24.2, 16.9).
+//  Tiles count whole, also where M or N fills a part of them alone (a few rows by tens of thousands of columns): the
+//  limits come of the sizes above, wide in both.
 struct MxPlan {
   int tile = 0, shares = 1;  // 0: by waves that share K
   MxPlan(int64_t M, int64_t N, int64_t K) {

@@ -2,9 +2,9 @@
 generation step runs in the place of ``fp8_routed_experts``.
 
 The grouped experts pad each expert's rows to 256; with a token or a few of them
-the layer is bound by the weights of the experts that are taken.  Here each of
-those is read once, from bf16 or from 4-bit weights.  No counterpart in the
-reference, which runs its grouped path at every size (train.py:2262-2299).
+the layer is bound by the weights of the experts that are taken.  Here those
+are read from memory once, from bf16 or from 4-bit weights.  No counterpart in
+the reference, which runs its grouped path at every size (train.py:2262-2299).
 There is no CPU fallback.
 """
 from __future__ import annotations
