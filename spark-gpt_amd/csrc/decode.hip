@@ -675,13 +675,12 @@ __global__ __launch_bounds__(256, W4 && NB > 1 ? 3 : 4) void decode_gateup_kerne
 // read again for each 2 C of them.  RAGGED: I is no multiple of a step.
 // h is in 32 bits.  A wave reads each value of a step once (16 lanes 64 columns
 // of a slot and part), splits it into three bf16 parts and hands them to the
-// matrix cores' lanes through its own LDS, 64 columns of K at a time.  Where the
-// slots take a quarter of the product's columns at most, their parts are columns
-// of their own: a third of the LDS reads and products, and the three sums meet
-// at the end.  (Layer of 2048 x 768, 8 of 128 experts, us: 4 tokens 4-bit 40.4, 16
-// tokens bf16 160; every lane splitting what it multiplies, without LDS, 46.6 and
-// 172; three products for few slots too 41.7 and 167; h in two bf16 parts as they
-// lie in memory, 17 bits of it, 38.6 and 168.)
+// matrix cores' lanes through its own LDS.  Where the slots take a quarter of the
+// product's columns at most, their parts are columns of their own: a third of the
+// LDS reads and products, and the three sums meet at the end.  (Layer of 2048 x
+// 768, 8 of 128 experts, in a graph, us: 4 tokens 4-bit 38.8, 16 tokens bf16 158.5;
+// every lane splitting what it multiplies, without LDS, 46.6 and 172; h in two
+// bf16 parts as they lie in memory, 17 bits of it, 38.4 and 168.)
 // With many slots an expert, h is what the CUs take most of (32 bits of each
 // slot beside C rows of weights): then SETS = 2 sets of 16 columns share it, and
 // gridDim.y work-groups share the steps of a column block; the last of them to
@@ -692,7 +691,7 @@ __global__ __launch_bounds__(512) void decode_down_kernel(DecodeArgs a) {
   constexpr int W = 8, P = 16 / C, CB = C * SETS, NB = 2;
   constexpr int kStep = P * Stretch<W4>::kStep, kSubs = Stretch<W4>::kPieces / 2;
   // rows of 64 bf16 values, 16 bytes further on by the banks from one to the next
-  constexpr int kHRow = 144, kMostTogether = SETS > 1 ? 1 : kSubs;
+  constexpr int kHRow = 144, kMostTogether = SETS > 1 ? 1 : kSubs;  // 64 columns a unit
   extern __shared__ __align__(16) float totals[];  // [W][T][CB]
   __shared__ __align__(16) uint8_t hparts[W][kMostTogether * 3 * 16 * kHRow];
   __shared__ short expert_of[kMaxExperts], slot_of[kSlots];
@@ -760,12 +759,16 @@ __global__ __launch_bounds__(512) void decode_down_kernel(DecodeArgs a) {
       const auto products = [&](auto blocks, auto loads) {
         constexpr int B = decltype(blocks)::value, X = decltype(loads)::value;
         constexpr int kRegs = SETS * (int)sizeof(typename WeightRows<W4>::Raw) / 4 + B * kSubs * X * 4;
-        // slots that are few enough have their parts in columns of their own: one product in the place of three
+        // slots that are few enough have their parts in columns of their own: one product in the place of three, and
+        // three steps a way through the LDS
         constexpr bool kApart = X == 1;
-        constexpr int kParts = kApart ? 1 : 3, kTogether = kApart ? 1 : kMostTogether;
-        // as many steps in flight as 256 registers hold
-        constexpr int kSpace = SETS > 1 ? 112 : kTogether > 1 ? 128 : 160;
-        constexpr int kInFlight = kSpace / kRegs < 8 ? kSpace / kRegs : 8;
+        constexpr int kParts = kApart ? 1 : 3, kTogether = kApart ? kSubs : kMostTogether;
+        constexpr int kSteps = kApart ? 3 * kMostTogether / kSubs : 1;
+        constexpr int kUnitRows = 16 * kParts, kPartRows = kApart ? 1 : 16;
+        // Steps in flight: three, or as many as 256 registers hold.  Up to eight are 49 KB of code in the place of 25 -
+        // 33, which each launch fetches anew (4 tokens 4-bit 40.2 us against 38.8, 16 tokens bf16 160.7, 158.5).
+        constexpr int kSpace = SETS > 1 ? 112 : kMostTogether > 1 ? 128 : 160;
+        constexpr int kInFlight = kSpace / kRegs < 3 ? kSpace / kRegs : 3;
         const float* hrow[B][X];
         uint32_t to[X];
 #pragma unroll
@@ -805,49 +808,61 @@ __global__ __launch_bounds__(512) void decode_down_kernel(DecodeArgs a) {
                   f[i][b][u][x] = *reinterpret_cast<const intx4*>(hrow[b][x] + s * kStep + 64 * u);
           }
           __builtin_amdgcn_sched_barrier(0);  // the loads stay ahead of the products
-#pragma unroll
-          for (int i = 0; i < U; ++i) {
+          Stretch<W4> fw[SETS];
+          const auto weights = [&](int i) {
             const int s = s0 + from + i;
-            Stretch<W4> fw[SETS];
 #pragma unroll
             for (int z = 0; z < SETS; ++z) {
               w.values(rw[i][z], fw[z]);
               if (RAGGED && s == steps - 1) w.zero_past(fw[z], I, s * kStep + part * Stretch<W4>::kStep, q);
             }
+          };
+#pragma unroll
+          for (int i0 = 0; i0 < U; i0 += kSteps) {
+            if constexpr (kSteps == 1) weights(i0);
 #pragma unroll
             for (int b = 0; b < B; ++b)
 #pragma unroll
               for (int u0 = 0; u0 < kSubs; u0 += kTogether) {
 #pragma unroll
-                for (int u = 0; u < kTogether; ++u)
+                for (int c = 0; c < kSteps && i0 + c < U; ++c)
 #pragma unroll
-                  for (int x = 0; x < X; ++x) {
-                    intx2 h[3];
-                    three_parts(f[i][b][u0 + u][x], h);
+                  for (int u = 0; u < kTogether; ++u)
 #pragma unroll
-                    for (int p = 0; p < 3; ++p)
-                      *reinterpret_cast<intx2*>(hs + (u * 48 + p * (kApart ? 1 : 16)) * kHRow + to[x]) = h[p];
-                  }
+                    for (int x = 0; x < X; ++x) {
+                      intx2 h[3];
+                      three_parts(f[i0 + c][b][u0 + u][x], h);
+#pragma unroll
+                      for (int p = 0; p < 3; ++p)
+                        *reinterpret_cast<intx2*>(hs + ((c * kTogether + u) * kUnitRows + p * kPartRows) * kHRow +
+                                                  to[x]) = h[p];
+                    }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                bf16x8 h[kTogether][2][kParts];
+                bf16x8 h[kSteps][kTogether][2][kParts];
 #pragma unroll
-                for (int u = 0; u < kTogether; ++u)
+                for (int c = 0; c < kSteps && i0 + c < U; ++c)
 #pragma unroll
-                  for (int j = 0; j < 2; ++j)
+                  for (int u = 0; u < kTogether; ++u)
 #pragma unroll
-                    for (int p = 0; p < kParts; ++p)
-                      h[u][j][p] =
-                          *reinterpret_cast<const bf16x8*>(hs + (u * 48 + p * 16 + r) * kHRow + 64 * j + 16 * q);
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                      for (int p = 0; p < kParts; ++p)
+                        h[c][u][j][p] = *reinterpret_cast<const bf16x8*>(
+                            hs + ((c * kTogether + u) * kUnitRows + p * 16 + r) * kHRow + 64 * j + 16 * q);
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-                for (int u = 0; u < kTogether; ++u)
+                for (int c = 0; c < kSteps && i0 + c < U; ++c) {
+                  if constexpr (kSteps > 1) weights(i0 + c);
 #pragma unroll
-                  for (int j = 0; j < 2; ++j)
+                  for (int u = 0; u < kTogether; ++u)
 #pragma unroll
-                    for (int p = 0; p < kParts; ++p)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
-                      for (int z = 0; z < SETS; ++z)
-                        acc[b][z] = mfma16(fw[z].w[2 * (u0 + u) + j], h[u][j][p], acc[b][z]);
+                      for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                        for (int z = 0; z < SETS; ++z)
+                          acc[b][z] = mfma16(fw[z].w[2 * (u0 + u) + j], h[c][u][j][p], acc[b][z]);
+                }
               }
           }
         });
@@ -961,12 +976,12 @@ template <bool W4>
 void launch_experts(DecodeArgs a, hipStream_t s) {
   // Columns a work-group of down: such that at D = 1024 (bf16), 2048 and 4096 there is one for each CU; narrower layers
   // leave CUs without one.  In a graph, us a layer with 4, 8 and 16 columns:
-  //  bf16  T = 16, D = 1024, 2 of 8 experts of 1536 32.9, 34.1, 37.9; T = 4, D = 512, the same experts 21.3, 22.7, 26.8;
+  //  bf16  T = 16, D = 1024, 2 of 8 experts of 1536 32.9, 34.1, 37.9; T = 4, D = 512, the same ones 21.3, 22.7, 26.8;
   //        T = 1, D = 2048, 8 of 128 of 768 31.5, 27.8, 30.6; T = 4, D = 4096, 2 of 16 of 1536 73.3, 63.8, 60.0
   //  4-bit T = 4, 8 of 128 of 768, D = 512 30.0, 31.9, 37.3; 1024 34.1, 35.2, 40.3; 2048 50.8, 40.1, 45.3; D = 4096, 8
   //        of 32 77.7, 55.9, 48.1
-  // Beyond 16 tokens 32 columns, whose steps are shared (T = 64, D = 2048, 6 of 64 of 1032: 185 against 227 with 16; T =
-  // 24, D = 1024, 2 of 8: 35.5 against 42.3; T = 16, the first of the layers above: 33.8).
+  // Beyond 16 tokens 32 columns, whose steps are shared (T = 64, D = 2048, 6 of 64 of 1032: 185 against 227 with 16;
+  // T = 24, D = 1024, 2 of 8: 35.5 against 42.3; T = 16, the first of the layers above: 33.8).
   const int C = a.T > 16 ? 32 : a.D >= 4096 ? 16 : !W4 && a.D < 2048 ? 4 : 8;
   const int step = (C < 16 ? 16 / C : 1) * Stretch<W4>::kStep;
   a.ldh = (a.I + step - 1) / step * step;
