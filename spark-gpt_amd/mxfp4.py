@@ -83,7 +83,7 @@ def _is_mxfp4(name: str, q, dims=(2,)) -> None:
 def _no_tangent(what: str, *tensors) -> None:
     """Refuses inputs of forward-mode differentiation: a dual tensor needs no gradient, so the paths without a node
     would drop its tangent."""
-    if not torch.compiler.is_compiling() and forward_ad._current_level >= 0 and any(
+    if forward_ad._current_level >= 0 and not torch.compiler.is_compiling() and any(
             isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what} has no forward-mode derivative")
 
