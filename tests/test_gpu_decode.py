@@ -489,3 +489,26 @@ def test_every_number_of_slots(dev, D, I, four):
         out, sel = sg.decode_routed_experts(x[:T], router, w_gu, w_down, 1)
         bad = ~((out.double() - ref[:T]).abs() <= bound[:T])
         assert not bad.any() and not sel.any(), (T, int(bad.sum()), out[bad][:4], ref[:T][bad][:4])
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("which,least", [("x", -128), ("w_gu", -128), ("w_down", -128), ("w_gu", -124),
+                                         ("w_down", -124)])
+@pytest.mark.parametrize("T", [1, 9, 24])
+def test_subnormal_values(dev, T, which, least, four):
+    """Subnormal tokens and weights (4-bit: scales from 2^-127 on) beside large ones count as what they are.  Gate and up
+    weights N(0, 2^-6) 2^-128 are nearly all zeros in 4 bits, below 2^-129, half the smallest code; no other case's are."""
+    x, router, w_gu, w_down = _layer(dev, T, 4, 64, 40, seed=T)
+    tiny = {"x": x, "w_gu": w_gu, "w_down": w_down}[which]
+    tiny.copy_((tiny.double() * 2.0 ** least).to(torch.bfloat16))
+    for t, power in ((x, 100 if which == "w_gu" else 0), (w_gu, 100 if which == "x" else 60 if which == "w_down" else 0)):
+        if power and t is not tiny:
+            t.copy_((t.double() * 2.0 ** power).to(torch.bfloat16))
+    if which in ("x", "w_gu"):  # h is tiny then: about 2^-60
+        w_down.copy_((w_down.double() * 2.0 ** 60).to(torch.bfloat16))
+    values = (w_gu, w_down)
+    if four:
+        values = (Q.quantized(w_gu).to(dev), Q.quantized(w_down).to(dev))
+        w_gu, w_down = sg.mxfp4_quantize(w_gu), sg.mxfp4_quantize(w_down)
+    out, _ = _check(x, router, w_gu, w_down, 2, values=values)
+    assert out.any(1).all() or (four and (which, least) == ("w_gu", -128))
