@@ -322,10 +322,10 @@ def test_same_layer_as_the_grouped_experts(dev):
 @pytest.mark.parametrize("four", [False, True])
 @pytest.mark.parametrize("T,D", [(1, 64), (1, 2048), (1, 4096), (9, 64), (9, 2048), (24, 64)])
 def test_h_keeps_its_32_bits(dev, T, D, four):
-    """Two columns of h, 64 (1 + 2^-8 + 2^-17) and 64 (1 + 2^-8), whose difference is the output: 2^-11, which the 17 bits
-    of two bf16 parts do not hold.  In steps of 2^-23 of 65, which h stays below: a sum of three products is off by 3, the
-    sigmoid by 1, the two products by 1 together; the difference of what two columns' three parts give, six products, by
-    12: 2 * 5 + 12 in all."""
+    """Two columns of h, 64 (1 + 2^-8 + 2^-17) and 64 (1 + 2^-8), whose difference is the output: 2^-11, which the 17
+    bits of two bf16 parts do not hold.  In steps of 2^-23 of 65, which h stays below: a sum of three products is off
+    by 3, the sigmoid by 1, the two products by 1 together; the difference of what two columns' three parts give, six
+    products, by 12: 2 * 5 + 12 in all."""
     x, router, w_gu, w_down = _layer(dev, T, 2, D, 16)
     for t in (x, router, w_gu, w_down):
         t.zero_()
@@ -344,7 +344,8 @@ def test_h_keeps_its_32_bits(dev, T, D, four):
 @pytest.mark.parametrize("four", [False, True])
 @pytest.mark.parametrize("T", [1, 9, 24])
 def test_infinities_in_h(dev, T, four):
-    """An infinity in one column of h is one in the output, of either sign; both, or a weight of zero beside it, are a NaN."""
+    """An infinity in one column of h is one in the output, of either sign; both, or a weight of zero beside it, are a
+    NaN."""
     def run(columns, zero_weight=False):
         x, router, w_gu, w_down = (torch.zeros_like(t) for t in _layer(dev, T, 2, 64, 16))
         x[:, 0] = 1
@@ -364,8 +365,8 @@ def test_infinities_in_h(dev, T, four):
 @pytest.mark.parametrize("four", [False, True])
 @pytest.mark.parametrize("T", [1, 6, 24])
 def test_silu_of_large_gates(dev, T, four):
-    """silu(g) less 64 v, v the fp32 value nearest to silu(g) / 64, for gates whose product with log2(e) rounds badly (off
-    by 26 steps of 2^-23 in the exponential).  In those steps of silu(g): the exponential is off by 1, the sum and the
+    """silu(g) less 64 v, v the fp32 value nearest to silu(g) / 64, for gates whose product with log2(e) rounds badly
+    (off by 26 steps of 2^-23 in the exponential).  In those steps of silu(g): the exponential is off by 1, the sum and the
     quotient by 1 together, v's three parts by 2, the down sums' six products by 6: 10."""
     x, router, w_gu, w_down = (torch.zeros_like(t) for t in _layer(dev, T, 2, 64, 16))
     g = -torch.tensor([61.25, 58.0, 54.75, 51.5, 48.25, 45.0], dtype=torch.float64, device=dev)
@@ -496,12 +497,13 @@ def test_every_number_of_slots(dev, D, I, four):
                                          ("w_down", -124)])
 @pytest.mark.parametrize("T", [1, 9, 24])
 def test_subnormal_values(dev, T, which, least, four):
-    """Subnormal tokens and weights (4-bit: scales from 2^-127 on) beside large ones count as what they are.  Gate and up
-    weights N(0, 2^-6) 2^-128 are nearly all zeros in 4 bits, below 2^-129, half the smallest code; no other case's are."""
+    """Subnormal tokens and weights (4-bit: scales from 2^-127 on) beside large ones count as what they are.  Gate and
+    up weights N(0, 2^-6) 2^-128 are nearly all zeros in 4 bits, below 2^-129, half the smallest code; no other case's
+    are."""
     x, router, w_gu, w_down = _layer(dev, T, 4, 64, 40, seed=T)
     tiny = {"x": x, "w_gu": w_gu, "w_down": w_down}[which]
     tiny.copy_((tiny.double() * 2.0 ** least).to(torch.bfloat16))
-    for t, power in ((x, 100 if which == "w_gu" else 0), (w_gu, 100 if which == "x" else 60 if which == "w_down" else 0)):
+    for t, power in ((x, {"w_gu": 100}.get(which, 0)), (w_gu, {"x": 100, "w_down": 60}.get(which, 0))):
         if power and t is not tiny:
             t.copy_((t.double() * 2.0 ** power).to(torch.bfloat16))
     if which in ("x", "w_gu"):  # h is tiny then: about 2^-60
