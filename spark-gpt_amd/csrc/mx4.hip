@@ -779,9 +779,9 @@ constexpr int64_t kMxMaxDim = (int64_t)1 << 31;
 //  512, 512, 24576 (15.8, 17.2) and 256, 256, 32768 (13.6, 15.4), but not at 128, 128, 65536 (24.2, 16.9).
 //  Tiles count whole, also where M or N fills a part of them alone, and the limits come of the sizes above, wide in
 //  both.  A few rows by very many columns, in a graph (us): 128 x 128 wins from N = 65536 on, also for one row (1,
-//  65536, 2048 15.7, 16 x 32 17.2; 64, 131072, 2048 36.4, 64 x 64 40.9), and loses at 16384 (8, 16384, 2048 8.2,
-//  16 x 32 5.8; 64, 16384, 4096 12.8, 64 x 64 10.4; 16384, 16, 8192 20.4, 64 x 32 13.9); 256 x 256, which the rule takes there for a
-//  long K, loses to 128 x 128 (8, 131072, 4096 59.4 and 53.5; 64, 65536, 4096 38.0 and 36.4).
+//  65536, 2048 15.7, 16 x 32 17.2; 64, 131072, 2048 36.4, 64 x 64 40.9), and loses at 16384 (8, 16384, 2048 8.2, 16 x
+//  32 5.8; 64, 16384, 4096 12.8, 64 x 64 10.4; 16384, 16, 8192 20.4, 64 x 32 13.9); 256 x 256, which the rule takes
+//  there for a long K, loses to 128 x 128 (8, 131072, 4096 59.4 and 53.5; 64, 65536, 4096 38.0 and 36.4).
 struct MxPlan {
   int tile = 0, shares = 1;  // 0: by waves that share K
   MxPlan(int64_t M, int64_t N, int64_t K) {
